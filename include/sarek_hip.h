@@ -673,6 +673,50 @@ int sarek_hip_gemm_f16_bias_relu_rowsum(const uint16_t *a, const uint16_t *b, co
 int sarek_hip_cast_f32_to_bf16(const float *in, uint16_t *out, int64_t n, sarek_hip_stream stream);
 int sarek_hip_cast_f32_to_f16(const float *in, uint16_t *out, int64_t n, sarek_hip_stream stream);
 
+/* ---------------------------------------------------------------------- */
+/* Microscaled 8- and 4-bit floating point: the matrices of a feed-forward layer and the operators on them (no counterpart in the
+ * reference).  A row of k values is held in blocks of 32; a block's scale is 2^E, E = floor(log2 of its largest magnitude) - 8 for
+ * SAREK_HIP_MX_FP8 (codes e4m3, up to 448) or - 2 for SAREK_HIP_MX_FP4 (codes e2m1, up to 6), held as the byte E + 127, at least 0.  A
+ * value v is the code nearest to v / 2^E, ties to the even code, past the largest as the largest.  A block with a NaN or an infinity
+ * has the byte 255 and stands for 32 NaNs.
+ * Layout: `codes` holds rows of kp = sarek_hip_mx_row_values(k) codes (k rounded up to 256), one byte each for FP8, two to a byte for
+ * FP4 (the first in the low half); `scales` rows of kp / 32 bytes.  What is behind k is zeros, and has to be where a caller brings
+ * codes of their own.  Codes start at a multiple of 16 bytes, scales of 8, as every row of such a matrix does.
+ * Types of the other matrices: float32, bf16 or fp16; their rows are `stride` elements apart (at least their length), at any alignment
+ * of an element.  rows = 0 (m = 0) is no error and writes nothing but sums over no rows; k and n are positive.                      */
+enum { SAREK_HIP_TYPE_F32 = 0, SAREK_HIP_TYPE_BF16 = 1, SAREK_HIP_TYPE_F16 = 2 };
+enum { SAREK_HIP_MX_FP8 = 0, SAREK_HIP_MX_FP4 = 1 };
+int64_t sarek_hip_mx_row_values(int64_t k);     /* 0 for k <= 0 */
+int sarek_hip_mx_quantize(const void *x, int type, int64_t x_stride, unsigned char *codes, unsigned char *scales, int format,
+                          int64_t rows, int64_t k, sarek_hip_stream stream);
+/* The values that codes and scales stand for, rounded to the type (bf16 and float32 hold them all exactly but for a type's least
+ * exponents).                                                                                                                       */
+int sarek_hip_mx_dequantize(const unsigned char *codes, const unsigned char *scales, int format, void *out, int type,
+                            int64_t out_stride, int64_t rows, int64_t k, sarek_hip_stream stream);
+/* h = x + residual, rounded to the type; rstd[row] = (mean of h^2 + eps)^-1/2; the 8-bit form of h rstd weight, all in 32 bits
+ * between.  x, residual, weight and h are of one type.  residual NULL: h is x, and is written only where h is not NULL.  rstd may be
+ * NULL.  h may be x or residual itself; anything else must not overlap.                                                            */
+int sarek_hip_rms_norm_mx(const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const void *weight, int type,
+                          float eps, void *h, int64_t h_stride, unsigned char *codes, unsigned char *scales, float *rstd,
+                          int64_t rows, int64_t k, sarek_hip_stream stream);
+/* The norm's gradient, the 8-bit rounding taken as the identity: for n = h rstd and g = weight dy
+ *   dx = rstd (g - n mean(n g)) + dh     (the gradient of x and of residual; dh, what comes to h past the norm, may be NULL)
+ *   dweight[c] = sum over the rows of dy n     (float32, the same bits on every run)
+ * dy, h, weight, dh and dx are of one type; dx may be dy or dh itself.  workspace: at least
+ * sarek_hip_rms_norm_backward_workspace_floats(rows, k) floats, SAREK_HIP_E_WORKSPACE else.                                       */
+int64_t sarek_hip_rms_norm_backward_workspace_floats(int64_t rows, int64_t k);
+int sarek_hip_rms_norm_backward(const void *dy, int64_t dy_stride, const void *h, int64_t h_stride, const void *weight,
+                                const float *rstd, const void *dh, int64_t dh_stride, int type, void *dx, int64_t dx_stride,
+                                float *dweight, int64_t rows, int64_t k, float *workspace, int64_t workspace_floats,
+                                sarek_hip_stream stream);
+/* C[m x n] = A[m x k] . B[n x k]^T (+ bias[col]) (then max(0, .) where relu is not 0; a NaN stays one): A microscaled in a_format, B in
+ * FP4 (a layer's weights, one row for each column of C), bias float32 or NULL, C of c_type, its rows c_stride elements apart.  Sums of
+ * FP4 with FP4 are held in 32 bits throughout.  FP8 with FP4: the matrix unit adds 128 products at a time on a grid of about 2^-14 of
+ * the largest of them (measured), so C is 16-bit there; float32 is SAREK_HIP_E_UNSUPPORTED.                                       */
+int sarek_hip_gemm_mx(const unsigned char *a_codes, const unsigned char *a_scales, int a_format, const unsigned char *b_codes,
+                      const unsigned char *b_scales, const float *bias, int relu, void *c, int c_type, int64_t c_stride, int64_t m,
+                      int64_t n, int64_t k, sarek_hip_stream stream);
+
 /* Persistent cache of compiled kernels: the reference's Framework_cache
  * (sarek/framework/Framework_cache.ml:63-141; used there by the Vulkan plugin,
  * sarek-vulkan/Vulkan_api.ml:1254-1283).  Directory: $XDG_CACHE_HOME, else

@@ -7,6 +7,7 @@ current stream only.
 """
 import ctypes as C
 import os
+from typing import NamedTuple
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # SAREK_HIP_MEASURE_BUILD=1 (bench.py --measure-build) loads the measurement build instead: the product's code plus the
@@ -36,6 +37,8 @@ E_PARSE = -6
 E_CODEGEN = -7
 E_BUFFER_TOO_SMALL = -8
 
+TYPE_F32, TYPE_BF16, TYPE_F16 = range(3)
+MX_FP8, MX_FP4 = range(2)
 LANG_CUDA, LANG_OPENCL, LANG_PTX, LANG_SPIRV, LANG_GLSL, LANG_HIP = range(6)
 ARG_BUFFER, ARG_INT32, ARG_INT64, ARG_FLOAT32, ARG_FLOAT64 = range(5)
 
@@ -153,6 +156,14 @@ SYMBOLS = {
     "sarek_hip_gemm_f16_bias_relu_rowsum": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "sarek_hip_cast_f32_to_bf16": (_i, [_vp, _vp, _i64, _vp]),
     "sarek_hip_cast_f32_to_f16": (_i, [_vp, _vp, _i64, _vp]),
+    "sarek_hip_mx_row_values": (_i64, [_i64]),
+    "sarek_hip_mx_quantize": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i64, _i64, _vp]),
+    "sarek_hip_mx_dequantize": (_i, [_vp, _vp, _i, _vp, _i, _i64, _i64, _i64, _vp]),
+    "sarek_hip_rms_norm_mx": (_i, [_vp, _i64, _vp, _i64, _vp, _i, _f, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "sarek_hip_rms_norm_backward_workspace_floats": (_i64, [_i64, _i64]),
+    "sarek_hip_rms_norm_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i, _vp, _i64, _vp, _i64, _i64, _vp,
+                                         _i64, _vp]),
+    "sarek_hip_gemm_mx": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _vp]),
     "sarek_hip_cache_dir": (_i, [C.c_char_p, _sz]),
     "sarek_hip_cache_compute_key": (_i, [C.c_char_p, C.c_char_p, C.c_char_p, C.c_char_p]),
     "sarek_hip_cache_get": (_i, [C.c_char_p, _vp, _sz, C.POINTER(_sz), C.POINTER(_i)]),
@@ -809,6 +820,156 @@ def cast_f16(x):
     out = torch.empty(x.shape, dtype=torch.float16, device=x.device)
     check(lib.sarek_hip_cast_f32_to_f16(_ptr(x), _ptr(out), x.numel(), _stream()))
     return out
+
+
+# ---------------------------------------------------------------------------
+# Microscaled 8- and 4-bit rows: quantisation, norm, products
+
+class MxTensor(NamedTuple):
+    """A matrix of k columns in microscaled 8- or 4-bit floating point.  codes: uint8 [rows, kp] (fmt "fp8", e4m3) or
+    [rows, kp / 2] (fmt "fp4", e2m1, the first of two in the low half of a byte), kp = mx_row_values(k); scales: uint8
+    [rows, kp / 32], a byte E + 127 for each 32 codes, which stand for their values times 2^E (255: for NaNs).  What is
+    behind column k is zeros."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    fmt: str
+    k: int
+
+    @property
+    def rows(self):
+        return self.codes.shape[0]
+
+
+_MX_FORMATS = {"fp8": MX_FP8, "fp4": MX_FP4}
+_MX_TYPES = {torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16}
+
+
+def mx_row_values(k):
+    """Codes in a row that holds k values: k rounded up to a multiple of 256."""
+    return (k + 255) & ~255
+
+
+def _need_rows(t, name, dtype=None, shape=None):
+    """A device matrix with adjacent columns, its rows at any distance; its distance from row to row."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in _MX_TYPES
+            and (t.stride(1) == 1 or t.shape[1] == 1)):
+        raise TypeError(f"{name}: expected a device matrix of float32, bfloat16 or float16 with adjacent columns")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected {tuple(shape)}, got {tuple(t.shape)}")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _need_mx(t, name):
+    if not isinstance(t, MxTensor) or t.fmt not in _MX_FORMATS:
+        raise TypeError(f"{name}: expected an MxTensor in fp8 or fp4")
+    _need(t.codes, torch.uint8, name + ".codes")
+    _need(t.scales, torch.uint8, name + ".scales")
+    kp = (t.k + 255) & ~255
+    if t.k < 1 or t.codes.dim() != 2 or t.codes.shape[1] != (kp if t.fmt == "fp8" else kp // 2) \
+            or t.scales.shape != (t.codes.shape[0], kp // 32):
+        raise ValueError(f"{name}: codes {tuple(t.codes.shape)} and scales {tuple(t.scales.shape)} are not {t.fmt} rows of {t.k}")
+
+
+def _mx_out(out, rows, k, fmt, like, name):
+    if fmt not in _MX_FORMATS:
+        raise ValueError(f"{name}: unknown format {fmt!r}")
+    if out is not None:
+        _need_mx(out, name)
+        if (out.rows, out.k, out.fmt) != (rows, k, fmt):
+            raise ValueError(f"{name}: out is {out.rows} x {out.k} in {out.fmt}, expected {rows} x {k} in {fmt}")
+        return out
+    kp = (k + 255) & ~255
+    return MxTensor(like.new_empty((rows, kp if fmt == "fp8" else kp // 2), dtype=torch.uint8),
+                    like.new_empty((rows, kp // 32), dtype=torch.uint8), fmt, k)
+
+
+def mx_quantize(x, fmt, out=None):
+    """The rows of x (float32, bfloat16 or float16) in "fp8" or "fp4", as an MxTensor."""
+    stride = _need_rows(x, "x")
+    rows, k = x.shape
+    q = _mx_out(out, rows, k, fmt, x, "mx_quantize")
+    check(lib.sarek_hip_mx_quantize(x.data_ptr(), _MX_TYPES[x.dtype], stride, q.codes.data_ptr(), q.scales.data_ptr(),
+                                    _MX_FORMATS[fmt], rows, k, _raw_stream()))
+    return q
+
+
+def mx_dequantize(q, dtype=torch.bfloat16, out=None):
+    """The values that an MxTensor stands for."""
+    _need_mx(q, "q")
+    if out is None:
+        out = q.codes.new_empty((q.rows, q.k), dtype=dtype)
+    stride = _need_rows(out, "out", dtype, (q.rows, q.k))
+    check(lib.sarek_hip_mx_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), _MX_FORMATS[q.fmt], out.data_ptr(),
+                                      _MX_TYPES[dtype], stride, q.rows, q.k, _raw_stream()))
+    return out
+
+
+def rms_norm_mx(x, weight, residual=None, eps=1e-6, out=None, h=None):
+    """h = x + residual (in x's type), rstd = (mean of h^2 + eps)^-1/2 of each row, and h * rstd * weight in "fp8".
+    Returns (MxTensor, h, rstd); without a residual h is x.  h: where the sum goes (x or residual itself, for instance)."""
+    stride = _need_rows(x, "x")
+    rows, k = x.shape
+    _need(weight, x.dtype, "weight")
+    if weight.shape != (k,):
+        raise ValueError(f"rms_norm_mx: {k} weights expected, got {tuple(weight.shape)}")
+    residual_stride = 0 if residual is None else _need_rows(residual, "residual", x.dtype, x.shape)
+    if h is None and residual is not None:
+        h = x.new_empty((rows, k))
+    h_stride = 0 if h is None else _need_rows(h, "h", x.dtype, x.shape)
+    q = _mx_out(out, rows, k, "fp8", x, "rms_norm_mx")
+    rstd = x.new_empty(rows, dtype=torch.float32)
+    check(lib.sarek_hip_rms_norm_mx(x.data_ptr(), stride, None if residual is None else residual.data_ptr(), residual_stride,
+                                    weight.data_ptr(), _MX_TYPES[x.dtype], eps, None if h is None else h.data_ptr(), h_stride,
+                                    q.codes.data_ptr(), q.scales.data_ptr(), rstd.data_ptr(), rows, k, _raw_stream()))
+    return q, x if h is None else h, rstd
+
+
+def rms_norm_backward(dy, h, weight, rstd, dh=None, out=None):
+    """The gradients of rms_norm_mx with the 8-bit rounding taken as the identity: dy for its output, dh for its h (None: no
+    gradient comes that way).  Returns (dx, dweight): dx is x's and the residual's, in their type; dweight is float32."""
+    stride = _need_rows(h, "h")
+    rows, k = h.shape
+    dy_stride = _need_rows(dy, "dy", h.dtype, h.shape)
+    dh_stride = 0 if dh is None else _need_rows(dh, "dh", h.dtype, h.shape)
+    _need(weight, h.dtype, "weight")
+    _need(rstd, torch.float32, "rstd")
+    if weight.shape != (k,) or rstd.shape != (rows,):
+        raise ValueError("rms_norm_backward: shape mismatch")
+    dx = h.new_empty((rows, k)) if out is None else out
+    dx_stride = _need_rows(dx, "out", h.dtype, h.shape)
+    dweight = h.new_empty(k, dtype=torch.float32)
+    workspace = h.new_empty(lib.sarek_hip_rms_norm_backward_workspace_floats(rows, k), dtype=torch.float32)
+    check(lib.sarek_hip_rms_norm_backward(dy.data_ptr(), dy_stride, h.data_ptr(), stride, weight.data_ptr(), rstd.data_ptr(),
+                                          None if dh is None else dh.data_ptr(), dh_stride, _MX_TYPES[h.dtype], dx.data_ptr(),
+                                          dx_stride, dweight.data_ptr(), rows, k, workspace.data_ptr(), workspace.numel(),
+                                          _raw_stream()))
+    return dx, dweight
+
+
+def gemm_mx(a, b, bias=None, relu=False, dtype=torch.bfloat16, out=None):
+    """a (rows of k values, "fp8" or "fp4") times the transpose of b (n rows of k values, "fp4"): [rows, n] in dtype, with
+    bias (float32, n values) added and, where asked, negative values set to 0.  An "fp8" a goes to 16-bit types."""
+    _need_mx(a, "a")
+    _need_mx(b, "b")
+    if b.fmt != "fp4":
+        raise ValueError("gemm_mx: b is held in fp4")
+    if a.k != b.k:
+        raise ValueError("gemm_mx: inner dimensions differ")
+    if dtype not in _MX_TYPES:
+        raise TypeError(f"gemm_mx: {dtype} is none of float32, bfloat16, float16")
+    m, n = a.rows, b.rows
+    if bias is not None:
+        _need(bias, torch.float32, "bias")
+        if bias.shape != (n,):
+            raise ValueError(f"gemm_mx: {n} biases expected, got {tuple(bias.shape)}")
+    c = a.codes.new_empty((m, n), dtype=dtype) if out is None else out
+    c_stride = _need_rows(c, "out", dtype, (m, n))
+    check(lib.sarek_hip_gemm_mx(a.codes.data_ptr(), a.scales.data_ptr(), _MX_FORMATS[a.fmt], b.codes.data_ptr(),
+                                b.scales.data_ptr(), None if bias is None else bias.data_ptr(), 1 if relu else 0, c.data_ptr(),
+                                _MX_TYPES[dtype], c_stride, m, n, a.k, _raw_stream()))
+    return c
 
 
 def make_args(items):
