@@ -8,6 +8,7 @@
 // place is free, as long as both operands and the scales agree: of 256 k, step s of two puts block 2 p + s in place p, so that a lane's
 // 4-bit codes of both steps are 32 bytes in a row and its scales two.
 // The weights are the first operand, so a lane's four results are four columns of one row of C.
+#include <type_traits>
 #include <utility>
 
 #include "gemm_common.hpp"
@@ -25,6 +26,14 @@ template <bool Fp8, int Step> __device__ __forceinline__ f32x4_t mfma_mx(u32x4_t
   const i32x8 wide = {static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3]), 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide, a, c, kFormatE2M1, Fp8 ? kFormatE4M3 : kFormatE2M1, Step, b_scales,
                                                           Step, a_scales);
+}
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+// 32 rows of each operand and 64 of k, two blocks: lane l brings row l % 32 of the block in place l / 32, and its scale.
+template <int Scale> __device__ __forceinline__ f32x16 mfma_mx32(u32x4 b, u32x4 a, f32x16 c, int b_scales, int a_scales) {
+  const i32x8 wide_b = {static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3]), 0, 0, 0, 0};
+  const i32x8 wide_a = {static_cast<int>(a[0]), static_cast<int>(a[1]), static_cast<int>(a[2]), static_cast<int>(a[3]), 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide_b, wide_a, c, kFormatE2M1, kFormatE2M1, Scale, b_scales, Scale, a_scales);
 }
 
 // One wave to a 16 x 16 tile of C, operands straight from memory.
@@ -96,24 +105,30 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
                                                            int m, int n, int kp, int tiles_m, int tiles_n) {
   constexpr int kStage = Fp8 ? 128 : 256;            // values of k in a stage: 128 bytes of a row of A
   constexpr int kRowB = Fp8 ? 64 : 128;              // bytes of a row of B in a stage
+  constexpr int kRing = Fp8 ? 3 : 2;                 // stages in LDS
   constexpr int kPerSpan = 512 / kStage;             // stages that 16 scale bytes of a row last
-  constexpr int kPeriod = 2 * kPerSpan;
+  constexpr int kPeriod = Fp8 ? 12 : 2;              // stages after which places in LDS and in the span repeat
   constexpr int kBytesA = 256 * 128, kBytesB = 256 * kRowB, kBytesS = 256 * 16;
   constexpr int kMovesA = kBytesA / 1024 / 8, kMovesB = kBytesB / 1024 / 8;   // transfers of a wave in a stage
+  constexpr int kRows = Fp8 ? 16 : 32;               // rows and columns of an MFMA
+  constexpr int kTilesA = 128 / kRows, kTilesB = 64 / kRows;
+  static_assert(kPeriod % kRing == 0 && kPeriod % kPerSpan == 0 && kRing * (kBytesA + kBytesB) + 2 * kBytesS <= 160 * 1024, "ring");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, place = lane >> 4;
-  const int wm = wave >> 1, wn = wave & 1;           // 64 rows of C by 128 columns to a wave
+  const int r = lane & (kRows - 1), place = lane / kRows;
+  const int wm = wave >> 2, wn = wave & 3;           // 128 rows of C by 64 columns to a wave
   int tm, tn;
   tile_of_block(tiles_m, tiles_n, 1, tm, tn);
   const int m0 = tm * 256, n0 = tn * 256;
   const int pitch_a = Fp8 ? kp : kp / 2, pitch_b = kp / 2, pitch_s = kp / kMxBlock;
   const int rows_a = min(256, m - m0), rows_b = min(256, n - n0);
-  // Rows past the end are out of the resources' range and read as zeros.
-  const __amdgpu_buffer_rsrc_t ra = make_rsrc(a + static_cast<int64_t>(m0) * pitch_a, static_cast<uint32_t>(rows_a) * pitch_a);
-  const __amdgpu_buffer_rsrc_t rb = make_rsrc(b + static_cast<int64_t>(n0) * pitch_b, static_cast<uint32_t>(rows_b) * pitch_b);
   const bool of_a = wave < 4;
+  const uint8_t *const a_from = a + static_cast<int64_t>(m0) * pitch_a, *const b_from = b + static_cast<int64_t>(n0) * pitch_b;
   const __amdgpu_buffer_rsrc_t rs = make_rsrc(of_a ? a_scales + static_cast<int64_t>(m0) * pitch_s : b_scales + static_cast<int64_t>(n0) * pitch_s,
                                               static_cast<uint32_t>(of_a ? rows_a : rows_b) * pitch_s);
+  // Where piece q (16 bytes) of a row lies in its row of LDS: at q ^ (row / 2 % 8) in rows of 128 bytes, q ^ place64(row) in rows of 64.  A
+  // ds_read_b128 is served 16 lanes at a time, row quads 0 and 3 of one place with 1 and 2 of the next and the other way round; they
+  // meet no bank twice so, whether they are of one piece or two.  (As lanes come, with pieces 2 p + step: 44 % of LDS cycles were conflicts.)
+  auto place64 = [](int row) { return ((row >> 2 ^ row >> 3) & 1) << 1 | (row >> 3 & 1); };
   uint32_t off_a[kMovesA], off_b[kMovesB];
 #pragma unroll
   for (int i = 0; i < kMovesA; ++i) {
@@ -124,81 +139,168 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
   for (int i = 0; i < kMovesB; ++i) {
     constexpr int chunks = kRowB / 16;
     const int row = (wave + 8 * i) * (64 / chunks) + lane / chunks;
-    off_b[i] = static_cast<uint32_t>(row) * pitch_b + (((lane % chunks) ^ (Fp8 ? (row >> 2) & 3 : (row >> 1) & 7)) << 4);
+    off_b[i] = static_cast<uint32_t>(row) * pitch_b + (((lane % chunks) ^ (Fp8 ? place64(row) : (row >> 1) & 7)) << 4);
   }
   const uint32_t off_s = static_cast<uint32_t>((wave & 3) * 64 + lane) * pitch_s;
   const int stages = kp / kStage, last_span = (stages - 1) / kPerSpan;
 
-  auto issue_codes = [&](char *la, char *lb, int s) {
-    const int at = min(s, stages - 1);
-#pragma unroll
-    for (int i = 0; i < kMovesA; ++i) dma16(ra, off_a[i], at * 128, la + (wave + 8 * i) * 1024);
-#pragma unroll
-    for (int i = 0; i < kMovesB; ++i) dma16(rb, off_b[i], at * kRowB, lb + (wave + 8 * i) * 1024);
+  // Rows past the end are out of the resources' range and read as zeros; past the last stage the range is empty, and nothing moves.
+  auto move_a = [&](char *la, int i, int s) {
+    dma16(make_rsrc(a_from, s < stages ? static_cast<uint32_t>(rows_a) * pitch_a : 0u), off_a[i], s * 128, la + (wave + 8 * i) * 1024);
+  };
+  auto move_b = [&](char *lb, int i, int s) {
+    dma16(make_rsrc(b_from, s < stages ? static_cast<uint32_t>(rows_b) * pitch_b : 0u), off_b[i], s * kRowB, lb + (wave + 8 * i) * 1024);
   };
   // A row's last span may be 8 bytes: then the 16 that end with the row are taken.
-  auto issue_scales = [&](char *ls, int span) { dma16(rs, off_s, min(min(span, last_span) * 16, pitch_s - 16), ls + wave * 1024); };
+  char *const ls = lds_ring<68, 2 * kBytesS>;
+  auto move_scales = [&](int span) { dma16(rs, off_s, min(min(span, last_span) * 16, pitch_s - 16), ls + wave * 1024); };
 
-  f32x4_t acc[4][8];
+  using Acc = std::conditional_t<Fp8, f32x4_t, f32x16>;
+  Acc acc[kTilesA][kTilesB];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < kTilesA; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  int sa[4], sb[8];
-  const uint32_t pick = (Fp8 ? static_cast<uint32_t>(place | (4 + place) << 8) : static_cast<uint32_t>(2 * place | (2 * place + 1) << 8)) | 0x0C0C0000u;
-  auto scales_of = [&](const char *at, bool short_span) {
-    u32x4 d = *reinterpret_cast<const u32x4 *>(at);
-    d[0] = short_span ? d[2] : d[0];
-    d[1] = short_span ? d[3] : d[1];
-    return static_cast<int>(__builtin_amdgcn_perm(d[1], d[0], pick) | __builtin_amdgcn_perm(d[3], d[2], pick) << 16);
-  };
-  const int a_at = (wm * 64 + r) * 128, b_at = (wn * 128 + r) * kRowB;
+    for (int j = 0; j < kTilesB; ++j)
+#pragma unroll
+      for (int e = 0; e < kRows * kRows / 64; ++e) acc[i][j][e] = 0.f;
 
-  auto stage = [&](auto ic, int s) {
-    constexpr int I = decltype(ic)::value, ring = I & 1, span = (I / kPerSpan) & 1, in_span = I % kPerSpan;
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));
-    barrier_no_fence();
-    if constexpr (in_span == 0) issue_scales(lds_ring<64 + (span ^ 1), 2 * kBytesS>, s / kPerSpan + 1);
-    issue_codes(lds_ring<60 + (ring ^ 1), kBytesA>, lds_ring<62 + (ring ^ 1), kBytesB>, s + 1);
-    const char *la = lds_ring<60 + ring, kBytesA>, *lb = lds_ring<62 + ring, kBytesB>, *ls = lds_ring<64 + span, 2 * kBytesS>;
-    if constexpr (in_span == 0) {
-      const bool short_span = s / kPerSpan * 16 + 16 > pitch_s;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sa[i] = scales_of(ls + (wm * 64 + i * 16 + r) * 16, short_span);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sb[j] = scales_of(ls + kBytesS + (wn * 128 + j * 16 + r) * 16, short_span);
+  // Scales: a lane reads the 16 bytes of a row's span and keeps those that its place needs, in the order of the steps.
+  constexpr int kWords = Fp8 ? 1 : 2;
+  int sa[kTilesA][kWords], sb[kTilesB][kWords];
+  u32x4 raw_a[Fp8 ? 2 : 4], raw_b[kTilesB];
+  const uint32_t pick = Fp8 ? static_cast<uint32_t>(place | (4 + place) << 8) | 0x0C0C0000u : 0x06040200u + place * 0x01010101u;
+  auto keep = [&](int (&to)[kWords], const u32x4 &d, bool short_span) {
+    const uint32_t d0 = short_span ? d[2] : d[0], d1 = short_span ? d[3] : d[1];
+    const uint32_t x = __builtin_amdgcn_perm(d1, d0, pick), y = __builtin_amdgcn_perm(d[3], d[2], pick);
+    if constexpr (Fp8) {
+      to[0] = static_cast<int>(x | y << 16);
+    } else {
+      to[0] = static_cast<int>(x);
+      to[1] = static_cast<int>(y);
     }
-    [&]<int... Steps>(std::integer_sequence<int, Steps...>) {
-      (
-          [&] {
-            constexpr int Step = Steps, sel = Fp8 ? in_span : in_span * 2 + Step;
-            i32x8 af[4];
+  };
+  // A lane's 16 bytes of the first row tile; what follows of the row is some bits away: the second half of 8-bit codes (4 pieces on), the
+  // steps of 4-bit ones (2 pieces each).
+  int a_at = (wm * 128 + r) * 128 + ((place ^ (r >> 1 & 7)) << 4);
+  int b_at = (wn * 64 + r) * kRowB + ((place ^ (Fp8 ? place64(r) : r >> 1 & 7)) << 4);
+  int sa_at = (wm * 128 + r) * 16, sb_at = kBytesS + (wn * 64 + r) * 16;
+  auto read = [](const char *p) { return *reinterpret_cast<const u32x4 *>(p); };
+  auto read_raw_a = [&](int i) { raw_a[i % (Fp8 ? 2 : 4)] = read(ls + sa_at + i * kRows * 16); };
+  auto read_raw_b = [&](int j) { raw_b[j] = read(ls + sb_at + j * kRows * 16); };
+
+  // Fragments.  8-bit: three row tiles of A in turn, B of this step and the next; 4-bit: both operands of this step and the next.  (A
+  // register more than there are, and its traffic waits for the transfers behind it in order.)
+  u32x4 alo[Fp8 ? 3 : 2 * kTilesA], ahi[Fp8 ? 3 : 1], bf[2][kTilesB];
+
+  // A stage's MFMAs, and before each what is to be read or moved meanwhile.  During the last eight the next stage's first fragments are
+  // read, after the barrier that says that it has landed and that this one has been read, and this one's place is filled again.
+  auto stage = [&](auto ic, int s) __attribute__((always_inline)) {
+    constexpr int I = decltype(ic)::value, ring = I % kRing, next = (I + 1) % kRing;
+    constexpr bool first_in_span = I % kPerSpan == 0, last_in_span = I % kPerSpan == kPerSpan - 1;
+    const char *const la = lds_ring<60 + ring, kBytesA>;
+    [[maybe_unused]] const char *const lb = lds_ring<64 + ring, kBytesB>;
+    const char *const la_next = lds_ring<60 + next, kBytesA>, *const lb_next = lds_ring<64 + next, kBytesB>;
+    const bool short_span = first_in_span && s / kPerSpan * 16 + 16 > pitch_s;
+    auto landed = [&]() __attribute__((always_inline)) {
+      // in flight may be what was asked for after the next stage: the stages behind it, and the scales where they went with the last
+      constexpr int later = (kRing - 2) * (kMovesA + kMovesB) + (kRing > 2 && I % kPerSpan == 1 ? 1 : 0);
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(later));
+      barrier_no_fence();
+    };
+    // the transfers of the stage that takes this one's place, in eight slots
+    auto refill = [&](int t) __attribute__((always_inline)) {
+      char *const to_a = lds_ring<60 + ring, kBytesA>, *const to_b = lds_ring<64 + ring, kBytesB>;
+      if (t < kMovesA) move_a(to_a, t, s + kRing);
+      else if (t < kMovesA + kMovesB) move_b(to_b, t - kMovesA, s + kRing);
+      if (t == 7 && first_in_span) move_scales(s / kPerSpan + 1);
+    };
+    asm volatile("" : "+v"(a_at), "+v"(b_at), "+v"(sa_at), "+v"(sb_at));   // (not one register for each place in LDS across the loop)
+    if constexpr (Fp8) {
+      constexpr int cur = I & 1;
+      if constexpr (first_in_span) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              u32x4 lo, hi = {0u, 0u, 0u, 0u};
-              if constexpr (Fp8) {
-                lo = *reinterpret_cast<const u32x4 *>(la + a_at + i * 2048 + ((place ^ (r >> 1)) << 4));
-                hi = *reinterpret_cast<const u32x4 *>(la + a_at + i * 2048 + (((4 + place) ^ (r >> 1)) << 4));
-              } else {
-                lo = *reinterpret_cast<const u32x4 *>(la + a_at + i * 2048 + (((2 * place + Step) ^ (r >> 1)) << 4));
-              }
-              af[i] = i32x8{static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
+        for (int j = 0; j < 4; ++j) keep(sb[j], raw_b[j], short_span);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i == 6) landed();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int t = (i - 6) * 4 + j;
+          const char *const from = i < 6 ? la + a_at + (i + 2) * 2048 : la_next + a_at + (i - 6) * 2048;
+          if (j == 0) alo[(8 * I + i + 2) % 3] = read(from);
+          if (j == 1) ahi[(8 * I + i + 2) % 3] = read(i < 6 ? la + (a_at ^ 64) + (i + 2) * 2048 : la_next + (a_at ^ 64) + (i - 6) * 2048);
+          if (first_in_span && j == 0) keep(sa[i], raw_a[i & 1], short_span);
+          if (first_in_span && j == 2 && i < 6) read_raw_a(i + 2);
+          if (i == 6) bf[cur ^ 1][j] = read(lb_next + b_at + j * 16 * kRowB);
+          if (i >= 6) refill(t);
+          if (last_in_span && i == 7) read_raw_b(j);
+          if (last_in_span && i == 7 && j >= 2) read_raw_a(j - 2);
+          const u32x4 lo = alo[(8 * I + i) % 3], hi = ahi[(8 * I + i) % 3];
+          const i32x8 af = {static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
                             static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
-            }
+          acc[i][j] = mfma_mx<true, I % 4>(bf[cur][j], af, acc[i][j], sb[j][0], sa[i][0]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    } else {
+      if constexpr (first_in_span) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int slot = Fp8 ? place ^ (r >> 2) : (2 * place + Step) ^ (r >> 1);
-              const u32x4_t bf = *reinterpret_cast<const u32x4_t *>(lb + b_at + j * 16 * kRowB + (slot << 4));
+        for (int j = 0; j < 2; ++j) keep(sb[j], raw_b[j], short_span);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) acc[i][j] = mfma_mx<Fp8, sel>(bf, af[i], acc[i][j], sb[j], sa[i]);
-            }
-          }(),
-          ...);
-    }(std::make_integer_sequence<int, Fp8 ? 1 : 2>{});
+        for (int i = 0; i < 4; ++i) keep(sa[i], raw_a[i], short_span);
+      }
+      [&]<int... Steps>(std::integer_sequence<int, Steps...>) {
+        (
+            [&] {
+              constexpr int Step = Steps, cur = Step & 1, number = I % kPerSpan * 4 + Step;
+              const char *const from_a = Step < 3 ? la : la_next, *const from_b = Step < 3 ? lb : lb_next;
+              const int bits = (Step + 1) % 4 << 5;
+              if (Step == 3) landed();
+#pragma unroll
+              for (int t = 0; t < 8; ++t) {
+                const int i = t >> 1, j = i & 1 ? 1 - (t & 1) : t & 1;
+                if (t == 0 || (t >= 3 && t < 6)) alo[(cur ^ 1) * 4 + (t == 0 ? 0 : t - 2)] = read(from_a + (a_at ^ bits) + (t == 0 ? 0 : t - 2) * 4096);
+                if (t == 1 || t == 2) bf[cur ^ 1][t - 1] = read(from_b + (b_at ^ bits) + (t - 1) * 4096);
+                if (Step == 3) refill(t);
+                if (Step == 3 && last_in_span && t >= 2) {
+                  if (t < 4) read_raw_b(t - 2);
+                  else read_raw_a(t - 4);
+                }
+                acc[i][j] = mfma_mx32<number % 4>(bf[cur][j], alo[cur * 4 + i], acc[i][j], sb[j][number / 4], sa[i][number / 4]);
+                __builtin_amdgcn_sched_barrier(0);
+              }
+            }(),
+            ...);
+      }(std::make_integer_sequence<int, 4>{});
+    }
   };
 
-  issue_scales(lds_ring<64, 2 * kBytesS>, 0);
-  issue_codes(lds_ring<60, kBytesA>, lds_ring<62, kBytesB>, 0);
+  move_scales(0);
+  [&]<int... Ss>(std::integer_sequence<int, Ss...>) {
+    (
+        [&] {
+#pragma unroll
+          for (int i = 0; i < kMovesA; ++i) move_a(lds_ring<60 + Ss, kBytesA>, i, Ss);
+#pragma unroll
+          for (int i = 0; i < kMovesB; ++i) move_b(lds_ring<64 + Ss, kBytesB>, i, Ss);
+        }(),
+        ...);
+  }(std::make_integer_sequence<int, kRing>{});
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((kRing - 1) * (kMovesA + kMovesB)));
+  barrier_no_fence();
+#pragma unroll
+  for (int j = 0; j < kTilesB; ++j) {
+    bf[0][j] = read(lds_ring<64, kBytesB> + b_at + j * kRows * kRowB);
+    read_raw_b(j);
+  }
+#pragma unroll
+  for (int i = 0; i < (Fp8 ? 2 : 4); ++i) {
+    alo[i] = read(lds_ring<60, kBytesA> + a_at + i * kRows * 128);
+    if constexpr (Fp8) ahi[i] = read(lds_ring<60, kBytesA> + (a_at ^ 64) + i * kRows * 128);
+    read_raw_a(i);
+  }
+  __builtin_amdgcn_sched_barrier(0);
   const int full = stages - stages % kPeriod;
   for (int s = 0; s < full; s += kPeriod)
     [&]<int... Is>(std::integer_sequence<int, Is...>) {
@@ -209,23 +311,56 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
   }(std::make_integer_sequence<int, kPeriod - 1>{});
   __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));   // the last, empty transfers, before the LDS is released
 
+  // C goes to memory by whole rows of the tile, put together in LDS in turns, 32 KiB of the four waves that share these rows at a time:
+  // piece q (16 bytes) of row r at q ^ (r % 16).  A lane has row r of a row tile, and four columns in a row for every four registers.
+  constexpr int kRowC = 256 * sizeof(T), kTurnRows = 32768 / kRowC, kTurns = 128 / kTurnRows, kPiece = 16 / sizeof(T);
+  char *const lc = wm == 0 ? lds_ring<60, kBytesA> : lds_ring<61, kBytesA>;
+  f32x4_t add[kTilesB][kRows * kRows / 256];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int col = n0 + wn * 128 + j * 16 + 4 * place;
-    f32x4_t add = {0.f, 0.f, 0.f, 0.f};
-    if (bias) {
+  for (int j = 0; j < kTilesB; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) add[e] = bias[min(col + e, n - 1)];
+    for (int q = 0; q < kRows * kRows / 256; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) add[j][q][e] = bias ? bias[min(n0 + wn * 64 + j * kRows + 8 * q + 4 * place + e, n - 1)] : 0.f;
+#pragma unroll
+  for (int turn = 0; turn < kTurns; ++turn) {
+    barrier_no_fence();   // every wave has left the K loop, or has read the turn before
+#pragma unroll
+    for (int u = 0; u < kTurnRows / kRows; ++u) {
+      const int i = turn * (kTurnRows / kRows) + u, row = u * kRows + r;
+#pragma unroll
+      for (int j = 0; j < kTilesB; ++j)
+#pragma unroll
+        for (int q = 0; q < kRows * kRows / 256; ++q) {
+          f32x4_t v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = acc[i][j][4 * q + e] + add[j][q][e];
+            if (relu) v[e] = v[e] < 0.f ? 0.f : v[e];
+          }
+          const int at = (wn * 64 + j * kRows + 8 * q + 4 * place) * static_cast<int>(sizeof(T));
+          store_four(reinterpret_cast<T *>(lc + row * kRowC + (at ^ (row & 15) << 4)), 4, v);
+        }
     }
+    wait_lds();
+    barrier_no_fence();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = m0 + wm * 64 + i * 16 + r;
-      f32x4_t v = acc[i][j] + add;
-      if (relu) {
+    for (int u = 0; u < kTurnRows * kRowC / 4096; ++u) {
+      const int row = wn * (kTurnRows / 4) + u * (1024 / kRowC) + lane * 16 / kRowC, at = lane * 16 % kRowC;
+      const u32x4 v = read(lc + row * kRowC + (at ^ (row & 15) << 4));
+      const int to_row = m0 + wm * 128 + turn * kTurnRows + row, col = n0 + lane % (kRowC / 16) * kPiece;
+      if (to_row >= m || col >= n) continue;
+      T *const to = c + to_row * c_stride + col;
+      if (col + kPiece <= n) {
+        *reinterpret_cast<u32x4_any *>(to) = v;
+      } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
+        for (int e = 0; e < kPiece; ++e) {
+          if (col + e >= n) continue;
+          if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(to)[e] = v[e];
+          else reinterpret_cast<uint16_t *>(to)[e] = static_cast<uint16_t>(v[e / 2] >> 16 * (e & 1));
+        }
       }
-      if (row < m && col < n) store_four(c + row * c_stride + col, n - col, v);
     }
   }
 }
