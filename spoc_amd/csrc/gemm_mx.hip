@@ -36,51 +36,7 @@ template <int Scale> __device__ __forceinline__ f32x16 mfma_mx32(u32x4 b, u32x4 
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide_b, wide_a, c, kFormatE2M1, kFormatE2M1, Scale, b_scales, Scale, a_scales);
 }
 
-// One wave to a 16 x 16 tile of C, operands straight from memory.
-template <bool Fp8, class T>
-__global__ __launch_bounds__(64) void gemm_mx_kernel(const uint8_t *__restrict__ a, const uint8_t *__restrict__ a_scales,
-                                                     const uint8_t *__restrict__ b, const uint8_t *__restrict__ b_scales,
-                                                     const float *__restrict__ bias, int relu, T *__restrict__ c, int64_t c_stride,
-                                                     int64_t m, int64_t n, int64_t kp) {
-  const int lane = threadIdx.x, r = lane & 15, place = lane >> 4;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 16, n0 = static_cast<int64_t>(blockIdx.x) * 16;
-  const int64_t arow = min(m0 + r, m - 1), brow = min(n0 + r, n - 1);   // rows past the end are the last one again: not stored
-  const uint8_t *const ap = a + arow * (Fp8 ? kp : kp / 2), *const bp = b + brow * (kp / 2);
-  const uint8_t *const as = a_scales + arow * (kp / kMxBlock), *const bs = b_scales + brow * (kp / kMxBlock);
-  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t u = 0; u < kp / kMxRow; ++u) {
-    const int sa = *reinterpret_cast<const uint16_t *>(as + u * 8 + 2 * place), sb = *reinterpret_cast<const uint16_t *>(bs + u * 8 + 2 * place);
-    u32x4_t bf[2];
-    i32x8 af[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf[s] = *reinterpret_cast<const u32x4_t *>(bp + u * 128 + place * 32 + s * 16);
-      u32x4_t lo, hi = {0u, 0u, 0u, 0u};
-      if constexpr (Fp8) {
-        const uint8_t *const p = ap + u * 256 + (2 * (place >> 1) + s) * 32 + (place & 1) * 16;
-        lo = *reinterpret_cast<const u32x4_t *>(p);
-        hi = *reinterpret_cast<const u32x4_t *>(p + 128);
-      } else {
-        lo = *reinterpret_cast<const u32x4_t *>(ap + u * 128 + place * 32 + s * 16);
-      }
-      af[s] = i32x8{static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
-                    static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
-    }
-    acc = mfma_mx<Fp8, 0>(bf[0], af[0], acc, sb, sa);
-    acc = mfma_mx<Fp8, 1>(bf[1], af[1], acc, sb, sa);
-  }
-  if (m0 + r >= m) return;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t col = n0 + 4 * place + j;
-    if (col >= n) continue;
-    float v = acc[j] + (bias ? bias[col] : 0.f);
-    if (relu) v = v < 0.f ? 0.f : v;
-    store_one(c + (m0 + r) * c_stride + col, v);
-  }
-}
-
-// ---- 256 x 256 tiles -----------------------------------------------------------------------------------------------------------------
+// ---- few rows ------------------------------------------------------------------------------------------------------------------------
 
 template <class T> __device__ __forceinline__ void store_four(T *p, int64_t count, f32x4_t v) {
   if (count >= 4) {
@@ -97,6 +53,147 @@ template <class T> __device__ __forceinline__ void store_four(T *p, int64_t coun
   for (int j = 0; j < 4; ++j)
     if (j < count) store_one(p + j, v[j]);
 }
+
+// Small tiles of C, both operands brought to LDS by transfers, kRing - 1 stages ahead.  Eight waves: WM by WN of them share out the tile of C, each
+// MT by NT row and column tiles of 16, and Q of them in each place take every Q-th step of 128 k; a stage is Q steps.  Their sums are added
+// in order at the end.
+template <bool Fp8, class T, int MT, int NT, int WM, int WN, int kRing>
+__global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__restrict__ a, const uint8_t *__restrict__ a_scales,
+                                                             const uint8_t *__restrict__ b, const uint8_t *__restrict__ b_scales,
+                                                             const float *__restrict__ bias, int relu, T *__restrict__ c,
+                                                             int64_t c_stride, int m, int n, int kp, int tiles_m, int tiles_n) {
+  constexpr int kPlaces = WM * WN, Q = 8 / kPlaces, kStage = Q * 128, kTM = 16 * MT * WM, kTN = 16 * NT * WN;
+  constexpr int kRowA = Fp8 ? kStage : kStage / 2, kRowB = kStage / 2;             // bytes of a row in a stage
+  constexpr int kBytesA = kTM * kRowA, kBytesB = kTN * kRowB, kWordsA = kTM * Q, kWordsB = kTN * Q;
+  constexpr int kBytes = kBytesA + kBytesB + (kWordsA + kWordsB) * 4;
+  constexpr int kMovesA = kBytesA / 8192, kMovesB = kBytesB / 8192, kMoves = kMovesA + kMovesB;   // a wave's transfers of a stage's codes
+  static_assert(kBytesA % 8192 == 0 && kBytesB % 8192 == 0 && kWordsA % 64 == 0 && kWordsB % 64 == 0 && (kWordsA + kWordsB) / 64 <= 8, "whole transfers");
+  static_assert(kRing * kBytes <= 160 * 1024 && (kRing - 2) * kMoves < 64, "LDS, vmcnt");
+  constexpr int kChunk = MT * NT * 1024;   // a wave's sums
+  static_assert((8 + kRing - 1) / kRing * kChunk <= kBytes, "the waves' sums go into the stages' places");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, place = lane >> 4;
+  const int q = wave / kPlaces, wm = wave % kPlaces / WN, wn = wave % WN;           // this wave's step and its part of the tile
+  int tm, tn;
+  tile_of_block(tiles_m, tiles_n, 1, tm, tn);
+  const int m0 = tm * kTM, n0 = tn * kTN;
+  const int pitch_a = Fp8 ? kp : kp / 2, pitch_b = kp / 2, pitch_s = kp / kMxBlock, steps = kp / 128, stages = (steps + Q - 1) / Q;
+  const uint32_t rows_a = static_cast<uint32_t>(min(m - m0, kTM)), rows_b = static_cast<uint32_t>(min(n - n0, kTN));
+  const __amdgpu_buffer_rsrc_t ra = make_rsrc(a + static_cast<int64_t>(m0) * pitch_a, rows_a * pitch_a);
+  const __amdgpu_buffer_rsrc_t rb = make_rsrc(b + static_cast<int64_t>(n0) * pitch_b, rows_b * pitch_b);
+  // Transfers: lanes past the rows that exist, or past a row's end in the last stage, are sent out of range and bring zeros.  A piece of 16
+  // bytes lies at its number in the row with the last bits turned by the row's (its quad's where a row is 128 bytes).
+  constexpr uint32_t kOutOfRange = 0x80000000u;   // (a tile's rows end below it, and so does what is added along k)
+  auto turn = [](int row, int row_bytes) { return (row_bytes >= 256 ? row & 15 : row >> 1 & 7) << 4; };
+  uint32_t off_a[kMovesA], off_b[kMovesB];
+  int at_a[kMovesA], at_b[kMovesB];    // where in the row, bytes
+#pragma unroll
+  for (int i = 0; i < kMovesA; ++i) {
+    const int in = (wave + 8 * i) * 1024 + lane * 16, row = in / kRowA;
+    at_a[i] = in % kRowA ^ turn(row, kRowA);
+    off_a[i] = row < static_cast<int>(rows_a) ? row * pitch_a + at_a[i] : kOutOfRange;
+  }
+#pragma unroll
+  for (int i = 0; i < kMovesB; ++i) {
+    const int in = (wave + 8 * i) * 1024 + lane * 16, row = in / kRowB;
+    at_b[i] = in % kRowB ^ turn(row, kRowB);
+    off_b[i] = row < static_cast<int>(rows_b) ? row * pitch_b + at_b[i] : kOutOfRange;
+  }
+  // Scales: a word of four to a row and step, step by step; each of the first waves brings 64 of them.
+  const bool scale_a = wave < kWordsA / 64;
+  const int word = (scale_a ? wave : wave - kWordsA / 64) * 64 + lane, word_row = word % (scale_a ? kTM : kTN), word_step = word / (scale_a ? kTM : kTN);
+  const __amdgpu_buffer_rsrc_t rs = make_rsrc(scale_a ? a_scales + static_cast<int64_t>(m0) * pitch_s : b_scales + static_cast<int64_t>(n0) * pitch_s, (scale_a ? rows_a : rows_b) * pitch_s);
+  const uint32_t off_s = word_step < Q && word_row < static_cast<int>(scale_a ? rows_a : rows_b) ? word_row * pitch_s + word_step * 4 : kOutOfRange;
+  auto move = [&](char *to, int s) __attribute__((always_inline)) {
+    if (wave < (kWordsA + kWordsB) / 64)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LDS_PTR void *)(to + kBytesA + kBytesB + wave * 256), 4,
+                                               static_cast<int>(s * Q + word_step < steps ? off_s + s * Q * 4 : kOutOfRange), 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kMovesA; ++i)
+      dma16(ra, s * kRowA + at_a[i] < pitch_a ? off_a[i] + s * kRowA : kOutOfRange, 0, to + (wave + 8 * i) * 1024);
+#pragma unroll
+    for (int i = 0; i < kMovesB; ++i)
+      dma16(rb, s * kRowB + at_b[i] < pitch_b ? off_b[i] + s * kRowB : kOutOfRange, 0, to + kBytesA + (wave + 8 * i) * 1024);
+  };
+  f32x4_t acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  auto read = [](const char *p) { return *reinterpret_cast<const u32x4 *>(p); };
+  const int row_a = wm * 16 * MT + r, row_b = wn * 16 * NT + r;
+  const int a_at = row_a * kRowA + (q * (Fp8 ? 128 : 64) + place * 16 ^ turn(r, kRowA)), b_at = kBytesA + row_b * kRowB + (q * 64 + place * 16 ^ turn(r, kRowB));
+  const int a_hi = row_a * kRowA + (q * 128 + 64 + place * 16 ^ turn(r, kRowA));
+  const int sa_at = kBytesA + kBytesB + (q * kTM + row_a) * 4 + place, sb_at = kBytesA + kBytesB + (kWordsA + q * kTN + row_b) * 4 + place;
+  auto stage = [&]<int I>(std::integral_constant<int, I>, int s) __attribute__((always_inline)) {
+    const char *const from = lds_ring<80 + I, kBytes>;
+    // What the next stages have in flight may stay there (of a wave with scales to bring, one transfer less).
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((kRing - 2) * kMoves));
+    barrier_no_fence();
+    move(lds_ring<80 + (I + kRing - 1) % kRing, kBytes>, s + kRing - 1);
+    u32x4 bf[NT];
+    int sb[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      bf[j] = read(from + b_at + j * 16 * kRowB);
+      sb[j] = static_cast<uint8_t>(from[sb_at + j * 64]);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const u32x4 lo = read(from + a_at + i * 16 * kRowA), hi = Fp8 ? read(from + a_hi + i * 16 * kRowA) : u32x4{0u, 0u, 0u, 0u};
+      const int sa = static_cast<uint8_t>(from[sa_at + i * 64]);
+      const i32x8 af = {static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
+                        static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = mfma_mx<Fp8, 0>(bf[j], af, acc[i][j], sb[j], sa);
+    }
+  };
+  [&]<int... Is>(std::integer_sequence<int, Is...>) { (move(lds_ring<80 + Is, kBytes>, Is), ...); }(std::make_integer_sequence<int, kRing - 1>{});
+  for (int s = 0; s < stages; s += kRing)
+    [&]<int... Is>(std::integer_sequence<int, Is...>) {
+      ((s + Is < stages ? stage(std::integral_constant<int, Is>{}, s + Is) : void()), ...);
+    }(std::make_integer_sequence<int, kRing>{});
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));   // the last, empty transfers: the stages' places take the sums
+  barrier_no_fence();
+  // Every wave's sums into LDS, a tile's 16 bytes of row r and column quad p at 4 r + p with the row turned by the column tile's number, then
+  // a thread to four columns of a row: its Q sums in order, and C by rows.
+  auto chunk = [&](int of) {   // the sums of wave `of`
+    char *base = lds_ring<80, kBytes>;
+    [&]<int... Is>(std::integer_sequence<int, Is...>) { ((base = of % kRing == Is ? lds_ring<80 + Is, kBytes> : base), ...); }(std::make_integer_sequence<int, kRing>{});
+    return reinterpret_cast<f32x4_t *>(base + of / kRing * kChunk);
+  };
+  f32x4_t *const to = chunk(wave);
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) to[(i * NT + j) * 64 + (r ^ (j & 3)) * 4 + place] = acc[i][j];
+  wait_lds();
+  barrier_no_fence();
+  constexpr int kQuads = kTN / 4, kRowsAtOnce = 512 / kQuads;   // of a row of the tile; rows that the threads cover at a time
+  const int col4 = threadIdx.x % kQuads, tile_j = col4 / 4 % NT, part_n = col4 / 4 / NT;
+  const int col = n0 + col4 * 4;
+  f32x4_t add = {0.f, 0.f, 0.f, 0.f};
+  if (bias) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) add[e] = bias[min(col + e, n - 1)];
+  }
+#pragma unroll
+  for (int turn_of = 0; turn_of < (kTM + kRowsAtOnce - 1) / kRowsAtOnce; ++turn_of) {
+    const int row_in = turn_of * kRowsAtOnce + threadIdx.x / kQuads, tile_i = row_in / 16 % MT, part_m = row_in / 16 / MT;
+    const int row = m0 + row_in;
+    if ((kTM % kRowsAtOnce && row_in >= kTM) || row >= m || col >= n) continue;
+    const int at = (tile_i * NT + tile_j) * 64 + ((row_in & 15) ^ (tile_j & 3)) * 4 + (col4 & 3);
+    f32x4_t v = chunk(part_m * WN + part_n)[at];
+#pragma unroll
+    for (int w = 1; w < Q; ++w) v += chunk(w * kPlaces + part_m * WN + part_n)[at];
+    v += add;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (relu) v[e] = v[e] < 0.f ? 0.f : v[e];
+    store_four(c + row * c_stride + col, n - col, v);
+  }
+}
+
+// ---- 256 x 256 tiles -----------------------------------------------------------------------------------------------------------------
 
 template <bool Fp8, class T>
 __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__restrict__ a, const uint8_t *__restrict__ a_scales,
@@ -368,6 +465,36 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
 }  // namespace
 }  // namespace sarek_hip
 
+namespace sarek_hip {
+namespace {
+
+// The kernels' tiles of C, and what a workgroup takes, us: `once` for its start and its end, `step` for 128 of k (8-bit and 4-bit rows).
+constexpr int kShapeCount = 8;
+struct Shape { int rows, columns; double once, step8, step4; };
+constexpr Shape kShapes[kShapeCount] = {{16, 16, 1.9, 0.056, 0.050},  {16, 32, 2.0, 0.085, 0.080},  {32, 32, 2.0, 0.115, 0.097}, {32, 64, 2.0, 0.168, 0.148},
+                                        {64, 32, 1.8, 0.184, 0.153},  {64, 64, 2.9, 0.240, 0.190},  {128, 128, 3.5, 0.420, 0.310}, {256, 256, 7.3, 1.200, 0.700}};
+
+// The one that the product takes least time on: a workgroup to a compute unit, as many in turn as there are too many.
+bool shape_serves(int shape, int64_t m, int64_t n, int64_t kp) {
+  if (shape < 0 || shape >= kShapeCount || (shape == kShapeCount - 1 && kp < 512)) return false;   // (its scales come 16 bytes of a row at a time)
+  return ceil_div(m, kShapes[shape].rows) * ceil_div(n, kShapes[shape].columns) < int64_t{1} << 22;   // below 2^32 threads
+}
+int best_shape(bool fp8, int64_t m, int64_t n, int64_t kp) {
+  int best = -1;
+  double least = 0.0;
+  for (int i = 0; i < kShapeCount; ++i) {
+    if (!shape_serves(i, m, n, kp)) continue;
+    const Shape &s = kShapes[i];
+    const int64_t tiles = ceil_div(m, s.rows) * ceil_div(n, s.columns);
+    const double us = static_cast<double>(ceil_div(tiles, compute_units())) * (s.once + static_cast<double>(kp / 128) * (fp8 ? s.step8 : s.step4));
+    if (best < 0 || us < least) least = us, best = i;
+  }
+  return best;
+}
+
+}  // namespace
+}  // namespace sarek_hip
+
 using namespace sarek_hip;
 
 extern "C" int sarek_hip_gemm_mx(const unsigned char *a_codes, const unsigned char *a_scales, int a_format, const unsigned char *b_codes,
@@ -380,29 +507,37 @@ extern "C" int sarek_hip_gemm_mx(const unsigned char *a_codes, const unsigned ch
   if (a_format == SAREK_HIP_MX_FP8 && c_type == SAREK_HIP_TYPE_F32)
     return fail(SAREK_HIP_E_UNSUPPORTED, "gemm_mx: products of 8-bit rows are not exact to float32's last bits: C is bf16 or fp16");
   if (c_stride < n) return fail(SAREK_HIP_E_INVALID_ARG, "gemm_mx: rows of C are %lld values apart, less than n = %lld", static_cast<long long>(c_stride), static_cast<long long>(n));
-  if (m > (int64_t{1} << 20) - 1 || n > 0x7FFFFFFF || k > 0x7FFFFFFF - kMxRow)
-    return fail(SAREK_HIP_E_UNSUPPORTED, "gemm_mx: m is below 2^20, n and k below 2^31");
+  if (m >= int64_t{1} << 20 || n >= int64_t{1} << 24 || k > int64_t{1} << 23)
+    return fail(SAREK_HIP_E_UNSUPPORTED, "gemm_mx: m is below 2^20, n below 2^24, k at most 2^23");
   if (m == 0) return SAREK_HIP_OK;
   if (!a_codes || !a_scales || !b_codes || !b_scales || !c) return fail(SAREK_HIP_E_INVALID_ARG, "gemm_mx: NULL pointer");
   if (misaligned(a_codes, a_scales) || misaligned(b_codes, b_scales)) return fail(SAREK_HIP_E_INVALID_ARG, "gemm_mx: codes start at multiples of 16 bytes, scales of 8");
   const int64_t kp = mx_row_values(k);
-  const int64_t tiles_m = ceil_div(m, 256), tiles_n = ceil_div(n, 256);
-  if (tunable("gemm_mx.tile", m >= 256 && n >= 256 ? 1 : 0) && kp >= 512 && kp <= (1 << 22) && tiles_m * tiles_n < (1 << 22))
-    return by_type(c_type, [&]<class T>(T *) {
-      const dim3 tiles(static_cast<unsigned>(tiles_m * tiles_n));
-      const auto run = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, tiles, dim3(512), 0, as_stream(stream), a_codes, a_scales, b_codes, b_scales, bias, relu, static_cast<T *>(c),
-                           c_stride, static_cast<int>(m), static_cast<int>(n), static_cast<int>(kp), static_cast<int>(tiles_m), static_cast<int>(tiles_n));
-        return check_launch("gemm_mx launch");
-      };
-      return a_format == SAREK_HIP_MX_FP8 ? run(gemm_mx_tile_kernel<true, T>) : run(gemm_mx_tile_kernel<false, T>);
-    });
-  const dim3 grid(static_cast<unsigned>(ceil_div(n, 16)), static_cast<unsigned>(ceil_div(m, 16)));
+  const bool fp8 = a_format == SAREK_HIP_MX_FP8;
+  const int forced = static_cast<int>(tunable("gemm_mx.shape", -1));
+  const int shape = shape_serves(forced, m, n, kp) ? forced : best_shape(fp8, m, n, kp);
+  if (shape < 0) return fail(SAREK_HIP_E_UNSUPPORTED, "gemm_mx: %lld x %lld is more than one launch covers", static_cast<long long>(m), static_cast<long long>(n));
   return by_type(c_type, [&]<class T>(T *) {
-    if (a_format == SAREK_HIP_MX_FP8)
-      hipLaunchKernelGGL((gemm_mx_kernel<true, T>), grid, dim3(64), 0, as_stream(stream), a_codes, a_scales, b_codes, b_scales, bias, relu, static_cast<T *>(c), c_stride, m, n, kp);
-    else
-      hipLaunchKernelGGL((gemm_mx_kernel<false, T>), grid, dim3(64), 0, as_stream(stream), a_codes, a_scales, b_codes, b_scales, bias, relu, static_cast<T *>(c), c_stride, m, n, kp);
-    return check_launch("gemm_mx launch");
+    const auto run = [&](auto kernel, int tile_m, int tile_n) {
+      const int64_t tiles_m = ceil_div(m, tile_m), tiles_n = ceil_div(n, tile_n);
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles_m * tiles_n)), dim3(512), 0, as_stream(stream), a_codes, a_scales, b_codes,
+                         b_scales, bias, relu, static_cast<T *>(c), c_stride, static_cast<int>(m), static_cast<int>(n), static_cast<int>(kp),
+                         static_cast<int>(tiles_m), static_cast<int>(tiles_n));
+      return check_launch("gemm_mx launch");
+    };
+    const auto small = [&]<int MT, int NT, int WM, int WN, int Ring8, int Ring4>(std::integer_sequence<int, MT, NT, WM, WN, Ring8, Ring4>) {
+      return fp8 ? run(gemm_mx_stream_kernel<true, T, MT, NT, WM, WN, Ring8>, 16 * MT * WM, 16 * NT * WN)
+                 : run(gemm_mx_stream_kernel<false, T, MT, NT, WM, WN, Ring4>, 16 * MT * WM, 16 * NT * WN);
+    };
+    switch (shape) {
+      case 0: return small(std::integer_sequence<int, 1, 1, 1, 1, 6, 6>{});
+      case 1: return small(std::integer_sequence<int, 1, 2, 1, 1, 4, 6>{});
+      case 2: return small(std::integer_sequence<int, 2, 1, 1, 2, 6, 6>{});
+      case 3: return small(std::integer_sequence<int, 2, 2, 1, 2, 4, 6>{});
+      case 4: return small(std::integer_sequence<int, 4, 1, 1, 2, 3, 6>{});
+      case 5: return small(std::integer_sequence<int, 4, 2, 1, 2, 3, 4>{});
+      case 6: return small(std::integer_sequence<int, 4, 4, 2, 2, 3, 4>{});
+      default: return fp8 ? run(gemm_mx_tile_kernel<true, T>, 256, 256) : run(gemm_mx_tile_kernel<false, T>, 256, 256);
+    }
   });
 }
