@@ -1,5 +1,5 @@
-// CPython extension spoc_amd._host: the launch calls of spoc_amd/sarek.py with their argument lists turned into the C
-// structures here.  A launch takes the HIP runtime 2.8 us; building the same structures with ctypes took 2.3 us more for
+// CPython extension spoc_amd._host: the launch calls of spoc_amd/sarek.py, and the operators of spoc_amd/hip.py on microscaled rows, with
+// their argument lists turned into the C ones here.  A launch takes the HIP runtime 2.8 us; building the same structures with ctypes took 2.3 us more for
 // one kernel and 5.3 us for a pipeline of two.  The entry points are those of the library the ctypes front end has loaded
 // (bind() gets their addresses), so there is one library per process whichever build it is, and their statuses come back
 // to the caller, who turns them into exceptions as for every other entry point.
@@ -7,6 +7,9 @@
 #include <Python.h>
 
 #include <cstring>
+#include <tuple>
+#include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "sarek_hip.h"
@@ -234,7 +237,52 @@ PyObject *fold_partials(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return PyLong_FromLong(status);
 }
 
-// bind(addresses of the five entry points above, in the order of their declaration)
+// The operators on microscaled rows, called with their C arguments: pointers and the stream as integers or None, numbers.  (ctypes takes
+// 1.7 us for the 9 arguments of mx_quantize, this 0.3.)
+decltype(&sarek_hip_mx_quantize) g_mx_quantize;
+decltype(&sarek_hip_mx_dequantize) g_mx_dequantize;
+decltype(&sarek_hip_rms_norm_mx) g_rms_norm_mx;
+decltype(&sarek_hip_rms_norm_backward) g_rms_norm_backward;
+decltype(&sarek_hip_gemm_mx) g_gemm_mx;
+
+template <typename T>
+T as_c(PyObject *o) {
+  if constexpr (std::is_pointer_v<T>) {
+    return o == Py_None ? nullptr : static_cast<T>(PyLong_AsVoidPtr(o));
+  } else if constexpr (std::is_floating_point_v<T>) {
+    return static_cast<T>(PyFloat_AsDouble(o));
+  } else {
+    const long long v = PyLong_AsLongLong(o);
+    if (v != static_cast<long long>(static_cast<T>(v))) PyErr_SetString(PyExc_OverflowError, "an integer argument does not fit its type");
+    return static_cast<T>(v);
+  }
+}
+template <typename... Args, size_t... Is>
+PyObject *call_with(int (*f)(Args...), PyObject *const *a, std::index_sequence<Is...>) {
+  const std::tuple<Args...> args{as_c<Args>(a[Is])...};
+  if (PyErr_Occurred()) return nullptr;
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = std::apply(f, args);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(status);
+}
+template <typename... Args>
+PyObject *call(int (*f)(Args...), PyObject *const *a, Py_ssize_t n, const char *what) {
+  if (!f) {
+    PyErr_SetString(PyExc_RuntimeError, "spoc_amd._host: bind_mx() has not been called");
+    return nullptr;
+  }
+  if (!arity(n, sizeof...(Args), what)) return nullptr;
+  return call_with(f, a, std::index_sequence_for<Args...>{});
+}
+PyObject *mx_quantize(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_mx_quantize, a, n, "mx_quantize"); }
+PyObject *mx_dequantize(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_mx_dequantize, a, n, "mx_dequantize"); }
+PyObject *rms_norm_mx(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_rms_norm_mx, a, n, "rms_norm_mx"); }
+PyObject *rms_norm_backward(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_rms_norm_backward, a, n, "rms_norm_backward"); }
+PyObject *gemm_mx(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_gemm_mx, a, n, "gemm_mx"); }
+
+// bind(addresses of the first five entry points above, in the order of their declaration)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
   if (!arity(n, 5, "bind")) return nullptr;
   void *p[5];
@@ -248,12 +296,32 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// bind_mx(addresses of the five on microscaled rows)
+PyObject *bind_mx(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (!arity(n, 5, "bind_mx")) return nullptr;
+  void *p[5];
+  for (int i = 0; i < 5; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
+  if (PyErr_Occurred()) return nullptr;
+  g_mx_dequantize = reinterpret_cast<decltype(g_mx_dequantize)>(p[1]);
+  g_rms_norm_mx = reinterpret_cast<decltype(g_rms_norm_mx)>(p[2]);
+  g_rms_norm_backward = reinterpret_cast<decltype(g_rms_norm_backward)>(p[3]);
+  g_gemm_mx = reinterpret_cast<decltype(g_gemm_mx)>(p[4]);
+  g_mx_quantize = reinterpret_cast<decltype(g_mx_quantize)>(p[0]);
+  Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(bind), METH_FASTCALL, "Addresses of the library's entry points."},
+    {"bind_mx", reinterpret_cast<PyCFunction>(bind_mx), METH_FASTCALL, "The same for the operators on microscaled rows."},
     {"run_vectors", reinterpret_cast<PyCFunction>(run_vectors), METH_FASTCALL, "sarek_hip_execute_run_vectors"},
     {"run_source", reinterpret_cast<PyCFunction>(run_source), METH_FASTCALL, "sarek_hip_execute_run_source"},
     {"run_pipeline", reinterpret_cast<PyCFunction>(run_pipeline), METH_FASTCALL, "sarek_hip_execute_run_pipeline"},
     {"fold_partials", reinterpret_cast<PyCFunction>(fold_partials), METH_FASTCALL, "sarek_hip_fold_partials_f64"},
+    {"mx_quantize", reinterpret_cast<PyCFunction>(mx_quantize), METH_FASTCALL, "sarek_hip_mx_quantize"},
+    {"mx_dequantize", reinterpret_cast<PyCFunction>(mx_dequantize), METH_FASTCALL, "sarek_hip_mx_dequantize"},
+    {"rms_norm_mx", reinterpret_cast<PyCFunction>(rms_norm_mx), METH_FASTCALL, "sarek_hip_rms_norm_mx"},
+    {"rms_norm_backward", reinterpret_cast<PyCFunction>(rms_norm_backward), METH_FASTCALL, "sarek_hip_rms_norm_backward"},
+    {"gemm_mx", reinterpret_cast<PyCFunction>(gemm_mx), METH_FASTCALL, "sarek_hip_gemm_mx"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Argument lists of launches, built natively.", -1, methods,

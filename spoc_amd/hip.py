@@ -7,7 +7,6 @@ current stream only.
 """
 import ctypes as C
 import os
-from typing import NamedTuple
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # SAREK_HIP_MEASURE_BUILD=1 (bench.py --measure-build) loads the measurement build instead: the product's code plus the
@@ -278,6 +277,9 @@ except ImportError as _e:
 _host.bind(*(C.cast(getattr(lib, _f), C.c_void_p).value for _f in (
     "sarek_hip_execute_run_vectors", "sarek_hip_execute_run_source", "sarek_hip_execute_run_pipeline",
     "sarek_hip_last_run_path", "sarek_hip_fold_partials_f64")))
+_host.bind_mx(*(C.cast(getattr(lib, _f), C.c_void_p).value for _f in (
+    "sarek_hip_mx_quantize", "sarek_hip_mx_dequantize", "sarek_hip_rms_norm_mx", "sarek_hip_rms_norm_backward",
+    "sarek_hip_gemm_mx")))
 
 
 def check(status):
@@ -825,21 +827,6 @@ def cast_f16(x):
 # ---------------------------------------------------------------------------
 # Microscaled 8- and 4-bit rows: quantisation, norm, products
 
-class MxTensor(NamedTuple):
-    """A matrix of k columns in microscaled 8- or 4-bit floating point.  codes: uint8 [rows, kp] (fmt "fp8", e4m3) or
-    [rows, kp / 2] (fmt "fp4", e2m1, the first of two in the low half of a byte), kp = mx_row_values(k); scales: uint8
-    [rows, kp / 32], a byte E + 127 for each 32 codes, which stand for their values times 2^E (255: for NaNs).  What is
-    behind column k is zeros."""
-    codes: torch.Tensor
-    scales: torch.Tensor
-    fmt: str
-    k: int
-
-    @property
-    def rows(self):
-        return self.codes.shape[0]
-
-
 _MX_FORMATS = {"fp8": MX_FP8, "fp4": MX_FP4}
 _MX_TYPES = {torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16}
 
@@ -849,126 +836,209 @@ def mx_row_values(k):
     return (k + 255) & ~255
 
 
-def _need_rows(t, name, dtype=None, shape=None):
-    """A device matrix with adjacent columns, its rows at any distance; its distance from row to row."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in _MX_TYPES
-            and (t.stride(1) == 1 or t.shape[1] == 1)):
-        raise TypeError(f"{name}: expected a device matrix of float32, bfloat16 or float16 with adjacent columns")
-    if dtype is not None and t.dtype != dtype:
-        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name}: expected {tuple(shape)}, got {tuple(t.shape)}")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+class MxTensor:
+    """A matrix of k columns in microscaled 8- or 4-bit floating point.  codes: uint8 [rows, kp] (fmt "fp8", e4m3) or
+    [rows, kp / 2] (fmt "fp4", e2m1, the first of two in the low half of a byte), kp = mx_row_values(k); scales: uint8
+    [rows, kp / 32], a byte E + 127 for each 32 codes, which stand for their values times 2^E (255: for NaNs).  What is
+    behind column k is zeros.  Both are contiguous, any rows of such a matrix are one too."""
+    __slots__ = ("fmt", "k", "rows", "_codes", "_scales", "_block", "_at")
+
+    def __init__(self, codes, scales, fmt, k):
+        if fmt not in _MX_FORMATS:
+            raise ValueError(f"MxTensor: unknown format {fmt!r}")
+        kp = (k + 255) & ~255
+        if not (isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.dtype == torch.uint8
+                and scales.dtype == torch.uint8 and codes.is_contiguous() and scales.is_contiguous()):
+            raise TypeError("MxTensor: expected contiguous uint8 tensors of codes and scales")
+        rows = codes.shape[0] if codes.dim() == 2 else -1
+        if k < 1 or codes.shape != (rows, kp if fmt == "fp8" else kp // 2) or scales.shape != (rows, kp // 32):
+            raise ValueError(f"MxTensor: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not {fmt} rows of {k}")
+        if codes.device != scales.device:
+            raise TypeError("MxTensor: codes and scales are on different devices")
+        self.fmt, self.k, self.rows, self._codes, self._scales, self._block = fmt, k, rows, codes, scales, None
+        self._at = (codes.data_ptr(), scales.data_ptr()) if codes.is_cuda else None
+
+    @classmethod
+    def _empty(cls, rows, k, fmt, like):
+        """One block of memory for both, on the device of `like`."""
+        self = cls.__new__(cls)
+        kp = (k + 255) & ~255
+        width = kp if fmt == "fp8" else kp >> 1
+        block = like.new_empty(rows * (width + (kp >> 5)), dtype=torch.uint8)
+        at = block.data_ptr()
+        self.fmt, self.k, self.rows, self._codes, self._scales, self._block = fmt, k, rows, None, None, block
+        self._at = (at, at + rows * width)
+        return self
+
+    def _part(self, name):
+        kp = (self.k + 255) & ~255
+        width = kp if self.fmt == "fp8" else kp >> 1
+        self._codes = self._block[:self.rows * width].view(self.rows, width)
+        self._scales = self._block[self.rows * width:].view(self.rows, kp >> 5)
+        return getattr(self, name)
+
+    @property
+    def codes(self):
+        return self._codes if self._codes is not None else self._part("_codes")
+
+    @property
+    def scales(self):
+        return self._scales if self._scales is not None else self._part("_scales")
+
+    def __repr__(self):
+        return f"MxTensor({self.rows} x {self.k}, {self.fmt})"
 
 
-def _need_mx(t, name):
-    if not isinstance(t, MxTensor) or t.fmt not in _MX_FORMATS:
-        raise TypeError(f"{name}: expected an MxTensor in fp8 or fp4")
-    _need(t.codes, torch.uint8, name + ".codes")
-    _need(t.scales, torch.uint8, name + ".scales")
-    kp = (t.k + 255) & ~255
-    if t.k < 1 or t.codes.dim() != 2 or t.codes.shape[1] != (kp if t.fmt == "fp8" else kp // 2) \
-            or t.scales.shape != (t.codes.shape[0], kp // 32):
-        raise ValueError(f"{name}: codes {tuple(t.codes.shape)} and scales {tuple(t.scales.shape)} are not {t.fmt} rows of {t.k}")
+def _mx_rows(t, name):
+    """(type, rows, columns, elements from row to row) of a device matrix with adjacent columns."""
+    kind = _MX_TYPES.get(t.dtype) if isinstance(t, torch.Tensor) and t.is_cuda else None
+    if kind is not None and t.dim() == 2:
+        (rows, k), (stride, step) = t.shape, t.stride()
+        if step == 1 or k == 1:
+            return kind, rows, k, stride if rows > 1 else max(stride, k)
+    raise TypeError(f"{name}: expected a device matrix of float32, bfloat16 or float16 with adjacent columns")
 
 
-def _mx_out(out, rows, k, fmt, like, name):
+def _mx_like(t, x, name):
+    """Elements from row to row of a matrix that has to have x's type and shape."""
+    _, rows, k, stride = _mx_rows(t, name)
+    if t.dtype != x.dtype:
+        raise TypeError(f"{name}: expected {x.dtype}, got {t.dtype}")
+    if (rows, k) != x.shape:
+        raise ValueError(f"{name}: expected {tuple(x.shape)}, got {tuple(t.shape)}")
+    return stride
+
+
+def _mx_at(q, name):
+    """Addresses of an MxTensor's codes and scales."""
+    if not isinstance(q, MxTensor) or q._at is None:
+        raise TypeError(f"{name}: expected an MxTensor on the device")
+    return q._at
+
+
+def _mx_out(out, rows, k, fmt, like):
     if fmt not in _MX_FORMATS:
-        raise ValueError(f"{name}: unknown format {fmt!r}")
-    if out is not None:
-        _need_mx(out, name)
-        if (out.rows, out.k, out.fmt) != (rows, k, fmt):
-            raise ValueError(f"{name}: out is {out.rows} x {out.k} in {out.fmt}, expected {rows} x {k} in {fmt}")
-        return out
-    kp = (k + 255) & ~255
-    return MxTensor(like.new_empty((rows, kp if fmt == "fp8" else kp // 2), dtype=torch.uint8),
-                    like.new_empty((rows, kp // 32), dtype=torch.uint8), fmt, k)
+        raise ValueError(f"unknown format {fmt!r}")
+    if out is None:
+        return MxTensor._empty(rows, k, fmt, like)
+    _mx_at(out, "out")
+    if (out.rows, out.k, out.fmt) != (rows, k, fmt):
+        raise ValueError(f"out: expected {rows} x {k} in {fmt}, got {out.rows} x {out.k} in {out.fmt}")
+    return out
+
+
+def _mx_weight(weight, dtype, k):
+    _need(weight, dtype, "weight")
+    if weight.shape != (k,):
+        raise ValueError(f"weight: {k} values expected, got {tuple(weight.shape)}")
+    return weight.data_ptr()
 
 
 def mx_quantize(x, fmt, out=None):
     """The rows of x (float32, bfloat16 or float16) in "fp8" or "fp4", as an MxTensor."""
-    stride = _need_rows(x, "x")
-    rows, k = x.shape
-    q = _mx_out(out, rows, k, fmt, x, "mx_quantize")
-    check(lib.sarek_hip_mx_quantize(x.data_ptr(), _MX_TYPES[x.dtype], stride, q.codes.data_ptr(), q.scales.data_ptr(),
-                                    _MX_FORMATS[fmt], rows, k, _raw_stream()))
+    kind, rows, k, stride = _mx_rows(x, "x")
+    q = _mx_out(out, rows, k, fmt, x)
+    codes, scales = q._at
+    status = _host.mx_quantize(x.data_ptr(), kind, stride, codes, scales, _MX_FORMATS[fmt], rows, k, _raw_stream())
+    if status != OK:
+        check(status)
     return q
 
 
 def mx_dequantize(q, dtype=torch.bfloat16, out=None):
     """The values that an MxTensor stands for."""
-    _need_mx(q, "q")
+    codes, scales = _mx_at(q, "q")
+    rows, k = q.rows, q.k
     if out is None:
-        out = q.codes.new_empty((q.rows, q.k), dtype=dtype)
-    stride = _need_rows(out, "out", dtype, (q.rows, q.k))
-    check(lib.sarek_hip_mx_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), _MX_FORMATS[q.fmt], out.data_ptr(),
-                                      _MX_TYPES[dtype], stride, q.rows, q.k, _raw_stream()))
+        if dtype not in _MX_TYPES:
+            raise TypeError(f"mx_dequantize: {dtype} is none of float32, bfloat16, float16")
+        out = (q._block if q._block is not None else q._codes).new_empty((rows, k), dtype=dtype)
+    kind, out_rows, out_k, stride = _mx_rows(out, "out")
+    if out.dtype != dtype or (out_rows, out_k) != (rows, k):
+        raise ValueError(f"out: expected {rows} x {k} of {dtype}, got {tuple(out.shape)} of {out.dtype}")
+    status = _host.mx_dequantize(codes, scales, _MX_FORMATS[q.fmt], out.data_ptr(), kind, stride, rows, k, _raw_stream())
+    if status != OK:
+        check(status)
     return out
 
 
 def rms_norm_mx(x, weight, residual=None, eps=1e-6, out=None, h=None):
     """h = x + residual (in x's type), rstd = (mean of h^2 + eps)^-1/2 of each row, and h * rstd * weight in "fp8".
     Returns (MxTensor, h, rstd); without a residual h is x.  h: where the sum goes (x or residual itself, for instance)."""
-    stride = _need_rows(x, "x")
-    rows, k = x.shape
-    _need(weight, x.dtype, "weight")
-    if weight.shape != (k,):
-        raise ValueError(f"rms_norm_mx: {k} weights expected, got {tuple(weight.shape)}")
-    residual_stride = 0 if residual is None else _need_rows(residual, "residual", x.dtype, x.shape)
-    if h is None and residual is not None:
-        h = x.new_empty((rows, k))
-    h_stride = 0 if h is None else _need_rows(h, "h", x.dtype, x.shape)
-    q = _mx_out(out, rows, k, "fp8", x, "rms_norm_mx")
+    kind, rows, k, stride = _mx_rows(x, "x")
+    weight_at = _mx_weight(weight, x.dtype, k)
+    residual_at, residual_stride, h_at, h_stride = None, 0, None, 0
+    if residual is not None:
+        residual_at, residual_stride = residual.data_ptr(), _mx_like(residual, x, "residual")
+        if h is None:
+            h = x.new_empty((rows, k))
+            h_at, h_stride = h.data_ptr(), k
+    if h is not None and h_at is None:
+        h_at, h_stride = h.data_ptr(), _mx_like(h, x, "h")
+    q = _mx_out(out, rows, k, "fp8", x)
     rstd = x.new_empty(rows, dtype=torch.float32)
-    check(lib.sarek_hip_rms_norm_mx(x.data_ptr(), stride, None if residual is None else residual.data_ptr(), residual_stride,
-                                    weight.data_ptr(), _MX_TYPES[x.dtype], eps, None if h is None else h.data_ptr(), h_stride,
-                                    q.codes.data_ptr(), q.scales.data_ptr(), rstd.data_ptr(), rows, k, _raw_stream()))
+    codes, scales = q._at
+    status = _host.rms_norm_mx(x.data_ptr(), stride, residual_at, residual_stride, weight_at, kind, eps, h_at, h_stride, codes,
+                               scales, rstd.data_ptr(), rows, k, _raw_stream())
+    if status != OK:
+        check(status)
     return q, x if h is None else h, rstd
 
 
 def rms_norm_backward(dy, h, weight, rstd, dh=None, out=None):
     """The gradients of rms_norm_mx with the 8-bit rounding taken as the identity: dy for its output, dh for its h (None: no
     gradient comes that way).  Returns (dx, dweight): dx is x's and the residual's, in their type; dweight is float32."""
-    stride = _need_rows(h, "h")
-    rows, k = h.shape
-    dy_stride = _need_rows(dy, "dy", h.dtype, h.shape)
-    dh_stride = 0 if dh is None else _need_rows(dh, "dh", h.dtype, h.shape)
-    _need(weight, h.dtype, "weight")
+    kind, rows, k, stride = _mx_rows(h, "h")
+    dy_stride = _mx_like(dy, h, "dy")
+    dh_at, dh_stride = (None, 0) if dh is None else (dh.data_ptr(), _mx_like(dh, h, "dh"))
+    weight_at = _mx_weight(weight, h.dtype, k)
     _need(rstd, torch.float32, "rstd")
-    if weight.shape != (k,) or rstd.shape != (rows,):
-        raise ValueError("rms_norm_backward: shape mismatch")
-    dx = h.new_empty((rows, k)) if out is None else out
-    dx_stride = _need_rows(dx, "out", h.dtype, h.shape)
+    if rstd.shape != (rows,):
+        raise ValueError(f"rstd: {rows} values expected, got {tuple(rstd.shape)}")
+    if out is None:
+        dx, dx_stride = h.new_empty((rows, k)), k
+    else:
+        dx, dx_stride = out, _mx_like(out, h, "out")
     dweight = h.new_empty(k, dtype=torch.float32)
-    workspace = h.new_empty(lib.sarek_hip_rms_norm_backward_workspace_floats(rows, k), dtype=torch.float32)
-    check(lib.sarek_hip_rms_norm_backward(dy.data_ptr(), dy_stride, h.data_ptr(), stride, weight.data_ptr(), rstd.data_ptr(),
-                                          None if dh is None else dh.data_ptr(), dh_stride, _MX_TYPES[h.dtype], dx.data_ptr(),
-                                          dx_stride, dweight.data_ptr(), rows, k, workspace.data_ptr(), workspace.numel(),
-                                          _raw_stream()))
+    floats = lib.sarek_hip_rms_norm_backward_workspace_floats(rows, k)
+    workspace = h.new_empty(floats, dtype=torch.float32)
+    status = _host.rms_norm_backward(dy.data_ptr(), dy_stride, h.data_ptr(), stride, weight_at, rstd.data_ptr(), dh_at, dh_stride,
+                                     kind, dx.data_ptr(), dx_stride, dweight.data_ptr(), rows, k, workspace.data_ptr(), floats,
+                                     _raw_stream())
+    if status != OK:
+        check(status)
     return dx, dweight
 
 
 def gemm_mx(a, b, bias=None, relu=False, dtype=torch.bfloat16, out=None):
     """a (rows of k values, "fp8" or "fp4") times the transpose of b (n rows of k values, "fp4"): [rows, n] in dtype, with
     bias (float32, n values) added and, where asked, negative values set to 0.  An "fp8" a goes to 16-bit types."""
-    _need_mx(a, "a")
-    _need_mx(b, "b")
+    (a_codes, a_scales), (b_codes, b_scales) = _mx_at(a, "a"), _mx_at(b, "b")
     if b.fmt != "fp4":
         raise ValueError("gemm_mx: b is held in fp4")
     if a.k != b.k:
         raise ValueError("gemm_mx: inner dimensions differ")
-    if dtype not in _MX_TYPES:
-        raise TypeError(f"gemm_mx: {dtype} is none of float32, bfloat16, float16")
     m, n = a.rows, b.rows
+    bias_at = None
     if bias is not None:
         _need(bias, torch.float32, "bias")
         if bias.shape != (n,):
-            raise ValueError(f"gemm_mx: {n} biases expected, got {tuple(bias.shape)}")
-    c = a.codes.new_empty((m, n), dtype=dtype) if out is None else out
-    c_stride = _need_rows(c, "out", dtype, (m, n))
-    check(lib.sarek_hip_gemm_mx(a.codes.data_ptr(), a.scales.data_ptr(), _MX_FORMATS[a.fmt], b.codes.data_ptr(),
-                                b.scales.data_ptr(), None if bias is None else bias.data_ptr(), 1 if relu else 0, c.data_ptr(),
-                                _MX_TYPES[dtype], c_stride, m, n, a.k, _raw_stream()))
+            raise ValueError(f"bias: {n} values expected, got {tuple(bias.shape)}")
+        bias_at = bias.data_ptr()
+    if out is None:
+        kind = _MX_TYPES.get(dtype)
+        if kind is None:
+            raise TypeError(f"gemm_mx: {dtype} is none of float32, bfloat16, float16")
+        c, c_stride = (a._block if a._block is not None else a._codes).new_empty((m, n), dtype=dtype), n
+    else:
+        c = out
+        kind, rows, columns, c_stride = _mx_rows(c, "out")
+        if c.dtype != dtype or (rows, columns) != (m, n):
+            raise ValueError(f"out: expected {m} x {n} of {dtype}, got {tuple(c.shape)} of {c.dtype}")
+    status = _host.gemm_mx(a_codes, a_scales, _MX_FORMATS[a.fmt], b_codes, b_scales, bias_at, 1 if relu else 0, c.data_ptr(), kind,
+                           c_stride, m, n, a.k, _raw_stream())
+    if status != OK:
+        check(status)
     return c
 
 
