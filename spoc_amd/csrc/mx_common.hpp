@@ -70,17 +70,52 @@ template <class T> __device__ __forceinline__ Raw8<T> load8(const T *p, int64_t 
     }
     return r;
   }
+  // Past the end the last value is loaded again and dropped: eight loads on their way at once, where conditional ones wait for each other.
+  const int last = static_cast<int>(count) - 1;
   if constexpr (sizeof(T) == 4) {
     r.lo = r.hi = f32x4v{0.f, 0.f, 0.f, 0.f};
+    if (last < 0) return r;
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < count) (j < 4 ? r.lo : r.hi)[j & 3] = p[j];
+    for (int j = 0; j < 8; ++j) v[j] = p[min(j, last)];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) (j < 4 ? r.lo : r.hi)[j & 3] = j <= last ? v[j] : 0.f;
   } else {
-    const uint16_t *q = reinterpret_cast<const uint16_t *>(p);
     r.w = u32x4_t{0u, 0u, 0u, 0u};
+    if (last < 0) return r;
+    const uint16_t *q = reinterpret_cast<const uint16_t *>(p);
+    uint32_t v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < count) r.w[j >> 1] |= static_cast<uint32_t>(q[j]) << (16 * (j & 1));
+    for (int j = 0; j < 8; ++j) v[j] = q[min(j, last)];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.w[j >> 1] |= j <= last ? v[j] << (16 * (j & 1)) : 0u;
+  }
+  return r;
+}
+
+// The same from column c of a row of k values, k at least 8: what begins past k - 8 is loaded from there and moved down, zeros behind it.
+// (No branch but for the lanes at a row's end, and few registers: kernels that hold a row load it so.)
+template <class T> __device__ __forceinline__ Raw8<T> load8_of_row(const T *row, int c, int k) {
+  const int from = min(c, k - 8), over = c - from;
+  Raw8<T> r = load8(row + from, 8);
+  if (over == 0) return r;
+  if constexpr (sizeof(T) == 4) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < 4 ? r.lo[j & 3] : r.hi[j & 3];
+#pragma unroll
+    for (int s = 1; s <= 4; s *= 2)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = over & s ? (j + s < 8 ? v[j + s] : 0.f) : v[j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) (j < 4 ? r.lo : r.hi)[j & 3] = over < 8 ? v[j] : 0.f;
+  } else {
+    typedef __attribute__((ext_vector_type(2))) unsigned long long u64x2_t;
+    u64x2_t v = __builtin_bit_cast(u64x2_t, r.w);
+    const int s = over * 16;
+    v[0] = s < 64 ? v[0] >> s | v[1] << 1 << (63 - s) : s < 128 ? v[1] >> (s - 64) : 0;
+    v[1] = s < 64 ? v[1] >> s : 0;
+    r.w = __builtin_bit_cast(u32x4_t, v);
   }
   return r;
 }

@@ -1,7 +1,7 @@
 // Rows in microscaled 8- and 4-bit floating point (layout: mx_common.hpp): bringing a matrix to them and back, the root-mean-square
 // norm that writes 8-bit rows for the product behind it, and that norm's gradient.  All of them pass over memory once.
 #include <algorithm>
-#include <type_traits>
+#include <utility>
 
 #include "mx_common.hpp"
 
@@ -67,25 +67,37 @@ __device__ __forceinline__ void write_codes(const float (&v)[8], uint8_t *__rest
 
 // ---- to 8 or 4 bits and back -------------------------------------------------------------------------------------------------------
 
-// One thread to eight values of the padded rows, four threads to a block.
-template <class T, bool Fp8>
-__global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ x, int64_t stride, uint8_t *__restrict__ codes,
-                                                          uint8_t *__restrict__ scales, int64_t rows, int64_t k, int64_t kp) {
-  for (int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; at < rows * kp; at += static_cast<int64_t>(gridDim.x) * 2048) {
-    const int64_t row = at / kp, c = at - row * kp;   // (the threads of a block of 32 stay together, kp being a multiple of 256)
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c < k) widen8<T>(load8(x + row * stride + c, k - c), v);
-    write_codes<Fp8>(v, codes + row * (Fp8 ? kp : kp / 2), scales + row * (kp / kMxBlock), c);
+// One thread to eight values of the padded rows, four threads to a block of 32, 32 to 256 values of one row.  Memory bounds both; with the
+// row found by a 64-bit division instead of a product they took @ and @ us for 11008 x 4096 from and to bf16.
+struct Rows {
+  uint32_t count, per_row, inverse;   // pieces of 256 values in all and of a row, and 2^32 over the latter, rounded down (2^32 - 1 for 1)
+};
+// Runs f(row, column) for the pieces that this thread takes part in.
+template <class F> __device__ __forceinline__ void each_piece(const Rows &p, F &&f) {
+  for (uint32_t u = blockIdx.x * 8 + threadIdx.x / 32; u < p.count; u += gridDim.x * 8) {
+    uint32_t row = __umulhi(u, p.inverse), left = u - row * p.per_row;   // at most two short
+    if (left >= p.per_row) ++row, left -= p.per_row;
+    if (left >= p.per_row) ++row, left -= p.per_row;
+    f(static_cast<int64_t>(row), static_cast<int64_t>(left) * kMxRow + (threadIdx.x & 31) * 8);
   }
 }
 
 template <class T, bool Fp8>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ x, int64_t stride, uint8_t *__restrict__ codes,
+                                                          uint8_t *__restrict__ scales, Rows pieces, int64_t k, int64_t kp) {
+  each_piece(pieces, [&](int64_t row, int64_t c) {
+    float v[8];
+    widen8<T>(load8(x + row * stride + c, k - c), v);
+    write_codes<Fp8>(v, codes + row * (Fp8 ? kp : kp / 2), scales + row * (kp / kMxBlock), c);
+  });
+}
+
+template <class T, bool Fp8>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
-                                                            T *__restrict__ out, int64_t stride, int64_t rows, int64_t k, int64_t kp) {
+                                                            T *__restrict__ out, int64_t stride, Rows pieces, int64_t k, int64_t kp) {
   typedef __attribute__((ext_vector_type(2))) float f32x2;
-  for (int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; at < rows * kp; at += static_cast<int64_t>(gridDim.x) * 2048) {
-    const int64_t row = at / kp, c = at - row * kp;
-    if (c >= k) continue;
+  each_piece(pieces, [&](int64_t row, int64_t c) {
+    if (c >= k) return;
     const uint32_t byte = scales[row * (kp / kMxBlock) + c / kMxBlock];
     const float scale = byte == 255 ? __uint_as_float(0x7FC00000u) : byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
     float v[8];
@@ -105,13 +117,12 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t *__res
       put(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.f, 3));
     }
     store8(out + row * stride + c, k - c, v);
-  }
+  });
 }
 
 // ---- norm --------------------------------------------------------------------------------------------------------------------------
 
-// The sum over the `Threads` threads of a row, in the same order on every run.  `shared`: Threads / 64 floats, not in use by the
-// previous sum any more.
+// The sum over the Threads threads of a row, in the same order on every run.  shared: Threads / 64 floats that nobody reads any more.
 template <int Threads> __device__ __forceinline__ float row_sum(float v, float *shared) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
@@ -125,106 +136,281 @@ template <int Threads> __device__ __forceinline__ float row_sum(float v, float *
   return v;
 }
 
-// h = x + residual rounded to T (h = x without one), r = (mean of h^2 + eps)^-1/2, and the 8-bit form of h r weight.  One workgroup to a
-// row, which it goes over twice: what the second turn reads of h, the first one has read or written.
-template <class T>
-__global__ __launch_bounds__(256) void rms_norm_kernel(const T *x, int64_t x_stride, const T *residual, int64_t residual_stride,
-                                                       const T *__restrict__ weight, float eps, T *h, int64_t h_stride,
-                                                       uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
-                                                       float *__restrict__ rstd, int64_t rows, int64_t k, int64_t kp) {
-  __shared__ float shared[4];
-  auto sums = [&](int64_t row, int64_t c, float (&v)[8]) {
-    widen8<T>(load8(x + row * x_stride + c, k - c), v);
-    if (residual) {
-      float w[8];
-      widen8<T>(load8(residual + row * residual_stride + c, k - c), w);
+template <class T> struct NormArgs {
+  const T *x, *residual, *weight;
+  T *h;
+  uint8_t *codes, *scales;
+  float *rstd;
+  int64_t x_stride, residual_stride, h_stride, rows, k, kp;
+  float eps;
+};
+
+// h = x + residual rounded to T (h = x without one), r = (mean of h^2 + eps)^-1/2, and the 8-bit form of h r weight.  Threads of a
+// workgroup to a row, Vectors times eight values each: the row stays in registers between its sum and its codes, so that memory is read
+// once and written once, which is what bounds it.
+template <class T, int Threads, int Vectors>
+__global__ __launch_bounds__(Threads < 256 ? 256 : Threads) void rms_norm_kernel(NormArgs<T> p) {
+  constexpr int kRows = Threads < 256 ? 256 / Threads : 1;
+  __shared__ float shared[Threads / 64];
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / Threads;
+  if (row >= p.rows) return;   // (a whole wave where there are several rows to a workgroup, and no barrier then)
+  const int first = static_cast<int>(threadIdx.x % Threads) * 8, k = static_cast<int>(p.k), kp = static_cast<int>(p.kp);
+  const T *const x = p.x + row * p.x_stride, *const residual = p.residual ? p.residual + row * p.residual_stride : nullptr;
+  Raw8<T> raw[Vectors], more[Vectors], w[Vectors];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = round_to<T>(v[j] + w[j]);
+  for (int v = 0; v < Vectors; ++v) {
+    const int c = first + v * Threads * 8;
+    raw[v] = load8_of_row(x, c, k);
+    if (residual) more[v] = load8_of_row(residual, c, k);
+    w[v] = load8_of_row(p.weight, c, k);
+  }
+  float h[Vectors][8], sum = 0.f;
+#pragma unroll
+  for (int v = 0; v < Vectors; ++v) {
+    widen8<T>(raw[v], h[v]);
+    if (residual) {
+      float m[8];
+      widen8<T>(more[v], m);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[v][j] = round_to<T>(h[v][j] + m[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += h[v][j] * h[v][j];
+  }
+  const float r = 1.f / sqrtf(row_sum<Threads>(sum, shared) / static_cast<float>(k) + p.eps);
+  if (p.rstd && first == 0) p.rstd[row] = r;
+#pragma unroll
+  for (int v = 0; v < Vectors; ++v) {
+    const int c = first + v * Threads * 8;
+    if (c >= kp) break;
+    if (p.h && c < k) store8(p.h + row * p.h_stride + c, k - c, h[v]);
+    float y[8];
+    widen8<T>(w[v], y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = c + j < k ? h[v][j] * r * y[j] : 0.f;   // (0 times an infinite or undefined r is not 0)
+    write_codes<true>(y, p.codes + row * kp, p.scales + row * (kp / kMxBlock), c);
+  }
+}
+
+// The same for rows that registers do not hold: a workgroup goes over its row twice.
+template <class T>
+__global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs<T> p) {
+  __shared__ float shared[16];
+  const int64_t row = blockIdx.x;
+  auto sums = [&](int64_t c, float (&v)[8]) {
+    widen8<T>(load8(p.x + row * p.x_stride + c, p.k - c), v);
+    if (p.residual) {
+      float m[8];
+      widen8<T>(load8(p.residual + row * p.residual_stride + c, p.k - c), m);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = round_to<T>(v[j] + m[j]);
     }
   };
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    float sum = 0.f;
-    for (int64_t c = threadIdx.x * 8; c < k; c += 256 * 8) {
-      float v[8];
-      sums(row, c, v);
+  float sum = 0.f;
+  for (int64_t c = threadIdx.x * 8; c < p.k; c += 1024 * 8) {
+    float v[8];
+    sums(c, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += v[j] * v[j];
+    for (int j = 0; j < 8; ++j) sum += v[j] * v[j];
+  }
+  const float r = 1.f / sqrtf(row_sum<1024>(sum, shared) / static_cast<float>(p.k) + p.eps);
+  if (p.rstd && threadIdx.x == 0) p.rstd[row] = r;
+  for (int64_t c = threadIdx.x * 8; c < p.kp; c += 1024 * 8) {
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (c < p.k) {
+      float w[8];
+      sums(c, v);
+      if (p.h) store8(p.h + row * p.h_stride + c, p.k - c, v);
+      widen8<T>(load8(p.weight + c, p.k - c), w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = v[j] * r * w[j];
     }
-    __syncthreads();
-    const float r = 1.f / sqrtf(row_sum<256>(sum, shared) / static_cast<float>(k) + eps);
-    if (rstd && threadIdx.x == 0) rstd[row] = r;
-    for (int64_t c = threadIdx.x * 8; c < kp; c += 256 * 8) {
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (c < k) {
-        float w[8];
-        sums(row, c, v);
-        if (h) store8(h + row * h_stride + c, k - c, v);
-        widen8<T>(load8(weight + c, k - c), w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = v[j] * r * w[j];
+    for (int j = 0; j < 8; ++j) v[j] = c + j < p.k ? v[j] : 0.f;
+    write_codes<true>(v, p.codes + row * p.kp, p.scales + row * (p.kp / kMxBlock), c);
+  }
+}
+
+// Calls f with (threads to a row, times eight values) for rows of k values; without any for longer ones than registers are made for, and for less than one load.  A
+// wave to a row up to 1024 values (no barrier), then 256 threads, then 512, the gradient's registers with eight waves to a compute unit being
+// as many as there are (with 256 threads of 32 values each 3000 x 8190 in fp16 took @ us).
+template <class F, class Long> int by_length(int64_t k, F &&f, Long &&longer) {
+  if (k < 8) return longer();   // (load8_of_row)
+  if (k <= 512) return f(std::integer_sequence<int, 64, 1>{});
+  if (k <= 1024) return f(std::integer_sequence<int, 64, 2>{});
+  if (k <= 2048) return f(std::integer_sequence<int, 256, 1>{});
+  if (k <= 4096) return f(std::integer_sequence<int, 256, 2>{});
+  if (k <= 8192) return f(std::integer_sequence<int, 512, 2>{});
+  if (k <= 16384) return f(std::integer_sequence<int, 512, 4>{});
+  return longer();
+}
+
+template <class T> struct BackwardArgs {
+  const T *dy, *h, *weight, *dh;
+  const float *rstd;
+  T *dx;
+  float *planes;
+  int64_t dy_stride, h_stride, dh_stride, dx_stride, rows, k;
+};
+
+// With n = h r and g = weight dy:  dx = r (g - n mean(n g)) + dh,  dweight = sum over the rows of dy n.  A workgroup takes every
+// gridDim.x-th row (or group of rows, a wave to a row) and keeps their share of dweight in registers; it goes into a plane of its own, and
+// rms_norm_planes_kernel adds the planes up in order.  The next row is asked for before this one's sum is waited for: memory bounds it.
+template <class T, int Threads, int Vectors>
+__global__ __launch_bounds__(Threads < 256 ? 256 : Threads) void rms_norm_backward_kernel(BackwardArgs<T> p) {
+  constexpr int kRows = Threads < 256 ? 256 / Threads : 1;
+  __shared__ float shared[2][Threads / 64];
+  __shared__ float parts[kRows > 1 ? kRows : 1][kRows > 1 ? Threads * Vectors * 8 : 1];
+  const int first = static_cast<int>(threadIdx.x % Threads) * 8, k = static_cast<int>(p.k), sub = threadIdx.x / Threads;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  float w[Vectors][8], dw[Vectors][8];
+#pragma unroll
+  for (int v = 0; v < Vectors; ++v) {
+    const int c = first + v * Threads * 8;
+    widen8<T>(load8_of_row(p.weight, c, k), w[v]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dw[v][j] = 0.f;
+  }
+  Raw8<T> dy[Vectors], h[Vectors];
+  float r = 0.f;
+  auto load = [&](int64_t row) {
+#pragma unroll
+    for (int v = 0; v < Vectors; ++v) {
+      const int c = first + v * Threads * 8;
+      dy[v] = load8_of_row(p.dy + row * p.dy_stride, c, k);
+      h[v] = load8_of_row(p.h + row * p.h_stride, c, k);
+    }
+    r = p.rstd[row];
+  };
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub;
+  if (row < p.rows) load(row);
+  for (int turn = 0; row < p.rows; row += step, turn ^= 1) {
+    float n[Vectors][8], g[Vectors][8], sum = 0.f;
+    Raw8<T> add[Vectors];
+    const float now = r;
+    if (p.dh)
+#pragma unroll
+      for (int v = 0; v < Vectors; ++v) add[v] = load8_of_row(p.dh + row * p.dh_stride, first + v * Threads * 8, k);
+#pragma unroll
+    for (int v = 0; v < Vectors; ++v) {
+      widen8<T>(dy[v], g[v]);
+      widen8<T>(h[v], n[v]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        n[v][j] *= now;
+        dw[v][j] += g[v][j] * n[v][j];
+        g[v][j] *= w[v][j];
+        sum += n[v][j] * g[v][j];
       }
+    }
+    if (row + step < p.rows) load(row + step);
+    const float mean = row_sum<Threads>(sum, shared[turn]) / static_cast<float>(k);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = c + j < k ? v[j] : 0.f;   // (0 times an infinite or undefined 1 / rms is not 0)
-      write_codes<true>(v, codes + row * kp, scales + row * (kp / kMxBlock), c);
+    for (int v = 0; v < Vectors; ++v) {
+      const int c = first + v * Threads * 8;
+      if (c >= k) break;
+      float out[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (p.dh) widen8<T>(add[v], out);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) out[j] += now * (g[v][j] - n[v][j] * mean);
+      store8(p.dx + row * p.dx_stride + c, k - c, out);
+    }
+  }
+  float *const plane = p.planes + blockIdx.x * p.k;
+  if constexpr (kRows > 1) {
+#pragma unroll
+    for (int v = 0; v < Vectors; ++v)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) parts[sub][first + v * Threads * 8 + j] = dw[v][j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < k; c += 256) {
+      float sum = 0.f;
+#pragma unroll
+      for (int q = 0; q < kRows; ++q) sum += parts[q][c];
+      plane[c] = sum;
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < Vectors; ++v) {
+      const int c = first + v * Threads * 8;
+      if (c < k) store8(plane + c, k - c, dw[v]);
     }
   }
 }
 
-// With n = h r and g = weight dy:  dx = r (g - n mean(n g)) + dh,  dweight = sum over the rows of dy n.  A workgroup takes every
-// gridDim.x-th row and leaves its rows' share of dweight in a plane of its own; rms_norm_planes_kernel adds the planes up in order.
+// The same for longer rows, which a workgroup goes over twice; its plane of dweight is in memory all along.
 template <class T>
-__global__ __launch_bounds__(256) void rms_norm_backward_kernel(const T *__restrict__ dy, int64_t dy_stride, const T *__restrict__ h,
-                                                                int64_t h_stride, const T *__restrict__ weight,
-                                                                const float *__restrict__ rstd, const T *dh, int64_t dh_stride, T *dx,
-                                                                int64_t dx_stride, float *__restrict__ planes, int64_t rows, int64_t k) {
-  __shared__ float shared[4];
-  float *const plane = planes + blockIdx.x * k;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const float r = rstd[row];
+__global__ __launch_bounds__(1024) void rms_norm_backward_long_kernel(BackwardArgs<T> p) {
+  __shared__ float shared[2][16];
+  float *const plane = p.planes + blockIdx.x * p.k;
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    const float r = p.rstd[row];
     float sum = 0.f;
-    for (int64_t c = threadIdx.x * 8; c < k; c += 256 * 8) {
+    for (int64_t c = threadIdx.x * 8; c < p.k; c += 1024 * 8) {
       float d[8], v[8], w[8];
-      widen8<T>(load8(dy + row * dy_stride + c, k - c), d);
-      widen8<T>(load8(h + row * h_stride + c, k - c), v);
-      widen8<T>(load8(weight + c, k - c), w);
+      widen8<T>(load8(p.dy + row * p.dy_stride + c, p.k - c), d);
+      widen8<T>(load8(p.h + row * p.h_stride + c, p.k - c), v);
+      widen8<T>(load8(p.weight + c, p.k - c), w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum += v[j] * r * (w[j] * d[j]);
     }
-    __syncthreads();
-    const float mean = row_sum<256>(sum, shared) / static_cast<float>(k);
-    for (int64_t c = threadIdx.x * 8; c < k; c += 256 * 8) {
+    const float mean = row_sum<1024>(sum, shared[turn]) / static_cast<float>(p.k);
+    for (int64_t c = threadIdx.x * 8; c < p.k; c += 1024 * 8) {
       float d[8], v[8], w[8], e[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      widen8<T>(load8(dy + row * dy_stride + c, k - c), d);
-      widen8<T>(load8(h + row * h_stride + c, k - c), v);
-      widen8<T>(load8(weight + c, k - c), w);
-      if (dh) widen8<T>(load8(dh + row * dh_stride + c, k - c), e);
+      widen8<T>(load8(p.dy + row * p.dy_stride + c, p.k - c), d);
+      widen8<T>(load8(p.h + row * p.h_stride + c, p.k - c), v);
+      widen8<T>(load8(p.weight + c, p.k - c), w);
+      if (p.dh) widen8<T>(load8(p.dh + row * p.dh_stride + c, p.k - c), e);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float n = v[j] * r;
-        if (c + j < k) plane[c + j] = (row == blockIdx.x ? 0.f : plane[c + j]) + d[j] * n;
+        if (c + j < p.k) plane[c + j] = (row == blockIdx.x ? 0.f : plane[c + j]) + d[j] * n;
         e[j] += r * (w[j] * d[j] - n * mean);
       }
-      store8(dx + row * dx_stride + c, k - c, e);
+      store8(p.dx + row * p.dx_stride + c, p.k - c, e);
     }
   }
 }
 
+// dweight[c] = the planes' values of column c, added in an order that their number fixes: 32 threads to 4 columns, each a share of the
+// planes, 32 columns (a line of every plane) to a workgroup.
 __global__ __launch_bounds__(256) void rms_norm_planes_kernel(const float *__restrict__ planes, float *__restrict__ dweight, int count,
                                                               int64_t k) {
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (c >= k) return;
-  float sum = 0.f;
-  for (int p = 0; p < count; ++p) sum += planes[p * k + c];
-  dweight[c] = sum;
+  __shared__ float sums[32][33];
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 32;
+  const int quad = threadIdx.x & 7, share = threadIdx.x >> 3;
+  const int64_t c = first + quad * 4;
+  f32x4v sum = {0.f, 0.f, 0.f, 0.f};
+  if (c + 4 <= k) {
+#pragma unroll 16
+    for (int q = share; q < count; q += 32) sum += *reinterpret_cast<const f32x4_any *>(planes + q * k + c);
+  } else if (c < k) {
+    for (int q = share; q < count; q += 32)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < k) sum[j] += planes[q * k + c + j];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sums[share][quad * 4 + j] = sum[j];
+  __syncthreads();
+  if (threadIdx.x < 32 && first + threadIdx.x < k) {
+    float total = 0.f;
+#pragma unroll
+    for (int q = 0; q < 32; ++q) total += sums[q][threadIdx.x];
+    dweight[first + threadIdx.x] = total;
+  }
 }
 
-int backward_planes(int64_t rows) { return static_cast<int>(std::min<int64_t>(rows, 512)); }
+// Workgroups of the gradient, each with a plane of k floats: two to a compute unit, one where the planes would take over 8 MiB (they are
+// written and read again), at most as many as there are (groups of) rows.
+int backward_planes(int64_t rows, int64_t k) { return static_cast<int>(std::min<int64_t>(k <= 1024 ? ceil_div(rows, 4) : rows, k <= 4096 ? 512 : 256)); }
 
 int check_matrix(const char *what, int64_t rows, int64_t k) {
   if (rows < 0 || k <= 0) return fail(SAREK_HIP_E_INVALID_ARG, "%s: rows must not be negative and k must be positive (%lld x %lld)", what,
                                       static_cast<long long>(rows), static_cast<long long>(k));
-  if (rows > 0x7FFFFFFF || k > 0x7FFFFFFF - kMxRow)
-    return fail(SAREK_HIP_E_UNSUPPORTED, "%s: %lld x %lld: rows and k are below 2^31", what, static_cast<long long>(rows), static_cast<long long>(k));
+  if (rows >= int64_t{1} << 22 || k > int64_t{1} << 28)   // (a workgroup of 1024 to a row: below 2^32 threads)
+    return fail(SAREK_HIP_E_UNSUPPORTED, "%s: %lld x %lld: rows are below 2^22, k at most 2^28", what, static_cast<long long>(rows), static_cast<long long>(k));
   return SAREK_HIP_OK;
 }
 // Workgroups for `wanted`, at most 2^21: a launch has below 2^32 threads, the kernels go on from there in turns.
@@ -232,6 +418,12 @@ dim3 grid_of(int64_t wanted) { return dim3(static_cast<unsigned>(std::min<int64_
 int check_stride(const char *what, const char *name, int64_t stride, int64_t k) {
   if (stride < k) return fail(SAREK_HIP_E_INVALID_ARG, "%s: rows of %s are %lld values apart, less than k = %lld", what, name,
                               static_cast<long long>(stride), static_cast<long long>(k));
+  return SAREK_HIP_OK;
+}
+int pieces_of(const char *what, int64_t rows, int64_t kp, Rows *out) {
+  const int64_t per_row = kp / kMxRow, count = rows * per_row;
+  if (count > 0x7FFFFFFF) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: 2^39 values or more", what);
+  *out = {static_cast<uint32_t>(count), static_cast<uint32_t>(per_row), per_row == 1 ? 0xFFFFFFFFu : static_cast<uint32_t>((int64_t{1} << 32) / per_row)};
   return SAREK_HIP_OK;
 }
 #define SAREK_MX_TRY(expr)                       \
@@ -258,12 +450,14 @@ int sarek_hip_mx_quantize(const void *x, int type, int64_t x_stride, unsigned ch
   if (!x || !codes || !scales) return fail(SAREK_HIP_E_INVALID_ARG, "mx_quantize: NULL pointer");
   if (misaligned(codes, scales)) return fail(SAREK_HIP_E_INVALID_ARG, "mx_quantize: codes start at multiples of 16 bytes, scales of 8");
   const int64_t kp = mx_row_values(k);
-  const dim3 grid = grid_of(ceil_div(rows * (kp / 8), 256));
+  Rows pieces;
+  SAREK_MX_TRY(pieces_of("mx_quantize", rows, kp, &pieces));
+  const dim3 grid = grid_of(ceil_div(pieces.count, 8));
   return by_type(type, [&]<class T>(T *) {
     if (format == SAREK_HIP_MX_FP8)
-      hipLaunchKernelGGL((mx_quantize_kernel<T, true>), grid, dim3(256), 0, as_stream(stream), static_cast<const T *>(x), x_stride, codes, scales, rows, k, kp);
+      hipLaunchKernelGGL((mx_quantize_kernel<T, true>), grid, dim3(256), 0, as_stream(stream), static_cast<const T *>(x), x_stride, codes, scales, pieces, k, kp);
     else
-      hipLaunchKernelGGL((mx_quantize_kernel<T, false>), grid, dim3(256), 0, as_stream(stream), static_cast<const T *>(x), x_stride, codes, scales, rows, k, kp);
+      hipLaunchKernelGGL((mx_quantize_kernel<T, false>), grid, dim3(256), 0, as_stream(stream), static_cast<const T *>(x), x_stride, codes, scales, pieces, k, kp);
     return check_launch("mx_quantize launch");
   });
 }
@@ -277,12 +471,14 @@ int sarek_hip_mx_dequantize(const unsigned char *codes, const unsigned char *sca
   if (!codes || !scales || !out) return fail(SAREK_HIP_E_INVALID_ARG, "mx_dequantize: NULL pointer");
   if (misaligned(codes, scales)) return fail(SAREK_HIP_E_INVALID_ARG, "mx_dequantize: codes start at multiples of 16 bytes, scales of 8");
   const int64_t kp = mx_row_values(k);
-  const dim3 grid = grid_of(ceil_div(rows * (kp / 8), 256));
+  Rows pieces;
+  SAREK_MX_TRY(pieces_of("mx_dequantize", rows, kp, &pieces));
+  const dim3 grid = grid_of(ceil_div(pieces.count, 8));
   return by_type(type, [&]<class T>(T *) {
     if (format == SAREK_HIP_MX_FP8)
-      hipLaunchKernelGGL((mx_dequantize_kernel<T, true>), grid, dim3(256), 0, as_stream(stream), codes, scales, static_cast<T *>(out), out_stride, rows, k, kp);
+      hipLaunchKernelGGL((mx_dequantize_kernel<T, true>), grid, dim3(256), 0, as_stream(stream), codes, scales, static_cast<T *>(out), out_stride, pieces, k, kp);
     else
-      hipLaunchKernelGGL((mx_dequantize_kernel<T, false>), grid, dim3(256), 0, as_stream(stream), codes, scales, static_cast<T *>(out), out_stride, rows, k, kp);
+      hipLaunchKernelGGL((mx_dequantize_kernel<T, false>), grid, dim3(256), 0, as_stream(stream), codes, scales, static_cast<T *>(out), out_stride, pieces, k, kp);
     return check_launch("mx_dequantize launch");
   });
 }
@@ -302,15 +498,24 @@ int sarek_hip_rms_norm_mx(const void *x, int64_t x_stride, const void *residual,
   if (residual && !h) return fail(SAREK_HIP_E_INVALID_ARG, "rms_norm_mx: a residual is added, but there is no h for the sum");
   const int64_t kp = mx_row_values(k);
   return by_type(type, [&]<class T>(T *) {
-    hipLaunchKernelGGL(rms_norm_kernel<T>, grid_of(rows), dim3(256), 0, as_stream(stream), static_cast<const T *>(x),
-                       x_stride, static_cast<const T *>(residual), residual_stride, static_cast<const T *>(weight), eps,
-                       static_cast<T *>(h), h_stride, codes, scales, rstd, rows, k, kp);
-    return check_launch("rms_norm_mx launch");
+    const NormArgs<T> args{static_cast<const T *>(x), static_cast<const T *>(residual), static_cast<const T *>(weight), static_cast<T *>(h),
+                           codes, scales, rstd, x_stride, residual_stride, h_stride, rows, k, kp, eps};
+    return by_length(
+        k,
+        [&]<int Threads, int Vectors>(std::integer_sequence<int, Threads, Vectors>) {
+          const dim3 grid(static_cast<unsigned>(ceil_div(rows, Threads < 256 ? 256 / Threads : 1)));
+          hipLaunchKernelGGL((rms_norm_kernel<T, Threads, Vectors>), grid, dim3(std::max(Threads, 256)), 0, as_stream(stream), args);
+          return check_launch("rms_norm_mx launch");
+        },
+        [&] {
+          hipLaunchKernelGGL(rms_norm_long_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(1024), 0, as_stream(stream), args);
+          return check_launch("rms_norm_mx launch");
+        });
   });
 }
 
 int64_t sarek_hip_rms_norm_backward_workspace_floats(int64_t rows, int64_t k) {
-  return rows <= 0 || k <= 0 ? 0 : backward_planes(rows) * k;
+  return rows <= 0 || k <= 0 ? 0 : backward_planes(rows, k) * k;
 }
 
 int sarek_hip_rms_norm_backward(const void *dy, int64_t dy_stride, const void *h, int64_t h_stride, const void *weight, const float *rstd,
@@ -327,15 +532,24 @@ int sarek_hip_rms_norm_backward(const void *dy, int64_t dy_stride, const void *h
   if (workspace_floats < sarek_hip_rms_norm_backward_workspace_floats(rows, k))
     return fail(SAREK_HIP_E_WORKSPACE, "rms_norm_backward: a workspace of %lld floats, %lld are needed", static_cast<long long>(workspace_floats),
                 static_cast<long long>(sarek_hip_rms_norm_backward_workspace_floats(rows, k)));
-  const int planes = rows > 0 ? backward_planes(rows) : 0;
+  const int planes = rows > 0 ? backward_planes(rows, k) : 0;
   return by_type(type, [&]<class T>(T *) {
     if (planes > 0) {
-      hipLaunchKernelGGL(rms_norm_backward_kernel<T>, dim3(planes), dim3(256), 0, as_stream(stream), static_cast<const T *>(dy), dy_stride,
-                         static_cast<const T *>(h), h_stride, static_cast<const T *>(weight), rstd, static_cast<const T *>(dh), dh_stride,
-                         static_cast<T *>(dx), dx_stride, workspace, rows, k);
+      const BackwardArgs<T> args{static_cast<const T *>(dy), static_cast<const T *>(h), static_cast<const T *>(weight), static_cast<const T *>(dh),
+                                 rstd, static_cast<T *>(dx), workspace, dy_stride, h_stride, dh_stride, dx_stride, rows, k};
+      by_length(
+          k,
+          [&]<int Threads, int Vectors>(std::integer_sequence<int, Threads, Vectors>) {
+            hipLaunchKernelGGL((rms_norm_backward_kernel<T, Threads, Vectors>), dim3(planes), dim3(std::max(Threads, 256)), 0, as_stream(stream), args);
+            return SAREK_HIP_OK;
+          },
+          [&] {
+            hipLaunchKernelGGL(rms_norm_backward_long_kernel<T>, dim3(planes), dim3(1024), 0, as_stream(stream), args);
+            return SAREK_HIP_OK;
+          });
       SAREK_MX_TRY(check_launch("rms_norm_backward launch"));
     }
-    hipLaunchKernelGGL(rms_norm_planes_kernel, dim3(static_cast<unsigned>(ceil_div(k, 256))), dim3(256), 0, as_stream(stream), workspace,
+    hipLaunchKernelGGL(rms_norm_planes_kernel, dim3(static_cast<unsigned>(ceil_div(k, 32))), dim3(256), 0, as_stream(stream), workspace,
                        dweight, planes, k);
     return check_launch("rms_norm_backward planes launch");
   });
