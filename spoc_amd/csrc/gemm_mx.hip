@@ -304,13 +304,14 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
       __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(later));
       barrier_no_fence();
     };
-    // the transfers of the stage that takes this one's place, in eight slots
-    auto refill = [&](int t) __attribute__((always_inline)) {
-      char *const to_a = lds_ring<60 + ring, kBytesA>, *const to_b = lds_ring<64 + ring, kBytesB>;
-      if (t < kMovesA) move_a(to_a, t, s + kRing);
-      else if (t < kMovesA + kMovesB) move_b(to_b, t - kMovesA, s + kRing);
-      if (t == 7 && first_in_span) move_scales(s / kPerSpan + 1);
+    // transfer t of the stage that takes the place of the one `ago` stages ago
+    auto refill = [&]<int Ago>(std::integral_constant<int, Ago>, int t) __attribute__((always_inline)) {
+      constexpr int to = (I + kRing - Ago) % kRing;
+      if (t < kMovesA) move_a(lds_ring<60 + to, kBytesA>, t, s - Ago + kRing);
+      else if (t < kMovesA + kMovesB) move_b(lds_ring<64 + to, kBytesB>, t - kMovesA, s - Ago + kRing);
     };
+    constexpr std::integral_constant<int, 0> this_one;
+    [[maybe_unused]] constexpr std::integral_constant<int, 1> one_before;
     asm volatile("" : "+v"(a_at), "+v"(b_at), "+v"(sa_at), "+v"(sb_at));   // (not one register for each place in LDS across the loop)
     if constexpr (Fp8) {
       constexpr int cur = I & 1;
@@ -323,14 +324,16 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
         if (i == 6) landed();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int t = (i - 6) * 4 + j;
           const char *const from = i < 6 ? la + a_at + (i + 2) * 2048 : la_next + a_at + (i - 6) * 2048;
           if (j == 0) alo[(8 * I + i + 2) % 3] = read(from);
           if (j == 1) ahi[(8 * I + i + 2) % 3] = read(i < 6 ? la + (a_at ^ 64) + (i + 2) * 2048 : la_next + (a_at ^ 64) + (i - 6) * 2048);
           if (first_in_span && j == 0) keep(sa[i], raw_a[i & 1], short_span);
           if (first_in_span && j == 2 && i < 6) read_raw_a(i + 2);
           if (i == 6) bf[cur ^ 1][j] = read(lb_next + b_at + j * 16 * kRowB);
-          if (i >= 6) refill(t);
+          // one transfer at a time: all of a workgroup's at once keep the path to LDS busy for 768 clocks, and the waves wait to issue them
+          if (i == 7 && j % 2 == 1) refill(this_one, j / 2);
+          if (i < 4 && j == 3) refill(one_before, i + 2);
+          if (i == 4 && j == 3 && I % kPerSpan == 1) move_scales(s / kPerSpan + 1);
           if (last_in_span && i == 7) read_raw_b(j);
           if (last_in_span && i == 7 && j >= 2) read_raw_a(j - 2);
           const u32x4 lo = alo[(8 * I + i) % 3], hi = ahi[(8 * I + i) % 3];
@@ -359,7 +362,8 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
                 const int i = t >> 1, j = i & 1 ? 1 - (t & 1) : t & 1;
                 if (t == 0 || (t >= 3 && t < 6)) alo[(cur ^ 1) * 4 + (t == 0 ? 0 : t - 2)] = read(from_a + (a_at ^ bits) + (t == 0 ? 0 : t - 2) * 4096);
                 if (t == 1 || t == 2) bf[cur ^ 1][t - 1] = read(from_b + (b_at ^ bits) + (t - 1) * 4096);
-                if (Step == 3) refill(t);
+                if (Step == 3) refill(this_one, t);
+                if (Step == 3 && t == 7 && first_in_span) move_scales(s / kPerSpan + 1);
                 if (Step == 3 && last_in_span && t >= 2) {
                   if (t < 4) read_raw_b(t - 2);
                   else read_raw_a(t - 4);
@@ -374,17 +378,21 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
   };
 
   move_scales(0);
+  // (8-bit: of the last of the three only what the stage before the first would have moved by now)
+  constexpr int kFirstMoves = Fp8 ? 2 : kMovesA + kMovesB;
   [&]<int... Ss>(std::integer_sequence<int, Ss...>) {
     (
         [&] {
+          constexpr int count = Ss == kRing - 1 ? kFirstMoves : kMovesA + kMovesB;
 #pragma unroll
-          for (int i = 0; i < kMovesA; ++i) move_a(lds_ring<60 + Ss, kBytesA>, i, Ss);
-#pragma unroll
-          for (int i = 0; i < kMovesB; ++i) move_b(lds_ring<64 + Ss, kBytesB>, i, Ss);
+          for (int t = 0; t < count; ++t) {
+            if (t < kMovesA) move_a(lds_ring<60 + Ss, kBytesA>, t, Ss);
+            else move_b(lds_ring<64 + Ss, kBytesB>, t - kMovesA, Ss);
+          }
         }(),
         ...);
   }(std::make_integer_sequence<int, kRing>{});
-  __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((kRing - 1) * (kMovesA + kMovesB)));
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((kRing - 2) * (kMovesA + kMovesB) + kFirstMoves));
   barrier_no_fence();
 #pragma unroll
   for (int j = 0; j < kTilesB; ++j) {
