@@ -901,12 +901,15 @@ def _mx_rows(t, name):
 
 def _mx_like(t, x, name):
     """Elements from row to row of a matrix that has to have x's type and shape."""
-    _, rows, k, stride = _mx_rows(t, name)
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == x.dtype and t.shape == x.shape:
+        stride, step = t.stride()
+        rows, k = t.shape
+        if step == 1 or k == 1:
+            return stride if rows > 1 else max(stride, k)
+    _mx_rows(t, name)
     if t.dtype != x.dtype:
         raise TypeError(f"{name}: expected {x.dtype}, got {t.dtype}")
-    if (rows, k) != x.shape:
-        raise ValueError(f"{name}: expected {tuple(x.shape)}, got {tuple(t.shape)}")
-    return stride
+    raise ValueError(f"{name}: expected {tuple(x.shape)}, got {tuple(t.shape)}")
 
 
 def _mx_at(q, name):
@@ -950,12 +953,14 @@ def mx_dequantize(q, dtype=torch.bfloat16, out=None):
     codes, scales = _mx_at(q, "q")
     rows, k = q.rows, q.k
     if out is None:
-        if dtype not in _MX_TYPES:
+        kind, stride = _MX_TYPES.get(dtype), k
+        if kind is None:
             raise TypeError(f"mx_dequantize: {dtype} is none of float32, bfloat16, float16")
-        out = (q._block if q._block is not None else q._codes).new_empty((rows, k), dtype=dtype)
-    kind, out_rows, out_k, stride = _mx_rows(out, "out")
-    if out.dtype != dtype or (out_rows, out_k) != (rows, k):
-        raise ValueError(f"out: expected {rows} x {k} of {dtype}, got {tuple(out.shape)} of {out.dtype}")
+        out = (q._block if q._block is not None else q._codes).new_empty(rows, k, dtype=dtype)
+    else:
+        kind, out_rows, out_k, stride = _mx_rows(out, "out")
+        if out.dtype != dtype or (out_rows, out_k) != (rows, k):
+            raise ValueError(f"out: expected {rows} x {k} of {dtype}, got {tuple(out.shape)} of {out.dtype}")
     status = _host.mx_dequantize(codes, scales, _MX_FORMATS[q.fmt], out.data_ptr(), kind, stride, rows, k, _raw_stream())
     if status != OK:
         check(status)
@@ -969,12 +974,14 @@ def rms_norm_mx(x, weight, residual=None, eps=1e-6, out=None, h=None):
     weight_at = _mx_weight(weight, x.dtype, k)
     residual_at, residual_stride, h_at, h_stride = None, 0, None, 0
     if residual is not None:
-        residual_at, residual_stride = residual.data_ptr(), _mx_like(residual, x, "residual")
+        residual_stride = _mx_like(residual, x, "residual")
+        residual_at = residual.data_ptr()
         if h is None:
-            h = x.new_empty((rows, k))
+            h = x.new_empty(rows, k)
             h_at, h_stride = h.data_ptr(), k
     if h is not None and h_at is None:
-        h_at, h_stride = h.data_ptr(), _mx_like(h, x, "h")
+        h_stride = _mx_like(h, x, "h")
+        h_at = h.data_ptr()
     q = _mx_out(out, rows, k, "fp8", x)
     rstd = x.new_empty(rows, dtype=torch.float32)
     codes, scales = q._at
@@ -990,13 +997,14 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, out=None):
     gradient comes that way).  Returns (dx, dweight): dx is x's and the residual's, in their type; dweight is float32."""
     kind, rows, k, stride = _mx_rows(h, "h")
     dy_stride = _mx_like(dy, h, "dy")
-    dh_at, dh_stride = (None, 0) if dh is None else (dh.data_ptr(), _mx_like(dh, h, "dh"))
+    dh_stride = 0 if dh is None else _mx_like(dh, h, "dh")
+    dh_at = None if dh is None else dh.data_ptr()
     weight_at = _mx_weight(weight, h.dtype, k)
     _need(rstd, torch.float32, "rstd")
     if rstd.shape != (rows,):
         raise ValueError(f"rstd: {rows} values expected, got {tuple(rstd.shape)}")
     if out is None:
-        dx, dx_stride = h.new_empty((rows, k)), k
+        dx, dx_stride = h.new_empty(rows, k), k
     else:
         dx, dx_stride = out, _mx_like(out, h, "out")
     dweight = h.new_empty(k, dtype=torch.float32)
@@ -1029,7 +1037,7 @@ def gemm_mx(a, b, bias=None, relu=False, dtype=torch.bfloat16, out=None):
         kind = _MX_TYPES.get(dtype)
         if kind is None:
             raise TypeError(f"gemm_mx: {dtype} is none of float32, bfloat16, float16")
-        c, c_stride = (a._block if a._block is not None else a._codes).new_empty((m, n), dtype=dtype), n
+        c, c_stride = (a._block if a._block is not None else a._codes).new_empty(m, n, dtype=dtype), n
     else:
         c = out
         kind, rows, columns, c_stride = _mx_rows(c, "out")
