@@ -249,7 +249,7 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
     dma16(make_rsrc(b_from, s < stages ? static_cast<uint32_t>(rows_b) * pitch_b : 0u), off_b[i], s * kRowB, lb + (wave + 8 * i) * 1024);
   };
   // A row's last span may be 8 bytes: then the 16 that end with the row are taken.
-  char *const ls = lds_ring<68, 2 * kBytesS>;
+  char *const ls = lds_ring<68, 2 * kBytesS + 16>;
   auto move_scales = [&](int span) { dma16(rs, off_s, min(min(span, last_span) * 16, pitch_s - 16), ls + wave * 1024); };
 
   using Acc = std::conditional_t<Fp8, f32x4_t, f32x16>;
@@ -261,20 +261,16 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
 #pragma unroll
       for (int e = 0; e < kRows * kRows / 64; ++e) acc[i][j][e] = 0.f;
 
-  // Scales: a lane reads the 16 bytes of a row's span and keeps those that its place needs, in the order of the steps.
+  // Scales: a lane reads the bytes of a row for 256 of k (8-bit; two stages) or 512 (4-bit; two stages too) and keeps those that its place
+  // needs, in the order of the steps.
+  using Raw = std::conditional_t<Fp8, u32x2_t, u32x4>;
   constexpr int kWords = Fp8 ? 1 : 2;
   int sa[kTilesA][kWords], sb[kTilesB][kWords];
-  u32x4 raw_a[Fp8 ? 2 : 4], raw_b[kTilesB];
+  Raw raw_a[Fp8 ? 2 : 4], raw_b[kTilesB];
   const uint32_t pick = Fp8 ? static_cast<uint32_t>(place | (4 + place) << 8) | 0x0C0C0000u : 0x06040200u + place * 0x01010101u;
-  auto keep = [&](int (&to)[kWords], const u32x4 &d, bool short_span) {
-    const uint32_t d0 = short_span ? d[2] : d[0], d1 = short_span ? d[3] : d[1];
-    const uint32_t x = __builtin_amdgcn_perm(d1, d0, pick), y = __builtin_amdgcn_perm(d[3], d[2], pick);
-    if constexpr (Fp8) {
-      to[0] = static_cast<int>(x | y << 16);
-    } else {
-      to[0] = static_cast<int>(x);
-      to[1] = static_cast<int>(y);
-    }
+  auto keep = [&](int (&to)[kWords], const Raw &d) {
+    to[0] = static_cast<int>(__builtin_amdgcn_perm(d[1], d[0], pick));
+    if constexpr (!Fp8) to[1] = static_cast<int>(__builtin_amdgcn_perm(d[3], d[2], pick));
   };
   // A lane's 16 bytes of the first row tile; what follows of the row is some bits away: the second half of 8-bit codes (4 pieces on), the
   // steps of 4-bit ones (2 pieces each).
@@ -282,8 +278,19 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
   int b_at = (wn * 64 + r) * kRowB + ((place ^ (Fp8 ? place64(r) : r >> 1 & 7)) << 4);
   int sa_at = (wm * 128 + r) * 16, sb_at = kBytesS + (wn * 64 + r) * 16;
   auto read = [](const char *p) { return *reinterpret_cast<const u32x4 *>(p); };
-  auto read_raw_a = [&](int i) { raw_a[i % (Fp8 ? 2 : 4)] = read(ls + sa_at + i * kRows * 16); };
-  auto read_raw_b = [&](int j) { raw_b[j] = read(ls + sb_at + j * kRows * 16); };
+  // Where in a row's 16 bytes those of stage s begin.  Of a span of 8 bytes they are the second half (which 4-bit rows, that have no second
+  // stage then, read first).
+  auto raw_at = [&](int s) { return (Fp8 ? (s / 2 & 1) * 8 : 0) + (s / kPerSpan * 16 + 16 > pitch_s ? 8 : 0); };
+  auto read_raw = [&](int at) {
+    if constexpr (Fp8) {
+      return *reinterpret_cast<const u32x2_t *>(ls + at);
+    } else {
+      typedef u32x4 u32x4_by8 __attribute__((aligned(8)));   // (past the row's 16 bytes: the next row's, not used)
+      return static_cast<u32x4>(*reinterpret_cast<const u32x4_by8 *>(ls + at));
+    }
+  };
+  auto read_raw_a = [&](int i, int at) { raw_a[i % (Fp8 ? 2 : 4)] = read_raw(sa_at + at + i * kRows * 16); };
+  auto read_raw_b = [&](int j, int at) { raw_b[j] = read_raw(sb_at + at + j * kRows * 16); };
 
   // Fragments.  8-bit: three row tiles of A in turn, B of this step and the next; 4-bit: both operands of this step and the next.  (A
   // register more than there are, and its traffic waits for the transfers behind it in order.)
@@ -293,15 +300,14 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
   // read, after the barrier that says that it has landed and that this one has been read, and this one's place is filled again.
   auto stage = [&](auto ic, int s) __attribute__((always_inline)) {
     constexpr int I = decltype(ic)::value, ring = I % kRing, next = (I + 1) % kRing;
-    constexpr bool first_in_span = I % kPerSpan == 0, last_in_span = I % kPerSpan == kPerSpan - 1;
+    constexpr bool first_of_two = I % 2 == 0;
     const char *const la = lds_ring<60 + ring, kBytesA>;
     [[maybe_unused]] const char *const lb = lds_ring<64 + ring, kBytesB>;
     const char *const la_next = lds_ring<60 + next, kBytesA>, *const lb_next = lds_ring<64 + next, kBytesB>;
-    const bool short_span = first_in_span && s / kPerSpan * 16 + 16 > pitch_s;
+    [[maybe_unused]] const int raw_now = raw_at(s), raw_next = raw_at(s + 1);
     auto landed = [&]() __attribute__((always_inline)) {
-      // in flight may be what was asked for after the next stage: the stages behind it, and the scales where they went with the last
-      constexpr int later = (kRing - 2) * (kMovesA + kMovesB) + (kRing > 2 && I % kPerSpan == 1 ? 1 : 0);
-      __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(later));
+      // in flight may be what was asked for after the next stage: the stages behind it
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((kRing - 2) * (kMovesA + kMovesB)));
       barrier_no_fence();
     };
     // transfer t of the stage that takes the place of the one `ago` stages ago
@@ -315,9 +321,9 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
     asm volatile("" : "+v"(a_at), "+v"(b_at), "+v"(sa_at), "+v"(sb_at));   // (not one register for each place in LDS across the loop)
     if constexpr (Fp8) {
       constexpr int cur = I & 1;
-      if constexpr (first_in_span) {
+      if constexpr (first_of_two) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) keep(sb[j], raw_b[j], short_span);
+        for (int j = 0; j < 4; ++j) keep(sb[j], raw_b[j]);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -327,28 +333,29 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
           const char *const from = i < 6 ? la + a_at + (i + 2) * 2048 : la_next + a_at + (i - 6) * 2048;
           if (j == 0) alo[(8 * I + i + 2) % 3] = read(from);
           if (j == 1) ahi[(8 * I + i + 2) % 3] = read(i < 6 ? la + (a_at ^ 64) + (i + 2) * 2048 : la_next + (a_at ^ 64) + (i - 6) * 2048);
-          if (first_in_span && j == 0) keep(sa[i], raw_a[i & 1], short_span);
-          if (first_in_span && j == 2 && i < 6) read_raw_a(i + 2);
+          if (first_of_two && j == 0) keep(sa[i], raw_a[i & 1]);
+          if (first_of_two && j == 2 && i < 6) read_raw_a(i + 2, raw_now);
           if (i == 6) bf[cur ^ 1][j] = read(lb_next + b_at + j * 16 * kRowB);
           // one transfer at a time: all of a workgroup's at once keep the path to LDS busy for 768 clocks, and the waves wait to issue them
           if (i == 7 && j % 2 == 1) refill(this_one, j / 2);
           if (i < 4 && j == 3) refill(one_before, i + 2);
-          if (i == 4 && j == 3 && I % kPerSpan == 1) move_scales(s / kPerSpan + 1);
-          if (last_in_span && i == 7) read_raw_b(j);
-          if (last_in_span && i == 7 && j >= 2) read_raw_a(j - 2);
+          // (all of the span's have been read before this stage's barrier; the next ones have landed at the next)
+          if (i == 7 && j == 0 && I % kPerSpan == 2) move_scales(s / kPerSpan + 1);
+          if (!first_of_two && i == 7) read_raw_b(j, raw_next);
+          if (!first_of_two && i == 7 && j >= 2) read_raw_a(j - 2, raw_next);
           const u32x4 lo = alo[(8 * I + i) % 3], hi = ahi[(8 * I + i) % 3];
           const i32x8 af = {static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
                             static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
-          acc[i][j] = mfma_mx<true, I % 4>(bf[cur][j], af, acc[i][j], sb[j][0], sa[i][0]);
+          acc[i][j] = mfma_mx<true, I % 2>(bf[cur][j], af, acc[i][j], sb[j][0], sa[i][0]);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
     } else {
-      if constexpr (first_in_span) {
+      if constexpr (first_of_two) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) keep(sb[j], raw_b[j], short_span);
+        for (int j = 0; j < 2; ++j) keep(sb[j], raw_b[j]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) keep(sa[i], raw_a[i], short_span);
+        for (int i = 0; i < 4; ++i) keep(sa[i], raw_a[i]);
       }
       [&]<int... Steps>(std::integer_sequence<int, Steps...>) {
         (
@@ -363,10 +370,10 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
                 if (t == 0 || (t >= 3 && t < 6)) alo[(cur ^ 1) * 4 + (t == 0 ? 0 : t - 2)] = read(from_a + (a_at ^ bits) + (t == 0 ? 0 : t - 2) * 4096);
                 if (t == 1 || t == 2) bf[cur ^ 1][t - 1] = read(from_b + (b_at ^ bits) + (t - 1) * 4096);
                 if (Step == 3) refill(this_one, t);
-                if (Step == 3 && t == 7 && first_in_span) move_scales(s / kPerSpan + 1);
-                if (Step == 3 && last_in_span && t >= 2) {
-                  if (t < 4) read_raw_b(t - 2);
-                  else read_raw_a(t - 4);
+                if (Step == 3 && t == 7 && first_of_two) move_scales(s / kPerSpan + 1);
+                if (Step == 3 && !first_of_two && t >= 2) {
+                  if (t < 4) read_raw_b(t - 2, raw_next);
+                  else read_raw_a(t - 4, raw_next);
                 }
                 acc[i][j] = mfma_mx32<number % 4>(bf[cur][j], alo[cur * 4 + i], acc[i][j], sb[j][number / 4], sa[i][number / 4]);
                 __builtin_amdgcn_sched_barrier(0);
@@ -397,13 +404,13 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
 #pragma unroll
   for (int j = 0; j < kTilesB; ++j) {
     bf[0][j] = read(lds_ring<64, kBytesB> + b_at + j * kRows * kRowB);
-    read_raw_b(j);
+    read_raw_b(j, raw_at(0));
   }
 #pragma unroll
   for (int i = 0; i < (Fp8 ? 2 : 4); ++i) {
     alo[i] = read(lds_ring<60, kBytesA> + a_at + i * kRows * 128);
     if constexpr (Fp8) ahi[i] = read(lds_ring<60, kBytesA> + (a_at ^ 64) + i * kRows * 128);
-    read_raw_a(i);
+    read_raw_a(i, raw_at(0));
   }
   __builtin_amdgcn_sched_barrier(0);
   const int full = stages - stages % kPeriod;
