@@ -147,6 +147,13 @@ __global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__re
       for (int j = 0; j < NT; ++j) acc[i][j] = mfma_mx<Fp8, 0>(bf[j], af, acc[i][j], sb[j], sa);
     }
   };
+  constexpr int kQuads = kTN / 4, kRowsAtOnce = 512 / kQuads;   // of a row of the tile; rows that the threads cover at a time
+  const int col4 = threadIdx.x % kQuads, col = n0 + col4 * 4;   // this thread's columns of C
+  f32x4_t add = {0.f, 0.f, 0.f, 0.f};
+  if (bias) {   // (before the first transfer: loads come in order)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) add[e] = bias[min(col + e, n - 1)];
+  }
   [&]<int... Is>(std::integer_sequence<int, Is...>) { (move(lds_ring<80 + Is, kBytes>, Is), ...); }(std::make_integer_sequence<int, kRing - 1>{});
   for (int s = 0; s < stages; s += kRing)
     [&]<int... Is>(std::integer_sequence<int, Is...>) {
@@ -168,14 +175,7 @@ __global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__re
     for (int j = 0; j < NT; ++j) to[(i * NT + j) * 64 + (r ^ (j & 3)) * 4 + place] = acc[i][j];
   wait_lds();
   barrier_no_fence();
-  constexpr int kQuads = kTN / 4, kRowsAtOnce = 512 / kQuads;   // of a row of the tile; rows that the threads cover at a time
-  const int col4 = threadIdx.x % kQuads, tile_j = col4 / 4 % NT, part_n = col4 / 4 / NT;
-  const int col = n0 + col4 * 4;
-  f32x4_t add = {0.f, 0.f, 0.f, 0.f};
-  if (bias) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) add[e] = bias[min(col + e, n - 1)];
-  }
+  const int tile_j = col4 / 4 % NT, part_n = col4 / 4 / NT;
 #pragma unroll
   for (int turn_of = 0; turn_of < (kTM + kRowsAtOnce - 1) / kRowsAtOnce; ++turn_of) {
     const int row_in = turn_of * kRowsAtOnce + threadIdx.x / kQuads, tile_i = row_in / 16 % MT, part_m = row_in / 16 / MT;
@@ -199,7 +199,7 @@ template <bool Fp8, class T>
 __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__restrict__ a, const uint8_t *__restrict__ a_scales,
                                                            const uint8_t *__restrict__ b, const uint8_t *__restrict__ b_scales,
                                                            const float *__restrict__ bias, int relu, T *__restrict__ c, int64_t c_stride,
-                                                           int m, int n, int kp, int tiles_m, int tiles_n) {
+                                                           int m, int n, int kp, int tiles_m, int tiles_n, bool past_caches) {
   constexpr int kStage = Fp8 ? 128 : 256;            // values of k in a stage: 128 bytes of a row of A
   constexpr int kRowB = Fp8 ? 64 : 128;              // bytes of a row of B in a stage
   constexpr int kRing = Fp8 ? 3 : 2;                 // stages in LDS
@@ -384,6 +384,14 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
     }
   };
 
+  // The bias of a lane's columns, before the first transfer: loads come in order, and at the end they would be waited for.
+  f32x4_t add[kTilesB][kRows * kRows / 256];
+#pragma unroll
+  for (int j = 0; j < kTilesB; ++j)
+#pragma unroll
+    for (int q = 0; q < kRows * kRows / 256; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) add[j][q][e] = bias ? bias[min(n0 + wn * 64 + j * kRows + 8 * q + 4 * place + e, n - 1)] : 0.f;
   move_scales(0);
   // (8-bit: of the last of the three only what the stage before the first would have moved by now)
   constexpr int kFirstMoves = Fp8 ? 2 : kMovesA + kMovesB;
@@ -427,13 +435,6 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
   // piece q (16 bytes) of row r at q ^ (r % 16).  A lane has row r of a row tile, and four columns in a row for every four registers.
   constexpr int kRowC = 256 * sizeof(T), kTurnRows = 32768 / kRowC, kTurns = 128 / kTurnRows, kPiece = 16 / sizeof(T);
   char *const lc = wm == 0 ? lds_ring<60, kBytesA> : lds_ring<61, kBytesA>;
-  f32x4_t add[kTilesB][kRows * kRows / 256];
-#pragma unroll
-  for (int j = 0; j < kTilesB; ++j)
-#pragma unroll
-    for (int q = 0; q < kRows * kRows / 256; ++q)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) add[j][q][e] = bias ? bias[min(n0 + wn * 64 + j * kRows + 8 * q + 4 * place + e, n - 1)] : 0.f;
 #pragma unroll
   for (int turn = 0; turn < kTurns; ++turn) {
     barrier_no_fence();   // every wave has left the K loop, or has read the turn before
@@ -464,7 +465,8 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
       if (to_row >= m || col >= n) continue;
       T *const to = c + to_row * c_stride + col;
       if (col + kPiece <= n) {
-        *reinterpret_cast<u32x4_any *>(to) = v;
+        if (past_caches) __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(to));
+        else *reinterpret_cast<u32x4_any *>(to) = v;
       } else {
 #pragma unroll
         for (int e = 0; e < kPiece; ++e) {
@@ -487,7 +489,7 @@ namespace {
 constexpr int kShapeCount = 8;
 struct Shape { int rows, columns; double once, step8, step4; };
 constexpr Shape kShapes[kShapeCount] = {{16, 16, 1.9, 0.056, 0.050},  {16, 32, 2.0, 0.085, 0.080},  {32, 32, 2.0, 0.115, 0.097}, {32, 64, 2.0, 0.168, 0.148},
-                                        {64, 32, 1.8, 0.184, 0.153},  {64, 64, 2.9, 0.240, 0.190},  {128, 128, 3.5, 0.420, 0.310}, {256, 256, 7.3, 1.200, 0.700}};
+                                        {64, 32, 1.8, 0.184, 0.153},  {64, 64, 2.9, 0.240, 0.190},  {128, 128, 6.0, 0.460, 0.360}, {256, 256, 7.5, 1.050, 0.650}};
 
 // The one that the product takes least time on: a workgroup to a compute unit, as many in turn as there are too many.
 bool shape_serves(int shape, int64_t m, int64_t n, int64_t kp) {
@@ -533,13 +535,15 @@ extern "C" int sarek_hip_gemm_mx(const unsigned char *a_codes, const unsigned ch
   const int shape = shape_serves(forced, m, n, kp) ? forced : best_shape(fp8, m, n, kp);
   if (shape < 0) return fail(SAREK_HIP_E_UNSUPPORTED, "gemm_mx: %lld x %lld is more than one launch covers", static_cast<long long>(m), static_cast<long long>(n));
   return by_type(c_type, [&]<class T>(T *) {
-    const auto run = [&](auto kernel, int tile_m, int tile_n) {
+    const auto run = [&](auto kernel, int tile_m, int tile_n, auto... more) {
       const int64_t tiles_m = ceil_div(m, tile_m), tiles_n = ceil_div(n, tile_n);
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles_m * tiles_n)), dim3(512), 0, as_stream(stream), a_codes, a_scales, b_codes,
                          b_scales, bias, relu, static_cast<T *>(c), c_stride, static_cast<int>(m), static_cast<int>(n), static_cast<int>(kp),
-                         static_cast<int>(tiles_m), static_cast<int>(tiles_n));
+                         static_cast<int>(tiles_m), static_cast<int>(tiles_n), more...);
       return check_launch("gemm_mx launch");
     };
+    const bool whole_lines = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(c_stride) * sizeof(T)) & 127) == 0;
+    const bool past_caches = whole_lines && m * n * static_cast<int64_t>(sizeof(T)) >= tunable("gemm_mx.past_caches_mib", 200) << 20;
     const auto small = [&]<int MT, int NT, int WM, int WN, int Ring8, int Ring4>(std::integer_sequence<int, MT, NT, WM, WN, Ring8, Ring4>) {
       return fp8 ? run(gemm_mx_stream_kernel<true, T, MT, NT, WM, WN, Ring8>, 16 * MT * WM, 16 * NT * WN)
                  : run(gemm_mx_stream_kernel<false, T, MT, NT, WM, WN, Ring4>, 16 * MT * WM, 16 * NT * WN);
@@ -552,7 +556,7 @@ extern "C" int sarek_hip_gemm_mx(const unsigned char *a_codes, const unsigned ch
       case 4: return small(std::integer_sequence<int, 4, 1, 1, 2, 3, 6>{});
       case 5: return small(std::integer_sequence<int, 4, 2, 1, 2, 3, 4>{});
       case 6: return small(std::integer_sequence<int, 4, 4, 2, 2, 3, 4>{});
-      default: return fp8 ? run(gemm_mx_tile_kernel<true, T>, 256, 256) : run(gemm_mx_tile_kernel<false, T>, 256, 256);
+      default: return fp8 ? run(gemm_mx_tile_kernel<true, T>, 256, 256, past_caches) : run(gemm_mx_tile_kernel<false, T>, 256, 256, past_caches);
     }
   });
 }
