@@ -72,52 +72,73 @@ __device__ __forceinline__ void write_codes(const float (&v)[8], uint8_t *__rest
 struct Rows {
   uint32_t count, per_row, inverse;   // pieces of 256 values in all and of a row, and 2^32 over the latter, rounded down (2^32 - 1 for 1)
 };
-// Runs f(row, column) for the pieces that this thread takes part in.
-template <class F> __device__ __forceinline__ void each_piece(const Rows &p, F &&f) {
-  for (uint32_t u = blockIdx.x * 8 + threadIdx.x / 32; u < p.count; u += gridDim.x * 8) {
-    uint32_t row = __umulhi(u, p.inverse), left = u - row * p.per_row;   // at most two short
-    if (left >= p.per_row) ++row, left -= p.per_row;
-    if (left >= p.per_row) ++row, left -= p.per_row;
-    f(static_cast<int64_t>(row), static_cast<int64_t>(left) * kMxRow + (threadIdx.x & 31) * 8);
+// The row and column of the eight values of piece u that are this thread's.
+__device__ __forceinline__ void place_of(const Rows &p, uint32_t u, int64_t &row, int64_t &column) {
+  uint32_t q = __umulhi(u, p.inverse), left = u - q * p.per_row;   // at most two short
+  if (left >= p.per_row) ++q, left -= p.per_row;
+  if (left >= p.per_row) ++q, left -= p.per_row;
+  row = q;
+  column = static_cast<int64_t>(left) * kMxRow + (threadIdx.x & 31) * 8;
+}
+template <class T, bool Fp8, int kAtOnce>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ x, int64_t stride, uint8_t *__restrict__ codes,
+                                                          uint8_t *__restrict__ scales, Rows pieces, int64_t k, int64_t kp) {
+  for (uint32_t u = blockIdx.x * (8 * kAtOnce) + threadIdx.x / 32; u < pieces.count; u += gridDim.x * (8 * kAtOnce)) {
+    int64_t row[kAtOnce], c[kAtOnce];
+    Raw8<T> raw[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (u + 8 * i >= pieces.count) break;
+      place_of(pieces, u + 8 * i, row[i], c[i]);
+      raw[i] = load8(x + row[i] * stride + c[i], k - c[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (u + 8 * i >= pieces.count) break;
+      float v[8];
+      widen8<T>(raw[i], v);
+      write_codes<Fp8>(v, codes + row[i] * (Fp8 ? kp : kp / 2), scales + row[i] * (kp / kMxBlock), c[i]);
+    }
   }
 }
 
-template <class T, bool Fp8>
-__global__ __launch_bounds__(256) void mx_quantize_kernel(const T *__restrict__ x, int64_t stride, uint8_t *__restrict__ codes,
-                                                          uint8_t *__restrict__ scales, Rows pieces, int64_t k, int64_t kp) {
-  each_piece(pieces, [&](int64_t row, int64_t c) {
-    float v[8];
-    widen8<T>(load8(x + row * stride + c, k - c), v);
-    write_codes<Fp8>(v, codes + row * (Fp8 ? kp : kp / 2), scales + row * (kp / kMxBlock), c);
-  });
-}
-
-template <class T, bool Fp8>
+template <class T, bool Fp8, int kAtOnce>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
                                                             T *__restrict__ out, int64_t stride, Rows pieces, int64_t k, int64_t kp) {
   typedef __attribute__((ext_vector_type(2))) float f32x2;
-  each_piece(pieces, [&](int64_t row, int64_t c) {
-    if (c >= k) return;
-    const uint32_t byte = scales[row * (kp / kMxBlock) + c / kMxBlock];
-    const float scale = byte == 255 ? __uint_as_float(0x7FC00000u) : byte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
-    float v[8];
-    auto put = [&](int j, f32x2 pair) { v[j] = pair.x * scale, v[j + 1] = pair.y * scale; };
-    if constexpr (Fp8) {
-      const u32x2_t q = *reinterpret_cast<const u32x2_t *>(codes + row * kp + c);
+  for (uint32_t u = blockIdx.x * (8 * kAtOnce) + threadIdx.x / 32; u < pieces.count; u += gridDim.x * (8 * kAtOnce)) {
+    int64_t row[kAtOnce], c[kAtOnce];
+    u32x2_t q[kAtOnce];
+    uint32_t byte[kAtOnce];
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        put(4 * w, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q[w], 1.f, false));
-        put(4 * w + 2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q[w], 1.f, true));
-      }
-    } else {
-      const uint32_t q = *reinterpret_cast<const uint32_t *>(codes + row * (kp / 2) + c / 2);
-      put(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.f, 0));
-      put(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.f, 1));
-      put(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.f, 2));
-      put(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.f, 3));
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (u + 8 * i >= pieces.count) break;
+      place_of(pieces, u + 8 * i, row[i], c[i]);
+      byte[i] = scales[row[i] * (kp / kMxBlock) + c[i] / kMxBlock];
+      if constexpr (Fp8) q[i] = *reinterpret_cast<const u32x2_t *>(codes + row[i] * kp + c[i]);
+      else q[i][0] = *reinterpret_cast<const uint32_t *>(codes + row[i] * (kp / 2) + c[i] / 2);
     }
-    store8(out + row * stride + c, k - c, v);
-  });
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (u + 8 * i >= pieces.count) break;
+      const float scale = byte[i] == 255 ? __uint_as_float(0x7FC00000u) : byte[i] == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(byte[i] << 23);
+      float v[8];
+      auto put = [&](int j, f32x2 pair) { v[j] = pair.x * scale, v[j + 1] = pair.y * scale; };
+      if constexpr (Fp8) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          put(4 * w, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q[i][w], 1.f, false));
+          put(4 * w + 2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q[i][w], 1.f, true));
+        }
+      } else {
+        put(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i][0], 1.f, 0));
+        put(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i][0], 1.f, 1));
+        put(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i][0], 1.f, 2));
+        put(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i][0], 1.f, 3));
+      }
+      store8(out + row[i] * stride + c[i], k - c[i], v);
+    }
+  }
 }
 
 // ---- norm --------------------------------------------------------------------------------------------------------------------------
@@ -420,6 +441,8 @@ int check_stride(const char *what, const char *name, int64_t stride, int64_t k) 
                               static_cast<long long>(stride), static_cast<long long>(k));
   return SAREK_HIP_OK;
 }
+// From here on a thread of mx_quantize and mx_dequantize asks for several pieces at once: eight workgroups to a compute unit then still.
+constexpr uint32_t kManyPieces = 1 << 16;
 int pieces_of(const char *what, int64_t rows, int64_t kp, Rows *out) {
   const int64_t per_row = kp / kMxRow, count = rows * per_row;
   if (count > 0x7FFFFFFF) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: 2^39 values or more", what);
@@ -452,13 +475,15 @@ int sarek_hip_mx_quantize(const void *x, int type, int64_t x_stride, unsigned ch
   const int64_t kp = mx_row_values(k);
   Rows pieces;
   SAREK_MX_TRY(pieces_of("mx_quantize", rows, kp, &pieces));
-  const dim3 grid = grid_of(ceil_div(pieces.count, 8));
   return by_type(type, [&]<class T>(T *) {
-    if (format == SAREK_HIP_MX_FP8)
-      hipLaunchKernelGGL((mx_quantize_kernel<T, true>), grid, dim3(256), 0, as_stream(stream), static_cast<const T *>(x), x_stride, codes, scales, pieces, k, kp);
-    else
-      hipLaunchKernelGGL((mx_quantize_kernel<T, false>), grid, dim3(256), 0, as_stream(stream), static_cast<const T *>(x), x_stride, codes, scales, pieces, k, kp);
-    return check_launch("mx_quantize launch");
+    const auto run = [&](auto kernel, int at_once) {
+      hipLaunchKernelGGL(kernel, grid_of(ceil_div(pieces.count, 8 * at_once)), dim3(256), 0, as_stream(stream), static_cast<const T *>(x), x_stride, codes,
+                         scales, pieces, k, kp);
+      return check_launch("mx_quantize launch");
+    };
+    constexpr int kMany = sizeof(T) == 4 ? 2 : 4;
+    if (pieces.count < kManyPieces) return format == SAREK_HIP_MX_FP8 ? run(mx_quantize_kernel<T, true, 1>, 1) : run(mx_quantize_kernel<T, false, 1>, 1);
+    return format == SAREK_HIP_MX_FP8 ? run(mx_quantize_kernel<T, true, kMany>, kMany) : run(mx_quantize_kernel<T, false, kMany>, kMany);
   });
 }
 
@@ -473,13 +498,14 @@ int sarek_hip_mx_dequantize(const unsigned char *codes, const unsigned char *sca
   const int64_t kp = mx_row_values(k);
   Rows pieces;
   SAREK_MX_TRY(pieces_of("mx_dequantize", rows, kp, &pieces));
-  const dim3 grid = grid_of(ceil_div(pieces.count, 8));
   return by_type(type, [&]<class T>(T *) {
-    if (format == SAREK_HIP_MX_FP8)
-      hipLaunchKernelGGL((mx_dequantize_kernel<T, true>), grid, dim3(256), 0, as_stream(stream), codes, scales, static_cast<T *>(out), out_stride, pieces, k, kp);
-    else
-      hipLaunchKernelGGL((mx_dequantize_kernel<T, false>), grid, dim3(256), 0, as_stream(stream), codes, scales, static_cast<T *>(out), out_stride, pieces, k, kp);
-    return check_launch("mx_dequantize launch");
+    const auto run = [&](auto kernel, int at_once) {
+      hipLaunchKernelGGL(kernel, grid_of(ceil_div(pieces.count, 8 * at_once)), dim3(256), 0, as_stream(stream), codes, scales, static_cast<T *>(out), out_stride,
+                         pieces, k, kp);
+      return check_launch("mx_dequantize launch");
+    };
+    if (pieces.count < kManyPieces) return format == SAREK_HIP_MX_FP8 ? run(mx_dequantize_kernel<T, true, 1>, 1) : run(mx_dequantize_kernel<T, false, 1>, 1);
+    return format == SAREK_HIP_MX_FP8 ? run(mx_dequantize_kernel<T, true, 4>, 4) : run(mx_dequantize_kernel<T, false, 4>, 4);
   });
 }
 
