@@ -67,8 +67,8 @@ __device__ __forceinline__ void write_codes(const float (&v)[8], uint8_t *__rest
 
 // ---- to 8 or 4 bits and back -------------------------------------------------------------------------------------------------------
 
-// One thread to eight values of the padded rows, four threads to a block of 32, 32 to 256 values of one row.  Memory bounds both; with the
-// row found by a 64-bit division instead of a product they took @ and @ us for 11008 x 4096 from and to bf16.
+// One thread to eight values of the padded rows, four threads to a block of 32, 32 to 256 values of one row.  Memory bounds both: 11008 x
+// 4096 in bf16 to 8 bits 26.9 us, back 26.1, 5.1 and 5.2 TB/s (one piece to a thread, the row by a 64-bit division: 29.5 and 31.3).
 struct Rows {
   uint32_t count, per_row, inverse;   // pieces of 256 values in all and of a row, and 2^32 over the latter, rounded down (2^32 - 1 for 1)
 };
@@ -252,17 +252,18 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs<T> p) {
   }
 }
 
-// Calls f with (threads to a row, times eight values) for rows of k values; without any for longer ones than registers are made for, and for less than one load.  A
-// wave to a row up to 1024 values (no barrier), then 256 threads, then 512, the gradient's registers with eight waves to a compute unit being
-// as many as there are (with 256 threads of 32 values each 3000 x 8190 in fp16 took @ us).
-template <class F, class Long> int by_length(int64_t k, F &&f, Long &&longer) {
+// Calls f with (threads to a row, times eight values) for rows of k values of `size` bytes; `longer` for those that registers are not made
+// for, and for less than one load.  A wave to a row up to 1024 values (no barrier), then 256 threads, then 512, and 1024 for float32, whose 32
+// values of a thread the gradient's registers would not hold (gradient of 3000 x 8190 in fp16, us: 256 threads 62.9, 512 46.5; 3000 x 12000
+// in float32: 512 threads 198, 1024 163; 2000 x 16384 in bf16: 512 threads 54, 1024 60).
+template <class F, class Long> int by_length(int64_t k, size_t size, F &&f, Long &&longer) {
   if (k < 8) return longer();   // (load8_of_row)
   if (k <= 512) return f(std::integer_sequence<int, 64, 1>{});
   if (k <= 1024) return f(std::integer_sequence<int, 64, 2>{});
   if (k <= 2048) return f(std::integer_sequence<int, 256, 1>{});
   if (k <= 4096) return f(std::integer_sequence<int, 256, 2>{});
   if (k <= 8192) return f(std::integer_sequence<int, 512, 2>{});
-  if (k <= 16384) return f(std::integer_sequence<int, 512, 4>{});
+  if (k <= 16384) return size == 4 ? f(std::integer_sequence<int, 1024, 2>{}) : f(std::integer_sequence<int, 512, 4>{});
   return longer();
 }
 
@@ -527,7 +528,7 @@ int sarek_hip_rms_norm_mx(const void *x, int64_t x_stride, const void *residual,
     const NormArgs<T> args{static_cast<const T *>(x), static_cast<const T *>(residual), static_cast<const T *>(weight), static_cast<T *>(h),
                            codes, scales, rstd, x_stride, residual_stride, h_stride, rows, k, kp, eps};
     return by_length(
-        k,
+        k, sizeof(T),
         [&]<int Threads, int Vectors>(std::integer_sequence<int, Threads, Vectors>) {
           const dim3 grid(static_cast<unsigned>(ceil_div(rows, Threads < 256 ? 256 / Threads : 1)));
           hipLaunchKernelGGL((rms_norm_kernel<T, Threads, Vectors>), grid, dim3(std::max(Threads, 256)), 0, as_stream(stream), args);
@@ -564,7 +565,7 @@ int sarek_hip_rms_norm_backward(const void *dy, int64_t dy_stride, const void *h
       const BackwardArgs<T> args{static_cast<const T *>(dy), static_cast<const T *>(h), static_cast<const T *>(weight), static_cast<const T *>(dh),
                                  rstd, static_cast<T *>(dx), workspace, dy_stride, h_stride, dh_stride, dx_stride, rows, k};
       by_length(
-          k,
+          k, sizeof(T),
           [&]<int Threads, int Vectors>(std::integer_sequence<int, Threads, Vectors>) {
             hipLaunchKernelGGL((rms_norm_backward_kernel<T, Threads, Vectors>), dim3(planes), dim3(std::max(Threads, 256)), 0, as_stream(stream), args);
             return SAREK_HIP_OK;
