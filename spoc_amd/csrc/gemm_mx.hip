@@ -103,16 +103,18 @@ __global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__re
   const int word = (scale_a ? wave : wave - kWordsA / 64) * 64 + lane, word_row = word % (scale_a ? kTM : kTN), word_step = word / (scale_a ? kTM : kTN);
   const __amdgpu_buffer_rsrc_t rs = make_rsrc(scale_a ? a_scales + static_cast<int64_t>(m0) * pitch_s : b_scales + static_cast<int64_t>(n0) * pitch_s, (scale_a ? rows_a : rows_b) * pitch_s);
   const uint32_t off_s = word_step < Q && word_row < static_cast<int>(scale_a ? rows_a : rows_b) ? word_row * pitch_s + word_step * 4 : kOutOfRange;
-  auto move = [&](char *to, int s) __attribute__((always_inline)) {
-    if (wave < (kWordsA + kWordsB) / 64)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LDS_PTR void *)(to + kBytesA + kBytesB + wave * 256), 4,
-                                               static_cast<int>(s * Q + word_step < steps ? off_s + s * Q * 4 : kOutOfRange), 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < kMovesA; ++i)
-      dma16(ra, s * kRowA + at_a[i] < pitch_a ? off_a[i] + s * kRowA : kOutOfRange, 0, to + (wave + 8 * i) * 1024);
-#pragma unroll
-    for (int i = 0; i < kMovesB; ++i)
-      dma16(rb, s * kRowB + at_b[i] < pitch_b ? off_b[i] + s * kRowB : kOutOfRange, 0, to + kBytesA + (wave + 8 * i) * 1024);
+  // Transfer `i` of stage s: its scales, then A's, then B's.
+  auto move = [&](char *to, int s, int i) __attribute__((always_inline)) {
+    if (i == 0) {
+      if (wave < (kWordsA + kWordsB) / 64)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LDS_PTR void *)(to + kBytesA + kBytesB + wave * 256), 4,
+                                                 static_cast<int>(s * Q + word_step < steps ? off_s + s * Q * 4 : kOutOfRange), 0, 0, 0);
+    } else if (i <= kMovesA) {
+      dma16(ra, s * kRowA + at_a[i - 1] < pitch_a ? off_a[i - 1] + s * kRowA : kOutOfRange, 0, to + (wave + 8 * (i - 1)) * 1024);
+    } else {
+      const int j = i - 1 - kMovesA;
+      dma16(rb, s * kRowB + at_b[j] < pitch_b ? off_b[j] + s * kRowB : kOutOfRange, 0, to + kBytesA + (wave + 8 * j) * 1024);
+    }
   };
   f32x4_t acc[MT][NT];
 #pragma unroll
@@ -129,9 +131,17 @@ __global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__re
     // What the next stages have in flight may stay there (of a wave with scales to bring, one transfer less).
     __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((kRing - 2) * kMoves));
     barrier_no_fence();
-    move(lds_ring<80 + (I + kRing - 1) % kRing, kBytes>, s + kRing - 1);
-    u32x4 bf[NT];
-    int sb[NT];
+    // All fragments are asked for before the first MFMA. Where a wave has several MFMAs of both operands, the transfers go one by one
+    // between them, as all at once keep the waves waiting to issue them (8000 x 500 x 16000 in 4 bits 55.2 us, so 53.0; 1024 x 4096 x
+    // 4096 in 8 bits 23.8, so 22.8); elsewhere there is too little to hide them behind, and they go first (64 x 32 tiles, with one
+    // fragment of B to a wave: 64 x 8192 x 8192 14.0 us, between the MFMAs 14.8).
+    constexpr bool kBetween = MT > 1 && NT > 1;
+    if constexpr (!kBetween) {
+#pragma unroll
+      for (int t = 0; t <= kMoves; ++t) move(lds_ring<80 + (I + kRing - 1) % kRing, kBytes>, s + kRing - 1, t);
+    }
+    u32x4 bf[NT], lo[MT], hi[Fp8 ? MT : 1];
+    int sb[NT], sa[MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       bf[j] = read(from + b_at + j * 16 * kRowB);
@@ -139,12 +149,28 @@ __global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__re
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const u32x4 lo = read(from + a_at + i * 16 * kRowA), hi = Fp8 ? read(from + a_hi + i * 16 * kRowA) : u32x4{0u, 0u, 0u, 0u};
-      const int sa = static_cast<uint8_t>(from[sa_at + i * 64]);
-      const i32x8 af = {static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
-                        static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
+      lo[i] = read(from + a_at + i * 16 * kRowA);
+      if constexpr (Fp8) hi[i] = read(from + a_hi + i * 16 * kRowA);
+      sa[i] = static_cast<uint8_t>(from[sa_at + i * 64]);
+    }
+    if constexpr (kBetween) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j] = mfma_mx<Fp8, 0>(bf[j], af, acc[i][j], sb[j], sa);
+    for (int i = 0; i < MT; ++i) {
+      const u32x4 high = Fp8 ? hi[Fp8 ? i : 0] : u32x4{0u, 0u, 0u, 0u};
+      const i32x8 af = {static_cast<int>(lo[i][0]), static_cast<int>(lo[i][1]), static_cast<int>(lo[i][2]), static_cast<int>(lo[i][3]),
+                        static_cast<int>(high[0]), static_cast<int>(high[1]), static_cast<int>(high[2]), static_cast<int>(high[3])};
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        // transfers (kMoves + 1) n / (MT NT) of the n-th MFMA and on
+        const int n = i * NT + j;
+        if constexpr (kBetween) {
+#pragma unroll
+          for (int t = (kMoves + 1) * n / (MT * NT); t < (kMoves + 1) * (n + 1) / (MT * NT); ++t)
+            move(lds_ring<80 + (I + kRing - 1) % kRing, kBytes>, s + kRing - 1, t);
+        }
+        acc[i][j] = mfma_mx<Fp8, 0>(bf[j], af, acc[i][j], sb[j], sa[i]);
+        if constexpr (kBetween) __builtin_amdgcn_sched_barrier(0);
+      }
     }
   };
   constexpr int kQuads = kTN / 4, kRowsAtOnce = 512 / kQuads;   // of a row of the tile; rows that the threads cover at a time
@@ -154,7 +180,14 @@ __global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__re
 #pragma unroll
     for (int e = 0; e < 4; ++e) add[e] = bias[min(col + e, n - 1)];
   }
-  [&]<int... Is>(std::integer_sequence<int, Is...>) { (move(lds_ring<80 + Is, kBytes>, Is), ...); }(std::make_integer_sequence<int, kRing - 1>{});
+  [&]<int... Is>(std::integer_sequence<int, Is...>) {
+    (
+        [&] {
+#pragma unroll
+          for (int t = 0; t <= kMoves; ++t) move(lds_ring<80 + Is, kBytes>, Is, t);
+        }(),
+        ...);
+  }(std::make_integer_sequence<int, kRing - 1>{});
   for (int s = 0; s < stages; s += kRing)
     [&]<int... Is>(std::integer_sequence<int, Is...>) {
       ((s + Is < stages ? stage(std::integral_constant<int, Is>{}, s + Is) : void()), ...);
@@ -485,11 +518,15 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
 namespace sarek_hip {
 namespace {
 
-// The kernels' tiles of C, and what a workgroup takes, us: `once` for its start and its end, `step` for 128 of k (8-bit and 4-bit rows).
-constexpr int kShapeCount = 8;
+// The kernels' tiles of C, and the weights that choose one, about us of a workgroup: `once` for its start and its end, a step for 128 of
+// k (8-bit and 4-bit rows). They rank the tiles and are no times: a workgroup alone on its compute unit takes 0.033 to 1.3 us a step,
+// and lines through those times choose worse (2048 x 4096 x 4096 in 8 bits 44.7 us with 128 x 128 for 41.2 with 256 x 256). Over 26
+// products of 1 to 8000 rows, each timed with every tile, the choice is at most 3 % behind the best (512 x 4096 x 4096 21.2 us for 20.5)
+// and 0.2 % on average. Tiles of 64 x 32 were the best of one of them, by 1.4 % (512 x 1024 x 8192 in 4 bits 11.3 us for 11.4).
+constexpr int kShapeCount = 7;
 struct Shape { int rows, columns; double once, step8, step4; };
-constexpr Shape kShapes[kShapeCount] = {{16, 16, 1.9, 0.056, 0.050},  {16, 32, 2.0, 0.085, 0.080},  {32, 32, 2.0, 0.115, 0.097}, {32, 64, 2.0, 0.168, 0.148},
-                                        {64, 32, 1.8, 0.184, 0.153},  {64, 64, 2.9, 0.240, 0.190},  {128, 128, 6.0, 0.460, 0.360}, {256, 256, 7.5, 1.050, 0.650}};
+constexpr Shape kShapes[kShapeCount] = {{16, 16, 1.9, 0.056, 0.050}, {16, 32, 2.0, 0.085, 0.080},   {32, 32, 2.0, 0.115, 0.097},  {32, 64, 2.0, 0.168, 0.148},
+                                        {64, 64, 2.9, 0.240, 0.190}, {128, 128, 6.0, 0.460, 0.360}, {256, 256, 7.5, 1.050, 0.650}};
 
 // The one that the product takes least time on: a workgroup to a compute unit, as many in turn as there are too many.
 bool shape_serves(int shape, int64_t m, int64_t n, int64_t kp) {
@@ -553,9 +590,8 @@ extern "C" int sarek_hip_gemm_mx(const unsigned char *a_codes, const unsigned ch
       case 1: return small(std::integer_sequence<int, 1, 2, 1, 1, 4, 6>{});
       case 2: return small(std::integer_sequence<int, 2, 1, 1, 2, 6, 6>{});
       case 3: return small(std::integer_sequence<int, 2, 2, 1, 2, 4, 6>{});
-      case 4: return small(std::integer_sequence<int, 4, 1, 1, 2, 3, 6>{});
-      case 5: return small(std::integer_sequence<int, 4, 2, 1, 2, 3, 4>{});
-      case 6: return small(std::integer_sequence<int, 4, 4, 2, 2, 3, 4>{});
+      case 4: return small(std::integer_sequence<int, 4, 2, 1, 2, 3, 4>{});
+      case 5: return small(std::integer_sequence<int, 4, 4, 2, 2, 3, 4>{});
       default: return fp8 ? run(gemm_mx_tile_kernel<true, T>, 256, 256, past_caches) : run(gemm_mx_tile_kernel<false, T>, 256, 256, past_caches);
     }
   });
