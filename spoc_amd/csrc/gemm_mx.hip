@@ -1,13 +1,16 @@
-// Products of microscaled rows with 4-bit weights (layout: mx_common.hpp) on v_mfma_scale_f32_16x16x128_f8f6f4:
+// Products of microscaled rows with 4-bit weights (layout: mx_common.hpp) on the matrix unit's scaled instructions:
 //   C[M x N] = A[M x K] . B[N x K]^T (+ bias) (ReLU),  A in e4m3 or e2m1, B in e2m1, sums in float32.
 //
-// The instruction takes 16 rows of each operand and 128 of k, four blocks of 32, and a scale byte for each row and block: lane l brings
-// row l % 16, and the scale of the block in place l / 16.  Of a 4-bit operand lane l's 16 bytes are that block too; of an 8-bit one its 32
-// bytes are half (l / 16) % 2 of the blocks in places l / 32 (first 16 bytes) and 2 + l / 32 (second).  (Measured: sums of 4-bit products
-// come out exact; 8-bit ones are added on a grid of about 2^-14 of the largest product of the 128.)  Which blocks of a row go to which
-// place is free, as long as both operands and the scales agree: of 256 k, step s of two puts block 2 p + s in place p, so that a lane's
-// 4-bit codes of both steps are 32 bytes in a row and its scales two.
-// The weights are the first operand, so a lane's four results are four columns of one row of C.
+// v_mfma_scale_f32_16x16x128_f8f6f4 takes 16 rows of each operand and 128 of k, four blocks of 32, and a scale byte for each row and
+// block: lane l brings row l % 16, and the scale of block l / 16.  Of a 4-bit operand its 16 bytes are that block too; of an 8-bit one
+// its first 16 bytes are values 16 (l / 16) and on, its second 64 + 16 (l / 16) and on.  The weights are the first operand, so a lane's
+// results are columns of one row of C, four in a row.
+// Sums of 4-bit products come out exact (until float32 rounds them); 8-bit ones are added on a grid of about 2^-14 of the largest product
+// of the 128 (measured: up to 4.7e-5 of the sum of the magnitudes), so C is 16-bit there.
+//
+// Streams of the instruction alone, random codes: 8-bit with 4-bit rows 4390 TFLOP/s, 4-bit ones 5830, on 32x32x64 6600 (16x16x128 is bound
+// by its issue there); the clock falls with the data, zeros reach 9600.  A copy reaches 5.4 TB/s.  Of few rows the weights' bytes are the
+// bound, of many the matrix unit: gemm_mx_stream_kernel and gemm_mx_tile_kernel.
 #include <type_traits>
 #include <utility>
 
@@ -54,9 +57,14 @@ template <class T> __device__ __forceinline__ void store_four(T *p, int64_t coun
     if (j < count) store_one(p + j, v[j]);
 }
 
-// Small tiles of C, both operands brought to LDS by transfers, kRing - 1 stages ahead.  Eight waves: WM by WN of them share out the tile of C, each
-// MT by NT row and column tiles of 16, and Q of them in each place take every Q-th step of 128 k; a stage is Q steps.  Their sums are added
-// in order at the end.
+// Small tiles of C, both operands brought to LDS by transfers, kRing - 1 stages ahead.  Eight waves: WM by WN of them share out the tile of
+// C, each MT by NT row and column tiles of 16, and Q of them in each place take every Q-th step of 128 k; a stage is Q steps.  Their sums
+// are added in order at the end.
+// Few rows are bound by the weights' bytes, and those by how many are under way: rings of 120 to 155 KB, a workgroup to a compute unit, so that
+// even one row of C keeps every one of them loading.  K is split over a workgroup's waves, not over workgroups: their sums
+// meet in LDS, with no second launch and no memory for them.  (Rows of B straight to registers: 64 x 8192 x 8192 26 us, so 13.2.)  8-bit
+// rows: 1 x 8192 x 8192 8.4 us, 4.2 TB/s; 61 x 11007 x 4095 11.7, its 172 tiles of 64 x 64 being less than the compute units; 512 x 4096 x
+// 4096 21.7, 1024 x 4096 x 4096 23.3, 1470 TFLOP/s, bound by a start and an end that no other workgroup covers (6 us).
 template <bool Fp8, class T, int MT, int NT, int WM, int WN, int kRing>
 __global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__restrict__ a, const uint8_t *__restrict__ a_scales,
                                                              const uint8_t *__restrict__ b, const uint8_t *__restrict__ b_scales,
@@ -228,6 +236,13 @@ __global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__re
 
 // ---- 256 x 256 tiles -----------------------------------------------------------------------------------------------------------------
 
+// Eight waves of 128 x 64 of C each, in registers.  Both operands go through LDS, by transfers that are issued a stage or two ahead and one at
+// a time between the MFMAs; a stage's last eight MFMAs come after the barrier for the next, whose first fragments are read under them.
+// 8-bit rows take stages of 128 k, three in LDS, on 16x16x128; 4-bit ones 256 k, two, on 32x32x64 (half the instructions).
+// Measured: 4095 x 11008 x 4096 in 8 bits 144 us, 2560 TFLOP/s, the matrix unit busy for 71 % of the time; 8192^3 in 4 bits, C float32,
+// 270 us, 4070 TFLOP/s, busy for 58 %.  What bounds it: with empty transfers (zeros) the same code takes 113 and 173 us, on real data that
+// lies in LDS 120 and 219 (the clock falls), all of it coming from the L2 137 and 249.  Not taken: a workgroup that goes on to its next
+// tile, its first stages moved during the last of this one (8192^3 267 to 330 us: the wait for transfers waits for C's stores, too).
 template <bool Fp8, class T>
 __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__restrict__ a, const uint8_t *__restrict__ a_scales,
                                                            const uint8_t *__restrict__ b, const uint8_t *__restrict__ b_scales,

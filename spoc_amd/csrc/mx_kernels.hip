@@ -157,9 +157,9 @@ template <int Threads> __device__ __forceinline__ float row_sum(float v, float *
   return v;
 }
 
-// 1 / sqrt(v) and what it is short by: the code of h r weight is one of a few, and the next one where r's last bit carries h r weight past
-// the middle between two, so the norm is rounded once, not three times (of 444 million codes
-// 221 then differ from those of 64 bits, for 273; one row of 4096 takes 3.2 us for 3.1, 4095 rows the same).  v = 0 or infinite: no remainder.
+// 1 / sqrt(v) and what it is short by: the next code is taken where an error of r's or of a product's last bit carries h r weight past the
+// middle between two, so the norm is rounded once, not three times (of 444 million codes 221 then differ from those of 64 bits, for
+// 273; one row of 4096 takes 3.2 us for 3.1, 4095 rows the same).  v = 0 or infinite: no remainder.
 struct Root { float r, low; };
 __device__ __forceinline__ Root inverse_root(float v) {
   const float r = 1.f / sqrtf(v), s = v * r;   // s: sqrt(v), which neither overflows nor loses bits where r r would
@@ -182,7 +182,8 @@ template <class T> struct NormArgs {
 
 // h = x + residual rounded to T (h = x without one), r = (mean of h^2 + eps)^-1/2, and the 8-bit form of h r weight.  Threads of a
 // workgroup to a row, Vectors times eight values each: the row stays in registers between its sum and its codes, so that memory is read
-// once and written once, which is what bounds it.
+// once and written once, which is what bounds it (4095 x 4096 in bf16 with a residual 20.3 us, 5.8 TB/s, some of it out of the caches; 999 x 11007 in float32,
+// four rows to a compute unit, 14.4, 3.8).
 template <class T, int Threads, int Vectors>
 __global__ __launch_bounds__(Threads < 256 ? 256 : Threads) void rms_norm_kernel(NormArgs<T> p) {
   constexpr int kRows = Threads < 256 ? 256 / Threads : 1;
@@ -268,18 +269,30 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs<T> p) {
 
 // Calls f with (threads to a row, times eight values) for rows of k values of `size` bytes; `longer` for those that registers are not made
 // for, and for less than one load.  A wave to a row up to 1024 values (no barrier), then 256 threads, then 512, and 1024 for float32, whose 32
-// values of a thread the gradient's registers would not hold (gradient of 3000 x 8190 in fp16, us: 256 threads 62.9, 512 46.5; 3000 x 12000
-// in float32: 512 threads 198, 1024 163; 2000 x 16384 in bf16: 512 threads 54, 1024 60).
-template <class F, class Long> int by_length(int64_t k, size_t size, F &&f, Long &&longer) {
+// values of a thread the gradient's registers would not hold (gradient of 3000 x 8190 in fp16, us: 256 threads 62.9, 512 46.5; 2000 x 16384
+// in bf16: 512 threads 54, 1024 60).  Three loads to a thread
+// where two of twice the threads would leave a quarter of them and more without values: past 8192 values always (3000 x 12000 in float32,
+// gradient 136 us, so 93; 4095 x 11008 in bf16, norm 73 us, so 62; 16 rows the same), below where the caller's many rows make up for
+// what a row alone takes longer: `wave3` a wave up to 1536 values, `block3` 256 threads up to 6144.
+template <class F, class Long> int by_length(int64_t k, size_t size, bool wave3, bool block3, F &&f, Long &&longer) {
   if (k < 8) return longer();   // (load8_of_row)
   if (k <= 512) return f(std::integer_sequence<int, 64, 1>{});
   if (k <= 1024) return f(std::integer_sequence<int, 64, 2>{});
+  if (k <= 1536 && wave3) return f(std::integer_sequence<int, 64, 3>{});
   if (k <= 2048) return f(std::integer_sequence<int, 256, 1>{});
   if (k <= 4096) return f(std::integer_sequence<int, 256, 2>{});
+  if (k <= 6144 && block3) return f(std::integer_sequence<int, 256, 3>{});
   if (k <= 8192) return f(std::integer_sequence<int, 512, 2>{});
+  if (k <= 12288) return f(std::integer_sequence<int, 512, 3>{});
   if (k <= 16384) return size == 4 ? f(std::integer_sequence<int, 1024, 2>{}) : f(std::integer_sequence<int, 512, 4>{});
   return longer();
 }
+// The norm's: of 16-bit rows from 2048 on (16000 x 1200 with a residual 38 us, so 28, 2000 x 1536 7.8, so 7.1, but 1000 x 1536 4.4, so 4.7;
+// 4000 x 5500 35.5, so 31.1, 500 x 5500 7.2, so 7.3).  Float32 rows, with twice the bytes under way, gain nothing (4000 x 5500 55.6, 54.9).
+bool norm_by_three(int64_t rows, size_t size) { return size == 2 && rows >= 2048; }
+// The gradient's, of a wave only: from 1024 rows on (16000 x 1200 in bf16 57 us, so 30, 1000 x 1536 8.6, so 8.2, 500 x 1536 12.0, so 12.3;
+// float32 76 us, so 46); 256 threads lose (4000 x 5500 in bf16 47 us, 55).
+bool gradient_by_three(int64_t rows) { return rows >= 1024; }
 
 template <class T> struct BackwardArgs {
   const T *dy, *h, *weight, *dh;
@@ -291,7 +304,8 @@ template <class T> struct BackwardArgs {
 
 // With n = h r and g = weight dy:  dx = r (g - n mean(n g)) + dh,  dweight = sum over the rows of dy n.  A workgroup takes every
 // gridDim.x-th row (or group of rows, a wave to a row) and keeps their share of dweight in registers; it goes into a plane of its own, and
-// rms_norm_planes_kernel adds the planes up in order.  The next row is asked for before this one's sum is waited for: memory bounds it.
+// rms_norm_planes_kernel adds the planes up in order.  The next row is asked for before this one's sum is waited for: memory bounds
+// it (8192 x 4096 in bf16 with dh 48.9 us and 4.7 for the planes, 5.0 TB/s).
 template <class T, int Threads, int Vectors>
 __global__ __launch_bounds__(Threads < 256 ? 256 : Threads) void rms_norm_backward_kernel(BackwardArgs<T> p) {
   constexpr int kRows = Threads < 256 ? 256 / Threads : 1;
@@ -440,7 +454,10 @@ __global__ __launch_bounds__(256) void rms_norm_planes_kernel(const float *__res
 
 // Workgroups of the gradient, each with a plane of k floats: two to a compute unit, one where the planes would take over 8 MiB (they are
 // written and read again), at most as many as there are (groups of) rows.
-int backward_planes(int64_t rows, int64_t k) { return static_cast<int>(std::min<int64_t>(k <= 1024 ? ceil_div(rows, 4) : rows, k <= 4096 ? 512 : 256)); }
+int backward_planes(int64_t rows, int64_t k) {
+  const bool wave = k <= 1024 || (k <= 1536 && gradient_by_three(rows));   // a wave to a row, four rows to a workgroup
+  return static_cast<int>(std::min<int64_t>(wave ? ceil_div(rows, 4) : rows, k <= 4096 ? 512 : 256));
+}
 
 int check_matrix(const char *what, int64_t rows, int64_t k) {
   if (rows < 0 || k <= 0) return fail(SAREK_HIP_E_INVALID_ARG, "%s: rows must not be negative and k must be positive (%lld x %lld)", what,
@@ -542,7 +559,7 @@ int sarek_hip_rms_norm_mx(const void *x, int64_t x_stride, const void *residual,
     const NormArgs<T> args{static_cast<const T *>(x), static_cast<const T *>(residual), static_cast<const T *>(weight), static_cast<T *>(h),
                            codes, scales, rstd, x_stride, residual_stride, h_stride, rows, k, kp, eps};
     return by_length(
-        k, sizeof(T),
+        k, sizeof(T), norm_by_three(rows, sizeof(T)), norm_by_three(rows, sizeof(T)),
         [&]<int Threads, int Vectors>(std::integer_sequence<int, Threads, Vectors>) {
           const dim3 grid(static_cast<unsigned>(ceil_div(rows, Threads < 256 ? 256 / Threads : 1)));
           hipLaunchKernelGGL((rms_norm_kernel<T, Threads, Vectors>), grid, dim3(std::max(Threads, 256)), 0, as_stream(stream), args);
@@ -579,7 +596,7 @@ int sarek_hip_rms_norm_backward(const void *dy, int64_t dy_stride, const void *h
       const BackwardArgs<T> args{static_cast<const T *>(dy), static_cast<const T *>(h), static_cast<const T *>(weight), static_cast<const T *>(dh),
                                  rstd, static_cast<T *>(dx), workspace, dy_stride, h_stride, dh_stride, dx_stride, rows, k};
       by_length(
-          k, sizeof(T),
+          k, sizeof(T), gradient_by_three(rows), false,
           [&]<int Threads, int Vectors>(std::integer_sequence<int, Threads, Vectors>) {
             hipLaunchKernelGGL((rms_norm_backward_kernel<T, Threads, Vectors>), dim3(planes), dim3(std::max(Threads, 256)), 0, as_stream(stream), args);
             return SAREK_HIP_OK;

@@ -162,6 +162,12 @@ def test_norm(hip, torch_cuda, rows, k, dtype, residual):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k", [(2048, 1025), (2051, 1536), (2047, 1536), (2049, 4100), (2048, 6144), (5, 8200), (40, 12288), (3, 12289)])
+def test_norm_of_three_loads_to_a_thread(hip, torch_cuda, rows, k, dtype):
+    test_norm(hip, torch_cuda, rows, k, dtype, True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_norm_in_place_and_strided(hip, torch_cuda, dtype):
     for rows, k in ((6, 300), (3, 2049), (2, 18001)):
         a, b = random_rows(rows, k, dtype, 1, 0.5), random_rows(rows, k, dtype, 2, 0.5)
@@ -226,6 +232,12 @@ def test_norm_backward_against_differences(hip, torch_cuda):
         along_w = (f(host(h), host(weight) + step * e) - f(host(h), host(weight) - step * e)) / (2 * step)
         assert abs((host(dx) * d).sum() - along_h) <= 1e-5 * np.abs(host(dx) * d).sum()
         assert abs((host(dw) * e).sum() - along_w) <= 1e-5 * np.abs(host(dw) * e).sum()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k", [(1024, 1025), (1030, 1536), (1023, 1536), (2051, 1100), (5, 8200), (40, 12288), (3, 12289)])
+def test_norm_backward_of_three_loads_to_a_thread(hip, torch_cuda, rows, k, dtype):
+    test_norm_backward(hip, torch_cuda, rows, k, dtype, True)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
