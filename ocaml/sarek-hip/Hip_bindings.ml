@@ -209,6 +209,35 @@ let cast_f32_to_bf16 =
 let cast_f32_to_f16 =
   bind "sarek_hip_cast_f32_to_f16"
     (ptr float @-> ptr uint16_t @-> int64_t @-> ptr void @-> returning int)
+
+(* Operators on microscaled rows (include/sarek_hip.h): types and formats are its enums *)
+let mx_row_values = bind "sarek_hip_mx_row_values" (int64_t @-> returning int64_t)
+let mx_quantize =
+  bind "sarek_hip_mx_quantize"
+    (ptr void @-> int @-> int64_t @-> ptr uchar @-> ptr uchar @-> int @-> int64_t @-> int64_t
+   @-> ptr void @-> returning int)
+let mx_dequantize =
+  bind "sarek_hip_mx_dequantize"
+    (ptr uchar @-> ptr uchar @-> int @-> ptr void @-> int @-> int64_t @-> int64_t @-> int64_t
+   @-> ptr void @-> returning int)
+let rms_norm_mx =
+  bind "sarek_hip_rms_norm_mx"
+    (ptr void @-> int64_t @-> ptr void @-> int64_t @-> ptr void @-> int @-> float @-> ptr void
+   @-> int64_t @-> ptr uchar @-> ptr uchar @-> ptr float @-> int64_t @-> int64_t @-> ptr void
+   @-> returning int)
+let rms_norm_backward_workspace_floats =
+  bind "sarek_hip_rms_norm_backward_workspace_floats" (int64_t @-> int64_t @-> returning int64_t)
+let rms_norm_backward =
+  bind "sarek_hip_rms_norm_backward"
+    (ptr void @-> int64_t @-> ptr void @-> int64_t @-> ptr void @-> ptr float @-> ptr void
+   @-> int64_t @-> int @-> ptr void @-> int64_t @-> ptr float @-> int64_t @-> int64_t
+   @-> ptr float @-> int64_t @-> ptr void @-> returning int)
+let gemm_mx =
+  bind "sarek_hip_gemm_mx"
+    (ptr uchar @-> ptr uchar @-> int @-> ptr uchar @-> ptr uchar @-> ptr float @-> int
+   @-> ptr void @-> int @-> int64_t @-> int64_t @-> int64_t @-> int64_t @-> ptr void
+   @-> returning int)
+
 let triad =
   bind "sarek_hip_triad_f32"
     (ptr float @-> ptr float @-> ptr float @-> float @-> int64_t @-> ptr void @-> returning int)

@@ -453,11 +453,9 @@ __global__ __launch_bounds__(256) void rms_norm_planes_kernel(const float *__res
 }
 
 // Workgroups of the gradient, each with a plane of k floats: two to a compute unit, one where the planes would take over 8 MiB (they are
-// written and read again), at most as many as there are (groups of) rows.
-int backward_planes(int64_t rows, int64_t k) {
-  const bool wave = k <= 1024 || (k <= 1536 && gradient_by_three(rows));   // a wave to a row, four rows to a workgroup
-  return static_cast<int>(std::min<int64_t>(wave ? ceil_div(rows, 4) : rows, k <= 4096 ? 512 : 256));
-}
+// written and read again), at most as many as there are (groups of) rows.  Never more for fewer rows: a workspace serves those, too (so
+// not by the groups of rows where only many rows go by groups).
+int backward_planes(int64_t rows, int64_t k) { return static_cast<int>(std::min<int64_t>(k <= 1024 ? ceil_div(rows, 4) : rows, k <= 4096 ? 512 : 256)); }
 
 int check_matrix(const char *what, int64_t rows, int64_t k) {
   if (rows < 0 || k <= 0) return fail(SAREK_HIP_E_INVALID_ARG, "%s: rows must not be negative and k must be positive (%lld x %lld)", what,

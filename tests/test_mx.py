@@ -101,3 +101,49 @@ def test_the_front_end_refuses_host_tensors_and_wrong_kinds(hip):
     assert q.rows == 2
     with pytest.raises(TypeError):
         hip.gemm_mx(q, q)                                                      # on the host
+
+
+def test_mx_tensor_is_checked(hip):
+    codes, scales = torch.zeros(2, 256, dtype=torch.uint8), torch.zeros(2, 8, dtype=torch.uint8)
+    q = hip.MxTensor(codes, scales, "fp8", 64)
+    assert (q.rows, q.k, q.fmt) == (2, 64, "fp8") and q.codes is codes and q.scales is scales
+    assert hip.MxTensor(codes, torch.zeros(2, 16, dtype=torch.uint8), "fp4", 257).k == 257
+    for bad in ((codes, scales, "fp8", 0), (codes, scales, "fp8", 257), (codes, scales, "fp4", 64), (codes, scales, "fp6", 64),
+                (codes, scales[:1], "fp8", 64), (codes.view(-1), scales, "fp8", 64), (codes, scales.view(4, 4), "fp8", 64)):
+        with pytest.raises(ValueError):
+            hip.MxTensor(*bad)
+    for bad in ((codes.float(), scales, "fp8", 64), (codes, scales.int(), "fp8", 64), (codes[:, ::2], scales, "fp4", 64), (None, scales, "fp8", 64)):
+        with pytest.raises(TypeError):
+            hip.MxTensor(*bad)
+
+
+def test_a_made_tensor_has_its_parts_in_one_block(hip):
+    for fmt, width in (("fp8", 512), ("fp4", 256)):
+        q = hip.MxTensor._empty(3, 300, fmt, torch.zeros(1))
+        at = q._at
+        assert q.codes.shape == (3, width) and q.scales.shape == (3, 16) and q.codes.is_contiguous() and q.scales.is_contiguous()
+        assert (q.codes.data_ptr(), q.scales.data_ptr()) == at and at[1] % 8 == 0
+        q.codes.fill_(1), q.scales.fill_(2)
+        assert int(q.codes.sum()) == 3 * width and int(q.scales.sum()) == 96
+
+
+def test_native_calls_check_their_arguments(hip):
+    """What goes to C through the extension: the number of the arguments, their kinds and their ranges; nothing is called else."""
+    good = [None, 0, 64, None, None, 0, 0, 64, None]
+    assert hip._host.mx_quantize(*good) == hip.OK
+    for i, bad, error in ((1, 1 << 31, OverflowError), (2, 1 << 63, OverflowError), (0, "x", TypeError), (5, 1.5, TypeError), (7, None, TypeError)):
+        with pytest.raises(error):
+            hip._host.mx_quantize(*good[:i], bad, *good[i + 1:])
+    for call, count in ((hip._host.mx_quantize, 9), (hip._host.mx_dequantize, 9), (hip._host.rms_norm_mx, 15),
+                        (hip._host.rms_norm_backward, 17), (hip._host.gemm_mx, 14), (hip._host.bind_mx, 5)):
+        for n in (0, count - 1, count + 1):
+            with pytest.raises(TypeError):
+                call(*[0] * n)
+
+
+def test_workspaces_grow_with_rows_to_a_limit(hip):
+    """A plane for each workgroup; what serves some rows serves fewer too."""
+    f = hip.lib.sarek_hip_rms_norm_backward_workspace_floats
+    for k in (1, 64, 1024, 1025, 1536, 1537, 4096, 4097, 20000):
+        planes = [f(rows, k) // k for rows in (*range(1, 4200), 1 << 14, 1 << 20)]
+        assert planes == sorted(planes) and planes[0] == 1 and planes[-1] == planes[-2] <= 512 and f(7, k) % k == 0
