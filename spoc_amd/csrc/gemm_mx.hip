@@ -5,12 +5,20 @@
 // block: lane l brings row l % 16, and the scale of block l / 16.  Of a 4-bit operand its 16 bytes are that block too; of an 8-bit one
 // its first 16 bytes are values 16 (l / 16) and on, its second 64 + 16 (l / 16) and on.  The weights are the first operand, so a lane's
 // results are columns of one row of C, four in a row.
-// Sums of 4-bit products come out exact (until float32 rounds them); 8-bit ones are added on a grid of about 2^-14 of the largest product
-// of the 128 (measured: up to 4.7e-5 of the sum of the magnitudes), so C is 16-bit there.
+// v_mfma_scale_f32_32x32x64_f8f6f4 is the same for 32 rows and 64 of k, lane l bringing row l % 32 and the scale of block l / 32; of an 8-bit
+// operand its first 16 bytes are values 16 (l / 32) and on, its second 32 + 16 (l / 32) and on.
 //
-// Streams of the instruction alone, random codes: 8-bit with 4-bit rows 4390 TFLOP/s, 4-bit ones 5830, on 32x32x64 6600 (16x16x128 is bound
-// by its issue there); the clock falls with the data, zeros reach 9600.  A copy reaches 5.4 TB/s.  Of few rows the weights' bytes are the
-// bound, of many the matrix unit: gemm_mx_stream_kernel and gemm_mx_tile_kernel.
+// How the instruction adds (measured): products of eight neighbours in k meet on a grid of 2^-13 of what the largest exponents among them
+// would give, and what is below is dropped; the eights of a block are then added exactly, and the blocks and C in float32.  4-bit products fit
+// the grid, so a block's sum is exact.  8-bit ones do not (2^-9 times 1/2 beside 448 times 6), so 8-bit codes are taken in two parts, of
+// magnitudes from 2 on and of those below (split), each with an instruction of its own: the products of either part fit the grid, 2^-3 beside up
+// to 2^11.4 and 2^-10 beside up to 2^3.5, and sums are float32 sums of exact products.  In one pass, twice as fast, C was up to 4.7e-5 of the sum
+// of the magnitudes off, a half and more of it where large products cancel.
+//
+// Streams of the instruction alone, random codes: 8-bit with 4-bit rows 4300 TFLOP/s, in two parts with the parting of their codes between
+// the instructions 2290 (the codes brought to bf16 and 16-bit instructions: 2050), 4-bit ones 5830, on 32x32x64 6600 (16x16x128 is bound by its
+// issue there); the clock falls with the data, zeros reach 9600 in 4 bits.  Of few rows the weights' bytes are the bound, of many the matrix
+// unit: gemm_mx_stream_kernel and gemm_mx_tile_kernel.
 #include <type_traits>
 #include <utility>
 
@@ -32,11 +40,23 @@ template <bool Fp8, int Step> __device__ __forceinline__ f32x4_t mfma_mx(u32x4_t
 }
 
 typedef __attribute__((ext_vector_type(16))) float f32x16;
-// 32 rows of each operand and 64 of k, two blocks: lane l brings row l % 32 of the block in place l / 32, and its scale.
-template <int Scale> __device__ __forceinline__ f32x16 mfma_mx32(u32x4 b, u32x4 a, f32x16 c, int b_scales, int a_scales) {
-  const i32x8 wide_b = {static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3]), 0, 0, 0, 0};
-  const i32x8 wide_a = {static_cast<int>(a[0]), static_cast<int>(a[1]), static_cast<int>(a[2]), static_cast<int>(a[3]), 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide_b, wide_a, c, kFormatE2M1, kFormatE2M1, Scale, b_scales, Scale, a_scales);
+template <bool Fp8, int Scale> __device__ __forceinline__ f32x16 mfma_mx32(u32x4 b, i32x8 a, f32x16 c, int b_scales, int a_scales) {
+  const i32x8 wide = {static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3]), 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide, a, c, kFormatE2M1, Fp8 ? kFormatE4M3 : kFormatE2M1, Scale, b_scales, Scale,
+                                                         a_scales);
+}
+
+__device__ __forceinline__ i32x8 join(u32x4 low, u32x4 high) {
+  return i32x8{static_cast<int>(low[0]), static_cast<int>(low[1]), static_cast<int>(low[2]), static_cast<int>(low[3]),
+               static_cast<int>(high[0]), static_cast<int>(high[1]), static_cast<int>(high[2]), static_cast<int>(high[3])};
+}
+// Four of a lane's e4m3 codes in two parts, zeros in the place of what is in the other: a magnitude from 2 on has the code's bit 6 set.
+__device__ __forceinline__ void split(i32x8 &codes, i32x8 &large, int word) {
+  typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+  const uint32_t c = static_cast<uint32_t>(codes[word]);
+  const u16x2 whole_bytes = __builtin_bit_cast(u16x2, c >> 6 & 0x01010101u) * u16x2{255, 255};
+  large[word] = static_cast<int>(c & __builtin_bit_cast(uint32_t, whole_bytes));
+  codes[word] = static_cast<int>(c & ~__builtin_bit_cast(uint32_t, whole_bytes));
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------
@@ -60,11 +80,11 @@ template <class T> __device__ __forceinline__ void store_four(T *p, int64_t coun
 // Small tiles of C, both operands brought to LDS by transfers, kRing - 1 stages ahead.  Eight waves: WM by WN of them share out the tile of
 // C, each MT by NT row and column tiles of 16, and Q of them in each place take every Q-th step of 128 k; a stage is Q steps.  Their sums
 // are added in order at the end.
-// Few rows are bound by the weights' bytes, and those by how many are under way: rings of 120 to 155 KB, a workgroup to a compute unit, so that
+// Few rows are bound by the weights' bytes, and those by how many are under way: rings of 102 to 153 KiB, a workgroup to a compute unit, so that
 // even one row of C keeps every one of them loading.  K is split over a workgroup's waves, not over workgroups: their sums
-// meet in LDS, with no second launch and no memory for them.  (Rows of B straight to registers: 64 x 8192 x 8192 26 us, so 13.2.)  8-bit
-// rows: 1 x 8192 x 8192 8.4 us, 4.2 TB/s; 61 x 11007 x 4095 11.7, its 172 tiles of 64 x 64 being less than the compute units; 512 x 4096 x
-// 4096 21.7, 1024 x 4096 x 4096 23.3, 1470 TFLOP/s, bound by a start and an end that no other workgroup covers (6 us).
+// meet in LDS, with no second launch and no memory for them.  8-bit rows: 1 x 8192 x 8192 9.0 us, 4.0 TB/s; 61 x 11007 x 4095 12.8, its 172
+// tiles of 64 x 64 being less than the compute units; 512 x 4096 x 4096 23.5, 1024 x 4096 x 4096 30.3, 1130 TFLOP/s, bound by a start and an
+// end that no other workgroup covers (6 us) and by the matrix unit, busy for half of the time.
 template <bool Fp8, class T, int MT, int NT, int WM, int WN, int kRing>
 __global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__restrict__ a, const uint8_t *__restrict__ a_scales,
                                                              const uint8_t *__restrict__ b, const uint8_t *__restrict__ b_scales,
@@ -139,11 +159,11 @@ __global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__re
     // What the next stages have in flight may stay there (of a wave with scales to bring, one transfer less).
     __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((kRing - 2) * kMoves));
     barrier_no_fence();
-    // All fragments are asked for before the first MFMA. Where a wave has several MFMAs of both operands, the transfers go one by one
-    // between them, as all at once keep the waves waiting to issue them (8000 x 500 x 16000 in 4 bits 55.2 us, so 53.0; 1024 x 4096 x
-    // 4096 in 8 bits 23.8, so 22.8); elsewhere there is too little to hide them behind, and they go first (64 x 32 tiles, with one
-    // fragment of B to a wave: 64 x 8192 x 8192 14.0 us, between the MFMAs 14.8).
-    constexpr bool kBetween = MT > 1 && NT > 1;
+    // All fragments are asked for before the first MFMA. Where a wave has four MFMA tiles and more, the transfers go one by one between the MFMAs,
+    // as all at once keep the waves waiting to issue them (61 x 11007 x 4095 in 8 bits 13.9 us, so 12.9; 512 x 4096 x 4096 25.5, so 23.5; 16 x
+    // 11008 x 4096 on 32 x 64 tiles 9.3, so 9.1); below there is too little to hide them behind, and they go first (16 x 4096 x 11008 on 16 x
+    // 32 tiles 9.5 us, between the MFMAs 10.0; 1 x 8192 x 8192 on 32 x 32 tiles in 4 bits 9.1 and 9.3).
+    constexpr bool kBetween = MT * NT >= 4;
     if constexpr (!kBetween) {
 #pragma unroll
       for (int t = 0; t <= kMoves; ++t) move(lds_ring<80 + (I + kRing - 1) % kRing, kBytes>, s + kRing - 1, t);
@@ -162,21 +182,33 @@ __global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__re
       sa[i] = static_cast<uint8_t>(from[sa_at + i * 64]);
     }
     if constexpr (kBetween) __builtin_amdgcn_sched_barrier(0);
+    // A fragment's parts: the large one's MFMAs and then the small one's.  The next fragment is parted between them.
+    constexpr int kParts = Fp8 ? 2 : 1, kMfmas = kParts * NT, kAll = MT * kMfmas;
+    i32x8 af[2], large[2];
+    auto take = [&](int i) { af[i & 1] = join(lo[i], Fp8 ? hi[Fp8 ? i : 0] : u32x4{0u, 0u, 0u, 0u}); };
+    take(0);
+    if constexpr (Fp8) {
+#pragma unroll
+      for (int w = 0; w < 8; ++w) split(af[0], large[0], w);
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const u32x4 high = Fp8 ? hi[Fp8 ? i : 0] : u32x4{0u, 0u, 0u, 0u};
-      const i32x8 af = {static_cast<int>(lo[i][0]), static_cast<int>(lo[i][1]), static_cast<int>(lo[i][2]), static_cast<int>(lo[i][3]),
-                        static_cast<int>(high[0]), static_cast<int>(high[1]), static_cast<int>(high[2]), static_cast<int>(high[3])};
+      if (i + 1 < MT) take(i + 1);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        // transfers (kMoves + 1) n / (MT NT) of the n-th MFMA and on
-        const int n = i * NT + j;
+      for (int t = 0; t < kMfmas; ++t) {
+        const int j = t % NT, n = i * kMfmas + t;
+        // transfers (kMoves + 1) n / kAll of the n-th MFMA and on
         if constexpr (kBetween) {
 #pragma unroll
-          for (int t = (kMoves + 1) * n / (MT * NT); t < (kMoves + 1) * (n + 1) / (MT * NT); ++t)
-            move(lds_ring<80 + (I + kRing - 1) % kRing, kBytes>, s + kRing - 1, t);
+          for (int u = (kMoves + 1) * n / kAll; u < (kMoves + 1) * (n + 1) / kAll; ++u)
+            move(lds_ring<80 + (I + kRing - 1) % kRing, kBytes>, s + kRing - 1, u);
         }
-        acc[i][j] = mfma_mx<Fp8, 0>(bf[j], af, acc[i][j], sb[j], sa[i]);
+        if constexpr (Fp8) {
+#pragma unroll
+          for (int w = 8 * t / kMfmas; w < 8 * (t + 1) / kMfmas; ++w)
+            if (i + 1 < MT) split(af[(i + 1) & 1], large[(i + 1) & 1], w);
+        }
+        acc[i][j] = mfma_mx<Fp8, 0>(bf[j], Fp8 && t < NT ? large[i & 1] : af[i & 1], acc[i][j], sb[j], sa[i]);
         if constexpr (kBetween) __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -236,18 +268,21 @@ __global__ __launch_bounds__(512) void gemm_mx_stream_kernel(const uint8_t *__re
 
 // ---- 256 x 256 tiles -----------------------------------------------------------------------------------------------------------------
 
-// Eight waves of 128 x 64 of C each, in registers.  Both operands go through LDS, by transfers that are issued a stage or two ahead and one at
-// a time between the MFMAs; a stage's last eight MFMAs come after the barrier for the next, whose first fragments are read under them.
-// 8-bit rows take stages of 128 k, three in LDS, on 16x16x128; 4-bit ones 256 k, two, on 32x32x64 (half the instructions).
-// Measured: 4095 x 11008 x 4096 in 8 bits 144 us, 2560 TFLOP/s, the matrix unit busy for 71 % of the time; 8192^3 in 4 bits, C float32,
-// 270 us, 4070 TFLOP/s, busy for 58 %.  What bounds it: with empty transfers (zeros) the same code takes 113 and 173 us, on real data that
-// lies in LDS 120 and 219 (the clock falls), all of it coming from the L2 137 and 249.  Not taken: a workgroup that goes on to its next
+// Eight waves, each with its part of C in registers.  Both operands go through LDS, by transfers that are issued a stage or two ahead and one
+// at a time between the MFMAs; before a stage's last step comes the barrier for the next stage, whose first fragments are read in that step.
+// 8-bit rows take stages of 128 k, three in LDS, and 64 x 128 of C to a wave: each of A's codes is parted by two waves (of 128 x 64 by
+// four), five instructions for four codes.  4-bit ones take 256 k, two, and 128 x 64.
+// Measured: 4095 x 11008 x 4096 in 8 bits 235 us, 1570 TFLOP/s, the matrix unit busy for 84 % of the time at 2.0 GHz; 8192^3 in 4 bits, C
+// float32, 270 us, 4070 TFLOP/s, busy for 56 % at 1.85 GHz.  What bounds 8-bit rows: the same on zeros takes 197 us, three turns of 66, where
+// 2.69 turns of 58 are the matrix unit's rate at 2.4 GHz; a turn's start and end are 8 of it, the clock on real data the rest.  4-bit rows: on
+// zeros 173 us, on real data that lies in LDS 219, all of it coming from the L2 249.  Not taken: a workgroup that goes on to its next
 // tile, its first stages moved during the last of this one (8192^3 267 to 330 us: the wait for transfers waits for C's stores, too).
 template <bool Fp8, class T>
 __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__restrict__ a, const uint8_t *__restrict__ a_scales,
                                                            const uint8_t *__restrict__ b, const uint8_t *__restrict__ b_scales,
                                                            const float *__restrict__ bias, int relu, T *__restrict__ c, int64_t c_stride,
                                                            int m, int n, int kp, int tiles_m, int tiles_n, bool past_caches) {
+  static_assert(!Fp8 || sizeof(T) == 2, "C of 8-bit rows is 16-bit");
   constexpr int kStage = Fp8 ? 128 : 256;            // values of k in a stage: 128 bytes of a row of A
   constexpr int kRowB = Fp8 ? 64 : 128;              // bytes of a row of B in a stage
   constexpr int kRing = Fp8 ? 3 : 2;                 // stages in LDS
@@ -255,12 +290,13 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
   constexpr int kPeriod = Fp8 ? 12 : 2;              // stages after which places in LDS and in the span repeat
   constexpr int kBytesA = 256 * 128, kBytesB = 256 * kRowB, kBytesS = 256 * 16;
   constexpr int kMovesA = kBytesA / 1024 / 8, kMovesB = kBytesB / 1024 / 8;   // transfers of a wave in a stage
-  constexpr int kRows = Fp8 ? 16 : 32;               // rows and columns of an MFMA
-  constexpr int kTilesA = 128 / kRows, kTilesB = 64 / kRows;
-  static_assert(kPeriod % kRing == 0 && kPeriod % kPerSpan == 0 && kRing * (kBytesA + kBytesB) + 2 * kBytesS <= 160 * 1024, "ring");
+  constexpr int kWavesN = Fp8 ? 2 : 4, kWavesM = 8 / kWavesN;
+  constexpr int kWaveRows = 256 / kWavesM, kWaveColumns = 256 / kWavesN;
+  constexpr int kTilesA = kWaveRows / 32, kTilesB = kWaveColumns / 32;
+  static_assert(kPeriod % kRing == 0 && kPeriod % kPerSpan == 0 && kRing * (kBytesA + kBytesB) + 2 * kBytesS + 1040 <= 160 * 1024, "ring");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & (kRows - 1), place = lane / kRows;
-  const int wm = wave >> 2, wn = wave & 3;           // 128 rows of C by 64 columns to a wave
+  const int r = lane & 31, place = lane >> 5;
+  const int wm = wave / kWavesN, wn = wave % kWavesN;
   int tm, tn;
   tile_of_block(tiles_m, tiles_n, 1, tm, tn);
   const int m0 = tm * 256, n0 = tn * 256;
@@ -270,21 +306,22 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
   const uint8_t *const a_from = a + static_cast<int64_t>(m0) * pitch_a, *const b_from = b + static_cast<int64_t>(n0) * pitch_b;
   const __amdgpu_buffer_rsrc_t rs = make_rsrc(of_a ? a_scales + static_cast<int64_t>(m0) * pitch_s : b_scales + static_cast<int64_t>(n0) * pitch_s,
                                               static_cast<uint32_t>(of_a ? rows_a : rows_b) * pitch_s);
-  // Where piece q (16 bytes) of a row lies in its row of LDS: at q ^ (row / 2 % 8) in rows of 128 bytes, q ^ place64(row) in rows of 64.  A
-  // ds_read_b128 is served 16 lanes at a time, row quads 0 and 3 of one place with 1 and 2 of the next and the other way round; they
-  // meet no bank twice so, whether they are of one piece or two.  (As lanes come, with pieces 2 p + step: 44 % of LDS cycles were conflicts.)
-  auto place64 = [](int row) { return ((row >> 2 ^ row >> 3) & 1) << 1 | (row >> 3 & 1); };
+  // Where piece q (16 bytes) of a row lies in its row of LDS: at q with its last bits turned by the row's, row / 2 % 8 in rows of 128 bytes, row /
+  // 8 % 4 in rows of 64.  A ds_read_b128 is served 16 lanes at a time, row quads 0, 3, 5 and 6 of eight and then the others; their pieces
+  // meet no bank twice so.  (Of the LDS cycles, which are 15 % of the time in 8 bits and 35 % in 4, 11 and 20 % are conflicts: of the scales' reads,
+  // 2 and 8 clocks each, and of C on its way out.  The counter grows with k by just the former.)
+  auto turn = [](int row, int row_bytes) { return row_bytes == 64 ? row >> 3 & 3 : row >> 1 & 7; };
   uint32_t off_a[kMovesA], off_b[kMovesB];
 #pragma unroll
   for (int i = 0; i < kMovesA; ++i) {
     const int row = (wave + 8 * i) * 8 + (lane >> 3);
-    off_a[i] = static_cast<uint32_t>(row) * pitch_a + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+    off_a[i] = static_cast<uint32_t>(row) * pitch_a + (((lane & 7) ^ turn(row, 128)) << 4);
   }
 #pragma unroll
   for (int i = 0; i < kMovesB; ++i) {
     constexpr int chunks = kRowB / 16;
     const int row = (wave + 8 * i) * (64 / chunks) + lane / chunks;
-    off_b[i] = static_cast<uint32_t>(row) * pitch_b + (((lane % chunks) ^ (Fp8 ? place64(row) : (row >> 1) & 7)) << 4);
+    off_b[i] = static_cast<uint32_t>(row) * pitch_b + (((lane % chunks) ^ turn(row, kRowB)) << 4);
   }
   const uint32_t off_s = static_cast<uint32_t>((wave & 3) * 64 + lane) * pitch_s;
   const int stages = kp / kStage, last_span = (stages - 1) / kPerSpan;
@@ -300,31 +337,30 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
   char *const ls = lds_ring<68, 2 * kBytesS + 16>;
   auto move_scales = [&](int span) { dma16(rs, off_s, min(min(span, last_span) * 16, pitch_s - 16), ls + wave * 1024); };
 
-  using Acc = std::conditional_t<Fp8, f32x4_t, f32x16>;
-  Acc acc[kTilesA][kTilesB];
+  f32x16 acc[kTilesA][kTilesB];
 #pragma unroll
   for (int i = 0; i < kTilesA; ++i)
 #pragma unroll
     for (int j = 0; j < kTilesB; ++j)
 #pragma unroll
-      for (int e = 0; e < kRows * kRows / 64; ++e) acc[i][j][e] = 0.f;
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
   // Scales: a lane reads the bytes of a row for 256 of k (8-bit; two stages) or 512 (4-bit; two stages too) and keeps those that its place
   // needs, in the order of the steps.
   using Raw = std::conditional_t<Fp8, u32x2_t, u32x4>;
   constexpr int kWords = Fp8 ? 1 : 2;
   int sa[kTilesA][kWords], sb[kTilesB][kWords];
-  Raw raw_a[Fp8 ? 2 : 4], raw_b[kTilesB];
-  const uint32_t pick = Fp8 ? static_cast<uint32_t>(place | (4 + place) << 8) | 0x0C0C0000u : 0x06040200u + place * 0x01010101u;
+  Raw raw_a[kTilesA], raw_b[kTilesB];
+  const uint32_t pick = 0x06040200u + place * 0x01010101u;
   auto keep = [&](int (&to)[kWords], const Raw &d) {
     to[0] = static_cast<int>(__builtin_amdgcn_perm(d[1], d[0], pick));
     if constexpr (!Fp8) to[1] = static_cast<int>(__builtin_amdgcn_perm(d[3], d[2], pick));
   };
-  // A lane's 16 bytes of the first row tile; what follows of the row is some bits away: the second half of 8-bit codes (4 pieces on), the
-  // steps of 4-bit ones (2 pieces each).
-  int a_at = (wm * 128 + r) * 128 + ((place ^ (r >> 1 & 7)) << 4);
-  int b_at = (wn * 64 + r) * kRowB + ((place ^ (Fp8 ? place64(r) : r >> 1 & 7)) << 4);
-  int sa_at = (wm * 128 + r) * 16, sb_at = kBytesS + (wn * 64 + r) * 16;
+  // A lane's 16 bytes of the first row tile; what follows of the row is some bits away: the second half of 8-bit codes (2 pieces on) and
+  // their next step (4), the steps of 4-bit ones (2 each).
+  int a_at = (wm * kWaveRows + r) * 128 + ((place ^ turn(r, 128)) << 4);
+  int b_at = (wn * kWaveColumns + r) * kRowB + ((place ^ turn(r, kRowB)) << 4);
+  int sa_at = (wm * kWaveRows + r) * 16, sb_at = kBytesS + (wn * kWaveColumns + r) * 16;
   auto read = [](const char *p) { return *reinterpret_cast<const u32x4 *>(p); };
   // Where in a row's 16 bytes those of stage s begin.  Of a span of 8 bytes they are the second half (which 4-bit rows, that have no second
   // stage then, read first).
@@ -337,74 +373,74 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
       return static_cast<u32x4>(*reinterpret_cast<const u32x4_by8 *>(ls + at));
     }
   };
-  auto read_raw_a = [&](int i, int at) { raw_a[i % (Fp8 ? 2 : 4)] = read_raw(sa_at + at + i * kRows * 16); };
-  auto read_raw_b = [&](int j, int at) { raw_b[j] = read_raw(sb_at + at + j * kRows * 16); };
+  auto read_raw_a = [&](int i, int at) { raw_a[i] = read_raw(sa_at + at + i * 512); };
+  auto read_raw_b = [&](int j, int at) { raw_b[j] = read_raw(sb_at + at + j * 512); };
 
-  // Fragments.  8-bit: three row tiles of A in turn, B of this step and the next; 4-bit: both operands of this step and the next.  (A
-  // register more than there are, and its traffic waits for the transfers behind it in order.)
-  u32x4 alo[Fp8 ? 3 : 2 * kTilesA], ahi[Fp8 ? 3 : 1], bf[2][kTilesB];
+  // Fragments.  B: of this step and the next.  A, 4-bit: the same; 8-bit: one after the other, its large part, and in three turns what is read,
+  // what is being parted, and the small part that is left of it.  (A register more than there are, and its traffic waits for the transfers
+  // behind it in order.)
+  u32x4 bf[2][kTilesB], alo[Fp8 ? 1 : 2 * kTilesA];
+  i32x8 af[Fp8 ? 3 : 1], large[Fp8 ? 2 : 1];
 
-  // A stage's MFMAs, and before each what is to be read or moved meanwhile.  During the last eight the next stage's first fragments are
+  // A stage's MFMAs, and before each what is to be read or moved meanwhile.  During the last step the next stage's first fragments are
   // read, after the barrier that says that it has landed and that this one has been read, and this one's place is filled again.
   auto stage = [&](auto ic, int s) __attribute__((always_inline)) {
     constexpr int I = decltype(ic)::value, ring = I % kRing, next = (I + 1) % kRing;
     constexpr bool first_of_two = I % 2 == 0;
     const char *const la = lds_ring<60 + ring, kBytesA>;
-    [[maybe_unused]] const char *const lb = lds_ring<64 + ring, kBytesB>;
+    const char *const lb = lds_ring<64 + ring, kBytesB>;
     const char *const la_next = lds_ring<60 + next, kBytesA>, *const lb_next = lds_ring<64 + next, kBytesB>;
-    [[maybe_unused]] const int raw_now = raw_at(s), raw_next = raw_at(s + 1);
+    [[maybe_unused]] const int raw_next = raw_at(s + 1);
     auto landed = [&]() __attribute__((always_inline)) {
       // in flight may be what was asked for after the next stage: the stages behind it
       __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((kRing - 2) * (kMovesA + kMovesB)));
       barrier_no_fence();
     };
-    // transfer t of the stage that takes the place of the one `ago` stages ago
-    auto refill = [&]<int Ago>(std::integral_constant<int, Ago>, int t) __attribute__((always_inline)) {
-      constexpr int to = (I + kRing - Ago) % kRing;
-      if (t < kMovesA) move_a(lds_ring<60 + to, kBytesA>, t, s - Ago + kRing);
-      else if (t < kMovesA + kMovesB) move_b(lds_ring<64 + to, kBytesB>, t - kMovesA, s - Ago + kRing);
+    // transfer t of the stage that takes the place of this one
+    auto refill = [&](int t) __attribute__((always_inline)) {
+      if (t < kMovesA) move_a(lds_ring<60 + ring, kBytesA>, t, s + kRing);
+      else if (t < kMovesA + kMovesB) move_b(lds_ring<64 + ring, kBytesB>, t - kMovesA, s + kRing);
     };
-    constexpr std::integral_constant<int, 0> this_one;
-    [[maybe_unused]] constexpr std::integral_constant<int, 1> one_before;
     asm volatile("" : "+v"(a_at), "+v"(b_at), "+v"(sa_at), "+v"(sb_at));   // (not one register for each place in LDS across the loop)
+    if constexpr (first_of_two) {
+#pragma unroll
+      for (int j = 0; j < kTilesB; ++j) keep(sb[j], raw_b[j]);
+#pragma unroll
+      for (int i = 0; i < kTilesA; ++i) keep(sa[i], raw_a[i]);
+    }
     if constexpr (Fp8) {
-      constexpr int cur = I & 1;
-      if constexpr (first_of_two) {
+      [&]<int... Steps>(std::integer_sequence<int, Steps...>) {
+        (
+            [&] {
+              constexpr int Step = Steps;
+              const char *const from_a = Step == 0 ? la : la_next, *const from_b = Step == 0 ? lb : lb_next;   // of the next step
+              if (Step == 1) landed();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) keep(sb[j], raw_b[j]);
-      }
+              for (int t = 0; t < 16; ++t) {
+                const int i = t >> 3, part = t >> 2 & 1, j = part == 0 ? t & 3 : 3 - (t & 3), f = 4 * I + 2 * Step + i;   // f: the fragment of A
+                const int at = a_at ^ (Step ^ 1) << 6;
+                if ((t & 7) < 2) {   // the fragment after the next, half by half
+                  const u32x4 half = read(from_a + (at ^ (t & 1) << 5) + i * 4096);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i == 6) landed();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const char *const from = i < 6 ? la + a_at + (i + 2) * 2048 : la_next + a_at + (i - 6) * 2048;
-          if (j == 0) alo[(8 * I + i + 2) % 3] = read(from);
-          if (j == 1) ahi[(8 * I + i + 2) % 3] = read(i < 6 ? la + (a_at ^ 64) + (i + 2) * 2048 : la_next + (a_at ^ 64) + (i - 6) * 2048);
-          if (first_of_two && j == 0) keep(sa[i], raw_a[i & 1]);
-          if (first_of_two && j == 2 && i < 6) read_raw_a(i + 2, raw_now);
-          if (i == 6) bf[cur ^ 1][j] = read(lb_next + b_at + j * 16 * kRowB);
-          // one transfer at a time: all of a workgroup's at once keep the path to LDS busy for 768 clocks, and the waves wait to issue them
-          if (i == 7 && j % 2 == 1) refill(this_one, j / 2);
-          if (i < 4 && j == 3) refill(one_before, i + 2);
-          // (all of the span's have been read before this stage's barrier; the next ones have landed at the next)
-          if (i == 7 && j == 0 && I % kPerSpan == 2) move_scales(s / kPerSpan + 1);
-          if (!first_of_two && i == 7) read_raw_b(j, raw_next);
-          if (!first_of_two && i == 7 && j >= 2) read_raw_a(j - 2, raw_next);
-          const u32x4 lo = alo[(8 * I + i) % 3], hi = ahi[(8 * I + i) % 3];
-          const i32x8 af = {static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
-                            static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
-          acc[i][j] = mfma_mx<true, I % 2>(bf[cur][j], af, acc[i][j], sb[j][0], sa[i][0]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
+                  for (int w = 0; w < 4; ++w) af[(f + 2) % 3][4 * (t & 1) + w] = static_cast<int>(half[w]);
+                }
+                if (t >= 2 && t < 6) bf[Step ^ 1][t - 2] = read(from_b + (b_at ^ (Step ^ 1) << 5) + (t - 2) * 32 * kRowB);
+                // (all of the span's scales have been read before this stage's barrier; the next ones have landed at the next)
+                if (Step == 1 && t == 1 && I % kPerSpan == 2) move_scales(s / kPerSpan + 1);
+                // one transfer at a time: all of a workgroup's at once keep the path to LDS busy for 768 clocks, and the waves wait to issue them
+                if (Step == 1 && t >= 2 && t % 2 == 0) refill(t / 2 - 1);
+                if (Step == 1 && !first_of_two && t >= 3 && t % 2 == 1) {
+                  if (t < 11) read_raw_b((t - 3) / 2, raw_next);
+                  else if (t < 15) read_raw_a((t - 11) / 2, raw_next);
+                }
+                split(af[(f + 1) % 3], large[(f + 1) % 2], t & 7);
+                acc[i][j] = mfma_mx32<true, I % 2 * 2 + Step>(bf[Step][j], part == 0 ? large[f % 2] : af[f % 3], acc[i][j], sb[j][0], sa[i][0]);
+                __builtin_amdgcn_sched_barrier(0);
+              }
+            }(),
+            ...);
+      }(std::make_integer_sequence<int, 2>{});
     } else {
-      if constexpr (first_of_two) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) keep(sb[j], raw_b[j]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) keep(sa[i], raw_a[i]);
-      }
       [&]<int... Steps>(std::integer_sequence<int, Steps...>) {
         (
             [&] {
@@ -417,13 +453,13 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
                 const int i = t >> 1, j = i & 1 ? 1 - (t & 1) : t & 1;
                 if (t == 0 || (t >= 3 && t < 6)) alo[(cur ^ 1) * 4 + (t == 0 ? 0 : t - 2)] = read(from_a + (a_at ^ bits) + (t == 0 ? 0 : t - 2) * 4096);
                 if (t == 1 || t == 2) bf[cur ^ 1][t - 1] = read(from_b + (b_at ^ bits) + (t - 1) * 4096);
-                if (Step == 3) refill(this_one, t);
+                if (Step == 3) refill(t);
                 if (Step == 3 && t == 7 && first_of_two) move_scales(s / kPerSpan + 1);
                 if (Step == 3 && !first_of_two && t >= 2) {
                   if (t < 4) read_raw_b(t - 2, raw_next);
                   else read_raw_a(t - 4, raw_next);
                 }
-                acc[i][j] = mfma_mx32<number % 4>(bf[cur][j], alo[cur * 4 + i], acc[i][j], sb[j][number / 4], sa[i][number / 4]);
+                acc[i][j] = mfma_mx32<false, number % 4>(bf[cur][j], join(alo[cur * 4 + i], u32x4{0u, 0u, 0u, 0u}), acc[i][j], sb[j][number / 4], sa[i][number / 4]);
                 __builtin_amdgcn_sched_barrier(0);
               }
             }(),
@@ -432,41 +468,50 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
     }
   };
 
-  // The bias of a lane's columns, before the first transfer: loads come in order, and at the end they would be waited for.
-  f32x4_t add[kTilesB][kRows * kRows / 256];
+  // The bias comes before the first transfer: loads come in order, and at the end it would be waited for.  4-bit rows have registers for that of
+  // a lane's columns; 8-bit ones put the tile's 256 values into LDS, zeros where there are none.
+  [[maybe_unused]] f32x4_t add[Fp8 ? 1 : kTilesB][4];
+  if constexpr (Fp8) {
+    if (of_a)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(bias ? bias + n0 : nullptr, bias ? static_cast<uint32_t>(rows_b) * 4 : 0u),
+                                               (LDS_PTR void *)(lds_ring<69, 1024> + wave * 256), 4, threadIdx.x * 4, 0, 0, 0);
+  } else {
 #pragma unroll
-  for (int j = 0; j < kTilesB; ++j)
+    for (int j = 0; j < kTilesB; ++j)
 #pragma unroll
-    for (int q = 0; q < kRows * kRows / 256; ++q)
+      for (int q = 0; q < 4; ++q)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) add[j][q][e] = bias ? bias[min(n0 + wn * 64 + j * kRows + 8 * q + 4 * place + e, n - 1)] : 0.f;
+        for (int e = 0; e < 4; ++e) add[j][q][e] = bias ? bias[min(n0 + wn * kWaveColumns + j * 32 + 8 * q + 4 * place + e, n - 1)] : 0.f;
+  }
   move_scales(0);
-  // (8-bit: of the last of the three only what the stage before the first would have moved by now)
-  constexpr int kFirstMoves = Fp8 ? 2 : kMovesA + kMovesB;
   [&]<int... Ss>(std::integer_sequence<int, Ss...>) {
     (
         [&] {
-          constexpr int count = Ss == kRing - 1 ? kFirstMoves : kMovesA + kMovesB;
 #pragma unroll
-          for (int t = 0; t < count; ++t) {
+          for (int t = 0; t < kMovesA + kMovesB; ++t) {
             if (t < kMovesA) move_a(lds_ring<60 + Ss, kBytesA>, t, Ss);
             else move_b(lds_ring<64 + Ss, kBytesB>, t - kMovesA, Ss);
           }
         }(),
         ...);
   }(std::make_integer_sequence<int, kRing>{});
-  __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((kRing - 2) * (kMovesA + kMovesB) + kFirstMoves));
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((kRing - 1) * (kMovesA + kMovesB)));
   barrier_no_fence();
 #pragma unroll
   for (int j = 0; j < kTilesB; ++j) {
-    bf[0][j] = read(lds_ring<64, kBytesB> + b_at + j * kRows * kRowB);
+    bf[0][j] = read(lds_ring<64, kBytesB> + b_at + j * 32 * kRowB);
     read_raw_b(j, raw_at(0));
   }
 #pragma unroll
-  for (int i = 0; i < (Fp8 ? 2 : 4); ++i) {
-    alo[i] = read(lds_ring<60, kBytesA> + a_at + i * kRows * 128);
-    if constexpr (Fp8) ahi[i] = read(lds_ring<60, kBytesA> + (a_at ^ 64) + i * kRows * 128);
+  for (int i = 0; i < kTilesA; ++i) {
+    const u32x4 first = read(lds_ring<60, kBytesA> + a_at + i * 4096);
+    if constexpr (Fp8) af[i] = join(first, read(lds_ring<60, kBytesA> + (a_at ^ 32) + i * 4096));
+    else alo[i] = first;
     read_raw_a(i, raw_at(0));
+  }
+  if constexpr (Fp8) {
+#pragma unroll
+    for (int w = 0; w < 8; ++w) split(af[0], large[0], w);
   }
   __builtin_amdgcn_sched_barrier(0);
   const int full = stages - stages % kPeriod;
@@ -479,37 +524,41 @@ __global__ __launch_bounds__(512) void gemm_mx_tile_kernel(const uint8_t *__rest
   }(std::make_integer_sequence<int, kPeriod - 1>{});
   __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));   // the last, empty transfers, before the LDS is released
 
-  // C goes to memory by whole rows of the tile, put together in LDS in turns, 32 KiB of the four waves that share these rows at a time:
-  // piece q (16 bytes) of row r at q ^ (r % 16).  A lane has row r of a row tile, and four columns in a row for every four registers.
-  constexpr int kRowC = 256 * sizeof(T), kTurnRows = 32768 / kRowC, kTurns = 128 / kTurnRows, kPiece = 16 / sizeof(T);
-  char *const lc = wm == 0 ? lds_ring<60, kBytesA> : lds_ring<61, kBytesA>;
+  // C goes to memory by whole rows of the tile, put together in LDS in turns, 64 KiB of the tile at a time, an equal share of it for the waves
+  // that share their rows: piece q (16 bytes) of row r at q ^ (r % 16).  A lane has row r of a row tile, and four columns in a row for every
+  // four registers.
+  constexpr int kRowC = 256 * sizeof(T), kShare = 65536 / kWavesM, kTurnRows = kShare / kRowC, kTurns = kWaveRows / kTurnRows, kPiece = 16 / sizeof(T);
+  static_assert(kTurnRows % 32 == 0 && kWaveRows % kTurnRows == 0, "whole row tiles");
+  char *const lc = (wm < kWavesM / 2 ? lds_ring<60, kBytesA> : lds_ring<61, kBytesA>) + wm % (kWavesM / 2) * kShare;
 #pragma unroll
-  for (int turn = 0; turn < kTurns; ++turn) {
+  for (int turn_of = 0; turn_of < kTurns; ++turn_of) {
     barrier_no_fence();   // every wave has left the K loop, or has read the turn before
 #pragma unroll
-    for (int u = 0; u < kTurnRows / kRows; ++u) {
-      const int i = turn * (kTurnRows / kRows) + u, row = u * kRows + r;
+    for (int u = 0; u < kTurnRows / 32; ++u) {
+      const int i = turn_of * (kTurnRows / 32) + u, row = u * 32 + r;
 #pragma unroll
       for (int j = 0; j < kTilesB; ++j)
 #pragma unroll
-        for (int q = 0; q < kRows * kRows / 256; ++q) {
+        for (int q = 0; q < 4; ++q) {
+          const int column = wn * kWaveColumns + j * 32 + 8 * q + 4 * place, at = column * static_cast<int>(sizeof(T));
           f32x4_t v;
+          if constexpr (Fp8) v = *reinterpret_cast<const f32x4_t *>(lds_ring<69, 1024> + column * 4);
+          else v = add[j][q];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            v[e] = acc[i][j][4 * q + e] + add[j][q][e];
+            v[e] += acc[i][j][4 * q + e];
             if (relu) v[e] = v[e] < 0.f ? 0.f : v[e];
           }
-          const int at = (wn * 64 + j * kRows + 8 * q + 4 * place) * static_cast<int>(sizeof(T));
           store_four(reinterpret_cast<T *>(lc + row * kRowC + (at ^ (row & 15) << 4)), 4, v);
         }
     }
     wait_lds();
     barrier_no_fence();
 #pragma unroll
-    for (int u = 0; u < kTurnRows * kRowC / 4096; ++u) {
-      const int row = wn * (kTurnRows / 4) + u * (1024 / kRowC) + lane * 16 / kRowC, at = lane * 16 % kRowC;
+    for (int u = 0; u < kShare / 1024 / kWavesN; ++u) {
+      const int row = wn * (kTurnRows / kWavesN) + u * (1024 / kRowC) + lane * 16 / kRowC, at = lane * 16 % kRowC;
       const u32x4 v = read(lc + row * kRowC + (at ^ (row & 15) << 4));
-      const int to_row = m0 + wm * 128 + turn * kTurnRows + row, col = n0 + lane % (kRowC / 16) * kPiece;
+      const int to_row = m0 + wm * kWaveRows + turn_of * kTurnRows + row, col = n0 + lane % (kRowC / 16) * kPiece;
       if (to_row >= m || col >= n) continue;
       T *const to = c + to_row * c_stride + col;
       if (col + kPiece <= n) {
@@ -534,14 +583,13 @@ namespace sarek_hip {
 namespace {
 
 // The kernels' tiles of C, and the weights that choose one, about us of a workgroup: `once` for its start and its end, a step for 128 of
-// k (8-bit and 4-bit rows). They rank the tiles and are no times: a workgroup alone on its compute unit takes 0.033 to 1.3 us a step,
-// and lines through those times choose worse (2048 x 4096 x 4096 in 8 bits 44.7 us with 128 x 128 for 41.2 with 256 x 256). Over 26
-// products of 1 to 8000 rows, each timed with every tile, the choice is at most 3 % behind the best (512 x 4096 x 4096 21.2 us for 20.5)
-// and 0.2 % on average. Tiles of 64 x 32 were the best of one of them, by 1.4 % (512 x 1024 x 8192 in 4 bits 11.3 us for 11.4).
+// k (8-bit and 4-bit rows). They rank the tiles and are no times. Over 48 products of 1 to 8000 rows, each timed with every tile, the choice is
+// behind the best by 0.1 % on average in 8 bits and at most 5.5 % (291 x 4798 x 286 9.8 us for 9.3), in 4 bits by 1.5 % and at most 14 % (926 x
+// 123 x 251 4.3 us for 3.8).
 constexpr int kShapeCount = 7;
 struct Shape { int rows, columns; double once, step8, step4; };
-constexpr Shape kShapes[kShapeCount] = {{16, 16, 1.9, 0.056, 0.050}, {16, 32, 2.0, 0.085, 0.080},   {32, 32, 2.0, 0.115, 0.097},  {32, 64, 2.0, 0.168, 0.148},
-                                        {64, 64, 2.9, 0.240, 0.190}, {128, 128, 6.0, 0.460, 0.360}, {256, 256, 7.5, 1.050, 0.650}};
+constexpr Shape kShapes[kShapeCount] = {{16, 16, 1.9, 0.077, 0.050}, {16, 32, 2.0, 0.110, 0.080},   {32, 32, 2.0, 0.144, 0.097},  {32, 64, 2.0, 0.175, 0.148},
+                                        {64, 64, 2.9, 0.248, 0.190}, {128, 128, 6.0, 0.600, 0.360}, {256, 256, 7.5, 2.050, 0.650}};
 
 // The one that the product takes least time on: a workgroup to a compute unit, as many in turn as there are too many.
 bool shape_serves(int shape, int64_t m, int64_t n, int64_t kp) {
@@ -574,7 +622,7 @@ extern "C" int sarek_hip_gemm_mx(const unsigned char *a_codes, const unsigned ch
                 static_cast<long long>(m), static_cast<long long>(n), static_cast<long long>(k));
   if (!known_format(a_format) || !known_type(c_type)) return fail(SAREK_HIP_E_INVALID_ARG, "gemm_mx: unknown format %d or type %d", a_format, c_type);
   if (a_format == SAREK_HIP_MX_FP8 && c_type == SAREK_HIP_TYPE_F32)
-    return fail(SAREK_HIP_E_UNSUPPORTED, "gemm_mx: products of 8-bit rows are not exact to float32's last bits: C is bf16 or fp16");
+    return fail(SAREK_HIP_E_UNSUPPORTED, "gemm_mx: C of 8-bit rows is bf16 or fp16");
   if (c_stride < n) return fail(SAREK_HIP_E_INVALID_ARG, "gemm_mx: rows of C are %lld values apart, less than n = %lld", static_cast<long long>(c_stride), static_cast<long long>(n));
   if (m >= int64_t{1} << 20 || n >= int64_t{1} << 24 || k > int64_t{1} << 23)
     return fail(SAREK_HIP_E_UNSUPPORTED, "gemm_mx: m is below 2^20, n below 2^24, k at most 2^23");
@@ -596,18 +644,25 @@ extern "C" int sarek_hip_gemm_mx(const unsigned char *a_codes, const unsigned ch
     };
     const bool whole_lines = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(c_stride) * sizeof(T)) & 127) == 0;
     const bool past_caches = whole_lines && m * n * static_cast<int64_t>(sizeof(T)) >= tunable("gemm_mx.past_caches_mib", 200) << 20;
-    const auto small = [&]<int MT, int NT, int WM, int WN, int Ring8, int Ring4>(std::integer_sequence<int, MT, NT, WM, WN, Ring8, Ring4>) {
-      return fp8 ? run(gemm_mx_stream_kernel<true, T, MT, NT, WM, WN, Ring8>, 16 * MT * WM, 16 * NT * WN)
-                 : run(gemm_mx_stream_kernel<false, T, MT, NT, WM, WN, Ring4>, 16 * MT * WM, 16 * NT * WN);
+    // (row tiles, column tiles of a wave; waves below and beside each other; stages in LDS.)  8-bit rows: waves below each other, so that
+    // every code is parted by one of them.
+    using std::integer_sequence;
+    const auto small = [&]<int... P8, int... P4>(integer_sequence<int, P8...>, integer_sequence<int, P4...>) {
+      if constexpr (sizeof(T) == 2)
+        if (fp8) return run(gemm_mx_stream_kernel<true, T, P8...>, kShapes[shape].rows, kShapes[shape].columns);
+      return run(gemm_mx_stream_kernel<false, T, P4...>, kShapes[shape].rows, kShapes[shape].columns);
     };
     switch (shape) {
-      case 0: return small(std::integer_sequence<int, 1, 1, 1, 1, 6, 6>{});
-      case 1: return small(std::integer_sequence<int, 1, 2, 1, 1, 4, 6>{});
-      case 2: return small(std::integer_sequence<int, 2, 1, 1, 2, 6, 6>{});
-      case 3: return small(std::integer_sequence<int, 2, 2, 1, 2, 4, 6>{});
-      case 4: return small(std::integer_sequence<int, 4, 2, 1, 2, 3, 4>{});
-      case 5: return small(std::integer_sequence<int, 4, 4, 2, 2, 3, 4>{});
-      default: return fp8 ? run(gemm_mx_tile_kernel<true, T>, 256, 256, past_caches) : run(gemm_mx_tile_kernel<false, T>, 256, 256, past_caches);
+      case 0: return small(integer_sequence<int, 1, 1, 1, 1, 6>{}, integer_sequence<int, 1, 1, 1, 1, 6>{});
+      case 1: return small(integer_sequence<int, 1, 2, 1, 1, 4>{}, integer_sequence<int, 1, 2, 1, 1, 6>{});
+      case 2: return small(integer_sequence<int, 1, 2, 2, 1, 6>{}, integer_sequence<int, 2, 1, 1, 2, 6>{});
+      case 3: return small(integer_sequence<int, 1, 4, 2, 1, 4>{}, integer_sequence<int, 2, 2, 1, 2, 6>{});
+      case 4: return small(integer_sequence<int, 2, 4, 2, 1, 3>{}, integer_sequence<int, 4, 2, 1, 2, 4>{});
+      case 5: return small(integer_sequence<int, 2, 8, 4, 1, 3>{}, integer_sequence<int, 4, 4, 2, 2, 4>{});
+      default:
+        if constexpr (sizeof(T) == 2)
+          if (fp8) return run(gemm_mx_tile_kernel<true, T>, 256, 256, past_caches);
+        return run(gemm_mx_tile_kernel<false, T>, 256, 256, past_caches);
     }
   });
 }
