@@ -1,5 +1,5 @@
 """Products of microscaled rows on every tile: how their sums are held, the tiles' rings and spans of scales all the way round, and
-results at the ends of the formats, against float64.
+results at the ends of the formats, against float64; and large quantisations against those of a few rows.
 
 Tolerances.  eps = 2^-24.  The products of a block of 32 are exact and add up exactly; blocks (those of 8-bit rows in two parts) are added
 one after the other, each with a rounding of at most a float32's last bit, 2 eps, and so are the sums of a workgroup's eight waves and the
@@ -91,3 +91,75 @@ def test_large_products_that_cancel_leave_the_small_ones(hip, torch_cuda, shape,
     want = hip.mx_dequantize(a, torch.float32).double() @ hip.mx_dequantize(b, torch.float32).double().t()
     with tuned(hip, shape=shape):
         assert torch.equal(hip.gemm_mx(a, b, dtype=dtype), want.float().to(dtype))
+
+
+# kp of 512 (one span of scales) to 4096 (the tiles' rings and periods all round), an odd multiple of 256 (a last span of 8 bytes) among them
+@pytest.mark.parametrize("k", [505, 768, 1530, 1792, 3300, 4090])
+@pytest.mark.parametrize("fmt,dtype", KINDS)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_every_tile_and_length_of_k(hip, torch_cuda, shape, fmt, dtype, k):
+    m, n = 300, 333
+    a, b, bias = operands(hip, m, n, k, fmt, k)
+    whole = torch.full((m * (n + 7) + 9,), 7.0, dtype=dtype, device="cuda")
+    c = whole[3:3 + m * (n + 7)].view(m, n + 7)[:, :n]
+    with tuned(hip, shape=shape):
+        check(hip, hip.gemm_mx(a, b, bias=bias, dtype=dtype, out=c), a, b, bias, False)
+        plain = hip.gemm_mx(a, b, dtype=dtype)
+        check(hip, plain, a, b, None, False)
+        assert torch.equal(plain, hip.gemm_mx(a, b, dtype=dtype))
+    c.fill_(7.0)
+    assert bool((whole == 7.0).all())
+
+
+@pytest.mark.parametrize("fmt,dtype", KINDS)
+def test_c_past_the_caches(hip, torch_cuda, fmt, dtype):
+    """Rows of C that are whole 128-byte lines, the last ones of a tile missing, and the same bits as through the caches; rows
+    that are not, where nothing changes."""
+    for m, n in ((700, 768), (300, 333)):
+        a, b, bias = operands(hip, m, n, 1100, fmt, n)
+        with tuned(hip, shape=6):
+            want = hip.gemm_mx(a, b, bias=bias, relu=True, dtype=dtype)
+        check(hip, want, a, b, bias, True)
+        out = torch.full((m + 3, n), 7.0, dtype=dtype, device="cuda")
+        with tuned(hip, shape=6, past_caches_mib=0):
+            hip.gemm_mx(a, b, bias=bias, relu=True, dtype=dtype, out=out[:m])
+        assert torch.equal(out[:m], want) and bool((out[m:] == 7.0).all())
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+@pytest.mark.parametrize("shape", [0, 3, 5, 6])
+def test_scales_far_apart(hip, torch_cuda, shape, fmt):
+    """Scales of A and B that cancel, results below the normal numbers (a rounding to a multiple of 2^-149 for each addition) and past the
+    largest one (of magnitudes only, so that no part of a sum passes it before the sum does)."""
+    m, n, k = 40, 70, 600
+    for up, down, kind in ((60, -60, "cancel"), (-70, 72, "cancel"), (-66, -66, "least"), (60, 66, "largest"), (60, 59, "largest")):
+        a, b, _ = operands(hip, m, n, k, fmt, 3)
+        if kind == "largest":
+            a.codes.bitwise_and_(0x7F if fmt == "fp8" else 0x77), b.codes.bitwise_and_(0x77)
+        for q, by in ((a, up), (b, down)):
+            q.scales.copy_(torch.where(q.scales > 0, q.scales.int() + by, 0).to(torch.uint8))
+        want = hip.mx_dequantize(a, torch.float32).double() @ hip.mx_dequantize(b, torch.float32).double().t()
+        size = hip.mx_dequantize(a, torch.float32).double().abs() @ hip.mx_dequantize(b, torch.float32).double().abs().t()
+        for dtype in (torch.bfloat16,) if fmt == "fp8" else (torch.bfloat16, torch.float32):
+            with tuned(hip, shape=shape):
+                c = hip.gemm_mx(a, b, dtype=dtype).double()
+            off = (2 * 19 + 13) * (2 * EPS32 * size + 2.0 ** -149)
+            bound = off + HALF_ULP[dtype] * (want.abs() + off) + LEAST[dtype]
+            top = torch.finfo(dtype).max
+            sure, never = want.abs() - off > top * (1 + 2 * HALF_ULP[dtype]), want.abs() + off < top
+            assert bool(((c - want).abs() <= bound)[never].all()) and bool((c.abs() == float("inf"))[sure].all())
+            assert bool(sure.any()) == (kind == "largest")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+def test_quantise_several_pieces_to_a_thread(hip, torch_cuda, fmt, dtype):
+    """A matrix of 2^16 pieces of 256 values and more, whose threads take several each, is what its rows are a few at a time."""
+    rows, k = 4099, 4100
+    x = torch.empty(rows, k, device="cuda").normal_(generator=generator(1)).mul_(torch.exp(torch.empty(rows, 1, device="cuda").normal_(0, 2, generator=generator(2)))).to(dtype)
+    q = hip.mx_quantize(x, fmt)
+    back = hip.mx_dequantize(q, dtype)
+    for first in range(0, rows, 1000):
+        part = hip.mx_quantize(x[first:first + 1000], fmt)
+        assert torch.equal(q.codes[first:first + 1000], part.codes) and torch.equal(q.scales[first:first + 1000], part.scales)
+        assert torch.equal(back[first:first + 1000], hip.mx_dequantize(part, dtype))
