@@ -1,7 +1,7 @@
 """The feed-forward layer of a transformer block on microscaled matrices: the residual's addition and the root-mean-square
 norm, a product with 4-bit weights, its bias and ReLU, 8 bits again, a second product.
 
-    python -m spoc_amd.feed_forward [tokens] [width] [inner]    # one pass each way on random data, checked against float64
+    python -m spoc_amd.feed_forward [tokens] [width] [inner]    # one pass each way on random data, both checked against float64
 """
 import torch
 
@@ -58,17 +58,21 @@ def main(argv=None):
     up_bias, down_bias = random(0.1, inner), random(0.1, width)
     layer = MxFeedForward(weight, up, down, up_bias, down_bias)
     y, h, kept = layer.train(x, residual)
-    grads = layer.backward(kept, random(0.1, tokens, width).bfloat16(), h)
+    dy = random(0.1, tokens, width).bfloat16()
+    grads = layer.backward(kept, dy, h)
 
-    h64 = h.double()
-    n = h64 / (h64.pow(2).mean(1, keepdim=True) + layer.eps).sqrt() * weight.double()
+    # float64, the ReLU as the layer chose, no rounding to 8 bits
+    leaves = {"dx": h, "dweight": weight, "dup_bias": up_bias, "ddown_bias": down_bias}
+    leaves = {name: t.double().detach().requires_grad_() for name, t in leaves.items()}
     values = lambda q: hip.mx_dequantize(q, torch.float32).double()  # noqa: E731
-    u = (n @ values(up).t() + up_bias.double()).clamp(min=0)
-    want = u @ values(down).t() + down_bias.double()
-    off = float((y.double() - want).norm() / want.norm())
-    print(f"{tokens} x {width} -> {inner} -> {width}: output within {off:.3f} of the layer without its roundings to 8 bits; "
-          f"gradients {', '.join(f'{k} {tuple(v.shape)}' for k, v in grads.items())}")
-    return 0 if off < 0.05 else 1
+    n = leaves["dx"] / (leaves["dx"].pow(2).mean(1, keepdim=True) + layer.eps).sqrt() * leaves["dweight"]
+    want = ((n @ values(up).t() + leaves["dup_bias"]) * (kept[2] > 0)) @ values(down).t() + leaves["ddown_bias"]
+    ((want * dy.double()).sum() + (leaves["dx"] * h.double()).sum()).backward()
+    away = lambda got, right: float((got.double() - right).norm() / right.norm())  # noqa: E731
+    off = {"y": (away(y, want.detach()), 0.05), **{name: (away(grads[name], t.grad), 0.02) for name, t in leaves.items()}}
+    print(f"{tokens} x {width} -> {inner} -> {width}: output and gradients within (of the layer in float64 without its roundings to 8 bits) "
+          + ", ".join(f"{name} {far:.4f}" for name, (far, _) in off.items()))
+    return 0 if all(far < most for far, most in off.values()) else 1
 
 
 if __name__ == "__main__":
