@@ -39,7 +39,7 @@ class MxFeedForward:
         dweight, dup_bias and ddown_bias.  The products go over the weights' values in 16 bits."""
         h, rstd, u = kept
         product = hip.gemm_bf16 if h.dtype == torch.bfloat16 else hip.gemm_f16
-        du = product(dy, hip.mx_dequantize(self.down, h.dtype)).masked_fill_(u <= 0, 0)
+        du = product(dy.contiguous(), hip.mx_dequantize(self.down, h.dtype))   # (the 16-bit products take adjacent rows).masked_fill_(u <= 0, 0)
         dn = product(du.to(h.dtype), hip.mx_dequantize(self.up, h.dtype)).to(h.dtype)
         dx, dweight = hip.rms_norm_backward(dn, h, self.weight, rstd, dh=dh)
         return {"dx": dx, "dweight": dweight, "dup_bias": du.sum(0), "ddown_bias": dy.float().sum(0)}

@@ -47,3 +47,33 @@ def test_the_command_checks_the_gradients(hip, torch_cuda, monkeypatch, wrong):
         return grads
     monkeypatch.setattr(feed_forward.MxFeedForward, "backward", off)
     assert feed_forward.main(["5", "300", "700"]) == 1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_of_strided_rows(hip, torch_cuda, dtype):
+    """dy, dh and the inputs as rows of larger matrices, at odd elements: the same bits as from matrices of their own."""
+    rows, k, inner = 37, 300, 520
+    layer, x, residual, dy, dh = made(hip, rows, k, inner, dtype, True)
+    apart = []
+    for i, t in enumerate((x, residual, dy, dh)):
+        whole = torch.full((rows * (k + 3 + i) + 9,), 5.0, dtype=dtype, device="cuda")
+        apart.append(whole[1 + i:1 + i + rows * (k + 3 + i)].view(rows, k + 3 + i)[:, :k])
+        apart[-1].copy_(t)
+    y, h, kept = layer.train(x, residual)
+    got = layer.train(*apart[:2])
+    assert torch.equal(got[0], y) and torch.equal(got[1], h)
+    want, grads = layer.backward(kept, dy, dh), layer.backward(got[2], *apart[2:])
+    assert all(torch.equal(grads[name], v) for name, v in want.items())
+    check_gradients(hip, layer, kept, want, dy, dh)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 19])
+@pytest.mark.parametrize("residual,dh,biases", [(False, False, False), (True, False, True), (False, True, True), (True, True, False)])
+def test_gradients_without_the_arguments_that_may_be_missing(hip, torch_cuda, rows, dtype, residual, dh, biases):
+    layer, x, more, dy, above = made(hip, rows, 260, 390, dtype, biases, seed=rows)
+    y, h, kept = layer.train(x, more if residual else None)
+    assert torch.equal(h, x + more if residual else x) and y.shape == x.shape
+    got = layer.backward(kept, dy, above if dh else None)
+    assert got["dx"].shape == x.shape and got["dx"].dtype == dtype
+    check_gradients(hip, layer, kept, got, dy, above if dh else None)
