@@ -38,11 +38,17 @@ class MxFeedForward:
         """Gradients for dy (of y) and dh (of h, None where nothing else uses it): a dict of dx (x's and the residual's),
         dweight, dup_bias and ddown_bias.  The products go over the weights' values in 16 bits."""
         h, rstd, u = kept
-        product = hip.gemm_bf16 if h.dtype == torch.bfloat16 else hip.gemm_f16
-        du = product(dy.contiguous(), hip.mx_dequantize(self.down, h.dtype))   # (the 16-bit products take adjacent rows).masked_fill_(u <= 0, 0)
-        dn = product(du.to(h.dtype), hip.mx_dequantize(self.up, h.dtype)).to(h.dtype)
+        du = _product(dy.contiguous(), hip.mx_dequantize(self.down, h.dtype)).masked_fill_(u <= 0, 0)   # (adjacent rows for the products)
+        dn = _product(du.to(h.dtype), hip.mx_dequantize(self.up, h.dtype)).to(h.dtype)
         dx, dweight = hip.rms_norm_backward(dn, h, self.weight, rstd, dh=dh)
         return {"dx": dx, "dweight": dweight, "dup_bias": du.sum(0), "ddown_bias": dy.float().sum(0)}
+
+
+def _product(a, b):
+    """a b of 16-bit matrices in float32; of no rows too, as the other operators serve them."""
+    if a.shape[0] == 0:
+        return a.new_empty(0, b.shape[1], dtype=torch.float32)
+    return (hip.gemm_bf16 if a.dtype == torch.bfloat16 else hip.gemm_f16)(a, b)
 
 
 def main(argv=None):

@@ -68,7 +68,7 @@ def test_gradients_of_strided_rows(hip, torch_cuda, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("rows", [1, 19])
+@pytest.mark.parametrize("rows", [0, 1, 19])
 @pytest.mark.parametrize("residual,dh,biases", [(False, False, False), (True, False, True), (False, True, True), (True, True, False)])
 def test_gradients_without_the_arguments_that_may_be_missing(hip, torch_cuda, rows, dtype, residual, dh, biases):
     layer, x, more, dy, above = made(hip, rows, 260, 390, dtype, biases, seed=rows)
