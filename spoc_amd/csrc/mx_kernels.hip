@@ -1,6 +1,7 @@
 // Rows in microscaled 8- and 4-bit floating point (layout: mx_common.hpp): bringing a matrix to them and back, the root-mean-square
 // norm that writes 8-bit rows for the product behind it, and that norm's gradient.  All of them pass over memory once.
 #include <algorithm>
+#include <type_traits>
 #include <utility>
 
 #include "mx_common.hpp"
@@ -267,32 +268,36 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs<T> p) {
   }
 }
 
-// Calls f with (threads to a row, times eight values) for rows of k values of `size` bytes; `longer` for those that registers are not made
+// Calls f with (threads to a row, times eight values) for rows of k values of type T; `longer` for those that registers are not made
 // for, and for less than one load.  A wave to a row up to 1024 values (no barrier), then 256 threads, then 512, and 1024 for float32, whose 32
 // values of a thread the gradient's registers would not hold (gradient of 3000 x 8190 in fp16, us: 256 threads 62.9, 512 46.5; 2000 x 16384
 // in bf16: 512 threads 54, 1024 60).  Three loads to a thread
 // where two of twice the threads would leave a quarter of them and more without values: past 8192 values always (3000 x 12000 in float32,
 // gradient 136 us, so 93; 4095 x 11008 in bf16, norm 73 us, so 62; 16 rows the same), below where the caller's many rows make up for
-// what a row alone takes longer: `wave3` a wave up to 1536 values, `block3` 256 threads up to 6144.
-template <class F, class Long> int by_length(int64_t k, size_t size, bool wave3, bool block3, F &&f, Long &&longer) {
+// what a row alone takes longer (`many`): for a caller with Wave3 a wave up to 1536 values, with Block3 256 threads up to 6144.
+template <class T, bool Wave3, bool Block3, class F, class Long> int by_length(int64_t k, bool many, F &&f, Long &&longer) {
   if (k < 8) return longer();   // (load8_of_row)
   if (k <= 512) return f(std::integer_sequence<int, 64, 1>{});
   if (k <= 1024) return f(std::integer_sequence<int, 64, 2>{});
-  if (k <= 1536 && wave3) return f(std::integer_sequence<int, 64, 3>{});
+  if constexpr (Wave3)
+    if (k <= 1536 && many) return f(std::integer_sequence<int, 64, 3>{});
   if (k <= 2048) return f(std::integer_sequence<int, 256, 1>{});
   if (k <= 4096) return f(std::integer_sequence<int, 256, 2>{});
-  if (k <= 6144 && block3) return f(std::integer_sequence<int, 256, 3>{});
+  if constexpr (Block3)
+    if (k <= 6144 && many) return f(std::integer_sequence<int, 256, 3>{});
   if (k <= 8192) return f(std::integer_sequence<int, 512, 2>{});
   if (k <= 12288) return f(std::integer_sequence<int, 512, 3>{});
-  if (k <= 16384) return size == 4 ? f(std::integer_sequence<int, 1024, 2>{}) : f(std::integer_sequence<int, 512, 4>{});
+  if (k <= 16384) return f(std::conditional_t<sizeof(T) == 4, std::integer_sequence<int, 1024, 2>, std::integer_sequence<int, 512, 4>>{});
   return longer();
 }
-// The norm's: of 16-bit rows from 2048 on (16000 x 1200 with a residual 38 us, so 28, 2000 x 1536 7.8, so 7.1, but 1000 x 1536 4.4, so 4.7;
-// 4000 x 5500 35.5, so 31.1, 500 x 5500 7.2, so 7.3).  Float32 rows, with twice the bytes under way, gain nothing (4000 x 5500 55.6, 54.9).
-bool norm_by_three(int64_t rows, size_t size) { return size == 2 && rows >= 2048; }
+// The norm's, of 16-bit rows: from 2048 rows on (16000 x 1200 with a residual 38 us, so 28; 4000 x 5500 35.5, so 31.1); of fewer some gain and
+// some lose (2000 x 1536 7.8, so 7.1; 1000 x 1536 4.4, so 4.7; 500 x 5500 7.2, so 7.3).  Float32 rows, with twice the bytes under way, gain
+// nothing (4000 x 5500 55.6, 54.9).
+template <class T> constexpr bool kNormByThree = sizeof(T) == 2;
+bool many_for_norm(int64_t rows) { return rows >= 2048; }
 // The gradient's, of a wave only: from 1024 rows on (16000 x 1200 in bf16 57 us, so 30, 1000 x 1536 8.6, so 8.2, 500 x 1536 12.0, so 12.3;
 // float32 76 us, so 46); 256 threads lose (4000 x 5500 in bf16 47 us, 55).
-bool gradient_by_three(int64_t rows) { return rows >= 1024; }
+bool many_for_gradient(int64_t rows) { return rows >= 1024; }
 
 template <class T> struct BackwardArgs {
   const T *dy, *h, *weight, *dh;
@@ -556,8 +561,8 @@ int sarek_hip_rms_norm_mx(const void *x, int64_t x_stride, const void *residual,
   return by_type(type, [&]<class T>(T *) {
     const NormArgs<T> args{static_cast<const T *>(x), static_cast<const T *>(residual), static_cast<const T *>(weight), static_cast<T *>(h),
                            codes, scales, rstd, x_stride, residual_stride, h_stride, rows, k, kp, eps};
-    return by_length(
-        k, sizeof(T), norm_by_three(rows, sizeof(T)), norm_by_three(rows, sizeof(T)),
+    return by_length<T, kNormByThree<T>, kNormByThree<T>>(
+        k, many_for_norm(rows),
         [&]<int Threads, int Vectors>(std::integer_sequence<int, Threads, Vectors>) {
           const dim3 grid(static_cast<unsigned>(ceil_div(rows, Threads < 256 ? 256 / Threads : 1)));
           hipLaunchKernelGGL((rms_norm_kernel<T, Threads, Vectors>), grid, dim3(std::max(Threads, 256)), 0, as_stream(stream), args);
@@ -593,8 +598,8 @@ int sarek_hip_rms_norm_backward(const void *dy, int64_t dy_stride, const void *h
     if (planes > 0) {
       const BackwardArgs<T> args{static_cast<const T *>(dy), static_cast<const T *>(h), static_cast<const T *>(weight), static_cast<const T *>(dh),
                                  rstd, static_cast<T *>(dx), workspace, dy_stride, h_stride, dh_stride, dx_stride, rows, k};
-      by_length(
-          k, sizeof(T), gradient_by_three(rows), false,
+      by_length<T, true, false>(
+          k, many_for_gradient(rows),
           [&]<int Threads, int Vectors>(std::integer_sequence<int, Threads, Vectors>) {
             hipLaunchKernelGGL((rms_norm_backward_kernel<T, Threads, Vectors>), dim3(planes), dim3(std::max(Threads, 256)), 0, as_stream(stream), args);
             return SAREK_HIP_OK;
