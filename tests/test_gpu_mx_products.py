@@ -163,3 +163,15 @@ def test_quantise_several_pieces_to_a_thread(hip, torch_cuda, fmt, dtype):
         part = hip.mx_quantize(x[first:first + 1000], fmt)
         assert torch.equal(q.codes[first:first + 1000], part.codes) and torch.equal(q.scales[first:first + 1000], part.scales)
         assert torch.equal(back[first:first + 1000], hip.mx_dequantize(part, dtype))
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_undefined_codes(hip, torch_cuda, shape):
+    """A code that is a NaN, in a block with a scale like any other, makes NaN of its row of C and of nothing else."""
+    m, n, k = 70, 90, 900
+    a, b, _ = operands(hip, m, n, k, "fp8", 9)
+    a.codes[3, 899], a.codes[40, 17] = 0x7F, 0xFF
+    want = torch.zeros(m, n, dtype=torch.bool, device="cuda")
+    want[3], want[40] = True, True
+    with tuned(hip, shape=shape):
+        assert torch.equal(torch.isnan(hip.gemm_mx(a, b)), want)
