@@ -31,7 +31,8 @@ extern "C" {
 
 /* 3: entry points added since 2 (sarek_hip_run_sources, sarek_hip_execute_run_pipeline, sarek_hip_rebuilt_source,
  * the library kernels, the stencil, layout and histogram kernels, sarek_hip_is_measurement_build, and the operators
- * on microscaled rows: sarek_hip_mx_*, sarek_hip_rms_norm_*, sarek_hip_gemm_mx); the measurement knobs and the
+ * on microscaled rows: sarek_hip_mx_*, sarek_hip_rms_norm_*, sarek_hip_gemm_mx, and on a paged cache: sarek_hip_rotary*,
+ * sarek_hip_kv_append, sarek_hip_attention_*); the measurement knobs and the
  * in-kernel clock probe left the product library; nothing that version 2 declared changed its meaning. */
 #define SAREK_HIP_ABI_VERSION 3
 
@@ -719,6 +720,70 @@ int sarek_hip_rms_norm_backward(const void *dy, int64_t dy_stride, const void *h
 int sarek_hip_gemm_mx(const unsigned char *a_codes, const unsigned char *a_scales, int a_format, const unsigned char *b_codes,
                       const unsigned char *b_scales, const float *bias, int relu, void *c, int c_type, int64_t c_stride, int64_t m,
                       int64_t n, int64_t k, sarek_hip_stream stream);
+
+/* ---------------------------------------------------------------------- */
+/* The attention layer that serves from a paged cache (no counterpart in the reference): rotary positions, the cache, and attention over it.
+ * Matrices of heads are [tokens, heads, head_dim] with adjacent values: heads are head_stride elements apart, tokens token_stride, at any
+ * alignment of an element.  Types: SAREK_HIP_TYPE_*; of the cache and of attention the 16-bit ones.  tokens = 0 is no error.
+ *
+ * Rotary positions.  Pair i of a head, i < pairs, is turned by the angle position times the pair's frequency, and multiplied by
+ * amplitude: (a, b) -> (a cos - b sin, a sin + b cos).  Pairs are the values i and i + pairs (interleaved 0) or 2 i and 2 i + 1
+ * (interleaved 1); what is behind value 2 pairs of a head stays as it is.  A frequency is held as the turns that it makes from position to
+ * position in units of 2^-64, modulo one turn, so that an angle is exact to 2^-24 turns of itself at any position;
+ * sarek_hip_rotary_turns brings radians (host memory) to that (host memory).                                                    */
+typedef struct {
+  const uint64_t *turns;   /* device memory, `pairs` of them */
+  int pairs, interleaved;
+  float amplitude;
+} sarek_hip_rotary_plan;
+int sarek_hip_rotary_turns(const double *radians, uint64_t *turns, int pairs);
+/* inverse not 0: by the angles' negatives (the gradient: of y = rotary(x) it takes dy to dx).  positions: one to a token, of
+ * position_bytes 4 or 8 (signed).  out may be x itself, with x's strides, and must not overlap it otherwise.                    */
+int sarek_hip_rotary(const sarek_hip_rotary_plan *plan, const void *x, int64_t x_token, int64_t x_head, int type, const void *positions,
+                     int position_bytes, int inverse, void *out, int64_t out_token, int64_t out_head, int64_t tokens, int heads,
+                     int head_dim, sarek_hip_stream stream);
+
+/* A cache [n_pages, page_size, heads, head_dim] of keys and one of values with the same strides (in elements; values of a head are
+ * adjacent).  head_dim is a multiple of 8 up to 256; keys and values start at a multiple of 16 bytes, strides are multiples of 8
+ * elements, none of its rows overlap.
+ * A call's tokens lie one sequence after the other: sequence b has tokens starts[b] to starts[b + 1] - 1, not decreasing, or the one
+ * token b where starts is NULL; they are the last of its lengths[b] keys.  Key p of sequence b lies in slot p % page_size of the page
+ * pages[b * pages_stride + p / page_size], p / page_size < max_pages.  lengths, starts and pages are int32 in device memory and are read
+ * when the kernels run.  Keys that the table has no room for are left out; an entry of the table that is no page of the cache is not
+ * written to and stands for keys and values of zeros.  Rows of tokens behind the last sequence are left as they are.             */
+typedef struct {
+  void *keys, *values;
+  int64_t page_stride, slot_stride, head_stride;
+  int64_t n_pages;
+  int page_size, heads, head_dim, type;
+} sarek_hip_kv_cache;
+/* Puts the tokens' k and v [tokens, cache->heads, head_dim] into their places, k turned by plan (NULL: as it is) at the position
+ * first + place in its sequence.  q (or NULL) [tokens, q_heads, head_dim] is turned likewise into q_out, which may be q itself; nothing
+ * else may overlap.  A page that the tokens go to belongs to one sequence.                                                       */
+int sarek_hip_kv_append(const sarek_hip_kv_cache *cache, const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token,
+                        int64_t v_head, const void *q, int64_t q_token, int64_t q_head, void *q_out, int64_t q_out_token,
+                        int64_t q_out_head, int q_heads, const sarek_hip_rotary_plan *plan, const int *pages, int64_t pages_stride,
+                        int max_pages, const int *lengths, const int *starts, int batch, int64_t tokens, int64_t first,
+                        sarek_hip_stream stream);
+/* out = softmax(scale q . keys) . values, head h of q with head h / (q_heads / cache->heads) of the cache; causal not 0: a token sees its
+ * sequence's keys up to its own.  A token that sees no key gets zeros.  lse (or NULL) [tokens, q_heads]: the natural logarithm of
+ * the sum of the exponents, minus infinity for no key.  Scores, their exponents' sums and the weighted values are held in float32.  A
+ * key that a token does not see takes no part in its sums, whatever the cache holds there.  scale is positive and finite.
+ * workspace: sarek_hip_attention_workspace_bytes, for the same arguments, of device memory (16 bytes aligned), SAREK_HIP_E_WORKSPACE else;
+ * one call at a time may use it.
+ * attention_shared: every sequence begins with the prefix_length keys of prefix_pages (device memory, at least prefix_length / page_size
+ * rounded up entries), which all its tokens see, and goes on with its own.  attention_paged is that without a prefix.              */
+int64_t sarek_hip_attention_workspace_bytes(const sarek_hip_kv_cache *cache, int q_heads, int batch, int64_t tokens, int max_pages,
+                                            int64_t prefix_length);
+int sarek_hip_attention_paged(const sarek_hip_kv_cache *cache, const void *q, int64_t q_token, int64_t q_head, int q_heads, void *out,
+                              int64_t out_token, int64_t out_head, float *lse, const int *pages, int64_t pages_stride, int max_pages,
+                              const int *lengths, const int *starts, int batch, int64_t tokens, int causal, float scale,
+                              void *workspace, int64_t workspace_bytes, sarek_hip_stream stream);
+int sarek_hip_attention_shared(const sarek_hip_kv_cache *cache, const void *q, int64_t q_token, int64_t q_head, int q_heads, void *out,
+                               int64_t out_token, int64_t out_head, float *lse, const int *prefix_pages, int64_t prefix_length,
+                               const int *pages, int64_t pages_stride, int max_pages, const int *lengths, const int *starts, int batch,
+                               int64_t tokens, int causal, float scale, void *workspace, int64_t workspace_bytes,
+                               sarek_hip_stream stream);
 
 /* Persistent cache of compiled kernels: the reference's Framework_cache
  * (sarek/framework/Framework_cache.ml:63-141; used there by the Vulkan plugin,

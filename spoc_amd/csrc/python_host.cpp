@@ -244,6 +244,11 @@ decltype(&sarek_hip_mx_dequantize) g_mx_dequantize;
 decltype(&sarek_hip_rms_norm_mx) g_rms_norm_mx;
 decltype(&sarek_hip_rms_norm_backward) g_rms_norm_backward;
 decltype(&sarek_hip_gemm_mx) g_gemm_mx;
+// and those on a paged cache
+decltype(&sarek_hip_rotary) g_rotary;
+decltype(&sarek_hip_kv_append) g_kv_append;
+decltype(&sarek_hip_attention_paged) g_attention_paged;
+decltype(&sarek_hip_attention_shared) g_attention_shared;
 
 template <typename T>
 T as_c(PyObject *o) {
@@ -270,7 +275,7 @@ PyObject *call_with(int (*f)(Args...), PyObject *const *a, std::index_sequence<I
 template <typename... Args>
 PyObject *call(int (*f)(Args...), PyObject *const *a, Py_ssize_t n, const char *what) {
   if (!f) {
-    PyErr_SetString(PyExc_RuntimeError, "spoc_amd._host: bind_mx() has not been called");
+    PyErr_SetString(PyExc_RuntimeError, "spoc_amd._host: bind_mx() and bind_attention() have not been called");
     return nullptr;
   }
   if (!arity(n, sizeof...(Args), what)) return nullptr;
@@ -281,6 +286,10 @@ PyObject *mx_dequantize(PyObject *, PyObject *const *a, Py_ssize_t n) { return c
 PyObject *rms_norm_mx(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_rms_norm_mx, a, n, "rms_norm_mx"); }
 PyObject *rms_norm_backward(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_rms_norm_backward, a, n, "rms_norm_backward"); }
 PyObject *gemm_mx(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_gemm_mx, a, n, "gemm_mx"); }
+PyObject *rotary(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_rotary, a, n, "rotary"); }
+PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_kv_append, a, n, "kv_append"); }
+PyObject *attention_paged(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_attention_paged, a, n, "attention_paged"); }
+PyObject *attention_shared(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_attention_shared, a, n, "attention_shared"); }
 
 // bind(addresses of the first five entry points above, in the order of their declaration)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
@@ -310,6 +319,19 @@ PyObject *bind_mx(PyObject *, PyObject *const *a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// bind_attention(addresses of the four on a paged cache)
+PyObject *bind_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (!arity(n, 4, "bind_attention")) return nullptr;
+  void *p[4];
+  for (int i = 0; i < 4; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
+  if (PyErr_Occurred()) return nullptr;
+  g_rotary = reinterpret_cast<decltype(g_rotary)>(p[0]);
+  g_kv_append = reinterpret_cast<decltype(g_kv_append)>(p[1]);
+  g_attention_paged = reinterpret_cast<decltype(g_attention_paged)>(p[2]);
+  g_attention_shared = reinterpret_cast<decltype(g_attention_shared)>(p[3]);
+  Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(bind), METH_FASTCALL, "Addresses of the library's entry points."},
     {"bind_mx", reinterpret_cast<PyCFunction>(bind_mx), METH_FASTCALL, "The same for the operators on microscaled rows."},
@@ -322,6 +344,11 @@ PyMethodDef methods[] = {
     {"rms_norm_mx", reinterpret_cast<PyCFunction>(rms_norm_mx), METH_FASTCALL, "sarek_hip_rms_norm_mx"},
     {"rms_norm_backward", reinterpret_cast<PyCFunction>(rms_norm_backward), METH_FASTCALL, "sarek_hip_rms_norm_backward"},
     {"gemm_mx", reinterpret_cast<PyCFunction>(gemm_mx), METH_FASTCALL, "sarek_hip_gemm_mx"},
+    {"bind_attention", reinterpret_cast<PyCFunction>(bind_attention), METH_FASTCALL, "The same for the operators on a paged cache."},
+    {"rotary", reinterpret_cast<PyCFunction>(rotary), METH_FASTCALL, "sarek_hip_rotary"},
+    {"kv_append", reinterpret_cast<PyCFunction>(kv_append), METH_FASTCALL, "sarek_hip_kv_append"},
+    {"attention_paged", reinterpret_cast<PyCFunction>(attention_paged), METH_FASTCALL, "sarek_hip_attention_paged"},
+    {"attention_shared", reinterpret_cast<PyCFunction>(attention_shared), METH_FASTCALL, "sarek_hip_attention_shared"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Argument lists of launches, built natively.", -1, methods,

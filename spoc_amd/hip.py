@@ -76,6 +76,18 @@ class Launch(C.Structure):
                 ("grid", C.c_int * 3), ("shared_mem_bytes", C.c_int), ("args", C.POINTER(Arg)), ("n_args", C.c_int)]
 
 
+class RotaryPlan(C.Structure):
+    """sarek_hip_rotary_plan."""
+    _fields_ = [("turns", C.c_void_p), ("pairs", C.c_int), ("interleaved", C.c_int), ("amplitude", C.c_float)]
+
+
+class KvCacheLayout(C.Structure):
+    """sarek_hip_kv_cache."""
+    _fields_ = [("keys", C.c_void_p), ("values", C.c_void_p), ("page_stride", C.c_int64), ("slot_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("n_pages", C.c_int64), ("page_size", C.c_int), ("heads", C.c_int),
+                ("head_dim", C.c_int), ("type", C.c_int)]
+
+
 class PipelineStage(C.Structure):
     """sarek_hip_pipeline_stage: one Execute.run_vectors call of a kernel sequence."""
     _fields_ = [("ir_text", C.c_char_p), ("block", C.c_int * 3), ("grid", C.c_int * 3),
@@ -163,6 +175,15 @@ SYMBOLS = {
     "sarek_hip_rms_norm_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i, _vp, _i64, _vp, _i64, _i64, _vp,
                                          _i64, _vp]),
     "sarek_hip_gemm_mx": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i64, _i64, _i64, _i64, _vp]),
+    "sarek_hip_rotary_turns": (_i, [_vp, _vp, _i]),
+    "sarek_hip_rotary": (_i, [_vp, _vp, _i64, _i64, _i, _vp, _i, _i, _vp, _i64, _i64, _i64, _i, _i, _vp]),
+    "sarek_hip_kv_append": (_i, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i, _vp, _vp, _i64, _i, _vp,
+                                 _vp, _i, _i64, _i64, _vp]),
+    "sarek_hip_attention_workspace_bytes": (_i64, [_vp, _i, _i, _i64, _i, _i64]),
+    "sarek_hip_attention_paged": (_i, [_vp, _vp, _i64, _i64, _i, _vp, _i64, _i64, _vp, _vp, _i64, _i, _vp, _vp, _i, _i64, _i, _f, _vp,
+                                       _i64, _vp]),
+    "sarek_hip_attention_shared": (_i, [_vp, _vp, _i64, _i64, _i, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i, _vp, _vp, _i, _i64,
+                                        _i, _f, _vp, _i64, _vp]),
     "sarek_hip_cache_dir": (_i, [C.c_char_p, _sz]),
     "sarek_hip_cache_compute_key": (_i, [C.c_char_p, C.c_char_p, C.c_char_p, C.c_char_p]),
     "sarek_hip_cache_get": (_i, [C.c_char_p, _vp, _sz, C.POINTER(_sz), C.POINTER(_i)]),
@@ -280,6 +301,8 @@ _host.bind(*(C.cast(getattr(lib, _f), C.c_void_p).value for _f in (
 _host.bind_mx(*(C.cast(getattr(lib, _f), C.c_void_p).value for _f in (
     "sarek_hip_mx_quantize", "sarek_hip_mx_dequantize", "sarek_hip_rms_norm_mx", "sarek_hip_rms_norm_backward",
     "sarek_hip_gemm_mx")))
+_host.bind_attention(*(C.cast(getattr(lib, _f), C.c_void_p).value for _f in (
+    "sarek_hip_rotary", "sarek_hip_kv_append", "sarek_hip_attention_paged", "sarek_hip_attention_shared")))
 
 
 def check(status):
@@ -1048,6 +1071,276 @@ def gemm_mx(a, b, bias=None, relu=False, dtype=torch.bfloat16, out=None):
     if status != OK:
         check(status)
     return c
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions, a paged cache of keys and values, attention over it
+
+_ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+class Rotary:
+    """Rotary positions of heads whose first `dim` values are turned: pair i by position times base^(-2 i / dim) radians.  layout
+    "half": a pair is the values i and i + dim / 2; "interleaved": 2 i and 2 i + 1.
+
+    scaling, for contexts `factor` times as long as the `trained` one: None; "linear" (every frequency divided by factor); "base"
+    (the base times factor^(dim / (dim - 2)): the slowest pair divided by factor, the fastest left); "ramp" (pairs that make at most
+    `low` turns in `trained` positions divided by factor, those that make `high` and more left, linear in the turns between).
+    amplitude multiplies what is turned.  frequencies (radians from position to position, dim / 2 of them) stand in for the formula."""
+
+    def __init__(self, dim, base=10000.0, layout="half", scaling=None, factor=1.0, trained=4096, low=1.0, high=32.0, amplitude=1.0,
+                 frequencies=None, device="cuda"):
+        if dim < 2 or dim % 2:
+            raise ValueError(f"Rotary: dim is even and positive, not {dim}")
+        if layout not in _ROTARY_LAYOUTS:
+            raise ValueError(f"Rotary: unknown layout {layout!r}")
+        if scaling not in (None, "linear", "base", "ramp"):
+            raise ValueError(f"Rotary: unknown scaling {scaling!r}")
+        if not (base > 0 and factor > 0 and trained > 0) or not high > low:
+            raise ValueError("Rotary: base, factor and trained are positive, high is above low")
+        if scaling == "base" and dim < 4:
+            raise ValueError('Rotary: scaling "base" needs a dim of 4 or more')
+        if frequencies is None:
+            if scaling == "base":
+                base = base * factor ** (dim / (dim - 2))
+            f = base ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+            if scaling == "linear":
+                f = f / factor
+            elif scaling == "ramp":
+                keep = ((trained * f / (2 * torch.pi) - low) / (high - low)).clamp(0, 1)
+                f = f * keep + f / factor * (1 - keep)
+        else:
+            f = torch.as_tensor(frequencies, dtype=torch.float64).cpu().contiguous()
+            if f.shape != (dim // 2,):
+                raise ValueError(f"Rotary: {dim // 2} frequencies expected, got {tuple(f.shape)}")
+        turns = torch.empty(dim // 2, dtype=torch.int64)
+        check(lib.sarek_hip_rotary_turns(f.data_ptr(), turns.data_ptr(), dim // 2))
+        self.dim, self.layout, self.amplitude, self.frequencies, self.turns = dim, layout, float(amplitude), f, turns.to(device)
+        self._plan = RotaryPlan(self.turns.data_ptr(), dim // 2, _ROTARY_LAYOUTS[layout], self.amplitude)
+        self._at = C.addressof(self._plan)
+
+    def __repr__(self):
+        return f"Rotary({self.dim}, {self.layout})"
+
+
+class KvCache:
+    """Keys and values [pages, page size, heads, head dim] (bfloat16 or float16, of the same strides, values of a head adjacent: views
+    of one block, or pages with their heads outermost, serve as well)."""
+
+    def __init__(self, keys, values):
+        for t, name in ((keys, "keys"), (values, "values")):
+            if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 4 and t.dtype in (torch.bfloat16, torch.float16)):
+                raise TypeError(f"KvCache: {name}: expected a device tensor [pages, page size, heads, head dim] of bfloat16 or float16")
+        if values.dtype != keys.dtype or values.device != keys.device:
+            raise TypeError("KvCache: keys and values differ in type or device")
+        if values.shape != keys.shape or values.stride() != keys.stride() or (keys.stride(3) != 1 and keys.shape[3] > 1):
+            raise ValueError(f"KvCache: keys {tuple(keys.shape)} with strides {keys.stride()}, values {tuple(values.shape)} with {values.stride()}: "
+                             "both are laid out alike, with adjacent values")
+        pages, page_size, heads, head_dim = keys.shape
+        if pages * page_size * heads == 0 or head_dim % 8 or not 8 <= head_dim <= 256:
+            raise ValueError(f"KvCache: {tuple(keys.shape)}: heads of a multiple of 8 values up to 256 are served, and nothing may be empty")
+        extents = sorted((s, n) for s, n in zip(keys.stride()[:3], keys.shape[:3]) if n > 1)
+        reach = head_dim
+        for stride, n in extents:
+            if stride < reach or stride % 8:
+                raise ValueError(f"KvCache: strides {keys.stride()}: multiples of 8, of rows that do not overlap")
+            reach = stride * (n - 1) + reach
+        if (keys.data_ptr() | values.data_ptr()) & 15:
+            raise ValueError("KvCache: keys and values start at multiples of 16 bytes")
+        self.keys, self.values, self.page_size, self.heads, self.head_dim = keys, values, page_size, heads, head_dim
+        self._layout = KvCacheLayout(keys.data_ptr(), values.data_ptr(), *keys.stride()[:3], pages, page_size, heads, head_dim, _MX_TYPES[keys.dtype])
+        self._at = C.addressof(self._layout)
+
+    @classmethod
+    def empty(cls, pages, page_size, heads, head_dim, dtype=torch.bfloat16, device="cuda"):
+        """A cache of its own memory."""
+        return cls(*torch.empty(2, pages, page_size, heads, head_dim, dtype=dtype, device=device).unbind(0))
+
+    def __repr__(self):
+        return f"KvCache({' x '.join(map(str, self.keys.shape))}, {self.keys.dtype})"
+
+
+def _here(device, name):
+    if device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"{name}: is on {device}, not on the current device")
+
+
+def _head_rows(t, name):
+    """(tokens, heads, head dim, elements from token to token, from head to head) of a device tensor of heads with adjacent values."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 3 and t.dtype in _MX_TYPES:
+        (tokens, heads, d), (token, head, step) = t.shape, t.stride()
+        if step == 1 or d == 1:
+            return tokens, heads, d, token, head
+    raise TypeError(f"{name}: expected a device tensor [tokens, heads, head dim] of float32, bfloat16 or float16 with adjacent values")
+
+
+def _rotated(x, positions, plan, out, inverse, name):
+    tokens, heads, d, token, head = _head_rows(x, name)
+    if not isinstance(plan, Rotary):
+        raise TypeError("plan: expected a Rotary")
+    if plan.dim > d:
+        raise ValueError(f"plan: turns {plan.dim} values, {name} has heads of {d}")
+    if not (isinstance(positions, torch.Tensor) and positions.is_cuda and positions.dtype in (torch.int64, torch.int32)
+            and positions.is_contiguous()):
+        raise TypeError("positions: expected a contiguous device tensor of int64 or int32")
+    if positions.shape != (tokens,):
+        raise ValueError(f"positions: {tokens} of them expected, got {tuple(positions.shape)}")
+    _here(x.device, name)
+    if positions.device != x.device or plan.turns.device != x.device:
+        raise ValueError(f"{name}, positions and plan are on different devices")
+    if out is None:
+        out = x.new_empty(tokens, heads, d)
+    out_token, out_head = _like_heads(out, x, "out")
+    status = _host.rotary(plan._at, x.data_ptr(), token, head, _MX_TYPES[x.dtype], positions.data_ptr(), positions.element_size(), inverse,
+                          out.data_ptr(), out_token, out_head, tokens, heads, d, _raw_stream())
+    if status != OK:
+        check(status)
+    return out
+
+
+def _like_heads(t, x, name):
+    _, _, _, token, head = _head_rows(t, name)
+    if t.dtype != x.dtype or t.device != x.device:
+        raise TypeError(f"{name}: expected {x.dtype} on {x.device}, got {t.dtype} on {t.device}")
+    if t.shape != x.shape:
+        raise ValueError(f"{name}: expected {tuple(x.shape)}, got {tuple(t.shape)}")
+    return token, head
+
+
+def rotary(x, positions, plan, out=None):
+    """x [tokens, heads, head dim] (float32, bfloat16 or float16) turned to its positions [tokens] (int64 or int32) by a Rotary.  out may be
+    x itself."""
+    return _rotated(x, positions, plan, out, 0, "x")
+
+
+def rotary_backward(dy, positions, plan, out=None):
+    """The gradient of rotary's x for dy, its output's: turned the other way."""
+    return _rotated(dy, positions, plan, out, 1, "dy")
+
+
+def _table(t, shape, name, device):
+    """A device tensor of int32, contiguous along its last dimension, of this shape (None: any)."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.int32 and t.dim() == len(shape)
+            and (t.stride(-1) == 1 or t.shape[-1] <= 1)):
+        raise TypeError(f"{name}: expected a device tensor of int32 of {len(shape)} dimension{'s' if len(shape) > 1 else ''} with adjacent values")
+    if any(want is not None and got != want for got, want in zip(t.shape, shape)):
+        raise ValueError(f"{name}: expected {' x '.join('any' if v is None else str(v) for v in shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name}: is on {t.device}, the cache on {device}")
+    return t.data_ptr()
+
+
+def _sequences(cache, pages, lengths, starts, tokens):
+    """The C arguments pages, pages_stride, max_pages, lengths, starts, batch."""
+    if not isinstance(cache, KvCache):
+        raise TypeError("cache: expected a KvCache")
+    device = cache.keys.device
+    _here(device, "cache")
+    lengths_at = _table(lengths, (None,), "lengths", device)
+    batch = lengths.shape[0]
+    pages_at = _table(pages, (batch, None), "pages", device)
+    starts_at = None if starts is None else _table(starts, (batch + 1,), "starts", device)
+    if starts is None and tokens != batch:
+        raise ValueError(f"without starts each of {batch} sequences has one token, but there are {tokens}")
+    return pages_at, max(pages.stride(0), pages.shape[1]), pages.shape[1], lengths_at, starts_at, batch
+
+
+def _cache_heads(t, cache, tokens, heads, name):
+    """Strides of a tensor that goes with the cache."""
+    got_tokens, got_heads, d, token, head = _head_rows(t, name)
+    if t.dtype != cache.keys.dtype:
+        raise TypeError(f"{name}: {t.dtype}, the cache holds {cache.keys.dtype}")
+    if t.device != cache.keys.device:
+        raise ValueError(f"{name}: is on {t.device}, the cache on {cache.keys.device}")
+    if d != cache.head_dim or (tokens is not None and got_tokens != tokens) or (heads is not None and got_heads != heads):
+        raise ValueError(f"{name}: expected {'any' if tokens is None else tokens} x {'any' if heads is None else heads} x {cache.head_dim}, got {tuple(t.shape)}")
+    return token, head
+
+
+def kv_append(k, v, cache, pages, lengths, starts=None, rotary=None, q=None, q_out=None, first=0):
+    """Puts k and v [tokens, heads of the cache, head dim] into a KvCache, k turned by `rotary` (a Rotary or None), and returns q
+    [tokens, heads, head dim] turned likewise (in q_out, which may be q itself; None without a q).
+
+    Sequence b of the batch has the tokens starts[b] to starts[b + 1] - 1 (starts None: the one token b); they are the last of its
+    lengths[b] keys.  Key p is in slot p % page size of page pages[b, p // page size] and at position first + p.  lengths [batch],
+    starts [batch + 1] and pages [batch, any] are int32 on the device.  A page that tokens go to belongs to one sequence; tokens that the
+    table has no room for, or no page of the cache, are not put anywhere.  Tokens behind the last sequence are left alone, in q_out too."""
+    if not isinstance(cache, KvCache):
+        raise TypeError("cache: expected a KvCache")
+    tokens = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() == 3 else 0
+    k_token, k_head = _cache_heads(k, cache, None, cache.heads, "k")
+    v_token, v_head = _cache_heads(v, cache, tokens, cache.heads, "v")
+    pages_at, pages_stride, max_pages, lengths_at, starts_at, batch = _sequences(cache, pages, lengths, starts, tokens)
+    plan_at = None
+    if rotary is not None:
+        if not isinstance(rotary, Rotary):
+            raise TypeError("rotary: expected a Rotary")
+        if rotary.dim > cache.head_dim:
+            raise ValueError(f"rotary: turns {rotary.dim} values of heads of {cache.head_dim}")
+        if rotary.turns.device != cache.keys.device:
+            raise ValueError(f"rotary: is on {rotary.turns.device}, the cache on {cache.keys.device}")
+        plan_at = rotary._at
+    q_at, q_token, q_head, q_out_at, q_out_token, q_out_head, q_heads = None, 0, 0, None, 0, 0, 0
+    if q is not None:
+        q_token, q_head = _cache_heads(q, cache, tokens, None, "q")
+        q_heads, q_at = q.shape[1], q.data_ptr()
+        if q_out is None:
+            q_out = q.new_empty(q.shape)
+        q_out_token, q_out_head = _cache_heads(q_out, cache, tokens, q_heads, "q_out")
+        q_out_at = q_out.data_ptr()
+    status = _host.kv_append(cache._at, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head, q_at, q_token, q_head, q_out_at, q_out_token,
+                             q_out_head, q_heads, plan_at, pages_at, pages_stride, max_pages, lengths_at, starts_at, batch, tokens, first, _raw_stream())
+    if status != OK:
+        check(status)
+    return q_out if q is not None else None
+
+
+def _attention(q, cache, prefix, pages, lengths, starts, causal, scale, out, lse):
+    if not isinstance(cache, KvCache):
+        raise TypeError("cache: expected a KvCache")
+    q_token, q_head = _cache_heads(q, cache, None, None, "q")
+    tokens, heads, d = q.shape
+    if heads == 0 or heads % cache.heads:
+        raise ValueError(f"q: {heads} heads over {cache.heads} of the cache")
+    table = _sequences(cache, pages, lengths, starts, tokens)
+    if out is None:
+        out = q.new_empty(tokens, heads, d)
+    out_token, out_head = _cache_heads(out, cache, tokens, heads, "out")
+    lse_at = None
+    if lse is not None:
+        _need(lse, torch.float32, "lse")
+        if lse.shape != (tokens, heads) or lse.device != q.device:
+            raise ValueError(f"lse: expected {tokens} x {heads} on {q.device}, got {tuple(lse.shape)} on {lse.device}")
+        lse_at = lse.data_ptr()
+    held = lib.sarek_hip_attention_workspace_bytes(cache._at, heads, table[5], tokens, table[2], 0 if prefix is None else prefix[1])
+    workspace = q.new_empty(held, dtype=torch.uint8) if held else None
+    tail = (*table, tokens, 1 if causal else 0, d ** -0.5 if scale is None else scale, None if workspace is None else workspace.data_ptr(), held, _raw_stream())
+    head = (cache._at, q.data_ptr(), q_token, q_head, heads, out.data_ptr(), out_token, out_head, lse_at)
+    status = _host.attention_paged(*head, *tail) if prefix is None else _host.attention_shared(*head, *prefix, *tail)
+    if status != OK:
+        check(status)
+    return out
+
+
+def attention_paged(q, cache, pages, lengths, starts=None, causal=True, scale=None, out=None, lse=None):
+    """softmax(scale q . keys) . values of q [tokens, heads, head dim] over a KvCache, whose heads serve as many of q's each as there are;
+    scale None: head dim ^ -1/2.  The sequences' tokens, lengths and pages: as for kv_append, the tokens' own keys are in the cache
+    already.  causal: a token sees its sequence's keys up to its own, otherwise all of them; a token that sees none gets zeros.
+    out: where the result goes; lse (float32 [tokens, heads]): gets the logarithm of the sum of the exponents, -inf where there is none.
+    Rows of tokens behind the last sequence are left as they are."""
+    return _attention(q, cache, None, pages, lengths, starts, causal, scale, out, lse)
+
+
+def attention_shared(q, cache, prefix_pages, prefix_length, pages, lengths, starts=None, causal=True, scale=None, out=None, lse=None):
+    """attention_paged for sequences that all begin with the prefix_length keys of prefix_pages (int32, one page after the other), which
+    are read once for all of them; pages and lengths are of what each sequence has behind the prefix (kv_append puts it there with
+    first=prefix_length)."""
+    if not isinstance(cache, KvCache):
+        raise TypeError("cache: expected a KvCache")
+    at = _table(prefix_pages, (None,), "prefix_pages", cache.keys.device)
+    if not 0 <= prefix_length <= prefix_pages.shape[0] * cache.page_size:
+        raise ValueError(f"prefix_length: {prefix_length} keys in {prefix_pages.shape[0]} pages of {cache.page_size}")
+    return _attention(q, cache, (at if prefix_length else None, prefix_length), pages, lengths, starts, causal, scale, out, lse)
 
 
 def make_args(items):
