@@ -1,11 +1,42 @@
 // Attention over a paged cache (layout: attention_common.hpp): for each token and head, softmax(scale q . keys) . values.
+//
+// All queries that meet the same keys go together: the rows of sequence b and key head h are its tokens times the group of q's heads that
+// share h, and a workgroup takes a tile of them against a stretch of the keys, in one pass over the keys with the running maximum m and
+// sum l of the softmax:
+//   s = scale q . k,   m' = max(m, s),   l' = l 2^(m - m') + sum 2^(s - m'),   o' = o 2^(m - m') + sum 2^(s - m') v
+// in units of log2 (scale log2(e) goes into the scores).  Both products are formed transposed, S^T = K Q^T and O^T = V^T P^T: a lane then has
+// all of its scores from one row, the maximum is one exchange between lanes, and the scores are in the lanes where the second product wants
+// its weights - only the order of the keys in a product differs, and V is read in that order.
+//
+// Two kernels.  Few rows to a sequence (single tokens) are bound by the bytes of the cache: attention_stream_kernel, 16 rows, every wave
+// with its own keys and its own transfers.  Many rows are bound by the matrix unit: attention_tile_kernel, 128 rows that share what a
+// workgroup brings to LDS.  Where rows are few for the card the keys are split into stretches of about the same length, and
+// attention_join_kernel joins what they leave (o, m and l in float32); the tiles and stretches are laid out by every workgroup for itself
+// from the lengths (Plan), which the host does not know.
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 #include "attention_common.hpp"
+#include "gemm_common.hpp"
 
 namespace sarek_hip {
 namespace {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4_t;
+
+// What one launch makes of the rows and keys.
+struct Pass {
+  int prefix;            // rows of all sequences against the prefix, or each sequence's against its own keys
+  int rows, unit;        // of a tile; keys in what a stretch has a whole number of
+  int target;            // about how many workgroups there are to be (0: no stretches, all of a sequence's keys in one)
+  int all;               // everything goes into the planes, for the join
+  int max_slots;
+  float *o;              // [slot][kv head][row][value]
+  f32x2_t *ml;           // [slot][kv head][row]
+};
 
 struct AttentionArgs {
   Batch batch;
@@ -13,68 +44,709 @@ struct AttentionArgs {
   void *out;
   float *lse;
   int64_t q_token, q_head, out_token, out_head;
-  int64_t page, slot, head;         // the cache's strides
-  int heads, group, head_dim, causal;
-  float scale;
+  int64_t page, slot, head, extent;         // the cache's strides and size, bytes
+  int heads, kv_heads, head_dim, causal;
+  Division group;
+  float scale;                              // times log2(e)
   const int *prefix;
   int prefix_length;
 };
 
-template <class T> __device__ __forceinline__ float widen(T v) { return load_one(&v); }
+// ---- which tile and stretch ----------------------------------------------------------------------------------------------------------
 
-// One wave to a token and head, 64 keys at a time: a lane to a key for the scores, a lane to every 64th value for the weighted sum.  The
-// running maximum and sum of the softmax, one pass over the keys.
-template <class T>
-__global__ __launch_bounds__(64) void attention_simple_kernel(AttentionArgs s) {
-  __shared__ float q[256];
-  const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, d = s.head_dim;
-  const int b = sequence_of(s.batch, token);
-  if (b >= s.batch.batch) return;
-  const Tokens mine = tokens_of(s.batch, b);
-  const int length = s.batch.lengths[b];
-  int64_t sees = s.causal ? static_cast<int64_t>(length) - mine.count + (token - mine.first) + 1 : length;
-  const int own = static_cast<int>(max(min(sees, static_cast<int64_t>(keys_held(s.batch, length))), int64_t{0}));
-  for (int i = lane; i < d; i += 64) q[i] = load_one(static_cast<const T *>(s.q) + token * s.q_token + head * s.q_head + i);
+// Inclusive sums over the lanes of a wave, by the row and bank shifts of the data-parallel moves (8 to 20 cycles each; an exchange
+// through LDS takes about 100).
+template <class V> __device__ __forceinline__ V scan_wave(V v) {
+  auto add = [&](auto ctrl, auto rows) {
+    const int moved = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, decltype(rows)::value, 0xF, true);
+    v += __builtin_bit_cast(V, moved);
+  };
+  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});   // row_shr:1, 2, 4, 8
+  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});   // row_bcast:15 into rows 1 and 3
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});   // row_bcast:31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+struct Work {
+  int first, count;      // tokens
+  int length, held;      // keys by lengths, and of these those that the table has room for
+  int tiles, units;
+};
+__device__ __forceinline__ Work work_of(const AttentionArgs &s, const Pass &p, int b) {
+  Work w = {0, 0, 0, 0, 0, 0};
+  if (p.prefix) {
+    if (b != 0) return w;
+    w.count = s.batch.starts ? min(max(s.batch.starts[s.batch.batch], 0), s.batch.tokens) : s.batch.batch;
+    w.length = w.held = s.prefix_length;
+  } else {
+    if (b >= s.batch.batch) return w;
+    const Tokens t = tokens_of(s.batch, b);
+    w.first = t.first, w.count = t.count;
+    w.length = s.batch.lengths[b];
+    w.held = keys_held(s.batch, w.length);
+  }
+  w.tiles = (w.count * static_cast<int>(s.group.size) + p.rows - 1) / p.rows;
+  w.units = (w.held + p.unit - 1) / p.unit;
+  return w;
+}
+__device__ __forceinline__ int sequences(const AttentionArgs &s, const Pass &p) { return p.prefix ? 1 : s.batch.batch; }
+// Units of keys to a stretch, for about p.target workgroups in all; every workgroup comes to the same number.
+__device__ __forceinline__ int units_at_once(const AttentionArgs &s, const Pass &p) {
+  if (p.target == 0) return INT32_MAX;
+  uint64_t all = 0;      // (whole numbers, then nothing but additions: no two kernels may round differently)
+  for (int b = threadIdx.x & 63, n = sequences(s, p); b < n; b += 64) {
+    const Work w = work_of(s, p, b);
+    all += static_cast<uint64_t>(w.tiles) * static_cast<uint32_t>(w.units);
+  }
+  const float total = __builtin_bit_cast(float, lane_of(__builtin_bit_cast(int, scan_wave(static_cast<float>(all))), 63));
+  return max(static_cast<int>(min(ceilf(total * static_cast<float>(s.kv_heads) / static_cast<float>(p.target)), 1e9f)), 1);
+}
+__device__ __forceinline__ int stretches(int units, int at_once) { return max((units + at_once - 1) / max(at_once, 1), 1); }
+
+struct Item {
+  int b;
+  int first, count, length, held;   // the sequence's, as above
+  int row0;                         // the tile's first row
+  int begin, end;                   // keys
+  int slot;                         // of the planes; -1: straight to out
+};
+// Tile and stretch number `item`; false past the last.  The last rows of a sequence come first: under a causal mask they have the most keys.
+__device__ __forceinline__ bool find_item(const AttentionArgs &s, const Pass &p, int item, Item &it) {
+  const int at_once = units_at_once(s, p), n = sequences(s, p), lane = threadIdx.x & 63;
+  int items = 0, slots = 0;
+  for (int b0 = 0; b0 < n; b0 += 64) {
+    const Work w = work_of(s, p, b0 + lane);
+    const int cut = stretches(w.units, at_once), mine = w.tiles * cut, kept = p.all || cut > 1 ? mine : 0;
+    const int upto = scan_wave(mine), slots_upto = scan_wave(kept);
+    const uint64_t past = __ballot(items + upto > item);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      const int cut_at = lane_of(cut, at), tiles = lane_of(w.tiles, at), units = lane_of(w.units, at);
+      const int local = item - items - lane_of(upto - mine, at), tile = tiles - 1 - local / cut_at, stretch = local % cut_at;
+      it.b = b0 + at, it.first = lane_of(w.first, at), it.count = lane_of(w.count, at);
+      it.length = lane_of(w.length, at), it.held = lane_of(w.held, at);
+      if (local < 0 || tile < 0) return false;
+      it.row0 = tile * p.rows;
+      it.slot = lane_of(kept, at) ? slots + lane_of(slots_upto - kept, at) + tile * cut_at + stretch : -1;
+      if (it.slot >= p.max_slots) return false;
+      const int keys = (units + cut_at - 1) / cut_at * p.unit;
+      const int last = static_cast<int>(divided(min(it.row0 + p.rows, it.count * static_cast<int>(s.group.size)) - 1, s.group));
+      const int64_t sees = s.causal && !p.prefix ? static_cast<int64_t>(it.length) - it.count + last + 1 : it.held;
+      it.begin = static_cast<int>(min(static_cast<int64_t>(stretch) * keys, static_cast<int64_t>(it.held)));
+      it.end = static_cast<int>(max(min(min(sees, static_cast<int64_t>(it.held)), static_cast<int64_t>(it.begin) + keys), static_cast<int64_t>(it.begin)));
+      return true;
+    }
+    items += lane_of(upto, 63), slots += lane_of(slots_upto, 63);
+  }
+  return false;
+}
+
+// ---- what both kernels share -----------------------------------------------------------------------------------------------------------
+
+// Keys and values of a tile in LDS: rows of 2 D bytes, the 16-byte pieces of a row at places turned by the key's last bits, so that neither
+// 16 keys of a column of pieces (K, ds_read_b128) nor 4 or 8 keys of a pair of them (V, ds_read_b64_tr_b16) meet in a bank.
+template <int D> __device__ __forceinline__ int turn_of_key(int key) { return D >= 128 ? key & 15 : key >> 1 & 7; }
+template <int D> __device__ __forceinline__ int turn_of_value(int key) {
+  return D >= 128 ? (key & 3) << 2 | (key >> 2 & 1) << 1 : (key >> 1 & 1) << 2 | (key >> 2 & 1) << 1;
+}
+
+__device__ const u32x4_t zero_block = {0u, 0u, 0u, 0u};
+
+// Where the rows of keys are.  Near: as an offset of 32 bits from the head's first, past the end (where a transfer brings zeros) for what is no
+// key; far, for caches past 2^32 bytes: 64 bits, negative for what is no key.
+template <bool Far> struct Rows;
+template <> struct Rows<false> { typedef uint32_t At; static constexpr uint32_t kNone = 0xFFFF0000u; };
+template <> struct Rows<true> { typedef int64_t At; static constexpr int64_t kNone = -1; };
+constexpr int64_t kNearBytes = 0xFFFF0000;
+
+struct Table {
+  const int *pages;
+  int end;               // of the stretch; at least 1
+};
+// The page of a key; any entry of the table for what is past the end.
+__device__ __forceinline__ int page_of(const AttentionArgs &s, const Table &t, int key) {
+  return t.pages[divided(static_cast<uint32_t>(min(key, t.end - 1)), s.batch.page_size)];
+}
+template <bool Far> __device__ __forceinline__ typename Rows<Far>::At row_of(const AttentionArgs &s, const Table &t, int key, int page) {
+  const uint32_t entry = divided(static_cast<uint32_t>(key), s.batch.page_size), in = static_cast<uint32_t>(key) - entry * s.batch.page_size.size;
+  if (key >= t.end || static_cast<uint32_t>(page) >= static_cast<uint32_t>(s.batch.n_pages)) return Rows<Far>::kNone;
+  if constexpr (Far) return page * s.page + in * s.slot;
+  else return static_cast<uint32_t>(page) * static_cast<uint32_t>(s.page) + in * static_cast<uint32_t>(s.slot);
+}
+// One transfer: 16 bytes of a row for each lane, zeros past head_dim.
+template <bool Far>
+__device__ __forceinline__ void move16(const char *base, __amdgpu_buffer_rsrc_t rsrc, typename Rows<Far>::At row, int piece, int pieces, char *to) {
+  if constexpr (Far) {
+    const char *from = row >= 0 && piece < pieces ? base + row + piece * 16 : reinterpret_cast<const char *>(&zero_block);
+    __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) void *>(reinterpret_cast<uintptr_t>(from)),
+                                     (LDS_PTR void *)to, 16, 0, 0);
+  } else {
+    dma16(rsrc, piece < pieces ? row + piece * 16 : Rows<false>::kNone, 0, to);
+  }
+}
+
+template <class T> struct Products;
+template <> struct Products<Bf16> {
+  static __device__ __forceinline__ f32x4_t mul(u32x4 a, u32x4 b, f32x4_t c) { return mfma16<true>(a, b, c); }
+  static __device__ __forceinline__ f32x16_t mul(u32x4 a, u32x4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return f32_pair_to_bf16(lo, hi); }
+  static __device__ __forceinline__ float low(uint32_t v) { return bf16_to_f32(v); }
+  static __device__ __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+  static constexpr uint32_t kExponent = 0x7F80u;
+};
+template <> struct Products<_Float16> {
+  static __device__ __forceinline__ f32x4_t mul(u32x4 a, u32x4 b, f32x4_t c) { return mfma16<false>(a, b, c); }
+  static __device__ __forceinline__ f32x16_t mul(u32x4 a, u32x4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return f32_pair_to_f16(lo, hi); }
+  static __device__ __forceinline__ float low(uint32_t v) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(v))); }
+  static __device__ __forceinline__ float high(uint32_t v) { return low(v >> 16); }
+  static constexpr uint32_t kExponent = 0x7C00u;
+};
+
+// Four consecutive keys of a column of V in each lane: lane i of 16 gives the address of 8 bytes of key i / 4, columns 4 (i % 4) on, and
+// gets the keys of column i.
+__device__ __forceinline__ u32x2_t read_turned(const char *p) {
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_PTR bf16x4_t *)p));
+}
+
+// Infinities and NaNs among values that some rows of the tile see and others do not: the product would bring them into all rows, 0 times
+// infinity being NaN.  They are set to 0 for it (clean), and added to the sums of those rows that see them (what is left of a
+// finite sum by an infinity does not matter).
+template <class T> __device__ __forceinline__ bool any_unbounded(u32x4_t v) {
+  constexpr uint32_t e = Products<T>::kExponent;
+  bool any = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) any |= (v[j] & e) == e || (v[j] >> 16 & e) == e;
+  return any;
+}
+template <class T> __device__ __forceinline__ u32x4_t cleaned(u32x4_t v) {
+  constexpr uint32_t e = Products<T>::kExponent;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if ((v[j] & e) == e) v[j] &= 0xFFFF0000u;
+    if ((v[j] >> 16 & e) == e) v[j] &= 0xFFFFu;
+  }
+  return v;
+}
+
+// The row of q that a lane works for.
+struct Row {
+  bool live;
+  int token, head;       // of the call
+  int limit;             // the keys it sees, at most the stretch's end
+};
+__device__ __forceinline__ Row row_at(const AttentionArgs &s, const Pass &p, const Item &it, int kv_head, int row) {
+  Row r;
+  const int group = static_cast<int>(s.group.size);
+  r.live = row < it.count * group;
+  const int token = static_cast<int>(divided(static_cast<uint32_t>(r.live ? row : 0), s.group));
+  r.token = it.first + token;
+  r.head = kv_head * group + (r.live ? row : 0) - token * group;
+  const int64_t sees = s.causal && !p.prefix ? static_cast<int64_t>(it.length) - it.count + token + 1 : it.held;
+  r.limit = r.live ? static_cast<int>(max(min(sees, static_cast<int64_t>(it.end)), int64_t{0})) : it.end;
+  return r;
+}
+template <class T> __device__ __forceinline__ u32x4 load_q(const AttentionArgs &s, const Row &r, int d) {
+  if (!r.live || d >= s.head_dim) return u32x4{0u, 0u, 0u, 0u};
+  return *reinterpret_cast<const u32x4_any *>(static_cast<const T *>(s.q) + r.token * s.q_token + r.head * s.q_head + d);
+}
+// Four values of a row's result.
+template <class T> __device__ __forceinline__ void store_out(const AttentionArgs &s, int token, int head, int d, f32x4_t v) {
+  typedef u32x2_t u32x2_any __attribute__((aligned(2)));
+  if (d < s.head_dim)
+    *reinterpret_cast<u32x2_any *>(static_cast<T *>(s.out) + token * s.out_token + head * s.out_head + d) =
+        u32x2_t{Products<T>::pack(v[0], v[1]), Products<T>::pack(v[2], v[3])};
+}
+__device__ __forceinline__ void store_lse(const AttentionArgs &s, int token, int head, float m, float l) {
+  if (s.lse) s.lse[static_cast<int64_t>(token) * s.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
+}
+// A maximum may lag behind its row by this much (log2): weights up to 2^8 lose nothing, and the sums are rescaled a few times instead of
+// at every new maximum.
+constexpr float kLag = 8.f;
+
+// ---- few rows ------------------------------------------------------------------------------------------------------------------------
+
+// A wave takes every kWaves-th tile of 32 keys of the stretch by itself: its transfers go into its own part of LDS, one tile ahead, and there
+// is no barrier until the waves' sums are joined at the end.
+constexpr int kStreamKeys = 32;
+template <int D> constexpr int kStreamWaves = D == 64 ? 4 : D == 128 ? 2 : 1;
+
+template <class T, int D, bool Far>
+__global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(AttentionArgs s, Pass p) {
+  constexpr int kWaves = kStreamWaves<D>, kRowBytes = 2 * D, kPieces = D / 8, kKeysMoved = 64 / kPieces, kMoves = kStreamKeys / kKeysMoved;
+  constexpr int kTileBytes = kStreamKeys * kRowBytes, kStage = kWaves * 2 * kTileBytes, kSteps = D / 32, kColumns = D / 16, kPitch = D + 4;
+  static_assert(kWaves * 16 * kPitch * 4 <= kStage && 2 * kMoves < 64, "the waves' sums go into a stage; vmcnt");
+  typedef typename Rows<Far>::At At;
+  typedef Products<T> P;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, quad = lane >> 4;
+  const int kv_head = static_cast<int>(blockIdx.x) % s.kv_heads;
+  Item it;
+  if (!find_item(s, p, static_cast<int>(blockIdx.x) / s.kv_heads, it)) return;
+  const Table table = {p.prefix ? s.prefix : s.batch.pages + it.b * s.batch.pages_stride, it.end};
+  const char *const keys = static_cast<const char *>(s.keys) + kv_head * s.head, *const values = static_cast<const char *>(s.values) + kv_head * s.head;
+  const uint32_t bytes = static_cast<uint32_t>(min(s.extent - kv_head * s.head, kNearBytes));
+  const __amdgpu_buffer_rsrc_t rk = make_rsrc(keys, Far ? 0u : bytes), rv = make_rsrc(values, Far ? 0u : bytes);
+  const int pieces = s.head_dim / 8, tiles = (it.end - it.begin + kStreamKeys - 1) / kStreamKeys;
+  auto key_of = [&](int tile) { return it.begin + tile * kStreamKeys + (lane & 31); };
+  auto issue = [&](char *to, At at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      const int key = i * kKeysMoved + lane / kPieces;
+      const At from = __shfl(at, key, 64);
+      move16<Far>(keys, rk, from, lane % kPieces ^ turn_of_key<D>(key), pieces, to + i * 1024);
+      move16<Far>(values, rv, from, lane % kPieces ^ turn_of_value<D>(key), pieces, to + kTileBytes + i * 1024);
+    }
+  };
+  int t = wave, page = 0;
+  if (t < tiles) {
+    page = page_of(s, table, key_of(t));
+    issue(lds_ring<0, kStage> + wave * 2 * kTileBytes, row_of<Far>(s, table, key_of(t), page));
+    page = page_of(s, table, key_of(t + kWaves));
+  }
+  const Row row = row_at(s, p, it, kv_head, it.row0 + l16);
+  int least = row.limit;
+#pragma unroll
+  for (int x = 1; x < 16; x *= 2) least = min(least, __shfl_xor(least, x, 64));
+  least = __builtin_amdgcn_readfirstlane(least);
+  u32x4 q[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) q[i] = load_q<T>(s, row, i * 32 + quad * 8);
+  f32x4_t o[kColumns];
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c) o[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;      // of this lane's row; l of this lane's keys
+
+  auto tile = [&](const char *from, int key0) __attribute__((always_inline)) {
+    f32x4_t score[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      score[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)
+        score[b] = P::mul(*reinterpret_cast<const u32x4 *>(from + (b * 16 + l16) * kRowBytes + ((i * 4 + quad) ^ turn_of_key<D>(l16)) * 16), q[i], score[b]);
+    }
+    const bool masked = key0 + kStreamKeys > least;
+    if (masked) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (key0 + j / 4 * 16 + quad * 4 + j % 4 >= row.limit) score[j / 4][j % 4] = -INFINITY;
+    }
+    float most = score[0][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) most = fmaxf(most, score[j / 4][j % 4]);
+    most = fmaxf(most, __shfl_xor(most, 16, 64));
+    most = fmaxf(most, __shfl_xor(most, 32, 64));
+    if (__any((most - m) * s.scale > kLag)) {
+      const float now = fmaxf(m, most), keep = now == m ? 1.f : __builtin_amdgcn_exp2f((m - now) * s.scale);
+      m = now;
+      l *= keep;
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) o[c] *= keep;
+    }
+    const float offset = m == -INFINITY ? 0.f : m * s.scale;
+    // The weights go into the product in two parts of the type, the second what the first's rounding has left: the matrix unit is idle for most of the
+    // time here, and the sums are those of 32-bit weights.
+    u32x4 big, small;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j / 2][j % 2 * 2], s.scale, -offset));
+      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j / 2][j % 2 * 2 + 1], s.scale, -offset));
+      l += x + y;
+      big[j] = P::pack(x, y);
+      small[j] = P::pack(x - P::low(big[j]), y - P::high(big[j]));
+    }
+    const char *const v = from + kTileBytes;
+    auto products = [&](auto clean) __attribute__((always_inline)) {
+      const int key = quad * 4 + (l16 >> 2);
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) {
+        const char *const at = v + key * kRowBytes + (2 * c ^ turn_of_value<D>(key)) * 16 + (l16 & 3) * 8;
+        const u32x2_t lo = read_turned(at), hi = read_turned(at + 16 * kRowBytes);
+        u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
+        if constexpr (decltype(clean)::value) a = cleaned<T>(a);
+        o[c] = P::mul(a, big, o[c]);
+        o[c] = P::mul(a, small, o[c]);
+      }
+    };
+    bool unbounded = false;
+    if (masked && least < it.end) {
+#pragma unroll
+      for (int i = 0; i < kMoves; ++i) unbounded |= any_unbounded<T>(*reinterpret_cast<const u32x4 *>(v + i * 1024 + lane * 16));
+      unbounded = __any(unbounded);
+    }
+    if (unbounded) {
+      for (int key = 0; key < kStreamKeys; ++key) {
+        if (key0 + key >= row.limit) continue;
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int d = c * 16 + quad * 4 + j;
+            const uint32_t x = *reinterpret_cast<const uint16_t *>(v + key * kRowBytes + (d / 8 ^ turn_of_value<D>(key)) * 16 + d % 8 * 2);
+            if ((x & P::kExponent) == P::kExponent) o[c][j] += P::low(x);
+          }
+      }
+      products(std::true_type{});
+    } else {
+      products(std::false_type{});
+    }
+  };
+  auto turn = [&]<int I>(std::integral_constant<int, I>) __attribute__((always_inline)) {
+    if (t + kWaves < tiles) {
+      issue(lds_ring<1 - I, kStage> + wave * 2 * kTileBytes, row_of<Far>(s, table, key_of(t + kWaves), page));
+      page = page_of(s, table, key_of(t + 2 * kWaves));
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(2 * kMoves));   // (the next tile's transfers may be under way)
+    } else {
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));
+    }
+    asm volatile("" ::: "memory");
+    tile(lds_ring<I, kStage> + wave * 2 * kTileBytes, it.begin + t * kStreamKeys);
+    t += kWaves;
+  };
+  while (t < tiles) {
+    turn(std::integral_constant<int, 0>{});
+    if (t < tiles) turn(std::integral_constant<int, 1>{});
+  }
+
+  // The waves' sums
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
   __syncthreads();
-  float most = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int part = 0; part < 2; ++part) {
-    const int keys = part ? own : s.prefix_length;
-    const int *const table = part ? s.batch.pages + b * s.batch.pages_stride : s.prefix;
-    for (int k0 = 0; k0 < keys; k0 += 64) {
-      const int key = k0 + lane;
-      float score = -INFINITY;
-      int64_t at = -1;
-      if (key < keys) {
-        const uint32_t entry = divided(key, s.batch.page_size);
-        const int page = table[entry];
-        score = 0.f;
-        if (page >= 0 && page < s.batch.n_pages) {
-          at = page * s.page + (key - static_cast<int64_t>(entry) * s.batch.page_size.size) * s.slot + head / s.group * s.head;
-          const T *const k = static_cast<const T *>(s.keys) + at;
-          for (int i = 0; i < d; ++i) score += q[i] * load_one(k + i);
+  float *const sums = reinterpret_cast<float *>(lds_ring<0, kStage>), *const ends = reinterpret_cast<float *>(lds_ring<1, kStage>);
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c) *reinterpret_cast<f32x4_t *>(sums + (wave * 16 + l16) * kPitch + c * 16 + quad * 4) = o[c];
+  if (quad == 0) ends[(wave * 16 + l16) * 2] = m * s.scale, ends[(wave * 16 + l16) * 2 + 1] = l;
+  __syncthreads();
+  constexpr int kParts = 4 * kWaves;      // threads to a row
+  const int r = threadIdx.x / kParts, part = threadIdx.x % kParts;
+  const Row mine = row_at(s, p, it, kv_head, it.row0 + r);
+  if (!mine.live) return;
+  float most = -INFINITY, total = 0.f, weight[kWaves];
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) most = fmaxf(most, ends[(w * 16 + r) * 2]);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    weight[w] = most == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ends[(w * 16 + r) * 2] - most);
+    total += weight[w] * ends[(w * 16 + r) * 2 + 1];
+  }
+  const float inverse = total == 0.f ? 0.f : 1.f / total;
+  const int64_t place = (static_cast<int64_t>(it.slot) * s.kv_heads + kv_head) * 16 + r;
+  for (int d = part * 4; d < D; d += kParts * 4) {
+    f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v += weight[w] * *reinterpret_cast<const f32x4_t *>(sums + (w * 16 + r) * kPitch + d);
+    if (it.slot < 0) store_out<T>(s, mine.token, mine.head, d, v * inverse);
+    else *reinterpret_cast<f32x4_t *>(p.o + place * D + d) = v;
+  }
+  if (part == 0) {
+    if (it.slot < 0) store_lse(s, mine.token, mine.head, most, total);
+    else p.ml[place] = f32x2_t{most, total};
+  }
+}
+
+// ---- many rows -----------------------------------------------------------------------------------------------------------------------
+
+// Four waves of 32 rows; a tile of keys and values goes to LDS for all of them, the next one while this one is worked on.
+template <int D> constexpr int kTileKeys = D == 256 ? 32 : 64;
+constexpr int kTileRows = 128;
+
+template <class T, int D, bool Far>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(AttentionArgs s, Pass p) {
+  constexpr int kKeys = kTileKeys<D>, kBlocks = kKeys / 32, kRowBytes = 2 * D, kPieces = D / 8, kKeysMoved = 64 / kPieces;
+  constexpr int kTileBytes = kKeys * kRowBytes, kMoves = kTileBytes / 4096, kMine = kMoves * kKeysMoved, kSteps = D / 16, kColumns = D / 32;
+  typedef typename Rows<Far>::At At;
+  typedef Products<T> P;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, l16 = lane & 15, half = lane >> 5;
+  const int kv_head = static_cast<int>(blockIdx.x) % s.kv_heads;
+  Item it;
+  if (!find_item(s, p, static_cast<int>(blockIdx.x) / s.kv_heads, it)) return;
+  const Table table = {p.prefix ? s.prefix : s.batch.pages + it.b * s.batch.pages_stride, it.end};
+  const char *const keys = static_cast<const char *>(s.keys) + kv_head * s.head, *const values = static_cast<const char *>(s.values) + kv_head * s.head;
+  const uint32_t bytes = static_cast<uint32_t>(min(s.extent - kv_head * s.head, kNearBytes));
+  const __amdgpu_buffer_rsrc_t rk = make_rsrc(keys, Far ? 0u : bytes), rv = make_rsrc(values, Far ? 0u : bytes);
+  const int pieces = s.head_dim / 8, tiles = (it.end - it.begin + kKeys - 1) / kKeys;
+  // This wave's transfers bring kMine keys of a tile; lane j looks up the j-th of them.
+  const int mine = lane % kMine, my_key = it.begin + (mine / kKeysMoved * 4 + wave) * kKeysMoved + mine % kKeysMoved;
+  auto issue = [&](char *to, At at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      const int key = (i * 4 + wave) * kKeysMoved + lane / kPieces;
+      const At from = __shfl(at, i * kKeysMoved + lane / kPieces, 64);
+      move16<Far>(keys, rk, from, lane % kPieces ^ turn_of_key<D>(key), pieces, to + (i * 4 + wave) * 1024);
+      move16<Far>(values, rv, from, lane % kPieces ^ turn_of_value<D>(key), pieces, to + kTileBytes + (i * 4 + wave) * 1024);
+    }
+  };
+  int page = 0;
+  if (tiles > 0) {
+    page = page_of(s, table, my_key);
+    issue(lds_ring<2, 2 * kTileBytes>, row_of<Far>(s, table, my_key, page));
+    page = page_of(s, table, my_key + kKeys);
+  }
+  const Row row = row_at(s, p, it, kv_head, it.row0 + wave * 32 + l32);
+  int least = row.limit, most_keys = row.live ? row.limit : it.begin;
+#pragma unroll
+  for (int x = 1; x < 32; x *= 2) least = min(least, __shfl_xor(least, x, 64)), most_keys = max(most_keys, __shfl_xor(most_keys, x, 64));
+  least = __builtin_amdgcn_readfirstlane(least), most_keys = __builtin_amdgcn_readfirstlane(most_keys);
+  u32x4 q[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) q[i] = load_q<T>(s, row, i * 16 + half * 8);
+  f32x16_t o[kColumns];
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[c][j] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  auto tile = [&](const char *from, int key0) __attribute__((always_inline)) {
+    f32x16_t score[kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) score[b][j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)
+        score[b] = P::mul(*reinterpret_cast<const u32x4 *>(from + (b * 32 + l32) * kRowBytes + ((i * 2 + half) ^ turn_of_key<D>(l32)) * 16), q[i], score[b]);
+    }
+    const bool masked = key0 + kKeys > least;
+    if (masked) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (key0 + b * 32 + j / 4 * 8 + half * 4 + j % 4 >= row.limit) score[b][j] = -INFINITY;
+    }
+    float most = score[0][0];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) most = fmaxf(most, score[b][j]);
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+    most = fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+    if (__any((most - m) * s.scale > kLag)) {
+      const float now = fmaxf(m, most), keep = now == m ? 1.f : __builtin_amdgcn_exp2f((m - now) * s.scale);
+      m = now;
+      l *= keep;
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) o[c] *= keep;
+    }
+    const float offset = m == -INFINITY ? 0.f : m * s.scale;
+    u32x4 weights[2 * kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[b][2 * j], s.scale, -offset));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[b][2 * j + 1], s.scale, -offset));
+        l += x + y;
+        weights[2 * b + j / 4][j % 4] = P::pack(x, y);
+      }
+    const char *const v = from + kTileBytes;
+    auto products = [&](auto clean) __attribute__((always_inline)) {
+      const int key = half * 4 + (l16 >> 2);
+#pragma unroll
+      for (int b = 0; b < 2 * kBlocks; ++b)
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) {
+          const char *const at = v + (b * 16 + key) * kRowBytes + ((c * 4 + (l32 >> 4) * 2) ^ turn_of_value<D>(key)) * 16 + (l16 & 3) * 8;
+          const u32x2_t lo = read_turned(at), hi = read_turned(at + 8 * kRowBytes);
+          u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
+          if constexpr (decltype(clean)::value) a = cleaned<T>(a);
+          o[c] = P::mul(a, weights[b], o[c]);
         }
-        score *= s.scale;
+    };
+    bool unbounded = false;
+    if (masked && least < it.end) {
+#pragma unroll
+      for (int i = 0; i < 4 * kMoves; ++i) unbounded |= any_unbounded<T>(*reinterpret_cast<const u32x4 *>(v + i * 1024 + lane * 16));
+      unbounded = __any(unbounded);
+    }
+    if (unbounded) {
+      for (int key = 0; key < kKeys; ++key) {
+        if (key0 + key >= row.limit) continue;
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int d = c * 32 + j / 4 * 8 + half * 4 + j % 4;
+            const uint32_t x = *reinterpret_cast<const uint16_t *>(v + key * kRowBytes + (d / 8 ^ turn_of_value<D>(key)) * 16 + d % 8 * 2);
+            if ((x & P::kExponent) == P::kExponent) o[c][j] += P::low(x);
+          }
       }
-      float top = score;
-      for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
-      const float now = fmaxf(most, top), before = now == most ? 1.f : expf(most - now);
-      const float p = key < keys ? expf(score - now) : 0.f;
-      float total = p;
-      for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x, 64);
-      sum = sum * before + total;
-      most = now;
-      for (int i = 0; i < 4; ++i) o[i] *= before;
-      for (int j = 0; j < min(64, keys - k0); ++j) {
-        const float pj = __shfl(p, j, 64);
-        const int64_t aj = __shfl(at, j, 64);
-        for (int i = 0; i < 4; ++i)
-          if (aj >= 0 && lane + 64 * i < d) o[i] += pj * load_one(static_cast<const T *>(s.values) + aj + lane + 64 * i);
-      }
+      products(std::true_type{});
+    } else {
+      products(std::false_type{});
+    }
+  };
+  auto turn = [&]<int I>(std::integral_constant<int, I>, int t) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));
+    barrier_no_fence();
+    if (t + 1 < tiles) {
+      issue(lds_ring<3 - I, 2 * kTileBytes>, row_of<Far>(s, table, my_key + (t + 1) * kKeys, page));
+      page = page_of(s, table, my_key + (t + 2) * kKeys);
+    }
+    if (it.begin + t * kKeys < most_keys) tile(lds_ring<2 + I, 2 * kTileBytes>, it.begin + t * kKeys);
+  };
+  for (int t = 0; t < tiles; t += 2) {
+    turn(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < tiles) turn(std::integral_constant<int, 1>{}, t + 1);
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  if (!row.live) return;
+  const float inverse = l == 0.f ? 0.f : 1.f / l;
+  const int64_t place = (static_cast<int64_t>(it.slot) * s.kv_heads + kv_head) * kTileRows + wave * 32 + l32;
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4_t v = {o[c][4 * j], o[c][4 * j + 1], o[c][4 * j + 2], o[c][4 * j + 3]};
+      const int d = c * 32 + j * 8 + half * 4;
+      if (it.slot < 0) store_out<T>(s, row.token, row.head, d, v * inverse);
+      else *reinterpret_cast<f32x4_t *>(p.o + place * D + d) = v;
+    }
+  if (half == 0) {
+    if (it.slot < 0) store_lse(s, row.token, row.head, m * s.scale, l);
+    else p.ml[place] = f32x2_t{m * s.scale, l};
+  }
+}
+
+// ---- the stretches' sums ---------------------------------------------------------------------------------------------------------------
+
+// The planes of one sequence: its first slot and how many stretches each of its tiles has; false where it has none.
+__device__ __forceinline__ bool find_planes(const AttentionArgs &s, const Pass &p, int b, int &slot, int &cut) {
+  const int at_once = units_at_once(s, p), lane = threadIdx.x & 63, n = sequences(s, p);
+  int slots = 0;
+  for (int b0 = 0; b0 < n; b0 += 64) {
+    const Work w = work_of(s, p, b0 + lane);
+    const int cuts = stretches(w.units, at_once), kept = p.all || cuts > 1 ? w.tiles * cuts : 0, upto = scan_wave(kept);
+    if (b < b0 + 64) {
+      slot = slots + lane_of(upto - kept, b - b0);
+      cut = lane_of(cuts, b - b0);
+      return lane_of(kept, b - b0) != 0;
+    }
+    slots += lane_of(upto, 63);
+  }
+  return false;
+}
+
+// A workgroup to a token and head: with M the largest of the planes' maxima, l = sum 2^(m - M) l, o = sum 2^(m - M) o / l.
+template <class T, int D> __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs s, Pass own, Pass before) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  __shared__ float sums[kGroups][D], totals[kGroups], tops[4];
+  const int token = blockIdx.x, head = blockIdx.y, b = sequence_of(s.batch, token), group = static_cast<int>(s.group.size);
+  if (b >= s.batch.batch) return;
+  const Tokens tokens = tokens_of(s.batch, b);
+  const int kv_head = head / group, in_group = head - kv_head * group;
+  int counts[2] = {0, 0};
+  int64_t places[2] = {0, 0};        // of the row in its first plane
+  if (before.all) {
+    int slot, cut;
+    const int row = token * group + in_group;
+    if (find_planes(s, before, 0, slot, cut) && (slot += row / before.rows * cut) + cut <= before.max_slots) {
+      counts[0] = cut;
+      places[0] = (static_cast<int64_t>(slot) * s.kv_heads + kv_head) * before.rows + row % before.rows;
     }
   }
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < d) store_one(static_cast<T *>(s.out) + token * s.out_token + head * s.out_head + lane + 64 * i, sum == 0.f ? 0.f : o[i] / sum);
-  if (s.lse && lane == 0) s.lse[static_cast<int64_t>(token) * s.heads + head] = sum == 0.f ? -INFINITY : most + logf(sum);
+  {
+    int slot, cut;
+    const int row = (token - tokens.first) * group + in_group;
+    if (row >= 0 && find_planes(s, own, b, slot, cut) && (slot += row / own.rows * cut) + cut <= own.max_slots) {
+      counts[1] = cut;
+      places[1] = (static_cast<int64_t>(slot) * s.kv_heads + kv_head) * own.rows + row % own.rows;
+    }
+  }
+  const int planes = counts[0] + counts[1];
+  if (planes == 0) return;           // the one workgroup that had the row has written it
+  auto place = [&](int j) { return j < counts[0] ? places[0] + static_cast<int64_t>(j) * s.kv_heads * before.rows : places[1] + static_cast<int64_t>(j - counts[0]) * s.kv_heads * own.rows; };
+  float top = -INFINITY;
+  for (int j = threadIdx.x; j < planes; j += 256) top = fmaxf(top, (j < counts[0] ? before.ml : own.ml)[place(j)][0]);
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const int part = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  for (int j = part; j < planes; j += kGroups) {
+    const f32x2_t ml = (j < counts[0] ? before.ml : own.ml)[place(j)];
+    const float weight = ml[0] == -INFINITY ? (ml[1] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml[0] - top);
+    l += weight * ml[1];
+    if (weight != 0.f) o += weight * *reinterpret_cast<const f32x4_t *>((j < counts[0] ? before.o : own.o) + place(j) * D + d);
+  }
+  *reinterpret_cast<f32x4_t *>(&sums[part][d]) = o;
+  if (d == 0) totals[part] = l;
+  __syncthreads();
+  if (part != 0) return;
+#pragma unroll
+  for (int j = 1; j < kGroups; ++j) o += *reinterpret_cast<const f32x4_t *>(&sums[j][d]), l += totals[j];
+  store_out<T>(s, token, head, d, o * (l == 0.f ? 0.f : 1.f / l));
+  if (d == 0) store_lse(s, token, head, top, l);
+}
+
+// ---- the host's part -------------------------------------------------------------------------------------------------------------------
+
+struct Launch {
+  bool tile;
+  int64_t items;         // for each kv head, at most
+  Pass pass;
+};
+// What the host knows: how many tokens, sequences and keys there are at most.  Stretches: about `target` workgroups where tiles alone are fewer.
+Launch plan(const sarek_hip_kv_cache *cache, int q_heads, int64_t sequences, int64_t tokens, int64_t keys, bool prefix, bool all) {
+  const int d = cache->head_dim;
+  const int64_t rows = tokens * (q_heads / cache->heads), heads = cache->heads;
+  Launch r;
+  r.tile = rows > 16 * sequences;
+  r.pass = {prefix, r.tile ? kTileRows : 16, 0, 0, all, 0, nullptr, nullptr};
+  r.pass.unit = r.tile ? (d <= 128 ? kTileKeys<128> : kTileKeys<256>) : kStreamKeys * (d <= 64 ? kStreamWaves<64> : d <= 128 ? kStreamWaves<128> : kStreamWaves<256>);
+  const int64_t most_tiles = rows / r.pass.rows + sequences, least_tiles = std::max<int64_t>(rows / r.pass.rows, 1), units = ceil_div(keys, r.pass.unit);
+  const int64_t wanted = r.tile ? 2 * compute_units() : 4 * compute_units();
+  if (units > 1 && least_tiles * heads < wanted) r.pass.target = static_cast<int>(wanted);
+  // (the number of units to a stretch comes from a float32 sum: a few items more)
+  r.items = r.pass.target == 0 ? most_tiles : std::min(most_tiles + wanted / heads + 8, most_tiles * units);
+  r.pass.max_slots = static_cast<int>(all ? r.items : r.pass.target == 0 ? 0 : std::min(r.items, 2 * wanted / heads + 8));
+  return r;
+}
+int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+int64_t plane_bytes(const sarek_hip_kv_cache *cache, const Launch &r) {
+  return static_cast<int64_t>(r.pass.max_slots) * cache->heads * r.pass.rows * (padded(cache->head_dim) + 4) * 4;
+}
+// The planes' places in the workspace: o, then m and l.
+char *place_planes(const sarek_hip_kv_cache *cache, Launch *r, char *at) {
+  const int64_t rows = static_cast<int64_t>(r->pass.max_slots) * cache->heads * r->pass.rows;
+  r->pass.o = reinterpret_cast<float *>(at);
+  r->pass.ml = reinterpret_cast<f32x2_t *>(at + rows * padded(cache->head_dim) * 4);
+  return at + plane_bytes(cache, *r);
+}
+
+template <class T, int D> int launch_all(const AttentionArgs &s, const Launch &own, const Launch *before, hipStream_t st) {
+  const bool far = s.extent > kNearBytes;
+  const auto one = [&](const Launch &r) {
+    const dim3 grid(static_cast<unsigned>(r.items * s.kv_heads));
+    if (r.tile) {
+      if (far) hipLaunchKernelGGL((attention_tile_kernel<T, D, true>), grid, dim3(256), 0, st, s, r.pass);
+      else hipLaunchKernelGGL((attention_tile_kernel<T, D, false>), grid, dim3(256), 0, st, s, r.pass);
+    } else {
+      if (far) hipLaunchKernelGGL((attention_stream_kernel<T, D, true>), grid, dim3(64 * kStreamWaves<D>), 0, st, s, r.pass);
+      else hipLaunchKernelGGL((attention_stream_kernel<T, D, false>), grid, dim3(64 * kStreamWaves<D>), 0, st, s, r.pass);
+    }
+    return check_launch("attention launch");
+  };
+  if (before) SAREK_ATTENTION_TRY(one(*before));
+  SAREK_ATTENTION_TRY(one(own));
+  if (own.pass.max_slots == 0) return SAREK_HIP_OK;
+  const Pass none = {0, 1, 1, 0, 0, 0, nullptr, nullptr};
+  hipLaunchKernelGGL((attention_join_kernel<T, D>), dim3(static_cast<unsigned>(s.batch.tokens), static_cast<unsigned>(s.heads)), dim3(256), 0, st, s, own.pass,
+                     before ? before->pass : none);
+  return check_launch("attention join launch");
 }
 
 int attention(const char *what, const sarek_hip_kv_cache *cache, const void *q, int64_t q_token, int64_t q_head, int q_heads, void *out,
@@ -85,7 +757,7 @@ int attention(const char *what, const sarek_hip_kv_cache *cache, const void *q, 
   AttentionArgs s;
   SAREK_ATTENTION_TRY(make_batch(what, cache, pages, pages_stride, max_pages, lengths, starts, batch, tokens, &s.batch));
   if (q_heads < 1 || q_heads % cache->heads != 0) return fail(SAREK_HIP_E_INVALID_ARG, "%s: %d heads of q over %d of the cache", what, q_heads, cache->heads);
-  if (q_heads > 65535) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: more than 65535 heads", what);
+  if (q_heads > 65535 || tokens * q_heads >= int64_t{1} << 30) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: more than 65535 heads, or 2^30 rows", what);
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail(SAREK_HIP_E_INVALID_ARG, "%s: the scale must be positive and finite", what);
   SAREK_ATTENTION_TRY(check_heads(what, "q", q_token, q_head, tokens, q_heads, cache->head_dim, false));
   SAREK_ATTENTION_TRY(check_heads(what, "out", out_token, out_head, tokens, q_heads, cache->head_dim, true));
@@ -96,15 +768,28 @@ int attention(const char *what, const sarek_hip_kv_cache *cache, const void *q, 
     return fail(SAREK_HIP_E_WORKSPACE, "%s: a workspace of %lld bytes, %lld are needed", what, static_cast<long long>(workspace_bytes), static_cast<long long>(need));
   if (tokens == 0 || batch == 0) return SAREK_HIP_OK;
   if (!q || !out || (need > 0 && !workspace)) return fail(SAREK_HIP_E_INVALID_ARG, "%s: NULL pointer", what);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return fail(SAREK_HIP_E_INVALID_ARG, "%s: a workspace starts at a multiple of 16 bytes", what);
+  const int d = cache->head_dim;
   s.q = q, s.keys = cache->keys, s.values = cache->values, s.out = out, s.lse = lse;
   s.q_token = q_token, s.q_head = q_head, s.out_token = out_token, s.out_head = out_head;
-  s.page = cache->page_stride, s.slot = cache->slot_stride, s.head = cache->head_stride;
-  s.heads = q_heads, s.group = q_heads / cache->heads, s.head_dim = cache->head_dim, s.causal = causal != 0, s.scale = scale;
+  s.page = cache->page_stride * 2, s.slot = cache->slot_stride * 2, s.head = cache->head_stride * 2;
+  s.extent = ((cache->n_pages - 1) * cache->page_stride + (cache->page_size - 1) * cache->slot_stride + (cache->heads - 1) * cache->head_stride + d) * 2;
+  s.heads = q_heads, s.kv_heads = cache->heads, s.head_dim = d, s.causal = causal != 0;
+  s.group = division_by(static_cast<uint32_t>(q_heads / cache->heads));
+  s.scale = scale * 1.44269504088896f;
   s.prefix = prefix_pages, s.prefix_length = static_cast<int>(prefix_length);
-  const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(q_heads));
-  if (cache->type == SAREK_HIP_TYPE_BF16) hipLaunchKernelGGL(attention_simple_kernel<Bf16>, grid, dim3(64), 0, as_stream(stream), s);
-  else hipLaunchKernelGGL(attention_simple_kernel<_Float16>, grid, dim3(64), 0, as_stream(stream), s);
-  return check_launch("attention launch");
+  const bool shared = prefix_length > 0;
+  Launch own = plan(cache, q_heads, batch, tokens, static_cast<int64_t>(max_pages) * cache->page_size, false, shared);
+  Launch before = plan(cache, q_heads, 1, tokens, prefix_length, true, true);
+  if (std::max(own.items, before.items) * cache->heads >= int64_t{1} << 24) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: 2^24 tiles of rows or more", what);
+  char *const rest = place_planes(cache, &own, static_cast<char *>(workspace));
+  if (shared) place_planes(cache, &before, rest);
+  const auto run = [&]<class T>(T *) {
+    const hipStream_t st = as_stream(stream);
+    const Launch *const first = shared ? &before : nullptr;
+    return d <= 64 ? launch_all<T, 64>(s, own, first, st) : d <= 128 ? launch_all<T, 128>(s, own, first, st) : launch_all<T, 256>(s, own, first, st);
+  };
+  return cache->type == SAREK_HIP_TYPE_BF16 ? run(static_cast<Bf16 *>(nullptr)) : run(static_cast<_Float16 *>(nullptr));
 }
 
 }  // namespace
@@ -115,8 +800,9 @@ using namespace sarek_hip;
 extern "C" {
 
 int64_t sarek_hip_attention_workspace_bytes(const sarek_hip_kv_cache *cache, int q_heads, int batch, int64_t tokens, int max_pages, int64_t prefix_length) {
-  (void)cache, (void)q_heads, (void)batch, (void)tokens, (void)max_pages, (void)prefix_length;
-  return 0;
+  if (!cache || cache->heads < 1 || q_heads < cache->heads || batch < 1 || tokens < 1 || max_pages < 0 || prefix_length < 0) return 0;
+  const Launch own = plan(cache, q_heads, batch, tokens, static_cast<int64_t>(max_pages) * cache->page_size, false, prefix_length > 0);
+  return plane_bytes(cache, own) + (prefix_length > 0 ? plane_bytes(cache, plan(cache, q_heads, 1, tokens, prefix_length, true, true)) : 0);
 }
 
 int sarek_hip_attention_paged(const sarek_hip_kv_cache *cache, const void *q, int64_t q_token, int64_t q_head, int q_heads, void *out,
