@@ -213,28 +213,33 @@ template <> struct Products<_Float16> {
 
 // Four consecutive keys of a column of V in each lane: lane i of 16 gives the address of 8 bytes of key i / 4, columns 4 (i % 4) on, and
 // gets the keys of column i.
-__device__ __forceinline__ u32x2_t read_turned(const char *p) {
-  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_PTR bf16x4_t *)p));
+__device__ __forceinline__ u32x2_t read_turned(const char *lds, int offset) {
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_PTR bf16x4_t *)(lds + offset)));
 }
 
 // Infinities and NaNs among values that some rows of the tile see and others do not: the product would bring them into all rows, 0 times
-// infinity being NaN.  They are set to 0 for it (clean), and added to the sums of those rows that see them (what is left of a
-// finite sum by an infinity does not matter).
-template <class T> __device__ __forceinline__ bool any_unbounded(u32x4_t v) {
-  constexpr uint32_t e = Products<T>::kExponent;
-  bool any = false;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) any |= (v[j] & e) == e || (v[j] >> 16 & e) == e;
-  return any;
-}
-template <class T> __device__ __forceinline__ u32x4_t cleaned(u32x4_t v) {
-  constexpr uint32_t e = Products<T>::kExponent;
+// infinity being NaN.  In tiles that some rows see in part they are set to 0 for the product, and `any` is told; behind the
+// last tile they are then added to the sums of those rows that see them (what else is in such a sum does not matter).
+// largest: the bits of the type's largest number, or 7FFF where all rows see the same keys and nothing is taken out.
+__device__ __forceinline__ u32x4_t cleaned(u32x4_t v, uint16_t largest, uint32_t &any) {
+  typedef __attribute__((ext_vector_type(2))) short s16x2_t;
+  const s16x2_t most = {static_cast<short>(largest), static_cast<short>(largest)};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if ((v[j] & e) == e) v[j] &= 0xFFFF0000u;
-    if ((v[j] >> 16 & e) == e) v[j] &= 0xFFFFu;
+    const s16x2_t over = (most - __builtin_bit_cast(s16x2_t, v[j] & 0x7FFF7FFFu)) >> 15;     // all ones or nothing, in 16 bits each
+    any |= __builtin_bit_cast(uint32_t, over);
+    v[j] &= ~__builtin_bit_cast(uint32_t, over);
   }
   return v;
+}
+// Four neighbouring values of a key's row from memory, the unbounded ones added to a row's sums.
+template <class T> __device__ __forceinline__ void add_unbounded(const char *from, f32x4_t &sums) {
+  const u32x2_t v = *reinterpret_cast<const u32x2_t *>(from);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t x = v[j / 2] >> (j % 2 * 16) & 0xFFFFu;
+    if ((x & Products<T>::kExponent) == Products<T>::kExponent) sums[j] += Products<T>::low(x);
+  }
 }
 
 // The row of q that a lane works for.
@@ -296,45 +301,59 @@ __global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(
   const __amdgpu_buffer_rsrc_t rk = make_rsrc(keys, Far ? 0u : bytes), rv = make_rsrc(values, Far ? 0u : bytes);
   const int pieces = s.head_dim / 8, tiles = (it.end - it.begin + kStreamKeys - 1) / kStreamKeys;
   auto key_of = [&](int tile) { return it.begin + tile * kStreamKeys + (lane & 31); };
+  const int mine = wave * 2 * kTileBytes;      // of a stage
   auto issue = [&](char *to, At at) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kMoves; ++i) {
       const int key = i * kKeysMoved + lane / kPieces;
       const At from = __shfl(at, key, 64);
-      move16<Far>(keys, rk, from, lane % kPieces ^ turn_of_key<D>(key), pieces, to + i * 1024);
-      move16<Far>(values, rv, from, lane % kPieces ^ turn_of_value<D>(key), pieces, to + kTileBytes + i * 1024);
+      move16<Far>(keys, rk, from, lane % kPieces ^ turn_of_key<D>(key), pieces, to + (mine + i * 1024));
+      move16<Far>(values, rv, from, lane % kPieces ^ turn_of_value<D>(key), pieces, to + (mine + kTileBytes + i * 1024));
     }
   };
-  int t = wave, page = 0;
-  if (t < tiles) {
-    page = page_of(s, table, key_of(t));
-    issue(lds_ring<0, kStage> + wave * 2 * kTileBytes, row_of<Far>(s, table, key_of(t), page));
-    page = page_of(s, table, key_of(t + kWaves));
-  }
+  // Loads come in order: the row of q before the first page, a page before the transfers that it is not for.
   const Row row = row_at(s, p, it, kv_head, it.row0 + l16);
+  u32x4 q[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) q[i] = load_q<T>(s, row, i * 32 + quad * 8);
+  int t = wave, page = 0;
+  if (t < tiles) page = page_of(s, table, key_of(t));
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) asm volatile("" : "+v"(q[i]));      // (waits for them here, not in the loop, where it would wait for transfers)
+  if (t < tiles) {
+    const At at = row_of<Far>(s, table, key_of(t), page);
+    page = page_of(s, table, key_of(t + kWaves));
+    asm volatile("" ::: "memory");
+    issue(lds_ring<0, kStage>, at);
+  }
   int least = row.limit;
 #pragma unroll
   for (int x = 1; x < 16; x *= 2) least = min(least, __shfl_xor(least, x, 64));
   least = __builtin_amdgcn_readfirstlane(least);
-  u32x4 q[kSteps];
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) q[i] = load_q<T>(s, row, i * 32 + quad * 8);
   f32x4_t o[kColumns];
 #pragma unroll
   for (int c = 0; c < kColumns; ++c) o[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;      // of this lane's row; l of this lane's keys
 
-  auto tile = [&](const char *from, int key0) __attribute__((always_inline)) {
+  const uint16_t largest = least < it.end ? P::kExponent - 1 : 0x7FFF;
+  uint32_t unbounded = 0;
+  // Where this lane reads: of step i and column tile c an XOR with the piece's number.  (Opaque: sums of pointers hide from the compiler which
+  // array is read, and it would wait for all transfers under way.)
+  int key_at = mine + l16 * kRowBytes + (quad ^ turn_of_key<D>(l16)) * 16;
+  int value_at = mine + (quad * 4 + (l16 >> 2)) * kRowBytes + turn_of_value<D>(quad * 4 + (l16 >> 2)) * 16 + (l16 & 3) * 8;
+  asm volatile("" : "+v"(key_at), "+v"(value_at));
+
+  auto tile = [&](auto masked, const char *from, int key0) __attribute__((always_inline)) {
+    constexpr bool kMasked = decltype(masked)::value;
     f32x4_t score[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       score[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < kSteps; ++i)
-        score[b] = P::mul(*reinterpret_cast<const u32x4 *>(from + (b * 16 + l16) * kRowBytes + ((i * 4 + quad) ^ turn_of_key<D>(l16)) * 16), q[i], score[b]);
+        score[b] = P::mul(*reinterpret_cast<const u32x4 *>(from + ((key_at ^ i << 6) + b * 16 * kRowBytes)), q[i], score[b]);
     }
-    const bool masked = key0 + kStreamKeys > least;
-    if (masked) {
+    if constexpr (kMasked) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (key0 + j / 4 * 16 + quad * 4 + j % 4 >= row.limit) score[j / 4][j % 4] = -INFINITY;
@@ -363,57 +382,52 @@ __global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(
       big[j] = P::pack(x, y);
       small[j] = P::pack(x - P::low(big[j]), y - P::high(big[j]));
     }
-    const char *const v = from + kTileBytes;
-    auto products = [&](auto clean) __attribute__((always_inline)) {
-      const int key = quad * 4 + (l16 >> 2);
 #pragma unroll
-      for (int c = 0; c < kColumns; ++c) {
-        const char *const at = v + key * kRowBytes + (2 * c ^ turn_of_value<D>(key)) * 16 + (l16 & 3) * 8;
-        const u32x2_t lo = read_turned(at), hi = read_turned(at + 16 * kRowBytes);
-        u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
-        if constexpr (decltype(clean)::value) a = cleaned<T>(a);
-        o[c] = P::mul(a, big, o[c]);
-        o[c] = P::mul(a, small, o[c]);
-      }
-    };
-    bool unbounded = false;
-    if (masked && least < it.end) {
-#pragma unroll
-      for (int i = 0; i < kMoves; ++i) unbounded |= any_unbounded<T>(*reinterpret_cast<const u32x4 *>(v + i * 1024 + lane * 16));
-      unbounded = __any(unbounded);
-    }
-    if (unbounded) {
-      for (int key = 0; key < kStreamKeys; ++key) {
-        if (key0 + key >= row.limit) continue;
-#pragma unroll
-        for (int c = 0; c < kColumns; ++c)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int d = c * 16 + quad * 4 + j;
-            const uint32_t x = *reinterpret_cast<const uint16_t *>(v + key * kRowBytes + (d / 8 ^ turn_of_value<D>(key)) * 16 + d % 8 * 2);
-            if ((x & P::kExponent) == P::kExponent) o[c][j] += P::low(x);
-          }
-      }
-      products(std::true_type{});
-    } else {
-      products(std::false_type{});
+    for (int c = 0; c < kColumns; ++c) {
+      const int at = (value_at ^ c << 5) + kTileBytes;
+      const u32x2_t lo = read_turned(from, at), hi = read_turned(from, at + 16 * kRowBytes);
+      u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
+      if constexpr (kMasked) a = cleaned(a, largest, unbounded);
+      o[c] = P::mul(a, big, o[c]);
+      o[c] = P::mul(a, small, o[c]);
     }
   };
   auto turn = [&]<int I>(std::integral_constant<int, I>) __attribute__((always_inline)) {
     if (t + kWaves < tiles) {
-      issue(lds_ring<1 - I, kStage> + wave * 2 * kTileBytes, row_of<Far>(s, table, key_of(t + kWaves), page));
+      const At at = row_of<Far>(s, table, key_of(t + kWaves), page);
       page = page_of(s, table, key_of(t + 2 * kWaves));
+      asm volatile("" ::: "memory");
+      issue(lds_ring<1 - I, kStage>, at);
       __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(2 * kMoves));   // (the next tile's transfers may be under way)
     } else {
       __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));
     }
     asm volatile("" ::: "memory");
-    tile(lds_ring<I, kStage> + wave * 2 * kTileBytes, it.begin + t * kStreamKeys);
+    const int key0 = it.begin + t * kStreamKeys;
+    const char *const from = lds_ring<I, kStage>;
+    if (key0 + kStreamKeys <= least) tile(std::false_type{}, from, key0);
+    else tile(std::true_type{}, from, key0);
     t += kWaves;
   };
   while (t < tiles) {
     turn(std::integral_constant<int, 0>{});
     if (t < tiles) turn(std::integral_constant<int, 1>{});
+  }
+  if (__any(unbounded != 0)) {
+    // Wave by wave the tiles are other ones: the keys from the first that is not seen by all rows on, of this wave's tiles.
+    for (int first = wave; first < tiles; first += kWaves) {
+      const int key0 = it.begin + first * kStreamKeys;
+      if (key0 + kStreamKeys <= least) continue;
+      for (int key = key0; key < min(key0 + kStreamKeys, it.end); ++key) {
+        const int64_t at = row_of<true>(s, table, key, page_of(s, table, key));
+        if (at < 0 || key >= row.limit) continue;
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) {
+          if (c * 16 + quad * 4 < s.head_dim) add_unbounded<T>(values + at + (c * 16 + quad * 4) * 2, o[c]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
   }
 
   // The waves' sums
@@ -427,8 +441,8 @@ __global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(
   __syncthreads();
   constexpr int kParts = 4 * kWaves;      // threads to a row
   const int r = threadIdx.x / kParts, part = threadIdx.x % kParts;
-  const Row mine = row_at(s, p, it, kv_head, it.row0 + r);
-  if (!mine.live) return;
+  const Row to = row_at(s, p, it, kv_head, it.row0 + r);
+  if (!to.live) return;
   float most = -INFINITY, total = 0.f, weight[kWaves];
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) most = fmaxf(most, ends[(w * 16 + r) * 2]);
@@ -443,11 +457,11 @@ __global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) v += weight[w] * *reinterpret_cast<const f32x4_t *>(sums + (w * 16 + r) * kPitch + d);
-    if (it.slot < 0) store_out<T>(s, mine.token, mine.head, d, v * inverse);
+    if (it.slot < 0) store_out<T>(s, to.token, to.head, d, v * inverse);
     else *reinterpret_cast<f32x4_t *>(p.o + place * D + d) = v;
   }
   if (part == 0) {
-    if (it.slot < 0) store_lse(s, mine.token, mine.head, most, total);
+    if (it.slot < 0) store_lse(s, to.token, to.head, most, total);
     else p.ml[place] = f32x2_t{most, total};
   }
 }
@@ -480,8 +494,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(A
     for (int i = 0; i < kMoves; ++i) {
       const int key = (i * 4 + wave) * kKeysMoved + lane / kPieces;
       const At from = __shfl(at, i * kKeysMoved + lane / kPieces, 64);
-      move16<Far>(keys, rk, from, lane % kPieces ^ turn_of_key<D>(key), pieces, to + (i * 4 + wave) * 1024);
-      move16<Far>(values, rv, from, lane % kPieces ^ turn_of_value<D>(key), pieces, to + kTileBytes + (i * 4 + wave) * 1024);
+      move16<Far>(keys, rk, from, lane % kPieces ^ turn_of_key<D>(key), pieces, to + ((i * 4 + wave) * 1024));
+      move16<Far>(values, rv, from, lane % kPieces ^ turn_of_value<D>(key), pieces, to + (kTileBytes + (i * 4 + wave) * 1024));
     }
   };
   int page = 0;
@@ -505,7 +519,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(A
     for (int j = 0; j < 16; ++j) o[c][j] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  auto tile = [&](const char *from, int key0) __attribute__((always_inline)) {
+  const uint16_t largest = least < it.end ? P::kExponent - 1 : 0x7FFF;
+  uint32_t unbounded = 0;
+  // Where this lane reads, as in the other kernel
+  int key_at = l32 * kRowBytes + (half ^ turn_of_key<D>(l32)) * 16;
+  int value_at = (half * 4 + (l16 >> 2)) * kRowBytes + ((l32 >> 4) * 2 ^ turn_of_value<D>(half * 4 + (l16 >> 2))) * 16 + (l16 & 3) * 8;
+  asm volatile("" : "+v"(key_at), "+v"(value_at));
+
+  auto tile = [&](auto masked, const char *from, int key0) __attribute__((always_inline)) {
+    constexpr bool kMasked = decltype(masked)::value;
     f32x16_t score[kBlocks];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
@@ -513,10 +535,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(A
       for (int j = 0; j < 16; ++j) score[b][j] = 0.f;
 #pragma unroll
       for (int i = 0; i < kSteps; ++i)
-        score[b] = P::mul(*reinterpret_cast<const u32x4 *>(from + (b * 32 + l32) * kRowBytes + ((i * 2 + half) ^ turn_of_key<D>(l32)) * 16), q[i], score[b]);
+        score[b] = P::mul(*reinterpret_cast<const u32x4 *>(from + ((key_at ^ i << 5) + b * 32 * kRowBytes)), q[i], score[b]);
     }
-    const bool masked = key0 + kKeys > least;
-    if (masked) {
+    if constexpr (kMasked) {
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
@@ -548,55 +569,51 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(A
         l += x + y;
         weights[2 * b + j / 4][j % 4] = P::pack(x, y);
       }
-    const char *const v = from + kTileBytes;
-    auto products = [&](auto clean) __attribute__((always_inline)) {
-      const int key = half * 4 + (l16 >> 2);
 #pragma unroll
-      for (int b = 0; b < 2 * kBlocks; ++b)
+    for (int b = 0; b < 2 * kBlocks; ++b)
 #pragma unroll
-        for (int c = 0; c < kColumns; ++c) {
-          const char *const at = v + (b * 16 + key) * kRowBytes + ((c * 4 + (l32 >> 4) * 2) ^ turn_of_value<D>(key)) * 16 + (l16 & 3) * 8;
-          const u32x2_t lo = read_turned(at), hi = read_turned(at + 8 * kRowBytes);
-          u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
-          if constexpr (decltype(clean)::value) a = cleaned<T>(a);
-          o[c] = P::mul(a, weights[b], o[c]);
-        }
-    };
-    bool unbounded = false;
-    if (masked && least < it.end) {
-#pragma unroll
-      for (int i = 0; i < 4 * kMoves; ++i) unbounded |= any_unbounded<T>(*reinterpret_cast<const u32x4 *>(v + i * 1024 + lane * 16));
-      unbounded = __any(unbounded);
-    }
-    if (unbounded) {
-      for (int key = 0; key < kKeys; ++key) {
-        if (key0 + key >= row.limit) continue;
-#pragma unroll
-        for (int c = 0; c < kColumns; ++c)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int d = c * 32 + j / 4 * 8 + half * 4 + j % 4;
-            const uint32_t x = *reinterpret_cast<const uint16_t *>(v + key * kRowBytes + (d / 8 ^ turn_of_value<D>(key)) * 16 + d % 8 * 2);
-            if ((x & P::kExponent) == P::kExponent) o[c][j] += P::low(x);
-          }
+      for (int c = 0; c < kColumns; ++c) {
+        const int at = (value_at ^ c << 6) + kTileBytes + b * 16 * kRowBytes;
+        const u32x2_t lo = read_turned(from, at), hi = read_turned(from, at + 8 * kRowBytes);
+        u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
+        if constexpr (kMasked) a = cleaned(a, largest, unbounded);
+        o[c] = P::mul(a, weights[b], o[c]);
       }
-      products(std::true_type{});
-    } else {
-      products(std::false_type{});
-    }
   };
-  auto turn = [&]<int I>(std::integral_constant<int, I>, int t) __attribute__((always_inline)) {
+  auto turn = [&]<int I>(std::integral_constant<int, I>, auto masked, int t) __attribute__((always_inline)) {
     __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));
     barrier_no_fence();
     if (t + 1 < tiles) {
       issue(lds_ring<3 - I, 2 * kTileBytes>, row_of<Far>(s, table, my_key + (t + 1) * kKeys, page));
       page = page_of(s, table, my_key + (t + 2) * kKeys);
     }
-    if (it.begin + t * kKeys < most_keys) tile(lds_ring<2 + I, 2 * kTileBytes>, it.begin + t * kKeys);
+    if (!decltype(masked)::value || it.begin + t * kKeys < most_keys) tile(masked, lds_ring<2 + I, 2 * kTileBytes>, it.begin + t * kKeys);
   };
-  for (int t = 0; t < tiles; t += 2) {
-    turn(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < tiles) turn(std::integral_constant<int, 1>{}, t + 1);
+  // Tiles that all of this wave's rows see, an even number of them, and the others.
+  const int whole = max(min((least - it.begin) / kKeys, tiles), 0) & ~1;
+  for (int t = 0; t < whole; t += 2) {
+    turn(std::integral_constant<int, 0>{}, std::false_type{}, t);
+    turn(std::integral_constant<int, 1>{}, std::false_type{}, t + 1);
+  }
+  for (int t = whole; t < tiles; t += 2) {
+    turn(std::integral_constant<int, 0>{}, std::true_type{}, t);
+    if (t + 1 < tiles) turn(std::integral_constant<int, 1>{}, std::true_type{}, t + 1);
+  }
+  if (__any(unbounded != 0)) {
+    for (int key = it.begin + whole * kKeys; key < it.end; ++key) {
+      const int64_t at = row_of<true>(s, table, key, page_of(s, table, key));
+      if (at < 0 || key >= row.limit) continue;
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f32x4_t v = {o[c][4 * j], o[c][4 * j + 1], o[c][4 * j + 2], o[c][4 * j + 3]};
+          if (c * 32 + j * 8 + half * 4 < s.head_dim) add_unbounded<T>(values + at + (c * 32 + j * 8 + half * 4) * 2, v);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[c][4 * j + k] = v[k];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    }
   }
 
   l += __shfl_xor(l, 32, 64);
