@@ -750,7 +750,7 @@ int sarek_hip_rotary(const sarek_hip_rotary_plan *plan, const void *x, int64_t x
  * token b where starts is NULL; they are the last of its lengths[b] keys.  Key p of sequence b lies in slot p % page_size of the page
  * pages[b * pages_stride + p / page_size], p / page_size < max_pages.  lengths, starts and pages are int32 in device memory and are read
  * when the kernels run.  Keys that the table has no room for are left out; an entry of the table that is no page of the cache is not
- * written to and stands for keys and values of zeros.  Rows of tokens behind the last sequence are left as they are.             */
+ * written to and stands for keys and values of zeros.  Rows of tokens before the first and behind the last sequence are left as they are.             */
 typedef struct {
   void *keys, *values;
   int64_t page_stride, slot_stride, head_stride;

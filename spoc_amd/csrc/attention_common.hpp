@@ -47,7 +47,7 @@ __device__ __forceinline__ Tokens tokens_of(const Batch &s, int b) {
 __device__ __forceinline__ int keys_held(const Batch &s, int length) {
   return max(min(static_cast<int64_t>(length), static_cast<int64_t>(s.max_pages) * s.page_size.size), int64_t{0});
 }
-// The sequence of a token that all lanes of the wave ask for; batch for tokens behind the last sequence.
+// The sequence of a token that all lanes of the wave ask for; batch for tokens behind the last sequence, the first one for those before it.
 __device__ __forceinline__ int sequence_of(const Batch &s, int token) {
   if (!s.starts) return min(token, s.batch);
   int ended = 0;

@@ -19,6 +19,7 @@
 
 #include "attention_common.hpp"
 #include "gemm_common.hpp"
+#include "tunables.hpp"
 
 namespace sarek_hip {
 namespace {
@@ -36,6 +37,7 @@ struct Pass {
   int max_slots;
   float *o;              // [slot][kv head][row][value]
   f32x2_t *ml;           // [slot][kv head][row]
+  u32x2_t *places;       // of each token's first row: its first slot, and the number of its stretches times 256 with its row in the tile
 };
 
 struct AttentionArgs {
@@ -94,17 +96,6 @@ __device__ __forceinline__ Work work_of(const AttentionArgs &s, const Pass &p, i
   return w;
 }
 __device__ __forceinline__ int sequences(const AttentionArgs &s, const Pass &p) { return p.prefix ? 1 : s.batch.batch; }
-// Units of keys to a stretch, for about p.target workgroups in all; every workgroup comes to the same number.
-__device__ __forceinline__ int units_at_once(const AttentionArgs &s, const Pass &p) {
-  if (p.target == 0) return INT32_MAX;
-  uint64_t all = 0;      // (whole numbers, then nothing but additions: no two kernels may round differently)
-  for (int b = threadIdx.x & 63, n = sequences(s, p); b < n; b += 64) {
-    const Work w = work_of(s, p, b);
-    all += static_cast<uint64_t>(w.tiles) * static_cast<uint32_t>(w.units);
-  }
-  const float total = __builtin_bit_cast(float, lane_of(__builtin_bit_cast(int, scan_wave(static_cast<float>(all))), 63));
-  return max(static_cast<int>(min(ceilf(total * static_cast<float>(s.kv_heads) / static_cast<float>(p.target)), 1e9f)), 1);
-}
 __device__ __forceinline__ int stretches(int units, int at_once) { return max((units + at_once - 1) / max(at_once, 1), 1); }
 
 struct Item {
@@ -113,36 +104,55 @@ struct Item {
   int row0;                         // the tile's first row
   int begin, end;                   // keys
   int slot;                         // of the planes; -1: straight to out
+  int stretch, cut;                 // which of how many of the tile
 };
-// Tile and stretch number `item`; false past the last.  The last rows of a sequence come first: under a causal mask they have the most keys.
+// Tile and stretch number `item`; false past the last.  Every workgroup finds its own, from the lengths of all.  The last rows of a sequence
+// come first: under a causal mask they have the most keys.
 __device__ __forceinline__ bool find_item(const AttentionArgs &s, const Pass &p, int item, Item &it) {
-  const int at_once = units_at_once(s, p), n = sequences(s, p), lane = threadIdx.x & 63;
+  const int n = sequences(s, p), lane = threadIdx.x & 63;
+  Work w = work_of(s, p, lane);
+  int at_once = INT32_MAX;           // units of keys to a stretch, for about p.target workgroups in all
+  if (p.target != 0) {
+    uint64_t all = static_cast<uint64_t>(w.tiles) * static_cast<uint32_t>(w.units);
+    for (int b = 64 + lane; b < n; b += 64) {
+      const Work more = work_of(s, p, b);
+      all += static_cast<uint64_t>(more.tiles) * static_cast<uint32_t>(more.units);
+    }
+    const float total = __builtin_bit_cast(float, lane_of(__builtin_bit_cast(int, scan_wave(static_cast<float>(all))), 63));
+    at_once = max(static_cast<int>(min(ceilf(total * static_cast<float>(s.kv_heads) / static_cast<float>(p.target)), 1e9f)), 1);
+  }
   int items = 0, slots = 0;
   for (int b0 = 0; b0 < n; b0 += 64) {
-    const Work w = work_of(s, p, b0 + lane);
+    if (b0 != 0) w = work_of(s, p, b0 + lane);
     const int cut = stretches(w.units, at_once), mine = w.tiles * cut, kept = p.all || cut > 1 ? mine : 0;
     const int upto = scan_wave(mine), slots_upto = scan_wave(kept);
     const uint64_t past = __ballot(items + upto > item);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
-      const int cut_at = lane_of(cut, at), tiles = lane_of(w.tiles, at), units = lane_of(w.units, at);
-      const int local = item - items - lane_of(upto - mine, at), tile = tiles - 1 - local / cut_at, stretch = local % cut_at;
+      const int tiles = lane_of(w.tiles, at), units = lane_of(w.units, at);
+      it.cut = lane_of(cut, at);
+      const int local = item - items - lane_of(upto - mine, at), tile = tiles - 1 - local / it.cut;
       it.b = b0 + at, it.first = lane_of(w.first, at), it.count = lane_of(w.count, at);
       it.length = lane_of(w.length, at), it.held = lane_of(w.held, at);
+      it.stretch = local % it.cut;
       if (local < 0 || tile < 0) return false;
       it.row0 = tile * p.rows;
-      it.slot = lane_of(kept, at) ? slots + lane_of(slots_upto - kept, at) + tile * cut_at + stretch : -1;
+      it.slot = lane_of(kept, at) ? slots + lane_of(slots_upto - kept, at) + tile * it.cut + it.stretch : -1;
       if (it.slot >= p.max_slots) return false;
-      const int keys = (units + cut_at - 1) / cut_at * p.unit;
+      const int keys = (units + it.cut - 1) / it.cut * p.unit;
       const int last = static_cast<int>(divided(min(it.row0 + p.rows, it.count * static_cast<int>(s.group.size)) - 1, s.group));
       const int64_t sees = s.causal && !p.prefix ? static_cast<int64_t>(it.length) - it.count + last + 1 : it.held;
-      it.begin = static_cast<int>(min(static_cast<int64_t>(stretch) * keys, static_cast<int64_t>(it.held)));
+      it.begin = static_cast<int>(min(static_cast<int64_t>(it.stretch) * keys, static_cast<int64_t>(it.held)));
       it.end = static_cast<int>(max(min(min(sees, static_cast<int64_t>(it.held)), static_cast<int64_t>(it.begin) + keys), static_cast<int64_t>(it.begin)));
       return true;
     }
     items += lane_of(upto, 63), slots += lane_of(slots_upto, 63);
   }
   return false;
+}
+// For the join: where the planes of this row's token are, by the workgroup that has its first row in its first stretch.
+__device__ __forceinline__ void tell_place(const Pass &p, const Item &it, int token, int row) {
+  p.places[token] = u32x2_t{static_cast<uint32_t>(it.slot), it.slot < 0 ? 0u : static_cast<uint32_t>(it.cut) << 8 | static_cast<uint32_t>(row)};
 }
 
 // ---- what both kernels share -----------------------------------------------------------------------------------------------------------
@@ -463,6 +473,7 @@ __global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(
   if (part == 0) {
     if (it.slot < 0) store_lse(s, to.token, to.head, most, total);
     else p.ml[place] = f32x2_t{most, total};
+    if (p.places && it.stretch == 0 && to.head == 0) tell_place(p, it, to.token, r);
   }
 }
 
@@ -632,79 +643,69 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(A
   if (half == 0) {
     if (it.slot < 0) store_lse(s, row.token, row.head, m * s.scale, l);
     else p.ml[place] = f32x2_t{m * s.scale, l};
+    if (p.places && it.stretch == 0 && row.head == 0) tell_place(p, it, row.token, wave * 32 + l32);
   }
 }
 
 // ---- the stretches' sums ---------------------------------------------------------------------------------------------------------------
 
-// The planes of one sequence: its first slot and how many stretches each of its tiles has; false where it has none.
-__device__ __forceinline__ bool find_planes(const AttentionArgs &s, const Pass &p, int b, int &slot, int &cut) {
-  const int at_once = units_at_once(s, p), lane = threadIdx.x & 63, n = sequences(s, p);
-  int slots = 0;
-  for (int b0 = 0; b0 < n; b0 += 64) {
-    const Work w = work_of(s, p, b0 + lane);
-    const int cuts = stretches(w.units, at_once), kept = p.all || cuts > 1 ? w.tiles * cuts : 0, upto = scan_wave(kept);
-    if (b < b0 + 64) {
-      slot = slots + lane_of(upto - kept, b - b0);
-      cut = lane_of(cuts, b - b0);
-      return lane_of(kept, b - b0) != 0;
-    }
-    slots += lane_of(upto, 63);
-  }
-  return false;
+// The planes of a row: how many, and the row's place in the first of them.
+struct Planes {
+  int count;
+  int64_t first, step;
+};
+__device__ __forceinline__ Planes planes_of(const AttentionArgs &s, const Pass &p, u32x2_t place, int kv_head, int in_group) {
+  const int cut = static_cast<int>(place[1] >> 8), row = static_cast<int>(place[1] & 255) + in_group, slot = static_cast<int>(place[0]) + row / p.rows * cut;
+  if (cut == 0 || slot < 0 || slot > p.max_slots - cut) return {0, 0, 0};      // (no place either for a token that starts out of order have left out)
+  return {cut, (static_cast<int64_t>(slot) * s.kv_heads + kv_head) * p.rows + row % p.rows, static_cast<int64_t>(s.kv_heads) * p.rows};
 }
 
-// A workgroup to a token and head: with M the largest of the planes' maxima, l = sum 2^(m - M) l, o = sum 2^(m - M) o / l.
-template <class T, int D> __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs s, Pass own, Pass before) {
+// D / 4 threads, `spread` times over, to a token and head: with M the largest of the planes' maxima, l = sum 2^(m - M) l, o = sum 2^(m - M) o / l,
+// every part of the threads with every spread-th plane, and the parts in order.
+template <class T, int D> __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs s, Pass own, Pass before, int spread) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
-  __shared__ float sums[kGroups][D], totals[kGroups], tops[4];
-  const int token = blockIdx.x, head = blockIdx.y, b = sequence_of(s.batch, token), group = static_cast<int>(s.group.size);
-  if (b >= s.batch.batch) return;
-  const Tokens tokens = tokens_of(s.batch, b);
-  const int kv_head = head / group, in_group = head - kv_head * group;
-  int counts[2] = {0, 0};
-  int64_t places[2] = {0, 0};        // of the row in its first plane
-  if (before.all) {
-    int slot, cut;
-    const int row = token * group + in_group;
-    if (find_planes(s, before, 0, slot, cut) && (slot += row / before.rows * cut) + cut <= before.max_slots) {
-      counts[0] = cut;
-      places[0] = (static_cast<int64_t>(slot) * s.kv_heads + kv_head) * before.rows + row % before.rows;
-    }
+  __shared__ float sums[kGroups][D], ends[kGroups][2];
+  const int group = static_cast<int>(s.group.size), part = static_cast<int>(threadIdx.x) / kLanes, d = threadIdx.x % kLanes * 4;
+  const int row = static_cast<int>(blockIdx.x) * (kGroups / spread) + part / spread, token = row / s.heads, head = row - token * s.heads;
+  const bool live = token >= (s.batch.starts ? s.batch.starts[0] : 0) && token < min(s.batch.starts ? s.batch.starts[s.batch.batch] : s.batch.batch, s.batch.tokens);
+  Planes of[2] = {{0, 0, 0}, {0, 0, 0}};
+  if (live) {
+    const int kv_head = head / group, in_group = head - kv_head * group;
+    const u32x2_t place = own.places[token];
+    if (before.all) of[0] = planes_of(s, before, before.places[token], kv_head, in_group);
+    of[1] = planes_of(s, own, place, kv_head, in_group);
   }
-  {
-    int slot, cut;
-    const int row = (token - tokens.first) * group + in_group;
-    if (row >= 0 && find_planes(s, own, b, slot, cut) && (slot += row / own.rows * cut) + cut <= own.max_slots) {
-      counts[1] = cut;
-      places[1] = (static_cast<int64_t>(slot) * s.kv_heads + kv_head) * own.rows + row % own.rows;
-    }
-  }
-  const int planes = counts[0] + counts[1];
-  if (planes == 0) return;           // the one workgroup that had the row has written it
-  auto place = [&](int j) { return j < counts[0] ? places[0] + static_cast<int64_t>(j) * s.kv_heads * before.rows : places[1] + static_cast<int64_t>(j - counts[0]) * s.kv_heads * own.rows; };
-  float top = -INFINITY;
-  for (int j = threadIdx.x; j < planes; j += 256) top = fmaxf(top, (j < counts[0] ? before.ml : own.ml)[place(j)][0]);
-#pragma unroll
-  for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
-  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  const int part = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+  const int planes = of[0].count + of[1].count;      // (none: the one workgroup that had the row has written it)
+  auto place = [&](int j) { return j < of[0].count ? of[0].first + j * of[0].step : of[1].first + (j - of[0].count) * of[1].step; };
+  float top = -INFINITY, l = 0.f;
+#pragma unroll 4
+  for (int j = part % spread; j < planes; j += spread) top = fmaxf(top, (j < of[0].count ? before.ml : own.ml)[place(j)][0]);
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  for (int j = part; j < planes; j += kGroups) {
-    const f32x2_t ml = (j < counts[0] ? before.ml : own.ml)[place(j)];
-    const float weight = ml[0] == -INFINITY ? (ml[1] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml[0] - top);
+#pragma unroll 4
+  for (int j = part % spread; j < planes; j += spread) {
+    const f32x2_t ml = (j < of[0].count ? before.ml : own.ml)[place(j)];
+    const f32x4_t more = *reinterpret_cast<const f32x4_t *>((j < of[0].count ? before.o : own.o) + place(j) * D + d);
+    // (a stretch without a key: m is minus infinity and all else 0; so is the m of one whose scores are all NaN, and its l is NaN)
+    const float weight = ml[0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[0] - top);
     l += weight * ml[1];
-    if (weight != 0.f) o += weight * *reinterpret_cast<const f32x4_t *>((j < counts[0] ? before.o : own.o) + place(j) * D + d);
+    o += weight * more;
   }
-  *reinterpret_cast<f32x4_t *>(&sums[part][d]) = o;
-  if (d == 0) totals[part] = l;
-  __syncthreads();
-  if (part != 0) return;
-#pragma unroll
-  for (int j = 1; j < kGroups; ++j) o += *reinterpret_cast<const f32x4_t *>(&sums[j][d]), l += totals[j];
+  if (spread > 1) {
+    *reinterpret_cast<f32x4_t *>(&sums[part][d]) = o;
+    if (d == 0) ends[part][0] = top, ends[part][1] = l;
+    __syncthreads();
+    if (part % spread != 0) return;
+    const float mine = top;
+    for (int j = 1; j < spread; ++j) top = fmaxf(top, ends[part + j][0]);
+    const float weight = mine == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mine - top);
+    l *= weight, o *= weight;
+    for (int j = 1; j < spread; ++j) {
+      const float w = ends[part + j][0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ends[part + j][0] - top);
+      l += w * ends[part + j][1];
+      o += w * *reinterpret_cast<const f32x4_t *>(&sums[part + j][d]);
+    }
+  }
+  if (planes == 0) return;
   store_out<T>(s, token, head, d, o * (l == 0.f ? 0.f : 1.f / l));
   if (d == 0) store_lse(s, token, head, top, l);
 }
@@ -722,10 +723,10 @@ Launch plan(const sarek_hip_kv_cache *cache, int q_heads, int64_t sequences, int
   const int64_t rows = tokens * (q_heads / cache->heads), heads = cache->heads;
   Launch r;
   r.tile = rows > 16 * sequences;
-  r.pass = {prefix, r.tile ? kTileRows : 16, 0, 0, all, 0, nullptr, nullptr};
+  r.pass = {prefix, r.tile ? kTileRows : 16, 0, 0, all, 0, nullptr, nullptr, nullptr};
   r.pass.unit = r.tile ? (d <= 128 ? kTileKeys<128> : kTileKeys<256>) : kStreamKeys * (d <= 64 ? kStreamWaves<64> : d <= 128 ? kStreamWaves<128> : kStreamWaves<256>);
   const int64_t most_tiles = rows / r.pass.rows + sequences, least_tiles = std::max<int64_t>(rows / r.pass.rows, 1), units = ceil_div(keys, r.pass.unit);
-  const int64_t wanted = r.tile ? 2 * compute_units() : 4 * compute_units();
+  const int64_t wanted = r.tile ? tunable("attention.tile_workgroups", 2 * compute_units()) : tunable("attention.stream_workgroups", 4 * compute_units());
   if (units > 1 && least_tiles * heads < wanted) r.pass.target = static_cast<int>(wanted);
   // (the number of units to a stretch comes from a float32 sum: a few items more)
   r.items = r.pass.target == 0 ? most_tiles : std::min(most_tiles + wanted / heads + 8, most_tiles * units);
@@ -733,15 +734,18 @@ Launch plan(const sarek_hip_kv_cache *cache, int q_heads, int64_t sequences, int
   return r;
 }
 int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-int64_t plane_bytes(const sarek_hip_kv_cache *cache, const Launch &r) {
-  return static_cast<int64_t>(r.pass.max_slots) * cache->heads * r.pass.rows * (padded(cache->head_dim) + 4) * 4;
+int64_t plane_bytes(const sarek_hip_kv_cache *cache, const Launch &r, int64_t tokens) {
+  if (r.pass.max_slots == 0) return 0;
+  return static_cast<int64_t>(r.pass.max_slots) * cache->heads * r.pass.rows * (padded(cache->head_dim) + 2) * 4 + (tokens + 1) / 2 * 16;
 }
-// The planes' places in the workspace: o, then m and l.
-char *place_planes(const sarek_hip_kv_cache *cache, Launch *r, char *at) {
+// The planes' places in the workspace: o, m and l, and where each token's are.
+char *place_planes(const sarek_hip_kv_cache *cache, Launch *r, int64_t tokens, char *at) {
+  if (r->pass.max_slots == 0) return at;
   const int64_t rows = static_cast<int64_t>(r->pass.max_slots) * cache->heads * r->pass.rows;
   r->pass.o = reinterpret_cast<float *>(at);
   r->pass.ml = reinterpret_cast<f32x2_t *>(at + rows * padded(cache->head_dim) * 4);
-  return at + plane_bytes(cache, *r);
+  r->pass.places = reinterpret_cast<u32x2_t *>(at + rows * (padded(cache->head_dim) + 2) * 4);
+  return at + plane_bytes(cache, *r, tokens);
 }
 
 template <class T, int D> int launch_all(const AttentionArgs &s, const Launch &own, const Launch *before, hipStream_t st) {
@@ -760,9 +764,14 @@ template <class T, int D> int launch_all(const AttentionArgs &s, const Launch &o
   if (before) SAREK_ATTENTION_TRY(one(*before));
   SAREK_ATTENTION_TRY(one(own));
   if (own.pass.max_slots == 0) return SAREK_HIP_OK;
-  const Pass none = {0, 1, 1, 0, 0, 0, nullptr, nullptr};
-  hipLaunchKernelGGL((attention_join_kernel<T, D>), dim3(static_cast<unsigned>(s.batch.tokens), static_cast<unsigned>(s.heads)), dim3(256), 0, st, s, own.pass,
-                     before ? before->pass : none);
+  const Pass none = {0, 1, 1, 0, 0, 0, nullptr, nullptr, nullptr};
+  // Rows that are few for the card take more threads each, which share the planes.
+  constexpr int kGroups = 1024 / D;
+  const int64_t rows = static_cast<int64_t>(s.batch.tokens) * s.heads;
+  int spread = 1;
+  while (spread < kGroups && rows * (D / 4) * spread < 512 * compute_units()) spread *= 2;
+  hipLaunchKernelGGL((attention_join_kernel<T, D>), dim3(static_cast<unsigned>(ceil_div(rows, kGroups / spread))), dim3(256), 0, st, s, own.pass,
+                     before ? before->pass : none, spread);
   return check_launch("attention join launch");
 }
 
@@ -799,8 +808,8 @@ int attention(const char *what, const sarek_hip_kv_cache *cache, const void *q, 
   Launch own = plan(cache, q_heads, batch, tokens, static_cast<int64_t>(max_pages) * cache->page_size, false, shared);
   Launch before = plan(cache, q_heads, 1, tokens, prefix_length, true, true);
   if (std::max(own.items, before.items) * cache->heads >= int64_t{1} << 24) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: 2^24 tiles of rows or more", what);
-  char *const rest = place_planes(cache, &own, static_cast<char *>(workspace));
-  if (shared) place_planes(cache, &before, rest);
+  char *const rest = place_planes(cache, &own, tokens, static_cast<char *>(workspace));
+  if (shared) place_planes(cache, &before, tokens, rest);
   const auto run = [&]<class T>(T *) {
     const hipStream_t st = as_stream(stream);
     const Launch *const first = shared ? &before : nullptr;
@@ -819,7 +828,7 @@ extern "C" {
 int64_t sarek_hip_attention_workspace_bytes(const sarek_hip_kv_cache *cache, int q_heads, int batch, int64_t tokens, int max_pages, int64_t prefix_length) {
   if (!cache || cache->heads < 1 || q_heads < cache->heads || batch < 1 || tokens < 1 || max_pages < 0 || prefix_length < 0) return 0;
   const Launch own = plan(cache, q_heads, batch, tokens, static_cast<int64_t>(max_pages) * cache->page_size, false, prefix_length > 0);
-  return plane_bytes(cache, own) + (prefix_length > 0 ? plane_bytes(cache, plan(cache, q_heads, 1, tokens, prefix_length, true, true)) : 0);
+  return plane_bytes(cache, own, tokens) + (prefix_length > 0 ? plane_bytes(cache, plan(cache, q_heads, 1, tokens, prefix_length, true, true), tokens) : 0);
 }
 
 int sarek_hip_attention_paged(const sarek_hip_kv_cache *cache, const void *q, int64_t q_token, int64_t q_head, int q_heads, void *out,

@@ -126,6 +126,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(RotaryArgs r, AppendArgs
   const int token = static_cast<int>(blockIdx.x), b = sequence_of(s.batch, token);
   if (b >= s.batch.batch) return;
   const Tokens mine = tokens_of(s.batch, b);
+  if (token < mine.first) return;
   const int64_t place = static_cast<int64_t>(s.batch.lengths[b]) - mine.count + (token - mine.first);
   const uint32_t entry = place >= 0 && place < INT32_MAX ? divided(static_cast<uint32_t>(place), s.batch.page_size) : 0xFFFFFFFFu;
   int page = -1;

@@ -310,6 +310,33 @@ def test_starts_that_do_not_fit_write_nothing_else(hip, torch_cuda):
     assert (block[:10] == 7).all() and (block[30:] == 7).all() and (cache.keys == 1).all()
 
 
+@pytest.mark.parametrize("prefix", [0, 40])
+@pytest.mark.parametrize("news", [[1, 2, 1], [30, 0, 40]])
+def test_tokens_before_the_first_sequence(hip, torch_cuda, prefix, news):
+    """They are left alone like those behind the last: in a batch that was cut out of a larger one."""
+    gen, dtype, lengths = torch.Generator().manual_seed(15), torch.bfloat16, [500, 20, 70]
+    pages, prefix_pages, n = table(lengths, 16, gen, prefix=-(-prefix // 16))
+    cache = cache_of(hip, n, 16, 2, 64, dtype)
+    fill(cache, pages, lengths, gen)
+    fill(cache, prefix_pages[None], [prefix], gen)
+    ends = [5 + sum(news[:b]) for b in range(4)]
+    q = queries(gen, ends[-1] + 3, 8, 64, dtype)
+    out = torch.full_like(q, 7.0)
+    if prefix:
+        hip.attention_shared(q, cache, prefix_pages, prefix, pages, ints(lengths), starts=ints(ends), out=out)
+    else:
+        hip.attention_paged(q, cache, pages, ints(lengths), starts=ints(ends), out=out)
+    want, tol, _, _ = ref.attention(q, cache.keys, cache.values, pages, lengths, ends, prefix=prefix_pages, prefix_length=prefix)
+    same, worst = ref.compare(out[5:ends[-1]], want[5:ends[-1]], tol[5:ends[-1]])
+    assert same and worst <= 1 and (out[:5] == 7).all() and (out[ends[-1]:] == 7).all()
+    k = torch.full((ends[-1] + 3, 2, 64), 3.0, dtype=dtype, device="cuda")
+    before, q_out = cache.keys.clone(), torch.full_like(q, 7.0)
+    hip.kv_append(k, k, cache, pages, ints(lengths), starts=ints(ends), q=q, q_out=q_out)
+    changed = (cache.keys != before).any(-1).any(-1) & ~before.isnan().any(-1).any(-1)
+    assert int(changed.sum()) == sum(news)
+    assert (q_out[:5] == 7).all() and (q_out[ends[-1]:] == 7).all() and torch.equal(q_out[5:ends[-1]], q[5:ends[-1]])
+
+
 def test_no_tokens_and_no_sequences(hip, torch_cuda):
     cache = cache_of(hip, 4, 16, 2, 64, torch.bfloat16)
     none = torch.empty(0, 4, 64, dtype=torch.bfloat16, device="cuda")
