@@ -479,14 +479,14 @@ __global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(
 
 // ---- many rows -----------------------------------------------------------------------------------------------------------------------
 
-// Four waves of 32 rows; a tile of keys and values goes to LDS for all of them, the next one while this one is worked on.
-template <int D> constexpr int kTileKeys = D == 256 ? 32 : 64;
-constexpr int kTileRows = 128;
+// Four waves of 32 rows; tiles of 32 keys go to LDS for all of them, three ahead.  While the softmax of tile j is on the vector unit, the
+// matrix unit forms the scores of tile j + 1; then come the weighted values of tile j.
+constexpr int kTileKeys = 32, kTileRows = 128, kTileRing = 4;
 
 template <class T, int D, bool Far>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(AttentionArgs s, Pass p) {
-  constexpr int kKeys = kTileKeys<D>, kBlocks = kKeys / 32, kRowBytes = 2 * D, kPieces = D / 8, kKeysMoved = 64 / kPieces;
-  constexpr int kTileBytes = kKeys * kRowBytes, kMoves = kTileBytes / 4096, kMine = kMoves * kKeysMoved, kSteps = D / 16, kColumns = D / 32;
+  constexpr int kRowBytes = 2 * D, kPieces = D / 8, kKeysMoved = 64 / kPieces, kTileBytes = kTileKeys * kRowBytes;
+  constexpr int kMoves = kTileBytes / 4096, kMine = kMoves * kKeysMoved, kSteps = D / 16, kColumns = D / 32;
   typedef typename Rows<Far>::At At;
   typedef Products<T> P;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, l16 = lane & 15, half = lane >> 5;
@@ -497,39 +497,62 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(A
   const char *const keys = static_cast<const char *>(s.keys) + kv_head * s.head, *const values = static_cast<const char *>(s.values) + kv_head * s.head;
   const uint32_t bytes = static_cast<uint32_t>(min(s.extent - kv_head * s.head, kNearBytes));
   const __amdgpu_buffer_rsrc_t rk = make_rsrc(keys, Far ? 0u : bytes), rv = make_rsrc(values, Far ? 0u : bytes);
-  const int pieces = s.head_dim / 8, tiles = (it.end - it.begin + kKeys - 1) / kKeys;
-  // This wave's transfers bring kMine keys of a tile; lane j looks up the j-th of them.
-  const int mine = lane % kMine, my_key = it.begin + (mine / kKeysMoved * 4 + wave) * kKeysMoved + mine % kKeysMoved;
-  auto issue = [&](char *to, At at) __attribute__((always_inline)) {
+  const int pieces = s.head_dim / 8, tiles = (it.end - it.begin + kTileKeys - 1) / kTileKeys;
+  // Loads come in order: the row of q before the first page, a page before the transfers that it is not for.
+  const Row row = row_at(s, p, it, kv_head, it.row0 + wave * 32 + l32);
+  u32x4 q[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) q[i] = load_q<T>(s, row, i * 16 + half * 8);
+  // This wave's transfers bring kMine keys of a tile; lane j looks up the j-th of them.  `from`: the rows of the last tile of keys that was asked
+  // for, whose values are asked for one tile later.
+  const int turn_of_mine = lane % kMine, my_key = it.begin + (turn_of_mine / kKeysMoved * 4 + wave) * kKeysMoved + turn_of_mine % kKeysMoved;
+  int page[kTileRing] = {};      // of this lane's key in the tiles to come, by their places in the ring
+  At from[kMoves];
+#pragma unroll
+  for (int i = 0; i < kMoves; ++i) from[i] = Rows<Far>::kNone;
+  auto look_up = [&](int place, int tile) __attribute__((always_inline)) { page[place] = page_of(s, table, my_key + tile * kTileKeys); };
+  // (A page is looked up a whole round ahead: as loads come in order, waiting for it is waiting for all transfers before it.)
+  auto move_keys = [&](char *to, int place, int tile) __attribute__((always_inline)) {
+    const At at = row_of<Far>(s, table, my_key + tile * kTileKeys, page[place]);
+    look_up(place, tile + kTileRing);
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < kMoves; ++i) {
-      const int key = (i * 4 + wave) * kKeysMoved + lane / kPieces;
-      const At from = __shfl(at, i * kKeysMoved + lane / kPieces, 64);
-      move16<Far>(keys, rk, from, lane % kPieces ^ turn_of_key<D>(key), pieces, to + ((i * 4 + wave) * 1024));
-      move16<Far>(values, rv, from, lane % kPieces ^ turn_of_value<D>(key), pieces, to + (kTileBytes + (i * 4 + wave) * 1024));
+      from[i] = __shfl(at, i * kKeysMoved + lane / kPieces, 64);
+      move16<Far>(keys, rk, from[i], lane % kPieces ^ turn_of_key<D>((i * 4 + wave) * kKeysMoved + lane / kPieces), pieces, to + ((i * 4 + wave) * 1024));
     }
   };
-  int page = 0;
+  auto move_values = [&](char *to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i)
+      move16<Far>(values, rv, from[i], lane % kPieces ^ turn_of_value<D>((i * 4 + wave) * kKeysMoved + lane / kPieces), pieces, to + ((i * 4 + wave) * 1024));
+  };
+  // Transfers come in the order K0 | V0 K1 | V1 K2 | V2 K3 | V3 K4 ...; what is behind the last tile brings zeros.
   if (tiles > 0) {
-    page = page_of(s, table, my_key);
-    issue(lds_ring<2, 2 * kTileBytes>, row_of<Far>(s, table, my_key, page));
-    page = page_of(s, table, my_key + kKeys);
+    look_up(0, 0), look_up(1, 1), look_up(2, 2), look_up(3, 3);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) asm volatile("" : "+v"(q[i]));      // (waits for them here, not in the loop, where it would wait for transfers)
+    move_keys(lds_ring<10, kTileBytes>, 0, 0);
+    move_values(lds_ring<20, kTileBytes>);
+    move_keys(lds_ring<11, kTileBytes>, 1, 1);
+    move_values(lds_ring<21, kTileBytes>);
+    move_keys(lds_ring<12, kTileBytes>, 2, 2);
+    move_values(lds_ring<22, kTileBytes>);
+    move_keys(lds_ring<13, kTileBytes>, 3, 3);
   }
-  const Row row = row_at(s, p, it, kv_head, it.row0 + wave * 32 + l32);
   int least = row.limit, most_keys = row.live ? row.limit : it.begin;
 #pragma unroll
   for (int x = 1; x < 32; x *= 2) least = min(least, __shfl_xor(least, x, 64)), most_keys = max(most_keys, __shfl_xor(most_keys, x, 64));
   least = __builtin_amdgcn_readfirstlane(least), most_keys = __builtin_amdgcn_readfirstlane(most_keys);
-  u32x4 q[kSteps];
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) q[i] = load_q<T>(s, row, i * 16 + half * 8);
-  f32x16_t o[kColumns];
+  f32x16_t o[kColumns], score;
 #pragma unroll
   for (int c = 0; c < kColumns; ++c)
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[c][j] = 0.f;
-  float m = -INFINITY, l = 0.f;
-
+#pragma unroll
+  for (int j = 0; j < 16; ++j) score[j] = 0.f;
+  float m = -INFINITY, l = 0.f, bound = -INFINITY;    // bound: the score from which m is to follow
+  const float lag = kLag / s.scale;
   const uint16_t largest = least < it.end ? P::kExponent - 1 : 0x7FFF;
   uint32_t unbounded = 0;
   // Where this lane reads, as in the other kernel
@@ -537,81 +560,85 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(A
   int value_at = (half * 4 + (l16 >> 2)) * kRowBytes + ((l32 >> 4) * 2 ^ turn_of_value<D>(half * 4 + (l16 >> 2))) * 16 + (l16 & 3) * 8;
   asm volatile("" : "+v"(key_at), "+v"(value_at));
 
-  auto tile = [&](auto masked, const char *from, int key0) __attribute__((always_inline)) {
+  auto scores = [&](const char *k, f32x16_t &sum) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sum[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) sum = P::mul(*reinterpret_cast<const u32x4 *>(k + (key_at ^ i << 5)), q[i], sum);
+  };
+  auto tile = [&](auto masked, const char *next, const char *v, int key0) __attribute__((always_inline)) {
     constexpr bool kMasked = decltype(masked)::value;
-    f32x16_t score[kBlocks];
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) score[b][j] = 0.f;
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i)
-        score[b] = P::mul(*reinterpret_cast<const u32x4 *>(from + ((key_at ^ i << 5) + b * 32 * kRowBytes)), q[i], score[b]);
-    }
     if constexpr (kMasked) {
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (key0 + b * 32 + j / 4 * 8 + half * 4 + j % 4 >= row.limit) score[b][j] = -INFINITY;
+      for (int j = 0; j < 16; ++j)
+        if (key0 + j / 4 * 8 + half * 4 + j % 4 >= row.limit) score[j] = -INFINITY;
     }
-    float most = score[0][0];
+    float most = score[0];
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) most = fmaxf(most, score[b][j]);
+    for (int j = 1; j < 16; ++j) most = fmaxf(most, score[j]);
     const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
     most = fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
-    if (__any((most - m) * s.scale > kLag)) {
+    if (__any(most > bound)) {
       const float now = fmaxf(m, most), keep = now == m ? 1.f : __builtin_amdgcn_exp2f((m - now) * s.scale);
-      m = now;
+      m = now, bound = now + lag;
       l *= keep;
 #pragma unroll
       for (int c = 0; c < kColumns; ++c) o[c] *= keep;
     }
     const float offset = m == -INFINITY ? 0.f : m * s.scale;
-    u32x4 weights[2 * kBlocks];
+    f32x16_t following;
+    scores(next, following);
+    u32x4 weights[2];
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
+    for (int j = 0; j < 8; ++j) {
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[2 * j], s.scale, -offset));
+      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[2 * j + 1], s.scale, -offset));
+      weights[j / 4][j % 4] = P::pack(x, y);
+      l += x + y;
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[b][2 * j], s.scale, -offset));
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[b][2 * j + 1], s.scale, -offset));
-        l += x + y;
-        weights[2 * b + j / 4][j % 4] = P::pack(x, y);
-      }
-#pragma unroll
-    for (int b = 0; b < 2 * kBlocks; ++b)
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int c = 0; c < kColumns; ++c) {
-        const int at = (value_at ^ c << 6) + kTileBytes + b * 16 * kRowBytes;
-        const u32x2_t lo = read_turned(from, at), hi = read_turned(from, at + 8 * kRowBytes);
+        const int at = (value_at ^ c << 6) + b * 16 * kRowBytes;
+        const u32x2_t lo = read_turned(v, at), hi = read_turned(v, at + 8 * kRowBytes);
         u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
         if constexpr (kMasked) a = cleaned(a, largest, unbounded);
         o[c] = P::mul(a, weights[b], o[c]);
       }
+    score = following;
   };
   auto turn = [&]<int I>(std::integral_constant<int, I>, auto masked, int t) __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));
+    // The keys of tile t + 1 and the values of tile t are there when no more than the next two tiles' transfers are under way.
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(4 * kMoves));
     barrier_no_fence();
-    if (t + 1 < tiles) {
-      issue(lds_ring<3 - I, 2 * kTileBytes>, row_of<Far>(s, table, my_key + (t + 1) * kKeys, page));
-      page = page_of(s, table, my_key + (t + 2) * kKeys);
-    }
-    if (!decltype(masked)::value || it.begin + t * kKeys < most_keys) tile(masked, lds_ring<2 + I, 2 * kTileBytes>, it.begin + t * kKeys);
+    move_values(lds_ring<20 + (I + 3) % 4, kTileBytes>);
+    move_keys(lds_ring<10 + I, kTileBytes>, I, t + 4);
+    const int key0 = it.begin + t * kTileKeys;
+    if (!decltype(masked)::value || key0 < most_keys) tile(masked, lds_ring<10 + (I + 1) % 4, kTileBytes>, lds_ring<20 + I, kTileBytes>, key0);
   };
-  // Tiles that all of this wave's rows see, an even number of them, and the others.
-  const int whole = max(min((least - it.begin) / kKeys, tiles), 0) & ~1;
-  for (int t = 0; t < whole; t += 2) {
+  if (tiles > 0) {
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(6 * kMoves));      // the first tile's keys
+    barrier_no_fence();
+    scores(lds_ring<10, kTileBytes>, score);
+  }
+  // Tiles that all of this wave's rows see, a whole number of rounds of the ring, and the others.
+  const int whole = max(min((least - it.begin) / kTileKeys, tiles), 0) & ~3;
+  for (int t = 0; t < whole; t += 4) {
     turn(std::integral_constant<int, 0>{}, std::false_type{}, t);
     turn(std::integral_constant<int, 1>{}, std::false_type{}, t + 1);
+    turn(std::integral_constant<int, 2>{}, std::false_type{}, t + 2);
+    turn(std::integral_constant<int, 3>{}, std::false_type{}, t + 3);
   }
-  for (int t = whole; t < tiles; t += 2) {
+  for (int t = whole; t < tiles; t += 4) {
     turn(std::integral_constant<int, 0>{}, std::true_type{}, t);
     if (t + 1 < tiles) turn(std::integral_constant<int, 1>{}, std::true_type{}, t + 1);
+    if (t + 2 < tiles) turn(std::integral_constant<int, 2>{}, std::true_type{}, t + 2);
+    if (t + 3 < tiles) turn(std::integral_constant<int, 3>{}, std::true_type{}, t + 3);
   }
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));   // the last, empty transfers, before the LDS is released
   if (__any(unbounded != 0)) {
-    for (int key = it.begin + whole * kKeys; key < it.end; ++key) {
+    for (int key = it.begin + whole * kTileKeys; key < it.end; ++key) {
       const int64_t at = row_of<true>(s, table, key, page_of(s, table, key));
       if (at < 0 || key >= row.limit) continue;
 #pragma unroll
@@ -724,7 +751,7 @@ Launch plan(const sarek_hip_kv_cache *cache, int q_heads, int64_t sequences, int
   Launch r;
   r.tile = rows > 16 * sequences;
   r.pass = {prefix, r.tile ? kTileRows : 16, 0, 0, all, 0, nullptr, nullptr, nullptr};
-  r.pass.unit = r.tile ? (d <= 128 ? kTileKeys<128> : kTileKeys<256>) : kStreamKeys * (d <= 64 ? kStreamWaves<64> : d <= 128 ? kStreamWaves<128> : kStreamWaves<256>);
+  r.pass.unit = r.tile ? 2 * kTileKeys : kStreamKeys * (d <= 64 ? kStreamWaves<64> : d <= 128 ? kStreamWaves<128> : kStreamWaves<256>);
   const int64_t most_tiles = rows / r.pass.rows + sequences, least_tiles = std::max<int64_t>(rows / r.pass.rows, 1), units = ceil_div(keys, r.pass.unit);
   const int64_t wanted = r.tile ? tunable("attention.tile_workgroups", 2 * compute_units()) : tunable("attention.stream_workgroups", 4 * compute_units());
   if (units > 1 && least_tiles * heads < wanted) r.pass.target = static_cast<int>(wanted);
