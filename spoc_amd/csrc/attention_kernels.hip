@@ -287,6 +287,53 @@ __device__ __forceinline__ void store_lse(const AttentionArgs &s, int token, int
 // at every new maximum.
 constexpr float kLag = 8.f;
 
+// The planes of a row: how many, and the row's place in the first of them.
+struct Planes {
+  int count;
+  int64_t first, step;
+};
+__device__ __forceinline__ Planes planes_of(const AttentionArgs &s, const Pass &p, u32x2_t place, int kv_head, int in_group) {
+  const int cut = static_cast<int>(place[1] >> 8), row = static_cast<int>(place[1] & 255) + in_group, slot = static_cast<int>(place[0]) + row / p.rows * cut;
+  if (cut == 0 || slot < 0 || slot > p.max_slots - cut) return {0, 0, 0};      // (no place either for a token that starts out of order have left out)
+  return {cut, (static_cast<int64_t>(slot) * s.kv_heads + kv_head) * p.rows + row % p.rows, static_cast<int64_t>(s.kv_heads) * p.rows};
+}
+
+// A row's sums so far, four columns of them, and what is added to them from planes: m and l and o of kAtOnce planes are asked for together.
+struct Sums {
+  float top, l;
+  f32x4_t o;
+};
+template <int D, int kAtOnce> __device__ __forceinline__ void add_planes(const Pass &p, const Planes &of, int d, Sums &a) {
+  for (int j0 = 0; j0 < of.count; j0 += kAtOnce) {
+    f32x2_t ml[kAtOnce];
+    f32x4_t o[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int64_t at = of.first + min(j0 + u, of.count - 1) * of.step;
+      ml[u] = p.ml[at];
+      o[u] = *reinterpret_cast<const f32x4_t *>(p.o + at * D + d);
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) asm volatile("" : "+v"(ml[u]), "+v"(o[u]));      // (all of them on their way: not each where it is used)
+    float top = a.top;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) top = fmaxf(top, ml[u][0]);
+    // (nothing without a key: m is minus infinity and all else 0; so is the m of a stretch whose scores are all NaN, and its l is NaN)
+    const float keep = a.top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(a.top - top);
+    a.top = top;
+    a.l *= keep;
+    a.o *= keep;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const bool there = j0 + u < of.count;      // (past the end: the last one again)
+      const float weight = ml[u][0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[u][0] - top);
+      a.l += there ? weight * ml[u][1] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) a.o[k] += there ? weight * o[u][k] : 0.f;
+    }
+  }
+}
+
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------
 
 // A wave takes every kWaves-th tile of 32 keys of the stretch by itself: its transfers go into its own part of LDS, one tile ahead, and there
@@ -295,7 +342,7 @@ constexpr int kStreamKeys = 32;
 template <int D> constexpr int kStreamWaves = D == 64 ? 4 : D == 128 ? 2 : 1;
 
 template <class T, int D, bool Far>
-__global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(AttentionArgs s, Pass p) {
+__global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(AttentionArgs s, Pass p, Pass before) {
   constexpr int kWaves = kStreamWaves<D>, kRowBytes = 2 * D, kPieces = D / 8, kKeysMoved = 64 / kPieces, kMoves = kStreamKeys / kKeysMoved;
   constexpr int kTileBytes = kStreamKeys * kRowBytes, kStage = kWaves * 2 * kTileBytes, kSteps = D / 32, kColumns = D / 16, kPitch = D + 4;
   static_assert(kWaves * 16 * kPitch * 4 <= kStage && 2 * kMoves < 64, "the waves' sums go into a stage; vmcnt");
@@ -449,31 +496,31 @@ __global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(
   for (int c = 0; c < kColumns; ++c) *reinterpret_cast<f32x4_t *>(sums + (wave * 16 + l16) * kPitch + c * 16 + quad * 4) = o[c];
   if (quad == 0) ends[(wave * 16 + l16) * 2] = m * s.scale, ends[(wave * 16 + l16) * 2 + 1] = l;
   __syncthreads();
-  constexpr int kParts = 4 * kWaves;      // threads to a row
-  const int r = threadIdx.x / kParts, part = threadIdx.x % kParts;
-  const Row to = row_at(s, p, it, kv_head, it.row0 + r);
-  if (!to.live) return;
-  float most = -INFINITY, total = 0.f, weight[kWaves];
+  // Threads by four columns of the rows that there are.  Where there is no other stretch the row is done, but for the prefix's planes.
+  constexpr int kThreads = 64 * kWaves, kQuads = D / 4;
+  const int live = min(16, it.count * static_cast<int>(s.group.size) - it.row0);
+  for (int column = threadIdx.x; column < live * kQuads; column += kThreads) {
+    const int r = column / kQuads, d = column % kQuads * 4;
+    const Row to = row_at(s, p, it, kv_head, it.row0 + r);
+    Sums a = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) most = fmaxf(most, ends[(w * 16 + r) * 2]);
+    for (int w = 0; w < kWaves; ++w) a.top = fmaxf(a.top, ends[(w * 16 + r) * 2]);
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    weight[w] = most == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ends[(w * 16 + r) * 2] - most);
-    total += weight[w] * ends[(w * 16 + r) * 2 + 1];
-  }
-  const float inverse = total == 0.f ? 0.f : 1.f / total;
-  const int64_t place = (static_cast<int64_t>(it.slot) * s.kv_heads + kv_head) * 16 + r;
-  for (int d = part * 4; d < D; d += kParts * 4) {
-    f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) v += weight[w] * *reinterpret_cast<const f32x4_t *>(sums + (w * 16 + r) * kPitch + d);
-    if (it.slot < 0) store_out<T>(s, to.token, to.head, d, v * inverse);
-    else *reinterpret_cast<f32x4_t *>(p.o + place * D + d) = v;
-  }
-  if (part == 0) {
-    if (it.slot < 0) store_lse(s, to.token, to.head, most, total);
-    else p.ml[place] = f32x2_t{most, total};
-    if (p.places && it.stretch == 0 && to.head == 0) tell_place(p, it, to.token, r);
+    for (int w = 0; w < kWaves; ++w) {
+      const float weight = a.top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ends[(w * 16 + r) * 2] - a.top);
+      a.l += weight * ends[(w * 16 + r) * 2 + 1];
+      a.o += weight * *reinterpret_cast<const f32x4_t *>(sums + (w * 16 + r) * kPitch + d);
+    }
+    if (it.slot < 0) {
+      if (before.all) add_planes<D, 16>(before, planes_of(s, before, before.places[to.token], kv_head, to.head - kv_head * static_cast<int>(s.group.size)), d, a);
+      store_out<T>(s, to.token, to.head, d, a.o * (a.l == 0.f ? 0.f : 1.f / a.l));
+      if (d == 0) store_lse(s, to.token, to.head, a.top, a.l);
+    } else {
+      const int64_t at = (static_cast<int64_t>(it.slot) * s.kv_heads + kv_head) * 16 + r;
+      *reinterpret_cast<f32x4_t *>(p.o + at * D + d) = a.o;
+      if (d == 0) p.ml[at] = f32x2_t{a.top, a.l};
+    }
+    if (p.places && it.stretch == 0 && to.head == 0 && d == 0) tell_place(p, it, to.token, r);
   }
 }
 
@@ -676,17 +723,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(A
 
 // ---- the stretches' sums ---------------------------------------------------------------------------------------------------------------
 
-// The planes of a row: how many, and the row's place in the first of them.
-struct Planes {
-  int count;
-  int64_t first, step;
-};
-__device__ __forceinline__ Planes planes_of(const AttentionArgs &s, const Pass &p, u32x2_t place, int kv_head, int in_group) {
-  const int cut = static_cast<int>(place[1] >> 8), row = static_cast<int>(place[1] & 255) + in_group, slot = static_cast<int>(place[0]) + row / p.rows * cut;
-  if (cut == 0 || slot < 0 || slot > p.max_slots - cut) return {0, 0, 0};      // (no place either for a token that starts out of order have left out)
-  return {cut, (static_cast<int64_t>(slot) * s.kv_heads + kv_head) * p.rows + row % p.rows, static_cast<int64_t>(s.kv_heads) * p.rows};
-}
-
 // D / 4 threads, `spread` times over, to a token and head: with M the largest of the planes' maxima, l = sum 2^(m - M) l, o = sum 2^(m - M) o / l,
 // every part of the threads with every spread-th plane, and the parts in order.
 template <class T, int D> __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs s, Pass own, Pass before, int spread) {
@@ -694,47 +730,40 @@ template <class T, int D> __global__ __launch_bounds__(256) void attention_join_
   __shared__ float sums[kGroups][D], ends[kGroups][2];
   const int group = static_cast<int>(s.group.size), part = static_cast<int>(threadIdx.x) / kLanes, d = threadIdx.x % kLanes * 4;
   const int row = static_cast<int>(blockIdx.x) * (kGroups / spread) + part / spread, token = row / s.heads, head = row - token * s.heads;
-  const bool live = token >= (s.batch.starts ? s.batch.starts[0] : 0) && token < min(s.batch.starts ? s.batch.starts[s.batch.batch] : s.batch.batch, s.batch.tokens);
-  Planes of[2] = {{0, 0, 0}, {0, 0, 0}};
-  if (live) {
+  const int end = min(s.batch.starts ? s.batch.starts[s.batch.batch] : s.batch.batch, s.batch.tokens), start = s.batch.starts ? s.batch.starts[0] : 0;
+  const int held = min(token, s.batch.tokens - 1);      // (asked for before it is known whether the token is one)
+  const u32x2_t place = own.places[held], place_before = before.all ? before.places[held] : u32x2_t{0u, 0u};
+  Sums a = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
+  int planes = 0;
+  if (token >= start && token < end) {
     const int kv_head = head / group, in_group = head - kv_head * group;
-    const u32x2_t place = own.places[token];
-    if (before.all) of[0] = planes_of(s, before, before.places[token], kv_head, in_group);
-    of[1] = planes_of(s, own, place, kv_head, in_group);
-  }
-  const int planes = of[0].count + of[1].count;      // (none: the one workgroup that had the row has written it)
-  auto place = [&](int j) { return j < of[0].count ? of[0].first + j * of[0].step : of[1].first + (j - of[0].count) * of[1].step; };
-  float top = -INFINITY, l = 0.f;
-#pragma unroll 4
-  for (int j = part % spread; j < planes; j += spread) top = fmaxf(top, (j < of[0].count ? before.ml : own.ml)[place(j)][0]);
-  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int j = part % spread; j < planes; j += spread) {
-    const f32x2_t ml = (j < of[0].count ? before.ml : own.ml)[place(j)];
-    const f32x4_t more = *reinterpret_cast<const f32x4_t *>((j < of[0].count ? before.o : own.o) + place(j) * D + d);
-    // (a stretch without a key: m is minus infinity and all else 0; so is the m of one whose scores are all NaN, and its l is NaN)
-    const float weight = ml[0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[0] - top);
-    l += weight * ml[1];
-    o += weight * more;
+    auto add = [&](const Pass &p, Planes of) __attribute__((always_inline)) {
+      planes += of.count;
+      of.count = (of.count - part % spread + spread - 1) / spread, of.first += part % spread * of.step, of.step *= spread;
+      if (spread > 1) add_planes<D, 8>(p, of, d, a);
+      else add_planes<D, 4>(p, of, d, a);
+    };
+    if (before.all) add(before, planes_of(s, before, place_before, kv_head, in_group));
+    add(own, planes_of(s, own, place, kv_head, in_group));
   }
   if (spread > 1) {
-    *reinterpret_cast<f32x4_t *>(&sums[part][d]) = o;
-    if (d == 0) ends[part][0] = top, ends[part][1] = l;
+    *reinterpret_cast<f32x4_t *>(&sums[part][d]) = a.o;
+    if (d == 0) ends[part][0] = a.top, ends[part][1] = a.l;
     __syncthreads();
     if (part % spread != 0) return;
-    const float mine = top;
-    for (int j = 1; j < spread; ++j) top = fmaxf(top, ends[part + j][0]);
-    const float weight = mine == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mine - top);
-    l *= weight, o *= weight;
+    const float mine = a.top;
+    for (int j = 1; j < spread; ++j) a.top = fmaxf(a.top, ends[part + j][0]);
+    const float keep = mine == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mine - a.top);
+    a.l *= keep, a.o *= keep;
     for (int j = 1; j < spread; ++j) {
-      const float w = ends[part + j][0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ends[part + j][0] - top);
-      l += w * ends[part + j][1];
-      o += w * *reinterpret_cast<const f32x4_t *>(&sums[part + j][d]);
+      const float weight = ends[part + j][0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ends[part + j][0] - a.top);
+      a.l += weight * ends[part + j][1];
+      a.o += weight * *reinterpret_cast<const f32x4_t *>(&sums[part + j][d]);
     }
   }
-  if (planes == 0) return;
-  store_out<T>(s, token, head, d, o * (l == 0.f ? 0.f : 1.f / l));
-  if (d == 0) store_lse(s, token, head, top, l);
+  if (planes == 0) return;           // the one workgroup that had the row has written it
+  store_out<T>(s, token, head, d, a.o * (a.l == 0.f ? 0.f : 1.f / a.l));
+  if (d == 0) store_lse(s, token, head, a.top, a.l);
 }
 
 // ---- the host's part -------------------------------------------------------------------------------------------------------------------
@@ -744,28 +773,32 @@ struct Launch {
   int64_t items;         // for each kv head, at most
   Pass pass;
 };
+int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+// What the planes of a launch take: o, m and l, and where each token's are.
+int64_t plane_bytes(const sarek_hip_kv_cache *cache, const Launch &r, int64_t tokens) {
+  if (r.pass.max_slots == 0) return 0;
+  const int64_t planes = static_cast<int64_t>(r.pass.max_slots) * cache->heads;
+  return planes * r.pass.rows * (padded(cache->head_dim) + 2) * 4 + (tokens + 1) / 2 * 16;
+}
 // What the host knows: how many tokens, sequences and keys there are at most.  Stretches: about `target` workgroups where tiles alone are fewer.
-Launch plan(const sarek_hip_kv_cache *cache, int q_heads, int64_t sequences, int64_t tokens, int64_t keys, bool prefix, bool all) {
+// own keys behind a prefix: few rows finish with the prefix's planes themselves where they are in one stretch each.
+enum { kAlone, kBehindPrefix, kPrefix };
+Launch plan(const sarek_hip_kv_cache *cache, int q_heads, int64_t sequences, int64_t tokens, int64_t keys, int what) {
   const int d = cache->head_dim;
   const int64_t rows = tokens * (q_heads / cache->heads), heads = cache->heads;
   Launch r;
   r.tile = rows > 16 * sequences;
-  r.pass = {prefix, r.tile ? kTileRows : 16, 0, 0, all, 0, nullptr, nullptr, nullptr};
+  r.pass = {what == kPrefix, r.tile ? kTileRows : 16, 0, 0, 0, 0, nullptr, nullptr, nullptr};
   r.pass.unit = r.tile ? 2 * kTileKeys : kStreamKeys * (d <= 64 ? kStreamWaves<64> : d <= 128 ? kStreamWaves<128> : kStreamWaves<256>);
-  const int64_t most_tiles = rows / r.pass.rows + sequences, least_tiles = std::max<int64_t>(rows / r.pass.rows, 1), units = ceil_div(keys, r.pass.unit);
-  const int64_t wanted = r.tile ? tunable("attention.tile_workgroups", 2 * compute_units()) : tunable("attention.stream_workgroups", 4 * compute_units());
-  if (units > 1 && least_tiles * heads < wanted) r.pass.target = static_cast<int>(wanted);
+  const int64_t most_tiles = rows / r.pass.rows + sequences, tiles = std::max(rows / r.pass.rows, std::min(tokens, sequences)), units = ceil_div(keys, r.pass.unit);
+  const int64_t wanted = r.tile ? tunable("attention.tile_workgroups", compute_units()) : tunable("attention.stream_workgroups", 3 * compute_units());
+  if (units > 1 && tiles * heads < (what == kBehindPrefix && !r.tile ? compute_units() : wanted)) r.pass.target = static_cast<int>(wanted);
+  r.pass.all = what == kPrefix || (what == kBehindPrefix && (r.tile || r.pass.target != 0));
   // (the number of units to a stretch comes from a float32 sum: a few items more)
   r.items = r.pass.target == 0 ? most_tiles : std::min(most_tiles + wanted / heads + 8, most_tiles * units);
-  r.pass.max_slots = static_cast<int>(all ? r.items : r.pass.target == 0 ? 0 : std::min(r.items, 2 * wanted / heads + 8));
+  r.pass.max_slots = static_cast<int>(r.pass.all ? r.items : r.pass.target == 0 ? 0 : std::min(r.items, 2 * wanted / heads + 8));
   return r;
 }
-int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-int64_t plane_bytes(const sarek_hip_kv_cache *cache, const Launch &r, int64_t tokens) {
-  if (r.pass.max_slots == 0) return 0;
-  return static_cast<int64_t>(r.pass.max_slots) * cache->heads * r.pass.rows * (padded(cache->head_dim) + 2) * 4 + (tokens + 1) / 2 * 16;
-}
-// The planes' places in the workspace: o, m and l, and where each token's are.
 char *place_planes(const sarek_hip_kv_cache *cache, Launch *r, int64_t tokens, char *at) {
   if (r->pass.max_slots == 0) return at;
   const int64_t rows = static_cast<int64_t>(r->pass.max_slots) * cache->heads * r->pass.rows;
@@ -777,21 +810,22 @@ char *place_planes(const sarek_hip_kv_cache *cache, Launch *r, int64_t tokens, c
 
 template <class T, int D> int launch_all(const AttentionArgs &s, const Launch &own, const Launch *before, hipStream_t st) {
   const bool far = s.extent > kNearBytes;
+  const Pass none = {0, 1, 1, 0, 0, 0, nullptr, nullptr, nullptr};
   const auto one = [&](const Launch &r) {
+    const Pass &then = before && !r.pass.prefix ? before->pass : none;      // (what the few rows' kernel joins with its own)
     const dim3 grid(static_cast<unsigned>(r.items * s.kv_heads));
     if (r.tile) {
       if (far) hipLaunchKernelGGL((attention_tile_kernel<T, D, true>), grid, dim3(256), 0, st, s, r.pass);
       else hipLaunchKernelGGL((attention_tile_kernel<T, D, false>), grid, dim3(256), 0, st, s, r.pass);
     } else {
-      if (far) hipLaunchKernelGGL((attention_stream_kernel<T, D, true>), grid, dim3(64 * kStreamWaves<D>), 0, st, s, r.pass);
-      else hipLaunchKernelGGL((attention_stream_kernel<T, D, false>), grid, dim3(64 * kStreamWaves<D>), 0, st, s, r.pass);
+      if (far) hipLaunchKernelGGL((attention_stream_kernel<T, D, true>), grid, dim3(64 * kStreamWaves<D>), 0, st, s, r.pass, then);
+      else hipLaunchKernelGGL((attention_stream_kernel<T, D, false>), grid, dim3(64 * kStreamWaves<D>), 0, st, s, r.pass, then);
     }
     return check_launch("attention launch");
   };
   if (before) SAREK_ATTENTION_TRY(one(*before));
   SAREK_ATTENTION_TRY(one(own));
   if (own.pass.max_slots == 0) return SAREK_HIP_OK;
-  const Pass none = {0, 1, 1, 0, 0, 0, nullptr, nullptr, nullptr};
   // Rows that are few for the card take more threads each, which share the planes.
   constexpr int kGroups = 1024 / D;
   const int64_t rows = static_cast<int64_t>(s.batch.tokens) * s.heads;
@@ -832,8 +866,8 @@ int attention(const char *what, const sarek_hip_kv_cache *cache, const void *q, 
   s.scale = scale * 1.44269504088896f;
   s.prefix = prefix_pages, s.prefix_length = static_cast<int>(prefix_length);
   const bool shared = prefix_length > 0;
-  Launch own = plan(cache, q_heads, batch, tokens, static_cast<int64_t>(max_pages) * cache->page_size, false, shared);
-  Launch before = plan(cache, q_heads, 1, tokens, prefix_length, true, true);
+  Launch own = plan(cache, q_heads, batch, tokens, static_cast<int64_t>(max_pages) * cache->page_size, shared ? kBehindPrefix : kAlone);
+  Launch before = plan(cache, q_heads, 1, tokens, prefix_length, kPrefix);
   if (std::max(own.items, before.items) * cache->heads >= int64_t{1} << 24) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: 2^24 tiles of rows or more", what);
   char *const rest = place_planes(cache, &own, tokens, static_cast<char *>(workspace));
   if (shared) place_planes(cache, &before, tokens, rest);
@@ -854,8 +888,8 @@ extern "C" {
 
 int64_t sarek_hip_attention_workspace_bytes(const sarek_hip_kv_cache *cache, int q_heads, int batch, int64_t tokens, int max_pages, int64_t prefix_length) {
   if (!cache || cache->heads < 1 || q_heads < cache->heads || batch < 1 || tokens < 1 || max_pages < 0 || prefix_length < 0) return 0;
-  const Launch own = plan(cache, q_heads, batch, tokens, static_cast<int64_t>(max_pages) * cache->page_size, false, prefix_length > 0);
-  return plane_bytes(cache, own, tokens) + (prefix_length > 0 ? plane_bytes(cache, plan(cache, q_heads, 1, tokens, prefix_length, true, true), tokens) : 0);
+  const Launch own = plan(cache, q_heads, batch, tokens, static_cast<int64_t>(max_pages) * cache->page_size, prefix_length > 0 ? kBehindPrefix : kAlone);
+  return plane_bytes(cache, own, tokens) + (prefix_length > 0 ? plane_bytes(cache, plan(cache, q_heads, 1, tokens, prefix_length, kPrefix), tokens) : 0);
 }
 
 int sarek_hip_attention_paged(const sarek_hip_kv_cache *cache, const void *q, int64_t q_token, int64_t q_head, int q_heads, void *out,

@@ -1,11 +1,14 @@
-// CPython extension spoc_amd._host: the launch calls of spoc_amd/sarek.py, and the operators of spoc_amd/hip.py on microscaled rows, with
-// their argument lists turned into the C ones here.  A launch takes the HIP runtime 2.8 us; building the same structures with ctypes took 2.3 us more for
+// CPython extension spoc_amd._host: the launch calls of spoc_amd/sarek.py, and the operators of spoc_amd/hip.py on microscaled rows and on
+// a paged cache, with their argument lists turned into the C ones here.  A launch takes the HIP runtime 2.8 us; building the same structures with ctypes took 2.3 us more for
 // one kernel and 5.3 us for a pipeline of two.  The entry points are those of the library the ctypes front end has loaded
 // (bind() gets their addresses), so there is one library per process whichever build it is, and their statuses come back
 // to the caller, who turns them into exceptions as for every other entry point.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <climits>
+#include <cmath>
+#include <cstdint>
 #include <cstring>
 #include <tuple>
 #include <type_traits>
@@ -291,6 +294,223 @@ PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(
 PyObject *attention_paged(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_attention_paged, a, n, "attention_paged"); }
 PyObject *attention_shared(PyObject *, PyObject *const *a, Py_ssize_t n) { return call(g_attention_shared, a, n, "attention_shared"); }
 
+// The operators on a paged cache with their tensors as they are.  The ordinary call is looked through and made here: the checks of
+// hip.py take 4 to 8 us of the interpreter, reading what they need of the tensors 0.25 us each.  Whatever is not as it has to be, and a call that
+// fails, gives None, and hip.py, which then goes through it with the same checks, says what it was.
+PyObject *g_tensor, *g_types[3], *g_int32, *g_int64, *g_get_device, *g_raw_stream;   // SAREK_HIP_TYPE_* order
+PyObject *s_shape, *s_stride, *s_dtype, *s_data_ptr, *s_get_device, *s_new_empty;
+decltype(&sarek_hip_attention_workspace_bytes) g_workspace_bytes;
+
+struct Held {      // a new reference, or none
+  PyObject *o;
+  explicit Held(PyObject *p) : o(p) {}
+  ~Held() { Py_XDECREF(o); }
+  Held(const Held &) = delete;
+  Held &operator=(const Held &) = delete;
+};
+struct TensorOf {
+  PyObject *dtype;             // (the type objects live as long as torch does)
+  long long shape[3], stride[3];
+  void *data;
+};
+bool as_longs(PyObject *tuple, int n, long long *out) {
+  if (!tuple || !PyTuple_Check(tuple) || PyTuple_GET_SIZE(tuple) != n) return false;
+  for (int i = 0; i < n; ++i) out[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(tuple, i));
+  return !PyErr_Occurred();
+}
+// A plain tensor of `dims` dimensions on that device, its last dimension adjacent
+bool read(PyObject *t, int dims, long device, TensorOf *out) {
+  if (reinterpret_cast<PyObject *>(Py_TYPE(t)) != g_tensor) return false;
+  const Held where(PyObject_CallMethodNoArgs(t, s_get_device));
+  if (!where.o || PyLong_AsLong(where.o) != device) return false;
+  const Held shape(PyObject_GetAttr(t, s_shape)), stride(PyObject_CallMethodNoArgs(t, s_stride)), dtype(PyObject_GetAttr(t, s_dtype)),
+      data(PyObject_CallMethodNoArgs(t, s_data_ptr));
+  if (!dtype.o || !data.o || !as_longs(shape.o, dims, out->shape) || !as_longs(stride.o, dims, out->stride)) return false;
+  out->dtype = dtype.o;
+  out->data = PyLong_AsVoidPtr(data.o);
+  return !PyErr_Occurred() && (out->stride[dims - 1] == 1 || out->shape[dims - 1] == 1);
+}
+bool same_shape(const TensorOf &a, const TensorOf &b) { return a.shape[0] == b.shape[0] && a.shape[1] == b.shape[1] && a.shape[2] == b.shape[2]; }
+// [tokens, heads, head dim] that go with a cache
+bool read_heads(PyObject *t, long device, PyObject *dtype, long long tokens, long long heads, long long d, TensorOf *out) {
+  return read(t, 3, device, out) && out->dtype == dtype && (tokens < 0 || out->shape[0] == tokens) && (heads < 0 || out->shape[1] == heads) && out->shape[2] == d;
+}
+// The device and its stream; false where an error is set
+bool here(long *device, void **stream) {
+  const Held index(PyObject_CallNoArgs(g_get_device));
+  if (!index.o) return false;
+  const Held raw(PyObject_CallOneArg(g_raw_stream, index.o));
+  if (!raw.o) return false;
+  *device = PyLong_AsLong(index.o);
+  *stream = PyLong_AsVoidPtr(raw.o);
+  return !PyErr_Occurred();
+}
+PyObject *long_way() {
+  PyErr_Clear();
+  Py_RETURN_NONE;
+}
+PyObject *new_like(PyObject *t) {
+  const Held shape(PyObject_GetAttr(t, s_shape));
+  return shape.o ? PyObject_CallMethodOneArg(t, s_new_empty, shape.o) : nullptr;
+}
+template <class Call> bool succeeds(Call call) {
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = call();
+  Py_END_ALLOW_THREADS
+  return status == SAREK_HIP_OK;
+}
+// What a Rotary and a KvCache hold for this: (address, values turned, device) and (address, heads, head dim, device, type)
+struct PlanOf {
+  const sarek_hip_rotary_plan *at;
+  long long dim, device;
+};
+bool read_plan(PyObject *o, PlanOf *out) {
+  long long v[3];
+  if (!as_longs(o, 3, v)) return false;
+  *out = {reinterpret_cast<const sarek_hip_rotary_plan *>(static_cast<uintptr_t>(v[0])), v[1], v[2]};
+  return true;
+}
+struct CacheOf {
+  const sarek_hip_kv_cache *at;
+  long long heads, d, device;
+  PyObject *dtype;
+};
+bool read_cache(PyObject *o, CacheOf *out) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 5) return false;
+  long long v[4];
+  for (int i = 0; i < 4; ++i) v[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(o, i));
+  *out = {reinterpret_cast<const sarek_hip_kv_cache *>(static_cast<uintptr_t>(v[0])), v[1], v[2], v[3], PyTuple_GET_ITEM(o, 4)};
+  return !PyErr_Occurred();
+}
+struct SequencesOf {
+  const int *pages, *lengths, *starts;
+  long long pages_stride;
+  int max_pages, batch;
+};
+bool read_sequences(PyObject *pages, PyObject *lengths, PyObject *starts, long device, long long tokens, SequencesOf *out) {
+  TensorOf p, l, s;
+  if (!read(lengths, 1, device, &l) || l.dtype != g_int32 || !read(pages, 2, device, &p) || p.dtype != g_int32 || p.shape[0] != l.shape[0] ||
+      l.shape[0] > INT32_MAX || p.shape[1] > INT32_MAX)
+    return false;
+  s.data = nullptr;
+  if (starts == Py_None) {
+    if (l.shape[0] != tokens) return false;
+  } else if (!read(starts, 1, device, &s) || s.dtype != g_int32 || s.shape[0] != l.shape[0] + 1) {
+    return false;
+  }
+  *out = {static_cast<const int *>(p.data), static_cast<const int *>(l.data), static_cast<const int *>(s.data),
+          p.stride[0] > p.shape[1] ? p.stride[0] : p.shape[1], static_cast<int>(p.shape[1]), static_cast<int>(l.shape[0])};
+  return true;
+}
+
+// rotary_tensors(x, positions, plan, out or None, inverse) -> out | None
+PyObject *rotary_tensors(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (!g_rotary || !g_tensor || !arity(n, 5, "rotary_tensors")) return long_way();
+  long device;
+  void *stream;
+  TensorOf x, at, to;
+  PlanOf plan;
+  if (!here(&device, &stream) || !read(a[0], 3, device, &x) || !read(a[1], 1, device, &at) || !read_plan(a[2], &plan)) return long_way();
+  int type = 0;
+  while (type < 3 && x.dtype != g_types[type]) ++type;
+  if (type == 3 || (at.dtype != g_int64 && at.dtype != g_int32) || at.shape[0] != x.shape[0] || plan.device != device || plan.dim > x.shape[2] ||
+      x.shape[1] > 65535 || x.shape[2] > 65536)
+    return long_way();
+  const Held out(a[3] == Py_None ? new_like(a[0]) : Py_NewRef(a[3]));
+  if (!out.o || !read(out.o, 3, device, &to) || to.dtype != x.dtype || !same_shape(to, x)) return long_way();
+  const int inverse = a[4] == Py_True;
+  if (!succeeds([&] {
+        return g_rotary(plan.at, x.data, x.stride[0], x.stride[1], type, at.data, at.dtype == g_int64 ? 8 : 4, inverse, to.data, to.stride[0], to.stride[1],
+                        x.shape[0], static_cast<int>(x.shape[1]), static_cast<int>(x.shape[2]), stream);
+      }))
+    return long_way();
+  return Py_NewRef(out.o);
+}
+
+// kv_append_tensors(k, v, cache, pages, lengths, starts or None, plan or None, q or None, q_out or None, first) -> q_out | False without a q | None
+PyObject *kv_append_tensors(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (!g_kv_append || !g_tensor || !arity(n, 10, "kv_append_tensors")) return long_way();
+  long device;
+  void *stream;
+  TensorOf k, v, q, to;
+  CacheOf cache;
+  PlanOf plan = {nullptr, 0, 0};
+  SequencesOf s;
+  if (!here(&device, &stream) || !read_cache(a[2], &cache) || cache.device != device || !read_heads(a[0], device, cache.dtype, -1, cache.heads, cache.d, &k) ||
+      !read_heads(a[1], device, cache.dtype, k.shape[0], cache.heads, cache.d, &v) || !read_sequences(a[3], a[4], a[5], device, k.shape[0], &s))
+    return long_way();
+  if (a[6] != Py_None && (!read_plan(a[6], &plan) || plan.device != device || plan.dim > cache.d)) return long_way();
+  const long long first = PyLong_AsLongLong(a[9]);
+  if (PyErr_Occurred()) return long_way();
+  const bool with_q = a[7] != Py_None;
+  const Held out(!with_q ? Py_NewRef(Py_False) : a[8] == Py_None ? new_like(a[7]) : Py_NewRef(a[8]));
+  q.data = to.data = nullptr, q.stride[0] = q.stride[1] = q.shape[1] = to.stride[0] = to.stride[1] = 0;
+  if (!out.o || (with_q && (!read_heads(a[7], device, cache.dtype, k.shape[0], -1, cache.d, &q) || q.shape[1] > 65535 || q.shape[1] < 1 ||
+                            !read_heads(out.o, device, cache.dtype, k.shape[0], q.shape[1], cache.d, &to))))
+    return long_way();
+  if (!succeeds([&] {
+        return g_kv_append(cache.at, k.data, k.stride[0], k.stride[1], v.data, v.stride[0], v.stride[1], q.data, q.stride[0], q.stride[1], to.data, to.stride[0],
+                           to.stride[1], static_cast<int>(q.shape[1]), plan.at, s.pages, s.pages_stride, s.max_pages, s.lengths, s.starts, s.batch, k.shape[0],
+                           first, stream);
+      }))
+    return long_way();
+  return Py_NewRef(out.o);
+}
+
+// attention_tensors(q, cache, prefix_pages or None, prefix_length, pages, lengths, starts or None, causal, scale or None, out or None, lse or None) -> out | None
+PyObject *attention_tensors(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (!g_attention_shared || !g_tensor || !arity(n, 11, "attention_tensors")) return long_way();
+  long device;
+  void *stream;
+  TensorOf q, to, lse, prefix;
+  CacheOf cache;
+  SequencesOf s;
+  if (!here(&device, &stream) || !read_cache(a[1], &cache) || cache.device != device || !read_heads(a[0], device, cache.dtype, -1, -1, cache.d, &q) ||
+      q.shape[1] < 1 || q.shape[1] > 65535 || q.shape[1] % cache.heads != 0 || !read_sequences(a[4], a[5], a[6], device, q.shape[0], &s))
+    return long_way();
+  prefix.data = lse.data = nullptr;
+  long long prefix_length = 0;
+  if (a[2] != Py_None) {
+    prefix_length = PyLong_AsLongLong(a[3]);
+    if (PyErr_Occurred() || !read(a[2], 1, device, &prefix) || prefix.dtype != g_int32 || prefix_length < 0 || prefix_length > prefix.shape[0] * cache.at->page_size)
+      return long_way();
+  }
+  if (a[10] != Py_None && (!read(a[10], 2, device, &lse) || lse.dtype != g_types[SAREK_HIP_TYPE_F32] || lse.shape[0] != q.shape[0] || lse.shape[1] != q.shape[1] ||
+                           (lse.shape[0] > 1 && lse.stride[0] != lse.shape[1])))
+    return long_way();
+  const int causal = PyObject_IsTrue(a[7]);
+  const double scale = a[8] == Py_None ? 1.0 / std::sqrt(static_cast<double>(cache.d)) : PyFloat_AsDouble(a[8]);
+  if (PyErr_Occurred()) return long_way();
+  const Held out(a[9] == Py_None ? new_like(a[0]) : Py_NewRef(a[9]));
+  if (!out.o || !read_heads(out.o, device, cache.dtype, q.shape[0], q.shape[1], cache.d, &to)) return long_way();
+  const int heads = static_cast<int>(q.shape[1]);
+  const int64_t held = g_workspace_bytes(cache.at, heads, s.batch, q.shape[0], s.max_pages, prefix_length);
+  TensorOf space;
+  space.data = nullptr;
+  const Held values(held > 0 ? Py_BuildValue("(L)", static_cast<long long>(held + 1) / 2) : nullptr);      // of q's type, of 2 bytes
+  const Held workspace(held > 0 ? PyObject_CallMethodOneArg(a[0], s_new_empty, values.o) : nullptr);
+  if (held > 0 && (!workspace.o || !read(workspace.o, 1, device, &space))) return long_way();
+  if (!succeeds([&] {
+        return g_attention_shared(cache.at, q.data, q.stride[0], q.stride[1], heads, to.data, to.stride[0], to.stride[1], static_cast<float *>(lse.data),
+                                  prefix_length > 0 ? static_cast<const int *>(prefix.data) : nullptr, prefix_length, s.pages, s.pages_stride, s.max_pages, s.lengths,
+                                  s.starts, s.batch, q.shape[0], causal, static_cast<float>(scale), space.data, held, stream);
+      }))
+    return long_way();
+  return Py_NewRef(out.o);
+}
+
+// bind_torch(Tensor, float32, bfloat16, float16, int32, int64, _cuda_getDevice, _cuda_getCurrentRawStream, address of attention_workspace_bytes)
+PyObject *bind_torch(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (!arity(n, 9, "bind_torch")) return nullptr;
+  void *const bytes = PyLong_AsVoidPtr(a[8]);
+  if (PyErr_Occurred()) return nullptr;
+  PyObject **const to[8] = {&g_tensor, &g_types[0], &g_types[1], &g_types[2], &g_int32, &g_int64, &g_get_device, &g_raw_stream};
+  for (int i = 0; i < 8; ++i) Py_XSETREF(*to[i], Py_NewRef(a[i]));
+  g_workspace_bytes = reinterpret_cast<decltype(g_workspace_bytes)>(bytes);
+  Py_RETURN_NONE;
+}
+
 // bind(addresses of the first five entry points above, in the order of their declaration)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
   if (!arity(n, 5, "bind")) return nullptr;
@@ -349,6 +569,10 @@ PyMethodDef methods[] = {
     {"kv_append", reinterpret_cast<PyCFunction>(kv_append), METH_FASTCALL, "sarek_hip_kv_append"},
     {"attention_paged", reinterpret_cast<PyCFunction>(attention_paged), METH_FASTCALL, "sarek_hip_attention_paged"},
     {"attention_shared", reinterpret_cast<PyCFunction>(attention_shared), METH_FASTCALL, "sarek_hip_attention_shared"},
+    {"bind_torch", reinterpret_cast<PyCFunction>(bind_torch), METH_FASTCALL, "What the next three need of torch."},
+    {"rotary_tensors", reinterpret_cast<PyCFunction>(rotary_tensors), METH_FASTCALL, "sarek_hip_rotary of tensors, None where it is not the ordinary call"},
+    {"kv_append_tensors", reinterpret_cast<PyCFunction>(kv_append_tensors), METH_FASTCALL, "sarek_hip_kv_append, likewise"},
+    {"attention_tensors", reinterpret_cast<PyCFunction>(attention_tensors), METH_FASTCALL, "sarek_hip_attention_paged and _shared, likewise"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Argument lists of launches, built natively.", -1, methods,
@@ -359,5 +583,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Argument lists of launche
 PyMODINIT_FUNC PyInit__host(void) {
   s_h = PyUnicode_InternFromString("_h");
   s_value = PyUnicode_InternFromString("value");
+  PyObject **const names[] = {&s_shape, &s_stride, &s_dtype, &s_data_ptr, &s_get_device, &s_new_empty};
+  const char *const texts[] = {"shape", "stride", "dtype", "data_ptr", "get_device", "new_empty"};
+  for (int i = 0; i < 6; ++i)
+    if (!(*names[i] = PyUnicode_InternFromString(texts[i]))) return nullptr;
   return s_h && s_value ? PyModule_Create(&module) : nullptr;
 }

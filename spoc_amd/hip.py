@@ -303,6 +303,8 @@ _host.bind_mx(*(C.cast(getattr(lib, _f), C.c_void_p).value for _f in (
     "sarek_hip_gemm_mx")))
 _host.bind_attention(*(C.cast(getattr(lib, _f), C.c_void_p).value for _f in (
     "sarek_hip_rotary", "sarek_hip_kv_append", "sarek_hip_attention_paged", "sarek_hip_attention_shared")))
+_host.bind_torch(torch.Tensor, torch.float32, torch.bfloat16, torch.float16, torch.int32, torch.int64, torch._C._cuda_getDevice,
+                 torch._C._cuda_getCurrentRawStream, C.cast(lib.sarek_hip_attention_workspace_bytes, C.c_void_p).value)
 
 
 def check(status):
@@ -1118,6 +1120,7 @@ class Rotary:
         self.dim, self.layout, self.amplitude, self.frequencies, self.turns = dim, layout, float(amplitude), f, turns.to(device)
         self._plan = RotaryPlan(self.turns.data_ptr(), dim // 2, _ROTARY_LAYOUTS[layout], self.amplitude)
         self._at = C.addressof(self._plan)
+        self._call = (self._at, dim, self.turns.get_device())      # what the native calls take
 
     def __repr__(self):
         return f"Rotary({self.dim}, {self.layout})"
@@ -1150,6 +1153,7 @@ class KvCache:
         self.keys, self.values, self.page_size, self.heads, self.head_dim = keys, values, page_size, heads, head_dim
         self._layout = KvCacheLayout(keys.data_ptr(), values.data_ptr(), *keys.stride()[:3], pages, page_size, heads, head_dim, _MX_TYPES[keys.dtype])
         self._at = C.addressof(self._layout)
+        self._call = (self._at, heads, head_dim, keys.get_device(), keys.dtype)
 
     @classmethod
     def empty(cls, pages, page_size, heads, head_dim, dtype=torch.bfloat16, device="cuda"):
@@ -1210,11 +1214,19 @@ def _like_heads(t, x, name):
 def rotary(x, positions, plan, out=None):
     """x [tokens, heads, head dim] (float32, bfloat16 or float16) turned to its positions [tokens] (int64 or int32) by a Rotary.  out may be
     x itself."""
+    if isinstance(plan, Rotary):
+        got = _host.rotary_tensors(x, positions, plan._call, out, False)
+        if got is not None:
+            return got
     return _rotated(x, positions, plan, out, 0, "x")
 
 
 def rotary_backward(dy, positions, plan, out=None):
     """The gradient of rotary's x for dy, its output's: turned the other way."""
+    if isinstance(plan, Rotary):
+        got = _host.rotary_tensors(dy, positions, plan._call, out, True)
+        if got is not None:
+            return got
     return _rotated(dy, positions, plan, out, 1, "dy")
 
 
@@ -1264,9 +1276,14 @@ def kv_append(k, v, cache, pages, lengths, starts=None, rotary=None, q=None, q_o
     Sequence b of the batch has the tokens starts[b] to starts[b + 1] - 1 (starts None: the one token b); they are the last of its
     lengths[b] keys.  Key p is in slot p % page size of page pages[b, p // page size] and at position first + p.  lengths [batch],
     starts [batch + 1] and pages [batch, any] are int32 on the device.  A page that tokens go to belongs to one sequence; tokens that the
-    table has no room for, or no page of the cache, are not put anywhere.  Tokens behind the last sequence are left alone, in q_out too."""
+    table has no room for, or no page of the cache, are not put anywhere.  Tokens before the first and behind the last sequence are left
+    alone, in q_out too."""
     if not isinstance(cache, KvCache):
         raise TypeError("cache: expected a KvCache")
+    if rotary is None or isinstance(rotary, Rotary):
+        got = _host.kv_append_tensors(k, v, cache._call, pages, lengths, starts, None if rotary is None else rotary._call, q, q_out, first)
+        if got is not None:
+            return got if got is not False else None
     tokens = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() == 3 else 0
     k_token, k_head = _cache_heads(k, cache, None, cache.heads, "k")
     v_token, v_head = _cache_heads(v, cache, tokens, cache.heads, "v")
@@ -1327,7 +1344,11 @@ def attention_paged(q, cache, pages, lengths, starts=None, causal=True, scale=No
     scale None: head dim ^ -1/2.  The sequences' tokens, lengths and pages: as for kv_append, the tokens' own keys are in the cache
     already.  causal: a token sees its sequence's keys up to its own, otherwise all of them; a token that sees none gets zeros.
     out: where the result goes; lse (float32 [tokens, heads]): gets the logarithm of the sum of the exponents, -inf where there is none.
-    Rows of tokens behind the last sequence are left as they are."""
+    Rows of tokens before the first and behind the last sequence are left as they are."""
+    if isinstance(cache, KvCache):
+        got = _host.attention_tensors(q, cache._call, None, 0, pages, lengths, starts, causal, scale, out, lse)
+        if got is not None:
+            return got
     return _attention(q, cache, None, pages, lengths, starts, causal, scale, out, lse)
 
 
@@ -1337,6 +1358,9 @@ def attention_shared(q, cache, prefix_pages, prefix_length, pages, lengths, star
     first=prefix_length)."""
     if not isinstance(cache, KvCache):
         raise TypeError("cache: expected a KvCache")
+    got = _host.attention_tensors(q, cache._call, prefix_pages, prefix_length, pages, lengths, starts, causal, scale, out, lse)
+    if got is not None:
+        return got
     at = _table(prefix_pages, (None,), "prefix_pages", cache.keys.device)
     if not 0 <= prefix_length <= prefix_pages.shape[0] * cache.page_size:
         raise ValueError(f"prefix_length: {prefix_length} keys in {prefix_pages.shape[0]} pages of {cache.page_size}")
