@@ -24,7 +24,6 @@
 namespace sarek_hip {
 namespace {
 
-typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4_t;
 
@@ -202,9 +201,6 @@ __device__ __forceinline__ void move16(const char *base, __amdgpu_buffer_rsrc_t 
 template <class T> struct Products;
 template <> struct Products<Bf16> {
   static __device__ __forceinline__ f32x4_t mul(u32x4 a, u32x4 b, f32x4_t c) { return mfma16<true>(a, b, c); }
-  static __device__ __forceinline__ f32x16_t mul(u32x4 a, u32x4 b, f32x16_t c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return f32_pair_to_bf16(lo, hi); }
   static __device__ __forceinline__ float low(uint32_t v) { return bf16_to_f32(v); }
   static __device__ __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
@@ -212,9 +208,6 @@ template <> struct Products<Bf16> {
 };
 template <> struct Products<_Float16> {
   static __device__ __forceinline__ f32x4_t mul(u32x4 a, u32x4 b, f32x4_t c) { return mfma16<false>(a, b, c); }
-  static __device__ __forceinline__ f32x16_t mul(u32x4 a, u32x4 b, f32x16_t c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return f32_pair_to_f16(lo, hi); }
   static __device__ __forceinline__ float low(uint32_t v) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(v))); }
   static __device__ __forceinline__ float high(uint32_t v) { return low(v >> 16); }
@@ -341,10 +334,10 @@ template <int D, int kAtOnce> __device__ __forceinline__ void add_planes(const P
 constexpr int kStreamKeys = 32;
 template <int D> constexpr int kStreamWaves = D == 64 ? 4 : D == 128 ? 2 : 1;
 
-template <class T, int D, bool Far>
+template <class T, int D, int Used, bool Far>
 __global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(AttentionArgs s, Pass p, Pass before) {
   constexpr int kWaves = kStreamWaves<D>, kRowBytes = 2 * D, kPieces = D / 8, kKeysMoved = 64 / kPieces, kMoves = kStreamKeys / kKeysMoved;
-  constexpr int kTileBytes = kStreamKeys * kRowBytes, kStage = kWaves * 2 * kTileBytes, kSteps = D / 32, kColumns = D / 16, kPitch = D + 4;
+  constexpr int kTileBytes = kStreamKeys * kRowBytes, kStage = kWaves * 2 * kTileBytes, kSteps = Used / 32, kColumns = Used / 16, kPitch = D + 4;
   static_assert(kWaves * 16 * kPitch * 4 <= kStage && 2 * kMoves < 64, "the waves' sums go into a stage; vmcnt");
   typedef typename Rows<Far>::At At;
   typedef Products<T> P;
@@ -497,7 +490,7 @@ __global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(
   if (quad == 0) ends[(wave * 16 + l16) * 2] = m * s.scale, ends[(wave * 16 + l16) * 2 + 1] = l;
   __syncthreads();
   // Threads by four columns of the rows that there are.  Where there is no other stretch the row is done, but for the prefix's planes.
-  constexpr int kThreads = 64 * kWaves, kQuads = D / 4;
+  constexpr int kThreads = 64 * kWaves, kQuads = Used / 4;
   const int live = min(16, it.count * static_cast<int>(s.group.size) - it.row0);
   for (int column = threadIdx.x; column < live * kQuads; column += kThreads) {
     const int r = column / kQuads, d = column % kQuads * 4;
@@ -526,17 +519,19 @@ __global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(
 
 // ---- many rows -----------------------------------------------------------------------------------------------------------------------
 
-// Four waves of 32 rows; tiles of 32 keys go to LDS for all of them, three ahead.  While the softmax of tile j is on the vector unit, the
-// matrix unit forms the scores of tile j + 1; then come the weighted values of tile j.
-constexpr int kTileKeys = 32, kTileRows = 128, kTileRing = 4;
+// Four waves of 32 rows, two blocks of 16; tiles of 32 keys go to LDS for all of them, three ahead.  While the softmax of tile j is on the vector
+// unit, the matrix unit forms the scores of tile j + 1; then come the weighted values of tile j.  Used: the values of a head, rounded up to 32 (D, the
+// length of a row in LDS, is a power of two).
+constexpr int kTileKeys = 32, kTileRing = 4;
 
-template <class T, int D, bool Far>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(AttentionArgs s, Pass p) {
+template <class T, int D, int Used, int Waves, bool Far>
+__global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_kernel(AttentionArgs s, Pass p) {
   constexpr int kRowBytes = 2 * D, kPieces = D / 8, kKeysMoved = 64 / kPieces, kTileBytes = kTileKeys * kRowBytes;
-  constexpr int kMoves = kTileBytes / 4096, kMine = kMoves * kKeysMoved, kSteps = D / 16, kColumns = D / 32;
+  constexpr int Blocks = 2, kMoves = kTileBytes / (1024 * Waves), kMine = kMoves * kKeysMoved, kSteps = Used / 32, kColumns = Used / 16;
+  static_assert(kMoves >= 1 && 6 * kMoves < 64, "whole transfers; vmcnt");
   typedef typename Rows<Far>::At At;
   typedef Products<T> P;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, l16 = lane & 15, half = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, quad = lane >> 4;
   const int kv_head = static_cast<int>(blockIdx.x) % s.kv_heads;
   Item it;
   if (!find_item(s, p, static_cast<int>(blockIdx.x) / s.kv_heads, it)) return;
@@ -545,122 +540,185 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(A
   const uint32_t bytes = static_cast<uint32_t>(min(s.extent - kv_head * s.head, kNearBytes));
   const __amdgpu_buffer_rsrc_t rk = make_rsrc(keys, Far ? 0u : bytes), rv = make_rsrc(values, Far ? 0u : bytes);
   const int pieces = s.head_dim / 8, tiles = (it.end - it.begin + kTileKeys - 1) / kTileKeys;
-  // Loads come in order: the row of q before the first page, a page before the transfers that it is not for.
-  const Row row = row_at(s, p, it, kv_head, it.row0 + wave * 32 + l32);
-  u32x4 q[kSteps];
+  // Loads come in order: the rows of q before the first page, a page before the transfers that it is not for.
+  Row row[Blocks];
+  u32x4 q[Blocks][kSteps];
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) q[i] = load_q<T>(s, row, i * 16 + half * 8);
-  // This wave's transfers bring kMine keys of a tile; lane j looks up the j-th of them.  `from`: the rows of the last tile of keys that was asked
-  // for, whose values are asked for one tile later.
-  const int turn_of_mine = lane % kMine, my_key = it.begin + (turn_of_mine / kKeysMoved * 4 + wave) * kKeysMoved + turn_of_mine % kKeysMoved;
-  int page[kTileRing] = {};      // of this lane's key in the tiles to come, by their places in the ring
-  At from[kMoves];
+  for (int r = 0; r < Blocks; ++r) {
+    row[r] = row_at(s, p, it, kv_head, it.row0 + wave * (16 * Blocks) + r * 16 + l16);
 #pragma unroll
-  for (int i = 0; i < kMoves; ++i) from[i] = Rows<Far>::kNone;
-  auto look_up = [&](int place, int tile) __attribute__((always_inline)) { page[place] = page_of(s, table, my_key + tile * kTileKeys); };
-  // (A page is looked up a whole round ahead: as loads come in order, waiting for it is waiting for all transfers before it.)
-  auto move_keys = [&](char *to, int place, int tile) __attribute__((always_inline)) {
-    const At at = row_of<Far>(s, table, my_key + tile * kTileKeys, page[place]);
-    look_up(place, tile + kTileRing);
+    for (int i = 0; i < kSteps; ++i) q[r][i] = load_q<T>(s, row[r], i * 32 + quad * 8);
+  }
+  // This wave's transfers bring kMine keys of a tile; lane j looks up the j-th of them: its entry of the table and its place in the page go on from tile
+  // to tile by additions.  A page is looked up a whole round of the ring ahead (as loads come in order, waiting for it is waiting for all
+  // transfers before it).  `from`: the rows of the last keys that were asked for, whose values are asked for one tile later.
+  const uint32_t size = s.batch.page_size.size, entries_on = divided(kTileKeys, s.batch.page_size), slots_on = kTileKeys - entries_on * size;
+  const int j_mine = lane % kMine;
+  int key = it.begin + (j_mine / kKeysMoved * Waves + wave) * kKeysMoved + j_mine % kKeysMoved;
+  uint32_t entry = divided(static_cast<uint32_t>(key), s.batch.page_size), in = static_cast<uint32_t>(key) - entry * size;
+  const uint32_t last_entry = divided(static_cast<uint32_t>(max(it.end - 1, 0)), s.batch.page_size);
+  int page[kTileRing] = {};
+  At in_page[kTileRing] = {}, in_page_next = static_cast<At>(in) * static_cast<At>(s.slot), from[kMoves];
+  const At slots_on_bytes = static_cast<At>(slots_on) * static_cast<At>(s.slot), page_of_slots = static_cast<At>(size) * static_cast<At>(s.slot);
+  uint32_t key_piece[kMoves], value_piece[kMoves];      // bytes from a row's start; past everything where the head ends before
+#pragma unroll
+  for (int i = 0; i < kMoves; ++i) {
+    const int k = (i * Waves + wave) * kKeysMoved + lane / kPieces, kp = lane % kPieces ^ turn_of_key<D>(k), vp = lane % kPieces ^ turn_of_value<D>(k);
+    key_piece[i] = kp < pieces ? kp * 16 : Rows<false>::kNone;
+    value_piece[i] = vp < pieces ? vp * 16 : Rows<false>::kNone;
+    from[i] = Rows<Far>::kNone;
+  }
+  auto look_up = [&](int place) __attribute__((always_inline)) {
+    page[place] = table.pages[min(entry, last_entry)];
+    in_page[place] = in_page_next;
+    entry += entries_on, in += slots_on, in_page_next += slots_on_bytes;
+    if (in >= size) ++entry, in -= size, in_page_next -= page_of_slots;
+  };
+  auto move = [&](const char *base, __amdgpu_buffer_rsrc_t rsrc, At at, uint32_t piece, char *to) __attribute__((always_inline)) {
+    if constexpr (Far) {
+      const char *source = at >= 0 && piece != Rows<false>::kNone ? base + at + piece : reinterpret_cast<const char *>(&zero_block);
+      __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) void *>(reinterpret_cast<uintptr_t>(source)), (LDS_PTR void *)to, 16, 0, 0);
+    } else {
+      dma16(rsrc, __builtin_elementwise_add_sat(at, piece), 0, to);
+    }
+  };
+  auto move_keys = [&](char *to, int place) __attribute__((always_inline)) {
+    At at = Rows<Far>::kNone;
+    if (key < it.end && static_cast<uint32_t>(page[place]) < static_cast<uint32_t>(s.batch.n_pages)) at = static_cast<At>(page[place]) * static_cast<At>(s.page) + in_page[place];
+    key += kTileKeys;
+    look_up(place);
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < kMoves; ++i) {
       from[i] = __shfl(at, i * kKeysMoved + lane / kPieces, 64);
-      move16<Far>(keys, rk, from[i], lane % kPieces ^ turn_of_key<D>((i * 4 + wave) * kKeysMoved + lane / kPieces), pieces, to + ((i * 4 + wave) * 1024));
+      move(keys, rk, from[i], key_piece[i], to + ((i * Waves + wave) * 1024));
     }
   };
   auto move_values = [&](char *to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kMoves; ++i)
-      move16<Far>(values, rv, from[i], lane % kPieces ^ turn_of_value<D>((i * 4 + wave) * kKeysMoved + lane / kPieces), pieces, to + ((i * 4 + wave) * 1024));
+    for (int i = 0; i < kMoves; ++i) move(values, rv, from[i], value_piece[i], to + ((i * Waves + wave) * 1024));
   };
   // Transfers come in the order K0 | V0 K1 | V1 K2 | V2 K3 | V3 K4 ...; what is behind the last tile brings zeros.
   if (tiles > 0) {
-    look_up(0, 0), look_up(1, 1), look_up(2, 2), look_up(3, 3);
+    look_up(0), look_up(1), look_up(2), look_up(3);
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) asm volatile("" : "+v"(q[i]));      // (waits for them here, not in the loop, where it would wait for transfers)
-    move_keys(lds_ring<10, kTileBytes>, 0, 0);
+    for (int r = 0; r < Blocks; ++r)
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) asm volatile("" : "+v"(q[r][i]));      // (waits for them here, not in the loop, where it would wait for transfers)
+    move_keys(lds_ring<10, kTileBytes>, 0);
     move_values(lds_ring<20, kTileBytes>);
-    move_keys(lds_ring<11, kTileBytes>, 1, 1);
+    move_keys(lds_ring<11, kTileBytes>, 1);
     move_values(lds_ring<21, kTileBytes>);
-    move_keys(lds_ring<12, kTileBytes>, 2, 2);
+    move_keys(lds_ring<12, kTileBytes>, 2);
     move_values(lds_ring<22, kTileBytes>);
-    move_keys(lds_ring<13, kTileBytes>, 3, 3);
+    move_keys(lds_ring<13, kTileBytes>, 3);
   }
-  int least = row.limit, most_keys = row.live ? row.limit : it.begin;
+  int least = INT32_MAX, most_keys = it.begin;
 #pragma unroll
-  for (int x = 1; x < 32; x *= 2) least = min(least, __shfl_xor(least, x, 64)), most_keys = max(most_keys, __shfl_xor(most_keys, x, 64));
+  for (int r = 0; r < Blocks; ++r) least = min(least, row[r].limit), most_keys = max(most_keys, row[r].live ? row[r].limit : it.begin);
+#pragma unroll
+  for (int x = 1; x < 16; x *= 2) least = min(least, __shfl_xor(least, x, 64)), most_keys = max(most_keys, __shfl_xor(most_keys, x, 64));
   least = __builtin_amdgcn_readfirstlane(least), most_keys = __builtin_amdgcn_readfirstlane(most_keys);
-  f32x16_t o[kColumns], score;
+  f32x4_t o[kColumns][Blocks], score[2][Blocks];      // score[keys 16 b on][rows 16 r on]
 #pragma unroll
   for (int c = 0; c < kColumns; ++c)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) o[c][j] = 0.f;
+    for (int r = 0; r < Blocks; ++r) o[c][r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m[Blocks], l[Blocks], bound[Blocks];    // bound: the score from which m is to follow
 #pragma unroll
-  for (int j = 0; j < 16; ++j) score[j] = 0.f;
-  float m = -INFINITY, l = 0.f, bound = -INFINITY;    // bound: the score from which m is to follow
+  for (int r = 0; r < Blocks; ++r) {
+    score[0][r] = score[1][r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    m[r] = bound[r] = -INFINITY, l[r] = 0.f;
+  }
   const float lag = kLag / s.scale;
   const uint16_t largest = least < it.end ? P::kExponent - 1 : 0x7FFF;
   uint32_t unbounded = 0;
   // Where this lane reads, as in the other kernel
-  int key_at = l32 * kRowBytes + (half ^ turn_of_key<D>(l32)) * 16;
-  int value_at = (half * 4 + (l16 >> 2)) * kRowBytes + ((l32 >> 4) * 2 ^ turn_of_value<D>(half * 4 + (l16 >> 2))) * 16 + (l16 & 3) * 8;
+  int key_at = l16 * kRowBytes + (quad ^ turn_of_key<D>(l16)) * 16;
+  int value_at = (quad * 4 + (l16 >> 2)) * kRowBytes + turn_of_value<D>(quad * 4 + (l16 >> 2)) * 16 + (l16 & 3) * 8;
   asm volatile("" : "+v"(key_at), "+v"(value_at));
 
-  auto scores = [&](const char *k, f32x16_t &sum) __attribute__((always_inline)) {
+  auto scores = [&](const char *k, f32x4_t (&sum)[2][Blocks]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) sum[j] = 0.f;
+    for (int b = 0; b < 2; ++b) {
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) sum = P::mul(*reinterpret_cast<const u32x4 *>(k + (key_at ^ i << 5)), q[i], sum);
+      for (int r = 0; r < Blocks; ++r) sum[b][r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const u32x4 a = *reinterpret_cast<const u32x4 *>(k + ((key_at ^ i << 6) + b * 16 * kRowBytes));
+#pragma unroll
+        for (int r = 0; r < Blocks; ++r) sum[b][r] = P::mul(a, q[r][i], sum[b][r]);
+      }
+    }
   };
   auto tile = [&](auto masked, const char *next, const char *v, int key0) __attribute__((always_inline)) {
     constexpr bool kMasked = decltype(masked)::value;
-    if constexpr (kMasked) {
+    float most[Blocks];
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (key0 + j / 4 * 8 + half * 4 + j % 4 >= row.limit) score[j] = -INFINITY;
-    }
-    float most = score[0];
+    for (int r = 0; r < Blocks; ++r) {
+      if constexpr (kMasked) {
 #pragma unroll
-    for (int j = 1; j < 16; ++j) most = fmaxf(most, score[j]);
-    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
-    most = fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
-    if (__any(most > bound)) {
-      const float now = fmaxf(m, most), keep = now == m ? 1.f : __builtin_amdgcn_exp2f((m - now) * s.scale);
-      m = now, bound = now + lag;
-      l *= keep;
-#pragma unroll
-      for (int c = 0; c < kColumns; ++c) o[c] *= keep;
-    }
-    const float offset = m == -INFINITY ? 0.f : m * s.scale;
-    f32x16_t following;
-    scores(next, following);
-    u32x4 weights[2];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[2 * j], s.scale, -offset));
-      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[2 * j + 1], s.scale, -offset));
-      weights[j / 4][j % 4] = P::pack(x, y);
-      l += x + y;
-    }
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int c = 0; c < kColumns; ++c) {
-        const int at = (value_at ^ c << 6) + b * 16 * kRowBytes;
-        const u32x2_t lo = read_turned(v, at), hi = read_turned(v, at + 8 * kRowBytes);
-        u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
-        if constexpr (kMasked) a = cleaned(a, largest, unbounded);
-        o[c] = P::mul(a, weights[b], o[c]);
+        for (int j = 0; j < 8; ++j)
+          if (key0 + j / 4 * 16 + quad * 4 + j % 4 >= row[r].limit) score[j / 4][r][j % 4] = -INFINITY;
       }
-    score = following;
+      most[r] = score[0][r][0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) most[r] = fmaxf(most[r], score[j / 4][r][j % 4]);
+    }
+    bool grows = false;
+#pragma unroll
+    for (int r = 0; r < Blocks; r += 2) {
+      // Two rows' maxima over the four quads of lanes: halves exchanged with one another's, quads of a half, and back to all lanes.
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(most[r]), __float_as_uint(most[r + 1]), false, false);
+      const float y = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+      const auto z = __builtin_amdgcn_permlane16_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+      const float w = fmaxf(__uint_as_float(z[0]), __uint_as_float(z[1]));
+      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(w), __float_as_uint(w), false, false);
+      most[r] = __uint_as_float(both[0]), most[r + 1] = __uint_as_float(both[1]);
+      grows |= most[r] > bound[r] || most[r + 1] > bound[r + 1];
+    }
+    if (__any(grows)) {
+#pragma unroll
+      for (int r = 0; r < Blocks; ++r) {
+        const float now = fmaxf(m[r], most[r]), keep = now == m[r] ? 1.f : __builtin_amdgcn_exp2f((m[r] - now) * s.scale);
+        m[r] = now, bound[r] = now + lag;
+        l[r] *= keep;
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) o[c][r] *= keep;
+      }
+    }
+    f32x4_t following[2][Blocks];
+    scores(next, following);
+    u32x4 weights[Blocks];
+#pragma unroll
+    for (int r = 0; r < Blocks; ++r) {
+      const float offset = m[r] == -INFINITY ? 0.f : m[r] * s.scale;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j / 2][r][j % 2 * 2], s.scale, -offset));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j / 2][r][j % 2 * 2 + 1], s.scale, -offset));
+        weights[r][j] = P::pack(x, y);
+        l[r] += x + y;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) {
+      const int at = value_at ^ c << 5;
+      const u32x2_t lo = read_turned(v, at), hi = read_turned(v, at + 16 * kRowBytes);
+      u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
+      if constexpr (kMasked) a = cleaned(a, largest, unbounded);
+#pragma unroll
+      for (int r = 0; r < Blocks; ++r) o[c][r] = P::mul(a, weights[r], o[c][r]);
+    }
+#pragma unroll
+    for (int r = 0; r < Blocks; ++r) score[0][r] = following[0][r], score[1][r] = following[1][r];
   };
   auto turn = [&]<int I>(std::integral_constant<int, I>, auto masked, int t) __attribute__((always_inline)) {
     // The keys of tile t + 1 and the values of tile t are there when no more than the next two tiles' transfers are under way.
     __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(4 * kMoves));
     barrier_no_fence();
     move_values(lds_ring<20 + (I + 3) % 4, kTileBytes>);
-    move_keys(lds_ring<10 + I, kTileBytes>, I, t + 4);
+    move_keys(lds_ring<10 + I, kTileBytes>, I);
     const int key0 = it.begin + t * kTileKeys;
     if (!decltype(masked)::value || key0 < most_keys) tile(masked, lds_ring<10 + (I + 1) % 4, kTileBytes>, lds_ring<20 + I, kTileBytes>, key0);
   };
@@ -685,39 +743,38 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(A
   }
   __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));   // the last, empty transfers, before the LDS is released
   if (__any(unbounded != 0)) {
-    for (int key = it.begin + whole * kTileKeys; key < it.end; ++key) {
-      const int64_t at = row_of<true>(s, table, key, page_of(s, table, key));
-      if (at < 0 || key >= row.limit) continue;
+    for (int k = it.begin + whole * kTileKeys; k < it.end; ++k) {
+      const int64_t at = row_of<true>(s, table, k, page_of(s, table, k));
+      if (at < 0) continue;
 #pragma unroll
       for (int c = 0; c < kColumns; ++c)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f32x4_t v = {o[c][4 * j], o[c][4 * j + 1], o[c][4 * j + 2], o[c][4 * j + 3]};
-          if (c * 32 + j * 8 + half * 4 < s.head_dim) add_unbounded<T>(values + at + (c * 32 + j * 8 + half * 4) * 2, v);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) o[c][4 * j + k] = v[k];
+        for (int r = 0; r < Blocks; ++r) {
+          if (k < row[r].limit && c * 16 + quad * 4 < s.head_dim) add_unbounded<T>(values + at + (c * 16 + quad * 4) * 2, o[c][r]);
           __builtin_amdgcn_sched_barrier(0);
         }
     }
   }
 
-  l += __shfl_xor(l, 32, 64);
-  if (!row.live) return;
-  const float inverse = l == 0.f ? 0.f : 1.f / l;
-  const int64_t place = (static_cast<int64_t>(it.slot) * s.kv_heads + kv_head) * kTileRows + wave * 32 + l32;
 #pragma unroll
-  for (int c = 0; c < kColumns; ++c)
+  for (int r = 0; r < Blocks; ++r) {
+    l[r] += __shfl_xor(l[r], 16, 64);
+    l[r] += __shfl_xor(l[r], 32, 64);
+    if (!row[r].live) continue;
+    const float inverse = l[r] == 0.f ? 0.f : 1.f / l[r];
+    const int in_tile = wave * (16 * Blocks) + r * 16 + l16;
+    const int64_t place = (static_cast<int64_t>(it.slot) * s.kv_heads + kv_head) * (16 * Blocks * Waves) + in_tile;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x4_t v = {o[c][4 * j], o[c][4 * j + 1], o[c][4 * j + 2], o[c][4 * j + 3]};
-      const int d = c * 32 + j * 8 + half * 4;
-      if (it.slot < 0) store_out<T>(s, row.token, row.head, d, v * inverse);
-      else *reinterpret_cast<f32x4_t *>(p.o + place * D + d) = v;
+    for (int c = 0; c < kColumns; ++c) {
+      const int d = c * 16 + quad * 4;
+      if (it.slot < 0) store_out<T>(s, row[r].token, row[r].head, d, o[c][r] * inverse);
+      else *reinterpret_cast<f32x4_t *>(p.o + place * D + d) = o[c][r];
     }
-  if (half == 0) {
-    if (it.slot < 0) store_lse(s, row.token, row.head, m * s.scale, l);
-    else p.ml[place] = f32x2_t{m * s.scale, l};
-    if (p.places && it.stretch == 0 && row.head == 0) tell_place(p, it, row.token, wave * 32 + l32);
+    if (quad == 0) {
+      if (it.slot < 0) store_lse(s, row[r].token, row[r].head, m[r] * s.scale, l[r]);
+      else p.ml[place] = f32x2_t{m[r] * s.scale, l[r]};
+      if (p.places && it.stretch == 0 && row[r].head == 0) tell_place(p, it, row[r].token, in_tile);
+    }
   }
 }
 
@@ -769,7 +826,7 @@ template <class T, int D> __global__ __launch_bounds__(256) void attention_join_
 // ---- the host's part -------------------------------------------------------------------------------------------------------------------
 
 struct Launch {
-  bool tile;
+  int waves;             // of 32 rows to a tile; 0: few rows
   int64_t items;         // for each kv head, at most
   Pass pass;
 };
@@ -787,13 +844,14 @@ Launch plan(const sarek_hip_kv_cache *cache, int q_heads, int64_t sequences, int
   const int d = cache->head_dim;
   const int64_t rows = tokens * (q_heads / cache->heads), heads = cache->heads;
   Launch r;
-  r.tile = rows > 16 * sequences;
-  r.pass = {what == kPrefix, r.tile ? kTileRows : 16, 0, 0, 0, 0, nullptr, nullptr, nullptr};
-  r.pass.unit = r.tile ? 2 * kTileKeys : kStreamKeys * (d <= 64 ? kStreamWaves<64> : d <= 128 ? kStreamWaves<128> : kStreamWaves<256>);
+  r.waves = rows <= 16 * sequences ? 0 : d > 64 && d <= 128 && rows / 256 * heads >= tunable("attention.large_tiles", 2 * compute_units()) ? 8 : 4;
+  const int tile_rows = r.waves ? 32 * r.waves : 16;
+  r.pass = {what == kPrefix, tile_rows, 0, 0, 0, 0, nullptr, nullptr, nullptr};
+  r.pass.unit = r.waves ? 2 * kTileKeys : kStreamKeys * (d <= 64 ? kStreamWaves<64> : d <= 128 ? kStreamWaves<128> : kStreamWaves<256>);
   const int64_t most_tiles = rows / r.pass.rows + sequences, tiles = std::max(rows / r.pass.rows, std::min(tokens, sequences)), units = ceil_div(keys, r.pass.unit);
-  const int64_t wanted = r.tile ? tunable("attention.tile_workgroups", compute_units()) : tunable("attention.stream_workgroups", 3 * compute_units());
-  if (units > 1 && tiles * heads < (what == kBehindPrefix && !r.tile ? compute_units() : wanted)) r.pass.target = static_cast<int>(wanted);
-  r.pass.all = what == kPrefix || (what == kBehindPrefix && (r.tile || r.pass.target != 0));
+  const int64_t wanted = r.waves ? tunable("attention.tile_workgroups", compute_units()) : tunable("attention.stream_workgroups", 3 * compute_units());
+  if (units > 1 && tiles * heads < (what == kBehindPrefix && !r.waves ? compute_units() : wanted)) r.pass.target = static_cast<int>(wanted);
+  r.pass.all = what == kPrefix || (what == kBehindPrefix && (r.waves || r.pass.target != 0));
   // (the number of units to a stretch comes from a float32 sum: a few items more)
   r.items = r.pass.target == 0 ? most_tiles : std::min(most_tiles + wanted / heads + 8, most_tiles * units);
   r.pass.max_slots = static_cast<int>(r.pass.all ? r.items : r.pass.target == 0 ? 0 : std::min(r.items, 2 * wanted / heads + 8));
@@ -808,18 +866,23 @@ char *place_planes(const sarek_hip_kv_cache *cache, Launch *r, int64_t tokens, c
   return at + plane_bytes(cache, *r, tokens);
 }
 
-template <class T, int D> int launch_all(const AttentionArgs &s, const Launch &own, const Launch *before, hipStream_t st) {
+template <class T, int D, int Used> int launch_all(const AttentionArgs &s, const Launch &own, const Launch *before, hipStream_t st) {
   const bool far = s.extent > kNearBytes;
   const Pass none = {0, 1, 1, 0, 0, 0, nullptr, nullptr, nullptr};
   const auto one = [&](const Launch &r) {
     const Pass &then = before && !r.pass.prefix ? before->pass : none;      // (what the few rows' kernel joins with its own)
     const dim3 grid(static_cast<unsigned>(r.items * s.kv_heads));
-    if (r.tile) {
-      if (far) hipLaunchKernelGGL((attention_tile_kernel<T, D, true>), grid, dim3(256), 0, st, s, r.pass);
-      else hipLaunchKernelGGL((attention_tile_kernel<T, D, false>), grid, dim3(256), 0, st, s, r.pass);
+    if (r.waves == 8) {
+      if constexpr (D == 128) {
+        if (far) hipLaunchKernelGGL((attention_tile_kernel<T, D, Used, 8, true>), grid, dim3(512), 0, st, s, r.pass);
+        else hipLaunchKernelGGL((attention_tile_kernel<T, D, Used, 8, false>), grid, dim3(512), 0, st, s, r.pass);
+      }
+    } else if (r.waves == 4) {
+      if (far) hipLaunchKernelGGL((attention_tile_kernel<T, D, Used, 4, true>), grid, dim3(256), 0, st, s, r.pass);
+      else hipLaunchKernelGGL((attention_tile_kernel<T, D, Used, 4, false>), grid, dim3(256), 0, st, s, r.pass);
     } else {
-      if (far) hipLaunchKernelGGL((attention_stream_kernel<T, D, true>), grid, dim3(64 * kStreamWaves<D>), 0, st, s, r.pass, then);
-      else hipLaunchKernelGGL((attention_stream_kernel<T, D, false>), grid, dim3(64 * kStreamWaves<D>), 0, st, s, r.pass, then);
+      if (far) hipLaunchKernelGGL((attention_stream_kernel<T, D, Used, true>), grid, dim3(64 * kStreamWaves<D>), 0, st, s, r.pass, then);
+      else hipLaunchKernelGGL((attention_stream_kernel<T, D, Used, false>), grid, dim3(64 * kStreamWaves<D>), 0, st, s, r.pass, then);
     }
     return check_launch("attention launch");
   };
@@ -874,7 +937,10 @@ int attention(const char *what, const sarek_hip_kv_cache *cache, const void *q, 
   const auto run = [&]<class T>(T *) {
     const hipStream_t st = as_stream(stream);
     const Launch *const first = shared ? &before : nullptr;
-    return d <= 64 ? launch_all<T, 64>(s, own, first, st) : d <= 128 ? launch_all<T, 128>(s, own, first, st) : launch_all<T, 256>(s, own, first, st);
+    if (d <= 64) return launch_all<T, 64, 64>(s, own, first, st);
+    if (d <= 96) return launch_all<T, 128, 96>(s, own, first, st);
+    if (d <= 128) return launch_all<T, 128, 128>(s, own, first, st);
+    return d <= 192 ? launch_all<T, 256, 192>(s, own, first, st) : launch_all<T, 256, 256>(s, own, first, st);
   };
   return cache->type == SAREK_HIP_TYPE_BF16 ? run(static_cast<Bf16 *>(nullptr)) : run(static_cast<_Float16 *>(nullptr));
 }
