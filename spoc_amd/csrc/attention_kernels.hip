@@ -527,7 +527,7 @@ constexpr int kTileKeys = 32, kTileRing = 4;
 template <class T, int D, int Used, int Waves, bool Far>
 __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_kernel(AttentionArgs s, Pass p) {
   constexpr int kRowBytes = 2 * D, kPieces = D / 8, kKeysMoved = 64 / kPieces, kTileBytes = kTileKeys * kRowBytes;
-  constexpr int Blocks = 2, kMoves = kTileBytes / (1024 * Waves), kMine = kMoves * kKeysMoved, kSteps = Used / 32, kColumns = Used / 16;
+  constexpr int Blocks = 2, kMoves = kTileBytes / (1024 * Waves), kSteps = Used / 32, kColumns = Used / 16;
   static_assert(kMoves >= 1 && 6 * kMoves < 64, "whole transfers; vmcnt");
   typedef typename Rows<Far>::At At;
   typedef Products<T> P;
@@ -549,17 +549,18 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) q[r][i] = load_q<T>(s, row[r], i * 32 + quad * 8);
   }
-  // This wave's transfers bring kMine keys of a tile; lane j looks up the j-th of them: its entry of the table and its place in the page go on from tile
-  // to tile by additions.  A page is looked up a whole round of the ring ahead (as loads come in order, waiting for it is waiting for all
-  // transfers before it).  `from`: the rows of the last keys that were asked for, whose values are asked for one tile later.
-  const uint32_t size = s.batch.page_size.size, entries_on = divided(kTileKeys, s.batch.page_size), slots_on = kTileKeys - entries_on * size;
-  const int j_mine = lane % kMine;
-  int key = it.begin + (j_mine / kKeysMoved * Waves + wave) * kKeysMoved + j_mine % kKeysMoved;
-  uint32_t entry = divided(static_cast<uint32_t>(key), s.batch.page_size), in = static_cast<uint32_t>(key) - entry * size;
+  // A wave looks up the rows that it moves in a round of the ring together, a lane to each (lane kMine u + j: the j-th of its kMine keys in the u-th
+  // tile), a round ahead; their pages are asked for a round before that (as loads come in order, waiting for one is waiting for all transfers
+  // before it).  `ahead`: the rows of the next keys to be asked for, handed to the lanes that move them a tile before; `from`: those of the
+  // last keys that were asked for, whose values are asked for one tile later.
+  constexpr int kMine = kMoves * kKeysMoved, kRound = kTileRing * kTileKeys;
+  static_assert(kMine * kTileRing <= 64, "a lane to each");
+  const uint32_t size = s.batch.page_size.size, entries_on = divided(kRound, s.batch.page_size), slots_on = kRound - entries_on * size;
   const uint32_t last_entry = divided(static_cast<uint32_t>(max(it.end - 1, 0)), s.batch.page_size);
-  int page[kTileRing] = {};
-  At in_page[kTileRing] = {}, in_page_next = static_cast<At>(in) * static_cast<At>(s.slot), from[kMoves];
-  const At slots_on_bytes = static_cast<At>(slots_on) * static_cast<At>(s.slot), page_of_slots = static_cast<At>(size) * static_cast<At>(s.slot);
+  const int j_mine = lane % kMine;
+  int key = it.begin + lane / kMine * kTileKeys + (j_mine / kKeysMoved * Waves + wave) * kKeysMoved + j_mine % kKeysMoved, page = 0;
+  uint32_t entry = divided(static_cast<uint32_t>(key), s.batch.page_size), in = static_cast<uint32_t>(key) - entry * size, in_of_page = 0;
+  At rows = Rows<Far>::kNone, ahead[kMoves], from[kMoves];
   uint32_t key_piece[kMoves], value_piece[kMoves];      // bytes from a row's start; past everything where the head ends before
 #pragma unroll
   for (int i = 0; i < kMoves; ++i) {
@@ -568,11 +569,22 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
     value_piece[i] = vp < pieces ? vp * 16 : Rows<false>::kNone;
     from[i] = Rows<Far>::kNone;
   }
-  auto look_up = [&](int place) __attribute__((always_inline)) {
-    page[place] = table.pages[min(entry, last_entry)];
-    in_page[place] = in_page_next;
-    entry += entries_on, in += slots_on, in_page_next += slots_on_bytes;
-    if (in >= size) ++entry, in -= size, in_page_next -= page_of_slots;
+  auto ask_for_pages = [&]() __attribute__((always_inline)) {
+    page = table.pages[min(entry, last_entry)];
+    in_of_page = in;
+    entry += entries_on, in += slots_on;
+    if (in >= size) ++entry, in -= size;
+  };
+  auto look_up = [&]() __attribute__((always_inline)) {      // the rows of the pages that were asked for last
+    rows = Rows<Far>::kNone;
+    if (key < it.end && static_cast<uint32_t>(page) < static_cast<uint32_t>(s.batch.n_pages)) rows = static_cast<At>(page) * static_cast<At>(s.page) + static_cast<At>(in_of_page) * static_cast<At>(s.slot);
+    key += kRound;
+    ask_for_pages();
+    asm volatile("" ::: "memory");
+  };
+  auto hand_out = [&](int place) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) ahead[i] = __shfl(rows, place * kMine + i * kKeysMoved + lane / kPieces, 64);
   };
   auto move = [&](const char *base, __amdgpu_buffer_rsrc_t rsrc, At at, uint32_t piece, char *to) __attribute__((always_inline)) {
     if constexpr (Far) {
@@ -582,15 +594,10 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
       dma16(rsrc, __builtin_elementwise_add_sat(at, piece), 0, to);
     }
   };
-  auto move_keys = [&](char *to, int place) __attribute__((always_inline)) {
-    At at = Rows<Far>::kNone;
-    if (key < it.end && static_cast<uint32_t>(page[place]) < static_cast<uint32_t>(s.batch.n_pages)) at = static_cast<At>(page[place]) * static_cast<At>(s.page) + in_page[place];
-    key += kTileKeys;
-    look_up(place);
-    asm volatile("" ::: "memory");
+  auto move_keys = [&](char *to) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kMoves; ++i) {
-      from[i] = __shfl(at, i * kKeysMoved + lane / kPieces, 64);
+      from[i] = ahead[i];
       move(keys, rk, from[i], key_piece[i], to + ((i * Waves + wave) * 1024));
     }
   };
@@ -599,19 +606,22 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
     for (int i = 0; i < kMoves; ++i) move(values, rv, from[i], value_piece[i], to + ((i * Waves + wave) * 1024));
   };
   // Transfers come in the order K0 | V0 K1 | V1 K2 | V2 K3 | V3 K4 ...; what is behind the last tile brings zeros.
+  if (tiles > 0) ask_for_pages();
+#pragma unroll
+  for (int r = 0; r < Blocks; ++r)
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) asm volatile("" : "+v"(q[r][i]));      // (waits for them here, not in the loop, where it would wait for transfers)
   if (tiles > 0) {
-    look_up(0), look_up(1), look_up(2), look_up(3);
-#pragma unroll
-    for (int r = 0; r < Blocks; ++r)
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) asm volatile("" : "+v"(q[r][i]));      // (waits for them here, not in the loop, where it would wait for transfers)
-    move_keys(lds_ring<10, kTileBytes>, 0);
+    look_up();
+    hand_out(0), move_keys(lds_ring<10, kTileBytes>);
     move_values(lds_ring<20, kTileBytes>);
-    move_keys(lds_ring<11, kTileBytes>, 1);
+    hand_out(1), move_keys(lds_ring<11, kTileBytes>);
     move_values(lds_ring<21, kTileBytes>);
-    move_keys(lds_ring<12, kTileBytes>, 2);
+    hand_out(2), move_keys(lds_ring<12, kTileBytes>);
     move_values(lds_ring<22, kTileBytes>);
-    move_keys(lds_ring<13, kTileBytes>, 3);
+    hand_out(3), move_keys(lds_ring<13, kTileBytes>);
+    look_up();
+    hand_out(0);
   }
   int least = INT32_MAX, most_keys = it.begin;
 #pragma unroll
@@ -638,14 +648,22 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
   int value_at = (quad * 4 + (l16 >> 2)) * kRowBytes + turn_of_value<D>(quad * 4 + (l16 >> 2)) * 16 + (l16 & 3) * 8;
   asm volatile("" : "+v"(key_at), "+v"(value_at));
 
-  auto scores = [&](const char *k, f32x4_t (&sum)[2][Blocks]) __attribute__((always_inline)) {
+  constexpr bool kEarly = Used <= 128;      // (registers)
+  u32x4 fragments[2][kSteps];
+  auto read_keys = [&](const char *k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) fragments[b][i] = *reinterpret_cast<const u32x4 *>(k + ((key_at ^ i << 6) + b * 16 * kRowBytes));
+  };
+  auto scores = [&](f32x4_t (&sum)[2][Blocks]) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
 #pragma unroll
       for (int r = 0; r < Blocks; ++r) sum[b][r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        const u32x4 a = *reinterpret_cast<const u32x4 *>(k + ((key_at ^ i << 6) + b * 16 * kRowBytes));
+        const u32x4 a = fragments[b][i];
 #pragma unroll
         for (int r = 0; r < Blocks; ++r) sum[b][r] = P::mul(a, q[r][i], sum[b][r]);
       }
@@ -653,6 +671,10 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
   };
   auto tile = [&](auto masked, const char *next, const char *v, int key0) __attribute__((always_inline)) {
     constexpr bool kMasked = decltype(masked)::value;
+    if constexpr (kEarly) {
+      read_keys(next);                            // (on their way while the maxima are formed)
+      __builtin_amdgcn_sched_barrier(0);
+    }
     float most[Blocks];
 #pragma unroll
     for (int r = 0; r < Blocks; ++r) {
@@ -688,7 +710,8 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
       }
     }
     f32x4_t following[2][Blocks];
-    scores(next, following);
+    if constexpr (!kEarly) read_keys(next);
+    scores(following);
     u32x4 weights[Blocks];
 #pragma unroll
     for (int r = 0; r < Blocks; ++r) {
@@ -718,14 +741,17 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
     __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(4 * kMoves));
     barrier_no_fence();
     move_values(lds_ring<20 + (I + 3) % 4, kTileBytes>);
-    move_keys(lds_ring<10 + I, kTileBytes>, I);
+    move_keys(lds_ring<10 + I, kTileBytes>);
+    if constexpr (I == 3) look_up();
+    hand_out((I + 1) % 4);
     const int key0 = it.begin + t * kTileKeys;
     if (!decltype(masked)::value || key0 < most_keys) tile(masked, lds_ring<10 + (I + 1) % 4, kTileBytes>, lds_ring<20 + I, kTileBytes>, key0);
   };
   if (tiles > 0) {
     __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(6 * kMoves));      // the first tile's keys
     barrier_no_fence();
-    scores(lds_ring<10, kTileBytes>, score);
+    read_keys(lds_ring<10, kTileBytes>);
+    scores(score);
   }
   // Tiles that all of this wave's rows see, a whole number of rounds of the ring, and the others.
   const int whole = max(min((least - it.begin) / kTileKeys, tiles), 0) & ~3;
