@@ -28,6 +28,46 @@ struct Batch {
   Division page_size;
 };
 
+typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+typedef __attribute__((ext_vector_type(2))) unsigned int place_t;
+
+// What one launch makes of the rows and keys.
+struct Pass {
+  int prefix;            // rows of all sequences against the prefix, or each sequence's against its own keys
+  int rows, unit;        // of a tile; keys in what a stretch has a whole number of
+  int target;            // about how many workgroups there are to be (0: no stretches, all of a sequence's keys in one)
+  int all;               // everything goes into the planes, for the join
+  int max_slots;
+  float *o;              // [slot][kv head][row][value]
+  f32x2_t *ml;           // [slot][kv head][row]
+  place_t *places;       // of each token's first row: its first slot, and the number of its stretches times 256 with its row in the tile
+};
+
+struct AttentionArgs {
+  Batch batch;
+  const void *q, *keys, *values;
+  void *out;
+  float *lse;
+  int64_t q_token, q_head, out_token, out_head;
+  int64_t page, slot, head, extent;         // the cache's strides and size, bytes
+  int heads, kv_heads, head_dim, causal;
+  Division group;
+  float scale;                              // times log2(e)
+  const int *prefix;
+  int prefix_length;
+};
+
+// The launches of one call (attention.hip plans them).
+struct Launch {
+  int waves;             // of 32 rows to a tile; 0: few rows
+  int64_t items;         // for each kv head, at most
+  Pass pass;
+};
+constexpr int kTileKeys = 32, kStreamKeys = 32;               // of a tile
+constexpr int stream_waves(int d) { return d <= 64 ? 4 : d <= 128 ? 2 : 1; }      // of a workgroup, by the padded head
+int launch_attention_bf16(const AttentionArgs &s, const Launch &own, const Launch *before, hipStream_t st);
+int launch_attention_f16(const AttentionArgs &s, const Launch &own, const Launch *before, hipStream_t st);
+
 namespace {
 
 __device__ __forceinline__ uint32_t divided(uint32_t n, const Division &by) {

@@ -13,45 +13,18 @@
 // workgroup brings to LDS.  Where rows are few for the card the keys are split into stretches of about the same length, and
 // attention_join_kernel joins what they leave (o, m and l in float32); the tiles and stretches are laid out by every workgroup for itself
 // from the lengths (Plan), which the host does not know.
+#pragma once
 #include <algorithm>
 #include <cmath>
 #include <utility>
 
 #include "attention_common.hpp"
 #include "gemm_common.hpp"
-#include "tunables.hpp"
 
 namespace sarek_hip {
 namespace {
 
-typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4_t;
-
-// What one launch makes of the rows and keys.
-struct Pass {
-  int prefix;            // rows of all sequences against the prefix, or each sequence's against its own keys
-  int rows, unit;        // of a tile; keys in what a stretch has a whole number of
-  int target;            // about how many workgroups there are to be (0: no stretches, all of a sequence's keys in one)
-  int all;               // everything goes into the planes, for the join
-  int max_slots;
-  float *o;              // [slot][kv head][row][value]
-  f32x2_t *ml;           // [slot][kv head][row]
-  u32x2_t *places;       // of each token's first row: its first slot, and the number of its stretches times 256 with its row in the tile
-};
-
-struct AttentionArgs {
-  Batch batch;
-  const void *q, *keys, *values;
-  void *out;
-  float *lse;
-  int64_t q_token, q_head, out_token, out_head;
-  int64_t page, slot, head, extent;         // the cache's strides and size, bytes
-  int heads, kv_heads, head_dim, causal;
-  Division group;
-  float scale;                              // times log2(e)
-  const int *prefix;
-  int prefix_length;
-};
 
 // ---- which tile and stretch ----------------------------------------------------------------------------------------------------------
 
@@ -331,12 +304,10 @@ template <int D, int kAtOnce> __device__ __forceinline__ void add_planes(const P
 
 // A wave takes every kWaves-th tile of 32 keys of the stretch by itself: its transfers go into its own part of LDS, one tile ahead, and there
 // is no barrier until the waves' sums are joined at the end.
-constexpr int kStreamKeys = 32;
-template <int D> constexpr int kStreamWaves = D == 64 ? 4 : D == 128 ? 2 : 1;
 
 template <class T, int D, int Used, bool Far>
-__global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(AttentionArgs s, Pass p, Pass before) {
-  constexpr int kWaves = kStreamWaves<D>, kRowBytes = 2 * D, kPieces = D / 8, kKeysMoved = 64 / kPieces, kMoves = kStreamKeys / kKeysMoved;
+__global__ __launch_bounds__(64 * stream_waves(D)) void attention_stream_kernel(AttentionArgs s, Pass p, Pass before) {
+  constexpr int kWaves = stream_waves(D), kRowBytes = 2 * D, kPieces = D / 8, kKeysMoved = 64 / kPieces, kMoves = kStreamKeys / kKeysMoved;
   constexpr int kTileBytes = kStreamKeys * kRowBytes, kStage = kWaves * 2 * kTileBytes, kSteps = Used / 32, kColumns = Used / 16, kPitch = D + 4;
   static_assert(kWaves * 16 * kPitch * 4 <= kStage && 2 * kMoves < 64, "the waves' sums go into a stage; vmcnt");
   typedef typename Rows<Far>::At At;
@@ -522,7 +493,7 @@ __global__ __launch_bounds__(64 * kStreamWaves<D>) void attention_stream_kernel(
 // Four waves of 32 rows, two blocks of 16; tiles of 32 keys go to LDS for all of them, three ahead.  While the softmax of tile j is on the vector
 // unit, the matrix unit forms the scores of tile j + 1; then come the weighted values of tile j.  Used: the values of a head, rounded up to 32 (D, the
 // length of a row in LDS, is a power of two).
-constexpr int kTileKeys = 32, kTileRing = 4;
+constexpr int kTileRing = 4;
 
 template <class T, int D, int Used, int Waves, bool Far>
 __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_kernel(AttentionArgs s, Pass p) {
@@ -849,48 +820,7 @@ template <class T, int D> __global__ __launch_bounds__(256) void attention_join_
   if (d == 0) store_lse(s, token, head, a.top, a.l);
 }
 
-// ---- the host's part -------------------------------------------------------------------------------------------------------------------
-
-struct Launch {
-  int waves;             // of 32 rows to a tile; 0: few rows
-  int64_t items;         // for each kv head, at most
-  Pass pass;
-};
-int padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-// What the planes of a launch take: o, m and l, and where each token's are.
-int64_t plane_bytes(const sarek_hip_kv_cache *cache, const Launch &r, int64_t tokens) {
-  if (r.pass.max_slots == 0) return 0;
-  const int64_t planes = static_cast<int64_t>(r.pass.max_slots) * cache->heads;
-  return planes * r.pass.rows * (padded(cache->head_dim) + 2) * 4 + (tokens + 1) / 2 * 16;
-}
-// What the host knows: how many tokens, sequences and keys there are at most.  Stretches: about `target` workgroups where tiles alone are fewer.
-// own keys behind a prefix: few rows finish with the prefix's planes themselves where they are in one stretch each.
-enum { kAlone, kBehindPrefix, kPrefix };
-Launch plan(const sarek_hip_kv_cache *cache, int q_heads, int64_t sequences, int64_t tokens, int64_t keys, int what) {
-  const int d = cache->head_dim;
-  const int64_t rows = tokens * (q_heads / cache->heads), heads = cache->heads;
-  Launch r;
-  r.waves = rows <= 16 * sequences ? 0 : d > 64 && d <= 128 && rows / 256 * heads >= tunable("attention.large_tiles", 2 * compute_units()) ? 8 : 4;
-  const int tile_rows = r.waves ? 32 * r.waves : 16;
-  r.pass = {what == kPrefix, tile_rows, 0, 0, 0, 0, nullptr, nullptr, nullptr};
-  r.pass.unit = r.waves ? 2 * kTileKeys : kStreamKeys * (d <= 64 ? kStreamWaves<64> : d <= 128 ? kStreamWaves<128> : kStreamWaves<256>);
-  const int64_t most_tiles = rows / r.pass.rows + sequences, tiles = std::max(rows / r.pass.rows, std::min(tokens, sequences)), units = ceil_div(keys, r.pass.unit);
-  const int64_t wanted = r.waves ? tunable("attention.tile_workgroups", compute_units()) : tunable("attention.stream_workgroups", 3 * compute_units());
-  if (units > 1 && tiles * heads < (what == kBehindPrefix && !r.waves ? compute_units() : wanted)) r.pass.target = static_cast<int>(wanted);
-  r.pass.all = what == kPrefix || (what == kBehindPrefix && (r.waves || r.pass.target != 0));
-  // (the number of units to a stretch comes from a float32 sum: a few items more)
-  r.items = r.pass.target == 0 ? most_tiles : std::min(most_tiles + wanted / heads + 8, most_tiles * units);
-  r.pass.max_slots = static_cast<int>(r.pass.all ? r.items : r.pass.target == 0 ? 0 : std::min(r.items, 2 * wanted / heads + 8));
-  return r;
-}
-char *place_planes(const sarek_hip_kv_cache *cache, Launch *r, int64_t tokens, char *at) {
-  if (r->pass.max_slots == 0) return at;
-  const int64_t rows = static_cast<int64_t>(r->pass.max_slots) * cache->heads * r->pass.rows;
-  r->pass.o = reinterpret_cast<float *>(at);
-  r->pass.ml = reinterpret_cast<f32x2_t *>(at + rows * padded(cache->head_dim) * 4);
-  r->pass.places = reinterpret_cast<u32x2_t *>(at + rows * (padded(cache->head_dim) + 2) * 4);
-  return at + plane_bytes(cache, *r, tokens);
-}
+// ---- launches --------------------------------------------------------------------------------------------------------------------------
 
 template <class T, int D, int Used> int launch_all(const AttentionArgs &s, const Launch &own, const Launch *before, hipStream_t st) {
   const bool far = s.extent > kNearBytes;
@@ -907,8 +837,8 @@ template <class T, int D, int Used> int launch_all(const AttentionArgs &s, const
       if (far) hipLaunchKernelGGL((attention_tile_kernel<T, D, Used, 4, true>), grid, dim3(256), 0, st, s, r.pass);
       else hipLaunchKernelGGL((attention_tile_kernel<T, D, Used, 4, false>), grid, dim3(256), 0, st, s, r.pass);
     } else {
-      if (far) hipLaunchKernelGGL((attention_stream_kernel<T, D, Used, true>), grid, dim3(64 * kStreamWaves<D>), 0, st, s, r.pass, then);
-      else hipLaunchKernelGGL((attention_stream_kernel<T, D, Used, false>), grid, dim3(64 * kStreamWaves<D>), 0, st, s, r.pass, then);
+      if (far) hipLaunchKernelGGL((attention_stream_kernel<T, D, Used, true>), grid, dim3(64 * stream_waves(D)), 0, st, s, r.pass, then);
+      else hipLaunchKernelGGL((attention_stream_kernel<T, D, Used, false>), grid, dim3(64 * stream_waves(D)), 0, st, s, r.pass, then);
     }
     return check_launch("attention launch");
   };
@@ -925,79 +855,13 @@ template <class T, int D, int Used> int launch_all(const AttentionArgs &s, const
   return check_launch("attention join launch");
 }
 
-int attention(const char *what, const sarek_hip_kv_cache *cache, const void *q, int64_t q_token, int64_t q_head, int q_heads, void *out,
-              int64_t out_token, int64_t out_head, float *lse, const int *prefix_pages, int64_t prefix_length, const int *pages,
-              int64_t pages_stride, int max_pages, const int *lengths, const int *starts, int batch, int64_t tokens, int causal, float scale,
-              void *workspace, int64_t workspace_bytes, sarek_hip_stream stream) {
-  SAREK_ATTENTION_TRY(check_cache(what, cache));
-  AttentionArgs s;
-  SAREK_ATTENTION_TRY(make_batch(what, cache, pages, pages_stride, max_pages, lengths, starts, batch, tokens, &s.batch));
-  if (q_heads < 1 || q_heads % cache->heads != 0) return fail(SAREK_HIP_E_INVALID_ARG, "%s: %d heads of q over %d of the cache", what, q_heads, cache->heads);
-  if (q_heads > 65535 || tokens * q_heads >= int64_t{1} << 30) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: more than 65535 heads, or 2^30 rows", what);
-  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(SAREK_HIP_E_INVALID_ARG, "%s: the scale must be positive and finite", what);
-  SAREK_ATTENTION_TRY(check_heads(what, "q", q_token, q_head, tokens, q_heads, cache->head_dim, false));
-  SAREK_ATTENTION_TRY(check_heads(what, "out", out_token, out_head, tokens, q_heads, cache->head_dim, true));
-  if (prefix_length < 0 || (prefix_length > 0 && !prefix_pages)) return fail(SAREK_HIP_E_INVALID_ARG, "%s: a prefix of %lld keys", what, static_cast<long long>(prefix_length));
-  if (prefix_length > int64_t{1} << 30) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: a prefix past 2^30 keys", what);
-  const int64_t need = sarek_hip_attention_workspace_bytes(cache, q_heads, batch, tokens, max_pages, prefix_length);
-  if (workspace_bytes < need)
-    return fail(SAREK_HIP_E_WORKSPACE, "%s: a workspace of %lld bytes, %lld are needed", what, static_cast<long long>(workspace_bytes), static_cast<long long>(need));
-  if (tokens == 0 || batch == 0) return SAREK_HIP_OK;
-  if (!q || !out || (need > 0 && !workspace)) return fail(SAREK_HIP_E_INVALID_ARG, "%s: NULL pointer", what);
-  if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return fail(SAREK_HIP_E_INVALID_ARG, "%s: a workspace starts at a multiple of 16 bytes", what);
-  const int d = cache->head_dim;
-  s.q = q, s.keys = cache->keys, s.values = cache->values, s.out = out, s.lse = lse;
-  s.q_token = q_token, s.q_head = q_head, s.out_token = out_token, s.out_head = out_head;
-  s.page = cache->page_stride * 2, s.slot = cache->slot_stride * 2, s.head = cache->head_stride * 2;
-  s.extent = ((cache->n_pages - 1) * cache->page_stride + (cache->page_size - 1) * cache->slot_stride + (cache->heads - 1) * cache->head_stride + d) * 2;
-  s.heads = q_heads, s.kv_heads = cache->heads, s.head_dim = d, s.causal = causal != 0;
-  s.group = division_by(static_cast<uint32_t>(q_heads / cache->heads));
-  s.scale = scale * 1.44269504088896f;
-  s.prefix = prefix_pages, s.prefix_length = static_cast<int>(prefix_length);
-  const bool shared = prefix_length > 0;
-  Launch own = plan(cache, q_heads, batch, tokens, static_cast<int64_t>(max_pages) * cache->page_size, shared ? kBehindPrefix : kAlone);
-  Launch before = plan(cache, q_heads, 1, tokens, prefix_length, kPrefix);
-  if (std::max(own.items, before.items) * cache->heads >= int64_t{1} << 24) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: 2^24 tiles of rows or more", what);
-  char *const rest = place_planes(cache, &own, tokens, static_cast<char *>(workspace));
-  if (shared) place_planes(cache, &before, tokens, rest);
-  const auto run = [&]<class T>(T *) {
-    const hipStream_t st = as_stream(stream);
-    const Launch *const first = shared ? &before : nullptr;
-    if (d <= 64) return launch_all<T, 64, 64>(s, own, first, st);
-    if (d <= 96) return launch_all<T, 128, 96>(s, own, first, st);
-    if (d <= 128) return launch_all<T, 128, 128>(s, own, first, st);
-    return d <= 192 ? launch_all<T, 256, 192>(s, own, first, st) : launch_all<T, 256, 256>(s, own, first, st);
-  };
-  return cache->type == SAREK_HIP_TYPE_BF16 ? run(static_cast<Bf16 *>(nullptr)) : run(static_cast<_Float16 *>(nullptr));
+template <class T> int launch_type(const AttentionArgs &s, const Launch &own, const Launch *before, hipStream_t st) {
+  const int d = s.head_dim;
+  if (d <= 64) return launch_all<T, 64, 64>(s, own, before, st);
+  if (d <= 96) return launch_all<T, 128, 96>(s, own, before, st);
+  if (d <= 128) return launch_all<T, 128, 128>(s, own, before, st);
+  return d <= 192 ? launch_all<T, 256, 192>(s, own, before, st) : launch_all<T, 256, 256>(s, own, before, st);
 }
 
 }  // namespace
 }  // namespace sarek_hip
-
-using namespace sarek_hip;
-
-extern "C" {
-
-int64_t sarek_hip_attention_workspace_bytes(const sarek_hip_kv_cache *cache, int q_heads, int batch, int64_t tokens, int max_pages, int64_t prefix_length) {
-  if (!cache || cache->heads < 1 || q_heads < cache->heads || batch < 1 || tokens < 1 || max_pages < 0 || prefix_length < 0) return 0;
-  const Launch own = plan(cache, q_heads, batch, tokens, static_cast<int64_t>(max_pages) * cache->page_size, prefix_length > 0 ? kBehindPrefix : kAlone);
-  return plane_bytes(cache, own, tokens) + (prefix_length > 0 ? plane_bytes(cache, plan(cache, q_heads, 1, tokens, prefix_length, kPrefix), tokens) : 0);
-}
-
-int sarek_hip_attention_paged(const sarek_hip_kv_cache *cache, const void *q, int64_t q_token, int64_t q_head, int q_heads, void *out,
-                              int64_t out_token, int64_t out_head, float *lse, const int *pages, int64_t pages_stride, int max_pages,
-                              const int *lengths, const int *starts, int batch, int64_t tokens, int causal, float scale, void *workspace,
-                              int64_t workspace_bytes, sarek_hip_stream stream) {
-  return attention("attention_paged", cache, q, q_token, q_head, q_heads, out, out_token, out_head, lse, nullptr, 0, pages, pages_stride, max_pages, lengths,
-                   starts, batch, tokens, causal, scale, workspace, workspace_bytes, stream);
-}
-
-int sarek_hip_attention_shared(const sarek_hip_kv_cache *cache, const void *q, int64_t q_token, int64_t q_head, int q_heads, void *out,
-                               int64_t out_token, int64_t out_head, float *lse, const int *prefix_pages, int64_t prefix_length,
-                               const int *pages, int64_t pages_stride, int max_pages, const int *lengths, const int *starts, int batch,
-                               int64_t tokens, int causal, float scale, void *workspace, int64_t workspace_bytes, sarek_hip_stream stream) {
-  return attention("attention_shared", cache, q, q_token, q_head, q_heads, out, out_token, out_head, lse, prefix_pages, prefix_length, pages, pages_stride,
-                   max_pages, lengths, starts, batch, tokens, causal, scale, workspace, workspace_bytes, stream);
-}
-
-}  // extern "C"

@@ -241,7 +241,7 @@ int make_batch(const char *what, const sarek_hip_kv_cache *cache, const int *pag
   if (batch > 1 && pages_stride < max_pages) return fail(SAREK_HIP_E_INVALID_ARG, "%s: rows of the page table are %lld apart, less than %d", what, static_cast<long long>(pages_stride), max_pages);
   if (!starts && tokens < batch) return fail(SAREK_HIP_E_INVALID_ARG, "%s: without starts each of %d sequences has a token, but there are %lld", what, batch, static_cast<long long>(tokens));
   if (static_cast<int64_t>(max_pages) * cache->page_size > (int64_t{1} << 30)) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: sequences past 2^30 keys", what);
-  if (tokens >= 1 << 24 || batch > 1 << 20) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: 2^24 tokens or more than 2^20 sequences", what);
+  if (tokens >= 1 << 24 || batch > 1 << 16) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: 2^24 tokens or more than 2^16 sequences", what);
   *out = {pages, lengths, starts, pages_stride, max_pages, batch, static_cast<int>(tokens), static_cast<int>(cache->n_pages), division_by(cache->page_size)};
   return SAREK_HIP_OK;
 }

@@ -61,7 +61,7 @@ def test_invalid_arguments(hip, call, bad):
 
 @pytest.mark.parametrize("call,bad", [
     (rotary, dict(heads=65536, x=P, xh=64, oh=64, xt=1 << 23, ot=1 << 23)), (append, dict(head_dim=60)), (append, dict(head_dim=264, head_stride=264, slot_stride=528, page_stride=528 * 16)),
-    (append, dict(tokens=1 << 24, starts=P)), (append, dict(batch=(1 << 20) + 1, tokens=(1 << 20) + 1)), (attend, dict(mp=1 << 27, ps=1 << 27)),
+    (append, dict(tokens=1 << 24, starts=P)), (append, dict(batch=(1 << 16) + 1, tokens=(1 << 16) + 1)), (attend, dict(tokens=1 << 23, starts=P, q_heads=8)), (attend, dict(batch=1 << 17, tokens=1 << 17)), (attend, dict(mp=1 << 27, ps=1 << 27)),
     (attend, dict(prefix=P, n=(1 << 30) + 1)), (attend, dict(head_dim=4))], ids=lambda v: v.__name__ if callable(v) else "-".join(v))
 def test_unsupported(hip, call, bad):
     assert call(hip, **bad) == hip.E_UNSUPPORTED

@@ -504,3 +504,69 @@ def test_random_calls(hip, torch_cuda):
                     layout=rng.choice(["plain", "heads first", "one block", "heads outermost"]), apart=rng.choice([0, 1, 8]), std=rng.choice([0.5, 2.0, 8.0]))
         print(turn, case, flush=True)
         run(hip, gen, **case)
+
+
+def test_many_sequences(hip, torch_cuda):
+    """More sequences than a wave has lanes, several times over: tiles, stretches and planes are found across the blocks of 64."""
+    gen = torch.Generator().manual_seed(16)
+    lengths = [int(v) for v in torch.randint(0, 40, (700,), generator=gen)]
+    lengths[333] = lengths[699] = 5000
+    news = [min(v, 1 + i % 3) for i, v in enumerate(lengths)]
+    run(hip, gen, "bf16", 64, 2, 1, 16, lengths)
+    run(hip, gen, "f16", 64, 2, 1, 16, lengths, news, pad=1)
+    run(hip, gen, "bf16", 64, 24, 1, 16, lengths[:200] + [4000], news[:200] + [3], prefix=200)
+
+
+def test_many_small_weights(hip, torch_cuda):
+    """One key far above 60000 others, whose weights of 2^-14 to 2^-17 (below fp16's normal numbers) are most of the sum."""
+    for dtype in ("f16", "bf16"):
+        gen = torch.Generator().manual_seed(17)
+        n, d = 60000, 64
+        pages, _, count = table([n], 64, gen)
+        cache = cache_of(hip, count, 64, 1, d, TYPES[dtype])
+        fill(cache, pages, [n], gen, key=0.1)
+        cache.values[:] = cache.values.abs()
+        for rows in (1, 40):
+            q = torch.ones(rows, 2, d, dtype=TYPES[dtype], device="cuda")
+            cache.keys[pages[0, 0].long(), 0, 0] = 11.0 / 8
+            lse = torch.empty(rows, 2, device="cuda")
+            starts = [0, rows]
+            got = hip.attention_paged(q, cache, pages, ints([n]), starts=ints(starts), causal=False, lse=lse)
+            want, tol, want_lse, lse_tol = ref.attention(q, cache.keys, cache.values, pages, [n], starts, False)
+            assert ref.compare(got, want, tol)[1] <= 1 and ref.compare(lse, want_lse, lse_tol)[1] <= 1
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-3, 3.0])
+def test_scales(hip, torch_cuda, scale):
+    gen = torch.Generator().manual_seed(18)
+    run(hip, gen, "bf16", 128, 4, 2, 16, [300, 5, 0, 77], scale=scale)
+    run(hip, gen, "f16", 128, 4, 2, 16, [300, 5, 77], [300, 2, 70], scale=scale)
+
+
+def test_tables_with_rows_apart(hip, torch_cuda):
+    """A page table that is a part of a wider one."""
+    gen = torch.Generator().manual_seed(19)
+    lengths = [40, 100]
+    pages, _, n = table(lengths, 16, gen)
+    wide = torch.full((2, pages.shape[1] + 5), -7, dtype=torch.int32, device="cuda")
+    wide[:, 2:2 + pages.shape[1]] = pages
+    cache = cache_of(hip, n, 16, 2, 64, torch.bfloat16)
+    fill(cache, pages, lengths, gen)
+    q = queries(gen, 2, 4, 64, torch.bfloat16)
+    assert torch.equal(hip.attention_paged(q, cache, wide[:, 2:2 + pages.shape[1]], ints(lengths)), hip.attention_paged(q, cache, pages, ints(lengths)))
+
+
+def test_on_a_stream_of_its_own(hip, torch_cuda):
+    """Everything runs on the current stream, behind what made its inputs there."""
+    gen = torch.Generator().manual_seed(20)
+    plan, pages = hip.Rotary(64), torch.arange(20, dtype=torch.int32).view(5, 4).cuda()
+    k, v, q = (torch.randn(5, h, 64, generator=gen).bfloat16().cuda() for h in (2, 2, 8))
+    want = step(hip, (k, v, q, plan), cache_of(hip, 20, 16, 2, 64, torch.bfloat16, fill=0.5), pages, ints([64, 33, 1, 20, 50]))
+    cache = cache_of(hip, 20, 16, 2, 64, torch.bfloat16, fill=0.5)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        late = [t + 0 for _ in range(20) for t in (k, v, q)][-3:]
+        got = step(hip, (*late, plan), cache, pages, ints([64, 33, 1, 20, 50]))
+    side.synchronize()
+    assert torch.equal(got, want)
