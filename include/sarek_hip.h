@@ -750,7 +750,9 @@ int sarek_hip_rotary(const sarek_hip_rotary_plan *plan, const void *x, int64_t x
  * token b where starts is NULL; they are the last of its lengths[b] keys.  Key p of sequence b lies in slot p % page_size of the page
  * pages[b * pages_stride + p / page_size], p / page_size < max_pages.  lengths, starts and pages are int32 in device memory and are read
  * when the kernels run.  Keys that the table has no room for are left out; an entry of the table that is no page of the cache is not
- * written to and stands for keys and values of zeros.  Rows of tokens before the first and behind the last sequence are left as they are.             */
+ * written to and stands for keys and values of zeros.  Rows of tokens before the first and behind the last sequence are left as they are.
+ * Served are (SAREK_HIP_E_UNSUPPORTED past that) below 2^24 tokens to a call, 2^16 sequences, 2^30 keys to a sequence or prefix, 65535
+ * heads; attention below 2^26 tokens times heads and 2^23 tiles of rows (16, 128 or 256 each, one more to a sequence) times the cache's heads. */
 typedef struct {
   void *keys, *values;
   int64_t page_stride, slot_stride, head_stride;
@@ -759,7 +761,7 @@ typedef struct {
 } sarek_hip_kv_cache;
 /* Puts the tokens' k and v [tokens, cache->heads, head_dim] into their places, k turned by plan (NULL: as it is) at the position
  * first + place in its sequence.  q (or NULL) [tokens, q_heads, head_dim] is turned likewise into q_out, which may be q itself; nothing
- * else may overlap.  A page that the tokens go to belongs to one sequence.                                                       */
+ * else may overlap.  A page that the tokens go to is in the table once.                                                          */
 int sarek_hip_kv_append(const sarek_hip_kv_cache *cache, const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token,
                         int64_t v_head, const void *q, int64_t q_token, int64_t q_head, void *q_out, int64_t q_out_token,
                         int64_t q_out_head, int q_heads, const sarek_hip_rotary_plan *plan, const int *pages, int64_t pages_stride,
@@ -767,7 +769,8 @@ int sarek_hip_kv_append(const sarek_hip_kv_cache *cache, const void *k, int64_t 
                         sarek_hip_stream stream);
 /* out = softmax(scale q . keys) . values, head h of q with head h / (q_heads / cache->heads) of the cache; causal not 0: a token sees its
  * sequence's keys up to its own.  A token that sees no key gets zeros.  lse (or NULL) [tokens, q_heads]: the natural logarithm of
- * the sum of the exponents, minus infinity for no key.  Scores, their exponents' sums and the weighted values are held in float32.  A
+ * the sum of the exponents, minus infinity for no key; one whose scores are all minus infinity counts as that.  out may be q itself, with
+ * its strides, and must not overlap it otherwise.  Scores, their exponents' sums and the weighted values are held in float32.  A
  * key that a token does not see takes no part in its sums, whatever the cache holds there.  scale is positive and finite.
  * workspace: sarek_hip_attention_workspace_bytes, for the same arguments, of device memory (16 bytes aligned), SAREK_HIP_E_WORKSPACE else;
  * one call at a time may use it.

@@ -31,7 +31,7 @@ Launch plan(const sarek_hip_kv_cache *cache, int q_heads, int64_t sequences, int
   r.pass = {what == kPrefix, tile_rows, 0, 0, 0, 0, nullptr, nullptr, nullptr};
   r.pass.unit = r.waves ? 2 * kTileKeys : kStreamKeys * stream_waves(d);
   const int64_t most_tiles = rows / r.pass.rows + sequences, tiles = std::max(rows / r.pass.rows, std::min(tokens, sequences)), units = ceil_div(keys, r.pass.unit);
-  const int64_t wanted = r.waves ? tunable("attention.tile_workgroups", compute_units()) : tunable("attention.stream_workgroups", 3 * compute_units());
+  const int64_t wanted = std::min<int64_t>(r.waves ? tunable("attention.tile_workgroups", compute_units()) : tunable("attention.stream_workgroups", 3 * compute_units()), 1 << 20);
   if (units > 1 && tiles * heads < (what == kBehindPrefix && !r.waves ? compute_units() : wanted)) r.pass.target = static_cast<int>(wanted);
   r.pass.all = what == kPrefix || (what == kBehindPrefix && (r.waves || r.pass.target != 0));
   // (the number of units to a stretch comes from a float32 sum: a few items more)

@@ -400,7 +400,7 @@ bool read_sequences(PyObject *pages, PyObject *lengths, PyObject *starts, long d
     return false;
   }
   *out = {static_cast<const int *>(p.data), static_cast<const int *>(l.data), static_cast<const int *>(s.data),
-          p.stride[0] > p.shape[1] ? p.stride[0] : p.shape[1], static_cast<int>(p.shape[1]), static_cast<int>(l.shape[0])};
+          l.shape[0] > 1 ? p.stride[0] : p.shape[1], static_cast<int>(p.shape[1]), static_cast<int>(l.shape[0])};
   return true;
 }
 

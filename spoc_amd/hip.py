@@ -1254,7 +1254,7 @@ def _sequences(cache, pages, lengths, starts, tokens):
     starts_at = None if starts is None else _table(starts, (batch + 1,), "starts", device)
     if starts is None and tokens != batch:
         raise ValueError(f"without starts each of {batch} sequences has one token, but there are {tokens}")
-    return pages_at, max(pages.stride(0), pages.shape[1]), pages.shape[1], lengths_at, starts_at, batch
+    return pages_at, pages.stride(0) if batch > 1 else pages.shape[1], pages.shape[1], lengths_at, starts_at, batch
 
 
 def _cache_heads(t, cache, tokens, heads, name):
@@ -1275,7 +1275,7 @@ def kv_append(k, v, cache, pages, lengths, starts=None, rotary=None, q=None, q_o
 
     Sequence b of the batch has the tokens starts[b] to starts[b + 1] - 1 (starts None: the one token b); they are the last of its
     lengths[b] keys.  Key p is in slot p % page size of page pages[b, p // page size] and at position first + p.  lengths [batch],
-    starts [batch + 1] and pages [batch, any] are int32 on the device.  A page that tokens go to belongs to one sequence; tokens that the
+    starts [batch + 1] and pages [batch, any] are int32 on the device.  A page that tokens go to is in the table once; tokens that the
     table has no room for, or no page of the cache, are not put anywhere.  Tokens before the first and behind the last sequence are left
     alone, in q_out too."""
     if not isinstance(cache, KvCache):
@@ -1343,7 +1343,7 @@ def attention_paged(q, cache, pages, lengths, starts=None, causal=True, scale=No
     """softmax(scale q . keys) . values of q [tokens, heads, head dim] over a KvCache, whose heads serve as many of q's each as there are;
     scale None: head dim ^ -1/2.  The sequences' tokens, lengths and pages: as for kv_append, the tokens' own keys are in the cache
     already.  causal: a token sees its sequence's keys up to its own, otherwise all of them; a token that sees none gets zeros.
-    out: where the result goes; lse (float32 [tokens, heads]): gets the logarithm of the sum of the exponents, -inf where there is none.
+    out: where the result goes, which may be q itself; lse (float32 [tokens, heads]): gets the logarithm of the sum of the exponents, -inf where there is none.
     Rows of tokens before the first and behind the last sequence are left as they are."""
     if isinstance(cache, KvCache):
         got = _host.attention_tensors(q, cache._call, None, 0, pages, lengths, starts, causal, scale, out, lse)

@@ -570,3 +570,52 @@ def test_on_a_stream_of_its_own(hip, torch_cuda):
         got = step(hip, (*late, plan), cache, pages, ints([64, 33, 1, 20, 50]))
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_tables_with_rows_on_each_other(hip, torch_cuda):
+    """An expanded page table has one row in memory: what lies behind it is not read as the others."""
+    cache = cache_of(hip, 4, 16, 2, 64, torch.bfloat16, fill=0.0)
+    q, lengths = torch.ones(2, 4, 64, dtype=torch.bfloat16, device="cuda"), ints([20, 30])
+    for pages in (ints([[0, 1]]).expand(2, 2), torch.arange(3, dtype=torch.int32, device="cuda").as_strided((2, 2), (1, 1))):
+        for call in (lambda: hip.attention_paged(q, cache, pages, lengths), lambda: hip.attention_shared(q, cache, ints([3]), 16, pages, lengths),
+                     lambda: hip.kv_append(q[:, :2], q[:, :2], cache, pages, lengths)):
+            with pytest.raises(hip.SarekHipError):
+                call()
+    one = ints([[0, 1]]).as_strided((1, 2), (0, 1))      # (the only row may lie anyhow)
+    assert torch.equal(hip.attention_paged(q[:1], cache, one, ints([20])), torch.zeros_like(q[:1]))
+
+
+@pytest.mark.parametrize("news,prefix", [(None, 0), ([40, 3], 0), ([2, 2], 100), ([60, 70], 100)])
+def test_out_may_be_q(hip, torch_cuda, news, prefix):
+    gen = torch.Generator().manual_seed(21)
+    lengths = [3000, 90]
+    pages, prefix_pages, n = table(lengths, 16, gen, prefix=-(-prefix // 16))
+    cache = cache_of(hip, n, 16, 2, 64, torch.bfloat16)
+    fill(cache, pages, lengths, gen)
+    fill(cache, prefix_pages[None], [prefix], gen)
+    q = queries(gen, 2 if news is None else sum(news), 8, 64, torch.bfloat16)
+    starts = None if news is None else ints([0, news[0], sum(news)])
+    call = lambda out: hip.attention_shared(q, cache, prefix_pages, prefix, pages, ints(lengths), starts=starts, out=out)  # noqa: E731
+    want = call(None)
+    assert call(q) is q and torch.equal(q, want)
+
+
+def test_many_heads(hip, torch_cuda):
+    gen = torch.Generator().manual_seed(22)
+    run(hip, gen, "f16", 8, 520, 520, 16, [70, 1, 0])
+    run(hip, gen, "bf16", 16, 600, 1, 16, [70, 9, 300], [3, 1, 2])
+
+
+@pytest.mark.parametrize("name,values", [("tile_workgroups", [-1, 0, 1, 7, 5000, 1 << 40]), ("stream_workgroups", [-1, 0, 1, 7, 5000, 1 << 40]), ("large_tiles", [0, 1 << 40])])
+def test_every_split_gives_the_same(hip, torch_cuda, name, values):
+    """What decides how the keys are split and which tiles are taken is free to be set."""
+    try:
+        for v in values:
+            hip.set_tunable("attention." + name, v)
+            gen = torch.Generator().manual_seed(23)
+            run(hip, gen, "bf16", 128, 8, 2, 16, [1500, 3, 400])
+            run(hip, gen, "f16", 128, 8, 2, 16, [1500, 30, 400], [300, 30, 1])
+            run(hip, gen, "bf16", 64, 8, 2, 16, [100, 3, 40], prefix=700)
+            run(hip, gen, "bf16", 128, 8, 2, 16, [100, 3, 400], [90, 3, 300], prefix=700)
+    finally:
+        hip.set_tunable("attention." + name, {"tile_workgroups": 256, "stream_workgroups": 768, "large_tiles": 512}[name])
