@@ -18,25 +18,46 @@ int64_t plane_bytes(const sarek_hip_kv_cache *cache, const Launch &r, int64_t to
   return planes * r.pass.rows * (padded(cache->head_dim) + 2) * 4 + (tokens + 1) / 2 * 16;
 }
 // What is launched, by what the host knows: how many tokens, sequences and keys there are at most.
-// Kernel: up to 16 rows to a sequence on average go to the kernel of few rows (XX), others to tiles of 128, and of 256 where those fill the card twice.
-// Stretches: where there are fewer tiles than that, the keys are cut for about `target` workgroups.  Own keys behind a prefix, few rows: a
-// workgroup to each tile where these fill the card, which then finishes with the prefix's planes; no launch for the join.
+//
+// Kernel.  Up to 16 rows to a sequence on average: the kernel of few rows; more: tiles of 128.  (us, 32 heads on 8 of 128, few rows / tiles: one
+// sequence of 4095 keys, 4 rows 16.3 / 19.0; 131071 keys 117 / 128; 64 of 2000, 20 rows 135 / 106, 16 rows 112 / 105.  Tiles are as fast from 8 rows on where
+// there are many sequences, but round the weights to 16 bits, which the kernel of few rows does not.)
+// Tiles of 256: heads of 65 to 128 values, long sequences that fill the card twice.  (One prompt, tiles of 256 / 128: 8192 tokens 526 / 537, 16384 2000 /
+// 2044; but 5000 231 / 219, and 16 prompts of 1000 242 / 222, for the rows past the ends and what the mask hides in a larger tile.)
+//
+// Stretches.  Where tiles are few for the card, the keys are cut: for as many workgroups as it takes at once if that comes out (find_item), two to
+// a compute unit for the kernel of few rows and tiles of 128, whose transfers it takes to keep the memory busy (8 sequences of 4000, one token: 512 workgroups 33.4, 256 36.9, 768 40.4;
+// 12 of 4000, which do not fill 512: 480 42.6, 576 55.8).  Few rows that do not come out get half as many again (61 sequences of 100 to 11007: 768 207, 512
+// 225).  Tiles are cut below one to a compute unit: planes of 128 rows cost as much as 6 units of keys (2000 tokens behind 6000: uncut 249, cut 284); and for half as many
+// workgroups where a stretch would have less than 12 units (64 behind 8128: 4 units 36.3, 8 units 32.3; 500 behind 7692: 32 units 90, 64 units 99).
+// No more than 256 stretches: 30000 keys of one head, 235 of them 21.1, 469 25.3 (131071: 256 31.6, 512 35.7, 128 37.9).
+// Own keys behind a prefix, few rows: a workgroup to each tile where these fill the card, which then finishes with the prefix's planes; no launch for
+// the join (61 sequences of up to 500 behind 8191: 57 with the join, 46).
 enum { kAlone, kBehindPrefix, kPrefix };
 Launch plan(const sarek_hip_kv_cache *cache, int q_heads, int64_t sequences, int64_t tokens, int64_t keys, int what) {
   const int d = cache->head_dim;
-  const int64_t rows = tokens * (q_heads / cache->heads), heads = cache->heads;
+  const int64_t rows = tokens * (q_heads / cache->heads), heads = cache->heads, units_at_once = compute_units();
+  const int64_t large = tunable("attention.large_rows", 25600);
+  const auto large_tiles = [&] { return large == 0 || (rows / 256 * heads >= 2 * units_at_once && rows >= large * sequences); };
   Launch r;
-  r.waves = rows <= 16 * sequences ? 0 : d > 64 && d <= 128 && rows / 256 * heads >= tunable("attention.large_tiles", 2 * compute_units()) ? 8 : 4;
-  const int tile_rows = r.waves ? 32 * r.waves : 16;
-  r.pass = {what == kPrefix, tile_rows, 0, 0, 0, 0, nullptr, nullptr, nullptr};
+  r.waves = rows <= 16 * sequences ? 0 : d > 64 && d <= 128 && large_tiles() ? 8 : 4;
+  r.pass = {};
+  r.pass.prefix = what == kPrefix;
+  r.pass.rows = r.waves ? 32 * r.waves : 16;
   r.pass.unit = r.waves ? 2 * kTileKeys : kStreamKeys * stream_waves(d);
   const int64_t most_tiles = rows / r.pass.rows + sequences, tiles = std::max(rows / r.pass.rows, std::min(tokens, sequences)), units = ceil_div(keys, r.pass.unit);
-  const int64_t wanted = std::min<int64_t>(r.waves ? tunable("attention.tile_workgroups", compute_units()) : tunable("attention.stream_workgroups", 3 * compute_units()), 1 << 20);
-  if (units > 1 && tiles * heads < (what == kBehindPrefix && !r.waves ? compute_units() : wanted)) r.pass.target = static_cast<int>(wanted);
+  const bool two_to_a_unit = r.waves != 8 && !(r.waves && d > 128);
+  const int64_t at_once = std::clamp<int64_t>(r.waves ? tunable("attention.tile_workgroups", 2 * compute_units()) / (two_to_a_unit ? 1 : 2)
+                                                      : tunable("attention.stream_workgroups", 2 * compute_units()), 0, 1 << 20);
+  const int64_t spread = r.waves ? at_once : at_once * 3 / 2;
+  if (units > 1 && at_once > 0 && tiles * heads < (r.waves || what == kBehindPrefix ? units_at_once : spread)) {
+    r.pass.target = static_cast<int>(at_once), r.pass.spread = static_cast<int>(spread);
+    r.pass.least_units = r.waves && two_to_a_unit ? 12 : 0;
+  }
   r.pass.all = what == kPrefix || (what == kBehindPrefix && (r.waves || r.pass.target != 0));
   // (the number of units to a stretch comes from a float32 sum: a few items more)
-  r.items = r.pass.target == 0 ? most_tiles : std::min(most_tiles + wanted / heads + 8, most_tiles * units);
-  r.pass.max_slots = static_cast<int>(r.pass.all ? r.items : r.pass.target == 0 ? 0 : std::min(r.items, 2 * wanted / heads + 8));
+  r.items = r.pass.target == 0 ? most_tiles : std::min(most_tiles + spread / heads + 8, most_tiles * units);
+  r.pass.max_slots = static_cast<int>(r.pass.all ? r.items : r.pass.target == 0 ? 0 : std::min(r.items, 2 * spread / heads + 8));
   return r;
 }
 char *place_planes(const sarek_hip_kv_cache *cache, Launch *r, int64_t tokens, char *at) {

@@ -35,7 +35,9 @@ typedef __attribute__((ext_vector_type(2))) unsigned int place_t;
 struct Pass {
   int prefix;            // rows of all sequences against the prefix, or each sequence's against its own keys
   int rows, unit;        // of a tile; keys in what a stretch has a whole number of
-  int target;            // about how many workgroups there are to be (0: no stretches, all of a sequence's keys in one)
+  int target;            // how many workgroups the card takes at once (0: no stretches, all of a sequence's keys in one)
+  int spread;            // about how many it gets where these do not come out
+  int least_units;       // where stretches would have fewer, half of `target`
   int all;               // everything goes into the planes, for the join
   int max_slots;
   float *o;              // [slot][kv head][row][value]

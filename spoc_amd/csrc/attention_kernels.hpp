@@ -70,6 +70,8 @@ __device__ __forceinline__ Work work_of(const AttentionArgs &s, const Pass &p, i
 __device__ __forceinline__ int sequences(const AttentionArgs &s, const Pass &p) { return p.prefix ? 1 : s.batch.batch; }
 __device__ __forceinline__ int stretches(int units, int at_once) { return max((units + at_once - 1) / max(at_once, 1), 1); }
 
+constexpr int kMostStretches = 256;      // of a sequence: as many planes a row has to be joined from
+
 struct Item {
   int b;
   int first, count, length, held;   // the sequence's, as above
@@ -83,20 +85,38 @@ struct Item {
 __device__ __forceinline__ bool find_item(const AttentionArgs &s, const Pass &p, int item, Item &it) {
   const int n = sequences(s, p), lane = threadIdx.x & 63;
   Work w = work_of(s, p, lane);
-  int at_once = INT32_MAX;           // units of keys to a stretch, for about p.target workgroups in all
+  int at_once = 1 << 30;             // units of keys to a stretch
   if (p.target != 0) {
+    // All workgroups at once, if stretches of up to a third more than their even share make that; otherwise more and shorter ones, which even out
+    // as they follow one another.
     uint64_t all = static_cast<uint64_t>(w.tiles) * static_cast<uint32_t>(w.units);
     for (int b = 64 + lane; b < n; b += 64) {
       const Work more = work_of(s, p, b);
       all += static_cast<uint64_t>(more.tiles) * static_cast<uint32_t>(more.units);
     }
-    const float total = __builtin_bit_cast(float, lane_of(__builtin_bit_cast(int, scan_wave(static_cast<float>(all))), 63));
-    at_once = max(static_cast<int>(min(ceilf(total * static_cast<float>(s.kv_heads) / static_cast<float>(p.target)), 1e9f)), 1);
+    const float total = __builtin_bit_cast(float, lane_of(__builtin_bit_cast(int, scan_wave(static_cast<float>(all))), 63)) * static_cast<float>(s.kv_heads);
+    const int target = total < static_cast<float>(p.target) * static_cast<float>(p.least_units) ? p.target / 2 : p.target;
+    const auto whole = [](float units) __attribute__((always_inline)) { return max(static_cast<int>(min(ceilf(units), 1e9f)), 1); };
+    const float even = total / static_cast<float>(target);
+    constexpr int kTries = 5;
+    int at[kTries], made[kTries];
+    float part[kTries];       // of a stretch that a unit is, a little less, so that a whole number of stretches is not rounded up
+#pragma unroll
+    for (int j = 0; j < kTries; ++j) at[j] = whole(even * (1.f + j / 12.f)), part[j] = __builtin_amdgcn_rcpf(static_cast<float>(at[j])) * (1.f - 1e-6f), made[j] = 0;
+    for (int b = 0; b < n; b += 64) {
+      const Work of = b == 0 ? w : work_of(s, p, b + lane);
+#pragma unroll
+      for (int j = 0; j < kTries; ++j) made[j] += of.tiles * max(static_cast<int>(ceilf(static_cast<float>(of.units) * part[j])), 1);
+    }
+    at_once = whole(target == p.target ? total / static_cast<float>(p.spread) : even);
+#pragma unroll
+    for (int j = kTries - 1; j >= 0; --j)
+      if (lane_of(scan_wave(made[j]), 63) * s.kv_heads <= target) at_once = at[j];
   }
   int items = 0, slots = 0;
   for (int b0 = 0; b0 < n; b0 += 64) {
     if (b0 != 0) w = work_of(s, p, b0 + lane);
-    const int cut = stretches(w.units, at_once), mine = w.tiles * cut, kept = p.all || cut > 1 ? mine : 0;
+    const int cut = min(stretches(w.units, at_once), kMostStretches), mine = w.tiles * cut, kept = p.all || cut > 1 ? mine : 0;
     const int upto = scan_wave(mine), slots_upto = scan_wave(kept);
     const uint64_t past = __ballot(items + upto > item);
     if (past != 0) {
@@ -824,7 +844,7 @@ template <class T, int D> __global__ __launch_bounds__(256) void attention_join_
 
 template <class T, int D, int Used> int launch_all(const AttentionArgs &s, const Launch &own, const Launch *before, hipStream_t st) {
   const bool far = s.extent > kNearBytes;
-  const Pass none = {0, 1, 1, 0, 0, 0, nullptr, nullptr, nullptr};
+  const Pass none = {};
   const auto one = [&](const Launch &r) {
     const Pass &then = before && !r.pass.prefix ? before->pass : none;      // (what the few rows' kernel joins with its own)
     const dim3 grid(static_cast<unsigned>(r.items * s.kv_heads));

@@ -606,7 +606,7 @@ def test_many_heads(hip, torch_cuda):
     run(hip, gen, "bf16", 16, 600, 1, 16, [70, 9, 300], [3, 1, 2])
 
 
-@pytest.mark.parametrize("name,values", [("tile_workgroups", [-1, 0, 1, 7, 5000, 1 << 40]), ("stream_workgroups", [-1, 0, 1, 7, 5000, 1 << 40]), ("large_tiles", [0, 1 << 40])])
+@pytest.mark.parametrize("name,values", [("tile_workgroups", [-1, 0, 1, 7, 5000, 1 << 40]), ("stream_workgroups", [-1, 0, 1, 7, 5000, 1 << 40]), ("large_rows", [0, 1 << 40])])
 def test_every_split_gives_the_same(hip, torch_cuda, name, values):
     """What decides how the keys are split and which tiles are taken is free to be set."""
     try:
@@ -618,4 +618,18 @@ def test_every_split_gives_the_same(hip, torch_cuda, name, values):
             run(hip, gen, "bf16", 64, 8, 2, 16, [100, 3, 40], prefix=700)
             run(hip, gen, "bf16", 128, 8, 2, 16, [100, 3, 400], [90, 3, 300], prefix=700)
     finally:
-        hip.set_tunable("attention." + name, {"tile_workgroups": 256, "stream_workgroups": 768, "large_tiles": 512}[name])
+        hip.set_tunable("attention." + name, {"tile_workgroups": 512, "stream_workgroups": 512, "large_rows": 25600}[name])
+
+
+def test_large_tiles(hip, torch_cuda):
+    """More than 25600 rows to a sequence that fill the card twice, so 256 to a workgroup."""
+    gen = torch.Generator().manual_seed(24)
+    run(hip, gen, "bf16", 72, 96, 6, 16, [1700], [1640])
+    run(hip, gen, "f16", 128, 64, 4, 20, [1700, 1800], [1650, 1800], causal=False)
+
+
+def test_more_keys_than_stretches_hold(hip, torch_cuda):
+    """One head of keys and few rows: as many stretches as a row may have, of several units each."""
+    gen = torch.Generator().manual_seed(25)
+    run(hip, gen, "bf16", 64, 2, 1, 64, [70001])
+    run(hip, gen, "f16", 256, 2, 1, 64, [9000, 30001])
