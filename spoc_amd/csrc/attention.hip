@@ -25,8 +25,9 @@ int64_t plane_bytes(const sarek_hip_kv_cache *cache, const Launch &r, int64_t to
 // Tiles of 256: heads of 65 to 128 values, long sequences that fill the card twice.  (One prompt, tiles of 256 / 128: 8192 tokens 526 / 537, 16384 2000 /
 // 2044; but 5000 231 / 219, and 16 prompts of 1000 242 / 222, for the rows past the ends and what the mask hides in a larger tile.)
 //
-// Stretches.  Where tiles are few for the card, the keys are cut: for as many workgroups as it takes at once if that comes out (find_item), two to
-// a compute unit for the kernel of few rows and tiles of 128, whose transfers it takes to keep the memory busy (8 sequences of 4000, one token: 512 workgroups 33.4, 256 36.9, 768 40.4;
+// Stretches.  Where tiles are few for the card, the keys are cut: for as many workgroups as it takes at once if that comes out (find_item).  That is two to
+// a compute unit for tiles of 128 and few rows of more than 64 values, whose transfers it takes to keep the memory busy (one token each: 8 sequences of 4000 512
+// workgroups 33.4, 256 36.9, 768 40.4; 131071 keys of 16 heads 194, 211, 218), one otherwise, or where there is no room for two (the same of 64 values 120, 113, 118;
 // 12 of 4000, which do not fill 512: 480 42.6, 576 55.8).  Few rows that do not come out get half as many again (61 sequences of 100 to 11007: 768 207, 512
 // 225).  Tiles are cut below one to a compute unit: planes of 128 rows cost as much as 6 units of keys (2000 tokens behind 6000: uncut 249, cut 284); and for half as many
 // workgroups where a stretch would have less than 12 units (64 behind 8128: 4 units 36.3, 8 units 32.3; 500 behind 7692: 32 units 90, 64 units 99).
@@ -46,9 +47,9 @@ Launch plan(const sarek_hip_kv_cache *cache, int q_heads, int64_t sequences, int
   r.pass.rows = r.waves ? 32 * r.waves : 16;
   r.pass.unit = r.waves ? 2 * kTileKeys : kStreamKeys * stream_waves(d);
   const int64_t most_tiles = rows / r.pass.rows + sequences, tiles = std::max(rows / r.pass.rows, std::min(tokens, sequences)), units = ceil_div(keys, r.pass.unit);
-  const bool two_to_a_unit = r.waves != 8 && !(r.waves && d > 128);
-  const int64_t at_once = std::clamp<int64_t>(r.waves ? tunable("attention.tile_workgroups", 2 * compute_units()) / (two_to_a_unit ? 1 : 2)
-                                                      : tunable("attention.stream_workgroups", 2 * compute_units()), 0, 1 << 20);
+  const bool two_to_a_unit = r.waves ? r.waves == 4 && d <= 128 : d > 64;
+  const int64_t wanted = r.waves ? tunable("attention.tile_workgroups", 2 * compute_units()) : tunable("attention.stream_workgroups", 2 * compute_units());
+  const int64_t at_once = std::clamp<int64_t>(two_to_a_unit ? wanted : wanted / 2, 0, 1 << 20);
   const int64_t spread = r.waves ? at_once : at_once * 3 / 2;
   if (units > 1 && at_once > 0 && tiles * heads < (r.waves || what == kBehindPrefix ? units_at_once : spread)) {
     r.pass.target = static_cast<int>(at_once), r.pass.spread = static_cast<int>(spread);

@@ -323,8 +323,9 @@ template <int D, int kAtOnce> __device__ __forceinline__ void add_planes(const P
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------
 
 // A wave takes every kWaves-th tile of 32 keys of the stretch by itself: its transfers go into its own part of LDS, one tile ahead, and there
-// is no barrier until the waves' sums are joined at the end.
-
+// is no barrier until the waves' sums are joined at the end.  The bytes of the cache bound it: 46 sequences of 100 to 11007 keys, 8 heads of
+// 128, 1.02 GB in 192 us, 5.3 TB/s (a large copy on this card: 5.1); 131071 keys of 16 heads of 64 in 101 us, 5.3.  The matrix unit is busy for 7 % of the time.  One
+// token of 4095 keys: 7.4 us for 17 MB, of which about 3 are a launch's start and the way to the first transfer (lengths, page, keys).
 template <class T, int D, int Used, bool Far>
 __global__ __launch_bounds__(64 * stream_waves(D)) void attention_stream_kernel(AttentionArgs s, Pass p, Pass before) {
   constexpr int kWaves = stream_waves(D), kRowBytes = 2 * D, kPieces = D / 8, kKeysMoved = 64 / kPieces, kMoves = kStreamKeys / kKeysMoved;
@@ -513,6 +514,14 @@ __global__ __launch_bounds__(64 * stream_waves(D)) void attention_stream_kernel(
 // Four waves of 32 rows, two blocks of 16; tiles of 32 keys go to LDS for all of them, three ahead.  While the softmax of tile j is on the vector
 // unit, the matrix unit forms the scores of tile j + 1; then come the weighted values of tile j.  Used: the values of a head, rounded up to 32 (D, the
 // length of a row in LDS, is a power of two).
+//
+// A prompt of 8192 tokens, 32 heads on 8 of 128 (Waves 8): 530 us, 1035 TFLOP/s of what the mask leaves; a matrix product reaches 1410 here.  The matrix unit is
+// busy for 47 % of the time, at 2.1 to 2.2 GHz, the power's bound.  Without the exponentials it took 535 of then 567 us, without the scores' product 412, without the
+// values' 460, without transfers 462: what is left is the softmax's vector instructions (4.3 to a matrix instruction) beside the matrix unit.  First without the
+// scores ahead 641, with 32 x 32 matrix instructions 552 for 547; 64 rows to a wave, one wave to a SIMD, 855.
+//
+// The weights are rounded to 16 bits for the second product (in two parts, as in the other kernel, it would be twice the work): off by up to half a step
+// each, 2^-9 of a sum's size in bf16 where they add up at random, the size of out's own rounding.  l is the sum of the weights before that rounding, so lse is not touched.
 constexpr int kTileRing = 4;
 
 template <class T, int D, int Used, int Waves, bool Far>
@@ -799,6 +808,8 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
 
 // D / 4 threads, `spread` times over, to a token and head: with M the largest of the planes' maxima, l = sum 2^(m - M) l, o = sum 2^(m - M) o / l,
 // every part of the threads with every spread-th plane, and the parts in order.
+// Latency bounds it, a row's table and then its planes: 4 to 5 us for 32 rows of 64 planes each (asked for together; one after the other 3 more).
+// 2500 x 13 rows of one to three planes of 80 values 9 us.
 template <class T, int D> __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs s, Pass own, Pass before, int spread) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
   __shared__ float sums[kGroups][D], ends[kGroups][2];
@@ -865,7 +876,7 @@ template <class T, int D, int Used> int launch_all(const AttentionArgs &s, const
   if (before) SAREK_ATTENTION_TRY(one(*before));
   SAREK_ATTENTION_TRY(one(own));
   if (own.pass.max_slots == 0) return SAREK_HIP_OK;
-  // Rows that are few for the card take more threads each, which share the planes.
+  // Rows that are few for the card take more threads each, which share the planes (one token of 4095 keys, both launches: 16.5 us, 22.7 without).
   constexpr int kGroups = 1024 / D;
   const int64_t rows = static_cast<int64_t>(s.batch.tokens) * s.heads;
   int spread = 1;

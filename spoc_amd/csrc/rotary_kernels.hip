@@ -6,7 +6,9 @@
 // position 10^6), and there is no reduction of the argument left for the sine.
 //
 // Memory bounds both kernels (two products and a sum to a value); a thread takes 8 pairs of a head, two accesses of 16 bytes each way in
-// 16-bit types, and where there are many tokens 4 heads, for which it forms the sines once.
+// 16-bit types, and where there are many tokens 4 heads, for which it forms the sines once (8192 x 32 x 128 bf16: 22 us, 6.1 TB/s; a
+// thread to each head 26).  One token of 32 heads: 2.8 us, a launch.  Appending 8190 tokens of 32 and 8 + 8 heads of 128 to pages in fp16: 38 us, 5.3 TB/s;
+// 16 tokens 4.5 us, the search for a token's sequence and its page before the first access.
 #include <cmath>
 
 #include "attention_common.hpp"
@@ -60,7 +62,7 @@ __device__ __forceinline__ Turned angles(const RotaryArgs &r, int64_t position, 
 
 // Piece `unit` of heads head to head + kHeads - 1, those of them below `heads`: 8 pairs, or 16 of the values behind the pairs.  All are asked for
 // before the first is written: out may be x, so the compiler would not put a load before an earlier store.  (8190 tokens of 32 and 8
-// heads appended: 58.7 us with each head's loads behind the stores of the one before.)
+// heads appended: 49.8 us, 58.7 with each head's loads behind the stores of the one before; launch and tensors among it.)
 template <class T, bool Interleaved, int kHeads>
 __device__ __forceinline__ void turn_pieces(const RotaryArgs &r, int64_t position, const T *x, int64_t x_head, T *out, int64_t out_head, int head, int heads,
                                             int unit) {
@@ -200,7 +202,9 @@ int make_plan(const char *what, const sarek_hip_rotary_plan *plan, int head_dim,
   *r = {plan->turns, plan->amplitude, plan->pairs, 0, head_dim, static_cast<int>(ceil_div(plan->pairs, kPairs)), static_cast<int>(ceil_div(head_dim - 2 * plan->pairs, 16))};
   return SAREK_HIP_OK;
 }
-// From here on (pieces of one head) a thread takes 4 heads; below that more threads, and so more loads at once, are worth the sines.
+// From here on (pieces of one head) a thread takes 4 heads; below that more threads, and so more loads at once, are worth the sines.  (Graphs of one
+// launch, us, 4 heads to a thread / 1, heads of 128 in bf16: 16384 x 4 17.5 / 16.6, 4096 x 8 16.5 / 16.8, 4096 x 32 17.5 / 21.2, 16384 x 8 17.6 / 21.1, 16384 x 32 46.8 / 53.7.)
+// Fewer than 4 heads leave a thread's places empty (16384 x 2: 16.4 / 17.8, x 3 17.4 / 16.7: no difference that stands out).
 constexpr int64_t kManyPieces = 1 << 19;
 
 }  // namespace
