@@ -324,7 +324,7 @@ template <int D, int kAtOnce> __device__ __forceinline__ void add_planes(const P
 
 // A wave takes every kWaves-th tile of 32 keys of the stretch by itself: its transfers go into its own part of LDS, one tile ahead, and there
 // is no barrier until the waves' sums are joined at the end.  The bytes of the cache bound it: 46 sequences of 100 to 11007 keys, 8 heads of
-// 128, 1.02 GB in 192 us, 5.3 TB/s (a large copy on this card: 5.1); 131071 keys of 16 heads of 64 in 101 us, 5.3.  The matrix unit is busy for 7 % of the time.  One
+// 128, 1.02 GB in 192 us, 5.3 TB/s (a large copy on this card: 5.1); 131071 keys of 16 heads of 64 in 98 us, 5.5.  The matrix unit is busy for 7 % of the time.  One
 // token of 4095 keys: 7.4 us for 17 MB, of which about 3 are a launch's start and the way to the first transfer (lengths, page, keys).
 template <class T, int D, int Used, bool Far>
 __global__ __launch_bounds__(64 * stream_waves(D)) void attention_stream_kernel(AttentionArgs s, Pass p, Pass before) {
