@@ -486,6 +486,7 @@ __global__ __launch_bounds__(64 * stream_waves(D)) void attention_stream_kernel(
   const int live = min(16, it.count * static_cast<int>(s.group.size) - it.row0);
   for (int column = threadIdx.x; column < live * kQuads; column += kThreads) {
     const int r = column / kQuads, d = column % kQuads * 4;
+    if (d >= s.head_dim) continue;
     const Row to = row_at(s, p, it, kv_head, it.row0 + r);
     Sums a = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -794,7 +795,7 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
     for (int c = 0; c < kColumns; ++c) {
       const int d = c * 16 + quad * 4;
       if (it.slot < 0) store_out<T>(s, row[r].token, row[r].head, d, o[c][r] * inverse);
-      else *reinterpret_cast<f32x4_t *>(p.o + place * D + d) = o[c][r];
+      else if (d < s.head_dim) *reinterpret_cast<f32x4_t *>(p.o + place * D + d) = o[c][r];
     }
     if (quad == 0) {
       if (it.slot < 0) store_lse(s, row[r].token, row[r].head, m[r] * s.scale, l[r]);
@@ -820,7 +821,7 @@ template <class T, int D> __global__ __launch_bounds__(256) void attention_join_
   const u32x2_t place = own.places[held], place_before = before.all ? before.places[held] : u32x2_t{0u, 0u};
   Sums a = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
   int planes = 0;
-  if (token >= start && token < end) {
+  if (token >= start && token < end && d < s.head_dim) {
     const int kv_head = head / group, in_group = head - kv_head * group;
     auto add = [&](const Pass &p, Planes of) __attribute__((always_inline)) {
       planes += of.count;
