@@ -516,7 +516,7 @@ __global__ __launch_bounds__(64 * stream_waves(D)) void attention_stream_kernel(
 // unit, the matrix unit forms the scores of tile j + 1; then come the weighted values of tile j.  Used: the values of a head, rounded up to 32 (D, the
 // length of a row in LDS, is a power of two).
 //
-// A prompt of 8192 tokens, 32 heads on 8 of 128 (Waves 8): 530 us, 1035 TFLOP/s of what the mask leaves; a matrix product reaches 1410 here.  The matrix unit is
+// A prompt of 8192 tokens, 32 heads on 8 of 128 (Waves 8): 526 us, 1045 TFLOP/s of what the mask leaves; a matrix product reaches 1410 here.  The matrix unit is
 // busy for 47 % of the time, at 2.1 to 2.2 GHz, the power's bound.  Without the exponentials it took 535 of then 567 us, without the scores' product 412, without the
 // values' 460, without transfers 462: what is left is the softmax's vector instructions (4.3 to a matrix instruction) beside the matrix unit.  First without the
 // scores ahead 641, with 32 x 32 matrix instructions 552 for 547; 64 rows to a wave, one wave to a SIMD, 855.
@@ -635,11 +635,11 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
   for (int c = 0; c < kColumns; ++c)
 #pragma unroll
     for (int r = 0; r < Blocks; ++r) o[c][r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m[Blocks], l[Blocks], bound[Blocks];    // bound: the score from which m is to follow
+  float m[Blocks], l[Blocks], bound[Blocks], offset[Blocks];    // bound: the score from which m is to follow; offset: scale times m, 0 before there is one
 #pragma unroll
   for (int r = 0; r < Blocks; ++r) {
     score[0][r] = score[1][r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    m[r] = bound[r] = -INFINITY, l[r] = 0.f;
+    m[r] = bound[r] = -INFINITY, l[r] = offset[r] = 0.f;
   }
   const float lag = kLag / s.scale;
   const uint16_t largest = least < it.end ? P::kExponent - 1 : 0x7FFF;
@@ -657,17 +657,14 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) fragments[b][i] = *reinterpret_cast<const u32x4 *>(k + ((key_at ^ i << 6) + b * 16 * kRowBytes));
   };
-  auto scores = [&](f32x4_t (&sum)[2][Blocks]) __attribute__((always_inline)) {
+  auto scores = [&](f32x4_t (&sum)[2][Blocks], int b) __attribute__((always_inline)) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int r = 0; r < Blocks; ++r) sum[b][r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int r = 0; r < Blocks; ++r) sum[b][r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < kSteps; ++i) {
+      const u32x4 a = fragments[b][i];
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const u32x4 a = fragments[b][i];
-#pragma unroll
-        for (int r = 0; r < Blocks; ++r) sum[b][r] = P::mul(a, q[r][i], sum[b][r]);
-      }
+      for (int r = 0; r < Blocks; ++r) sum[b][r] = P::mul(a, q[r][i], sum[b][r]);
     }
   };
   auto tile = [&](auto masked, const char *next, const char *v, int key0) __attribute__((always_inline)) {
@@ -704,7 +701,7 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
 #pragma unroll
       for (int r = 0; r < Blocks; ++r) {
         const float now = fmaxf(m[r], most[r]), keep = now == m[r] ? 1.f : __builtin_amdgcn_exp2f((m[r] - now) * s.scale);
-        m[r] = now, bound[r] = now + lag;
+        m[r] = now, bound[r] = now + lag, offset[r] = now == -INFINITY ? 0.f : now * s.scale;
         l[r] *= keep;
 #pragma unroll
         for (int c = 0; c < kColumns; ++c) o[c][r] *= keep;
@@ -712,27 +709,43 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
     }
     f32x4_t following[2][Blocks];
     if constexpr (!kEarly) read_keys(next);
-    scores(following);
-    u32x4 weights[Blocks];
-#pragma unroll
-    for (int r = 0; r < Blocks; ++r) {
-      const float offset = m[r] == -INFINITY ? 0.f : m[r] * s.scale;
+    u32x4 weights[Blocks], values[kColumns];
+    auto weigh = [&](int r) __attribute__((always_inline)) {
+      const float less = kEarly ? offset[r] : m[r] == -INFINITY ? 0.f : m[r] * s.scale;      // (registers again: heads of 256, held 195 us, formed 192)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j / 2][r][j % 2 * 2], s.scale, -offset));
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j / 2][r][j % 2 * 2 + 1], s.scale, -offset));
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j / 2][r][j % 2 * 2], s.scale, -less));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j / 2][r][j % 2 * 2 + 1], s.scale, -less));
         weights[r][j] = P::pack(x, y);
         l[r] += x + y;
       }
+    };
+    auto read_values = [&](int c) __attribute__((always_inline)) {
+      const int at = value_at ^ c << 5;
+      const u32x2_t lo = read_turned(v, at), hi = read_turned(v, at + 16 * kRowBytes);
+      values[c] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    if constexpr (kEarly) {
+      // Values are asked for as soon as half of the keys' registers are free, not each where it is used (16 prompts of 1000 223 to 217 us).
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        scores(following, b);
+        weigh(b);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = b * kColumns / 2; c < (b + 1) * kColumns / 2; ++c) read_values(c);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      scores(following, 0), scores(following, 1);
+      weigh(0), weigh(1);
     }
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) {
-      const int at = value_at ^ c << 5;
-      const u32x2_t lo = read_turned(v, at), hi = read_turned(v, at + 16 * kRowBytes);
-      u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
-      if constexpr (kMasked) a = cleaned(a, largest, unbounded);
+      if constexpr (!kEarly) read_values(c);
+      if constexpr (kMasked) values[c] = cleaned(values[c], largest, unbounded);
 #pragma unroll
-      for (int r = 0; r < Blocks; ++r) o[c][r] = P::mul(a, weights[r], o[c][r]);
+      for (int r = 0; r < Blocks; ++r) o[c][r] = P::mul(values[c], weights[r], o[c][r]);
     }
 #pragma unroll
     for (int r = 0; r < Blocks; ++r) score[0][r] = following[0][r], score[1][r] = following[1][r];
@@ -752,7 +765,7 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
     __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(6 * kMoves));      // the first tile's keys
     barrier_no_fence();
     read_keys(lds_ring<10, kTileBytes>);
-    scores(score);
+    scores(score, 0), scores(score, 1);
   }
   // Tiles that all of this wave's rows see, a whole number of rounds of the ring, and the others.
   const int whole = max(min((least - it.begin) / kTileKeys, tiles), 0) & ~3;
