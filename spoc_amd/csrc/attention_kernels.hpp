@@ -12,7 +12,7 @@
 // with its own keys and its own transfers.  Many rows are bound by the matrix unit: attention_tile_kernel, 128 rows that share what a
 // workgroup brings to LDS.  Where rows are few for the card the keys are split into stretches of about the same length, and
 // attention_join_kernel joins what they leave (o, m and l in float32); the tiles and stretches are laid out by every workgroup for itself
-// from the lengths (Plan), which the host does not know.
+// from the lengths (find_item), which the host does not know.
 #pragma once
 #include <algorithm>
 #include <cmath>
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(64 * stream_waves(D)) void attention_stream_kernel(
 
 // ---- many rows -----------------------------------------------------------------------------------------------------------------------
 
-// Four waves of 32 rows, two blocks of 16; tiles of 32 keys go to LDS for all of them, three ahead.  While the softmax of tile j is on the vector
+// Four or eight waves of 32 rows, two blocks of 16; tiles of 32 keys go to LDS for all of them, three ahead.  While the softmax of tile j is on the vector
 // unit, the matrix unit forms the scores of tile j + 1; then come the weighted values of tile j.  Used: the values of a head, rounded up to 32 (D, the
 // length of a row in LDS, is a power of two).
 //

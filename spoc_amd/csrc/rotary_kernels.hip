@@ -122,6 +122,13 @@ __device__ __forceinline__ void turn_pieces(const RotaryArgs &r, int64_t positio
   }
   // The last pairs, fewer than 8
   const int a_count = Interleaved ? 2 * left : left, b_count = Interleaved ? 2 * left - 8 : left;
+  if constexpr (kHeads == 1) {
+    const Raw8<T> ra = load8(x + head * x_head + a_at, a_count), rb = load8(x + head * x_head + b_at, b_count);
+    turned(angles(r, position, unit), ra, rb, u, v);
+    store8(out + head * out_head + a_at, a_count, u);
+    store8(out + head * out_head + b_at, b_count, v);
+    return;
+  }
   const Turned t = angles(r, position, unit);
 #pragma unroll 1
   for (int h = head; h < min(head + kHeads, heads); ++h) {
