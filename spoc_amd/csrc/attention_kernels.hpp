@@ -198,6 +198,7 @@ template <> struct Products<Bf16> {
   static __device__ __forceinline__ float low(uint32_t v) { return bf16_to_f32(v); }
   static __device__ __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
   static constexpr uint32_t kExponent = 0x7F80u;
+  static constexpr float kRaised = 0.f;
 };
 template <> struct Products<_Float16> {
   static __device__ __forceinline__ f32x4_t mul(u32x4 a, u32x4 b, f32x4_t c) { return mfma16<false>(a, b, c); }
@@ -205,7 +206,13 @@ template <> struct Products<_Float16> {
   static __device__ __forceinline__ float low(uint32_t v) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(v))); }
   static __device__ __forceinline__ float high(uint32_t v) { return low(v >> 16); }
   static constexpr uint32_t kExponent = 0x7C00u;
+  static constexpr float kRaised = 7.f;
 };
+// What is taken from a row's scores (log2) before the exponential: its maximum, less kRaised, so that weights, their sum and the weighted values are all held
+// 2^kRaised times as large.  fp16 has steps of 2^-24 below 2^-14 and nothing below 2^-25: of weights up to 1 thousands that are small would be lost to the product,
+// though not to their sum (131071 keys 18 natural units below another one, whose value is 0: 1e-4 for 2e-3).  With kLag they stay
+// below 2^15 and are off by 2^-32 of the largest at most.  bf16's exponents are float32's.
+template <class T> __device__ __forceinline__ float offset_of(float m, float scale) { return __builtin_fmaf(m, scale, -Products<T>::kRaised); }
 
 // Four consecutive keys of a column of V in each lane: lane i of 16 gives the address of 8 bytes of key i / 4, columns 4 (i % 4) on, and
 // gets the keys of column i.
@@ -269,7 +276,7 @@ template <class T> __device__ __forceinline__ void store_out(const AttentionArgs
 __device__ __forceinline__ void store_lse(const AttentionArgs &s, int token, int head, float m, float l) {
   if (s.lse) s.lse[static_cast<int64_t>(token) * s.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
 }
-// A maximum may lag behind its row by this much (log2): weights up to 2^8 lose nothing, and the sums are rescaled a few times instead of
+// A maximum may lag behind its row by this much (log2): weights up to 2^8 times as large lose nothing, and the sums are rescaled a few times instead of
 // at every new maximum.
 constexpr float kLag = 8.f;
 
@@ -412,9 +419,9 @@ __global__ __launch_bounds__(64 * stream_waves(D)) void attention_stream_kernel(
 #pragma unroll
       for (int c = 0; c < kColumns; ++c) o[c] *= keep;
     }
-    const float offset = m == -INFINITY ? 0.f : m * s.scale;
+    const float offset = m == -INFINITY ? 0.f : offset_of<T>(m, s.scale);
     // The weights go into the product in two parts of the type, the second what the first's rounding has left: the matrix unit is idle for most of the
-    // time here, and the sums are those of 32-bit weights.
+    // time here.  They are off by 2^-16 of themselves in bf16, 2^-22 in fp16 (and 2^-32 of the largest), which out's own rounding hides.
     u32x4 big, small;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -479,7 +486,7 @@ __global__ __launch_bounds__(64 * stream_waves(D)) void attention_stream_kernel(
   float *const sums = reinterpret_cast<float *>(lds_ring<0, kStage>), *const ends = reinterpret_cast<float *>(lds_ring<1, kStage>);
 #pragma unroll
   for (int c = 0; c < kColumns; ++c) *reinterpret_cast<f32x4_t *>(sums + (wave * 16 + l16) * kPitch + c * 16 + quad * 4) = o[c];
-  if (quad == 0) ends[(wave * 16 + l16) * 2] = m * s.scale, ends[(wave * 16 + l16) * 2 + 1] = l;
+  if (quad == 0) ends[(wave * 16 + l16) * 2] = offset_of<T>(m, s.scale), ends[(wave * 16 + l16) * 2 + 1] = l;
   __syncthreads();
   // Threads by four columns of the rows that there are.  Where there is no other stretch the row is done, but for the prefix's planes.
   constexpr int kThreads = 64 * kWaves, kQuads = Used / 4;
@@ -635,7 +642,7 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
   for (int c = 0; c < kColumns; ++c)
 #pragma unroll
     for (int r = 0; r < Blocks; ++r) o[c][r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m[Blocks], l[Blocks], bound[Blocks], offset[Blocks];    // bound: the score from which m is to follow; offset: scale times m, 0 before there is one
+  float m[Blocks], l[Blocks], bound[Blocks], offset[Blocks];    // bound: the score from which m is to follow; offset: of m, 0 before there is one
 #pragma unroll
   for (int r = 0; r < Blocks; ++r) {
     score[0][r] = score[1][r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -701,7 +708,7 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
 #pragma unroll
       for (int r = 0; r < Blocks; ++r) {
         const float now = fmaxf(m[r], most[r]), keep = now == m[r] ? 1.f : __builtin_amdgcn_exp2f((m[r] - now) * s.scale);
-        m[r] = now, bound[r] = now + lag, offset[r] = now == -INFINITY ? 0.f : now * s.scale;
+        m[r] = now, bound[r] = now + lag, offset[r] = now == -INFINITY ? 0.f : offset_of<T>(now, s.scale);
         l[r] *= keep;
 #pragma unroll
         for (int c = 0; c < kColumns; ++c) o[c][r] *= keep;
@@ -711,7 +718,7 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
     if constexpr (!kEarly) read_keys(next);
     u32x4 weights[Blocks], values[kColumns];
     auto weigh = [&](int r) __attribute__((always_inline)) {
-      const float less = kEarly ? offset[r] : m[r] == -INFINITY ? 0.f : m[r] * s.scale;      // (registers again: heads of 256, held 195 us, formed 192)
+      const float less = kEarly ? offset[r] : m[r] == -INFINITY ? 0.f : offset_of<T>(m[r], s.scale);      // (registers again: heads of 256, held 195 us, formed 192)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j / 2][r][j % 2 * 2], s.scale, -less));
@@ -811,8 +818,8 @@ __global__ __launch_bounds__(64 * Waves, D == 256 ? 1 : 2) void attention_tile_k
       else if (d < s.head_dim) *reinterpret_cast<f32x4_t *>(p.o + place * D + d) = o[c][r];
     }
     if (quad == 0) {
-      if (it.slot < 0) store_lse(s, row[r].token, row[r].head, m[r] * s.scale, l[r]);
-      else p.ml[place] = f32x2_t{m[r] * s.scale, l[r]};
+      if (it.slot < 0) store_lse(s, row[r].token, row[r].head, offset_of<T>(m[r], s.scale), l[r]);
+      else p.ml[place] = f32x2_t{offset_of<T>(m[r], s.scale), l[r]};
       if (p.places && it.stretch == 0 && row[r].head == 0) tell_place(p, it, row[r].token, in_tile);
     }
   }
