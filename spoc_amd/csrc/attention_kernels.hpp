@@ -191,12 +191,15 @@ __device__ __forceinline__ void move16(const char *base, __amdgpu_buffer_rsrc_t 
   }
 }
 
+// pack: two values of the type, rounded; pack_below: the largest below them (0 of 0), which are not negative.
+__device__ __forceinline__ uint32_t before(float v) { return __builtin_elementwise_sub_sat(__float_as_uint(v), 1u); }
 template <class T> struct Products;
 template <> struct Products<Bf16> {
   static __device__ __forceinline__ f32x4_t mul(u32x4 a, u32x4 b, f32x4_t c) { return mfma16<true>(a, b, c); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return f32_pair_to_bf16(lo, hi); }
   static __device__ __forceinline__ float low(uint32_t v) { return bf16_to_f32(v); }
   static __device__ __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+  static __device__ __forceinline__ uint32_t pack_below(float lo, float hi) { return __builtin_amdgcn_perm(before(hi), before(lo), 0x07060302u); }
   static constexpr uint32_t kExponent = 0x7F80u;
   static constexpr float kRaised = 0.f;
 };
@@ -205,6 +208,9 @@ template <> struct Products<_Float16> {
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return f32_pair_to_f16(lo, hi); }
   static __device__ __forceinline__ float low(uint32_t v) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(v))); }
   static __device__ __forceinline__ float high(uint32_t v) { return low(v >> 16); }
+  static __device__ __forceinline__ uint32_t pack_below(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(before(lo)), __uint_as_float(before(hi))));
+  }
   static constexpr uint32_t kExponent = 0x7C00u;
   static constexpr float kRaised = 7.f;
 };
@@ -420,15 +426,16 @@ __global__ __launch_bounds__(64 * stream_waves(D)) void attention_stream_kernel(
       for (int c = 0; c < kColumns; ++c) o[c] *= keep;
     }
     const float offset = m == -INFINITY ? 0.f : offset_of<T>(m, s.scale);
-    // The weights go into the product in two parts of the type, the second what the first's rounding has left: the matrix unit is idle for most of the
-    // time here.  They are off by 2^-16 of themselves in bf16, 2^-22 in fp16 (and 2^-32 of the largest), which out's own rounding hides.
+    // The weights go into the product in two parts of the type, the second what the first leaves: the matrix unit is idle for most of the time here.  They are
+    // off by 2^-15 of themselves in bf16, 2^-21 in fp16 (and 2^-32 of the largest), which out's own rounding hides.  The first is below the weight, so that
+    // both are positive: an infinity among the values times 0, or times parts of both signs, is NaN.  (Rounded to nearest it is half as far off, and no faster.)
     u32x4 big, small;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j / 2][j % 2 * 2], s.scale, -offset));
       const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j / 2][j % 2 * 2 + 1], s.scale, -offset));
       l += x + y;
-      big[j] = P::pack(x, y);
+      big[j] = P::pack_below(x, y);
       small[j] = P::pack(x - P::low(big[j]), y - P::high(big[j]));
     }
 #pragma unroll

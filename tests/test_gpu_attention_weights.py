@@ -2,7 +2,8 @@
 rounds them once more than it says would not pass.
 
 With p the weights relative to a row's largest, S their sum, and h = eps / 2 of the type, the largest error of a rounding, relative to the value:
-  few rows (up to 16 to a sequence): a weight is two parts of the type, so off by h^2 of itself;
+  few rows (up to 16 to a sequence): a weight is two parts of the type, the first below it by up to 2 h of it and the second what is left, rounded: off by
+  2 h^2 of itself;
   tiles of rows: it is rounded to the type once, off by h of itself;
   fp16: besides by 2^-32 of the largest at most, half of the smallest step 2^-24 of weights that are held 2^7 times as large.
 The queries and keys are such that scores are exact sums: an exponent's argument is then off by 2^-24 of itself for the scale and for the product each, the
@@ -28,7 +29,7 @@ def exactly(q, k, v, seen, scale, parts):
     total = p.sum(1, keepdim=True)
     o, size = p @ v / total, p @ v.abs() / total
     exponent = torch.where(p > 0, p * 2.0 ** -21 * (1 + torch.where(p > 0, s.amax(1, keepdim=True) - s, 0.0)), 0.0)
-    rest = (p * h ** parts + exponent) @ v.abs() / total + o.abs() * (exponent.sum(1, keepdim=True) / total + 2.0 ** -22) + (size + o.abs()) * n * 2.0 ** -24
+    rest = (p * (2 * h * h if parts == 2 else h) + exponent) @ v.abs() / total + o.abs() * (exponent.sum(1, keepdim=True) / total + 2.0 ** -22) + (size + o.abs()) * n * 2.0 ** -24
     if q.dtype == torch.float16:
         rest = rest + 2.0 ** -32 * (seen.double() @ v.abs()) / total
     own = h * o.abs() + (2.0 ** -25 if q.dtype == torch.float16 else 0)
@@ -160,6 +161,7 @@ def rounded_weights(q, k, v, scale, parts, raised):
     x = x / x.amax(1, keepdim=True)
     held = (x * 2.0 ** raised).to(q.dtype).double()
     if parts == 2:
+        held = torch.where(held < x * 2.0 ** raised, held, (held * (1 - torch.finfo(q.dtype).eps)).to(q.dtype).double())
         held = held + (x * 2.0 ** raised - held).to(q.dtype).double()
     return (held @ v.double() / 2.0 ** raised / x.sum(1, keepdim=True)).to(q.dtype)
 
