@@ -1358,7 +1358,8 @@ def attention_shared(q, cache, prefix_pages, prefix_length, pages, lengths, star
     first=prefix_length)."""
     if not isinstance(cache, KvCache):
         raise TypeError("cache: expected a KvCache")
-    got = _host.attention_tensors(q, cache._call, prefix_pages, prefix_length, pages, lengths, starts, causal, scale, out, lse)
+    # (None would be a call without a prefix there)
+    got = None if prefix_pages is None else _host.attention_tensors(q, cache._call, prefix_pages, prefix_length, pages, lengths, starts, causal, scale, out, lse)
     if got is not None:
         return got
     at = _table(prefix_pages, (None,), "prefix_pages", cache.keys.device)
