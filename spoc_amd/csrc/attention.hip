@@ -83,6 +83,8 @@ int attention(const char *what, const sarek_hip_kv_cache *cache, const void *q, 
   if (!(scale > 0.f) || !std::isfinite(scale * kLog2E)) return fail(SAREK_HIP_E_INVALID_ARG, "%s: the scale must be positive and finite", what);
   SAREK_ATTENTION_TRY(check_heads(what, "q", q_token, q_head, tokens, q_heads, cache->head_dim, false));
   SAREK_ATTENTION_TRY(check_heads(what, "out", out_token, out_head, tokens, q_heads, cache->head_dim, true));
+  if (q && q == out && ((tokens > 1 && q_token != out_token) || (q_heads > 1 && q_head != out_head)))
+    return fail(SAREK_HIP_E_INVALID_ARG, "%s: out is q with other strides", what);
   if (prefix_length < 0 || (prefix_length > 0 && !prefix_pages)) return fail(SAREK_HIP_E_INVALID_ARG, "%s: a prefix of %lld keys", what, static_cast<long long>(prefix_length));
   if (prefix_length > int64_t{1} << 30) return fail(SAREK_HIP_E_UNSUPPORTED, "%s: a prefix past 2^30 keys", what);
   const int64_t need = sarek_hip_attention_workspace_bytes(cache, q_heads, batch, tokens, max_pages, prefix_length);

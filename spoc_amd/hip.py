@@ -1343,7 +1343,7 @@ def attention_paged(q, cache, pages, lengths, starts=None, causal=True, scale=No
     """softmax(scale q . keys) . values of q [tokens, heads, head dim] over a KvCache, whose heads serve as many of q's each as there are;
     scale None: head dim ^ -1/2.  The sequences' tokens, lengths and pages: as for kv_append, the tokens' own keys are in the cache
     already.  causal: a token sees its sequence's keys up to its own, otherwise all of them; a token that sees none gets zeros.
-    out: where the result goes, which may be q itself; lse (float32 [tokens, heads]): gets the logarithm of the sum of the exponents, -inf where there is none.
+    out: where the result goes, which may be q itself (not q's memory in another order); lse (float32 [tokens, heads]): gets the logarithm of the sum of the exponents, -inf where there is none.
     Rows of tokens before the first and behind the last sequence are left as they are."""
     if isinstance(cache, KvCache):
         got = _host.attention_tensors(q, cache._call, None, 0, pages, lengths, starts, causal, scale, out, lse)
