@@ -40,7 +40,7 @@ class MxAttention:
             hip.attention_paged(q, cache, pages, lengths, starts=starts, out=o)
         else:
             hip.attention_shared(q, cache, prefix[0], prefix[1], pages, lengths, starts=starts, out=o)
-        y = hip.gemm_mx(hip.mx_quantize(o.view(tokens, -1), "fp8"), self.output, dtype=x.dtype)
+        y = hip.gemm_mx(hip.mx_quantize(o.flatten(1), "fp8"), self.output, dtype=x.dtype)
         return y, h
 
 

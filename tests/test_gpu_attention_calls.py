@@ -33,3 +33,17 @@ def test_out_in_the_memory_of_q_in_another_order_is_refused(hip, cache):
         with pytest.raises(hip.SarekHipError, match="other strides"):
             call(out)
         assert call(q.view(4, 4, 64)) is not None
+
+
+@pytest.mark.parametrize("prefix", [0, 20])
+def test_a_layer_of_no_tokens(hip, cache, prefix):
+    from spoc_amd.attention import MxAttention
+    random = lambda *shape: hip.mx_quantize(torch.randn(*shape, device="cuda"), "fp4")  # noqa: E731
+    layer = MxAttention(torch.ones(256, dtype=torch.bfloat16, device="cuda"), random(8 * 64, 256), random(256, 4 * 64), 4, 2, hip.Rotary(64))
+    none = torch.empty(0, 256, dtype=torch.bfloat16, device="cuda")
+    shared = (ints(2, 3), prefix) if prefix else None
+    for more in (dict(starts=ints(0, 0)), dict(starts=ints(0, 0), residual=none)):
+        y, h = layer(none, cache, ints([0]), ints(5), prefix=shared, **more)
+        assert y.shape == h.shape == (0, 256) and y.dtype == h.dtype == torch.bfloat16
+    y, h = layer(none, cache, torch.empty(0, 1, dtype=torch.int32, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda"), prefix=shared)
+    assert y.shape == h.shape == (0, 256) and (cache.keys == 0).all() and (cache.values == 0).all()
