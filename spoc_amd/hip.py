@@ -1280,6 +1280,8 @@ def kv_append(k, v, cache, pages, lengths, starts=None, rotary=None, q=None, q_o
     alone, in q_out too."""
     if not isinstance(cache, KvCache):
         raise TypeError("cache: expected a KvCache")
+    if q is None and q_out is not None:
+        raise ValueError("q_out: there is no q")
     if rotary is None or isinstance(rotary, Rotary):
         got = _host.kv_append_tensors(k, v, cache._call, pages, lengths, starts, None if rotary is None else rotary._call, q, q_out, first)
         if got is not None:

@@ -47,3 +47,10 @@ def test_a_layer_of_no_tokens(hip, cache, prefix):
         assert y.shape == h.shape == (0, 256) and y.dtype == h.dtype == torch.bfloat16
     y, h = layer(none, cache, torch.empty(0, 1, dtype=torch.int32, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda"), prefix=shared)
     assert y.shape == h.shape == (0, 256) and (cache.keys == 0).all() and (cache.values == 0).all()
+
+
+def test_a_place_for_q_without_a_q_is_refused(hip, cache):
+    with pytest.raises(ValueError):
+        hip.kv_append(heads(n=2), heads(n=2), cache, ints([0, 1], [2, 3]), ints(5, 6), q_out=heads())
+    assert (cache.keys == 0).all()
+    assert hip.kv_append(heads(n=2), heads(n=2), cache, ints([0, 1], [2, 3]), ints(5, 6)) is None
