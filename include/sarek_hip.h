@@ -729,7 +729,8 @@ int sarek_hip_gemm_mx(const unsigned char *a_codes, const unsigned char *a_scale
  * Rotary positions.  Pair i of a head, i < pairs, is turned by the angle position times the pair's frequency, and multiplied by
  * amplitude: (a, b) -> (a cos - b sin, a sin + b cos).  Pairs are the values i and i + pairs (interleaved 0) or 2 i and 2 i + 1
  * (interleaved 1); what is behind value 2 pairs of a head stays as it is.  A frequency is held as the turns that it makes from position to
- * position in units of 2^-64, modulo one turn, so that an angle is exact to 2^-24 turns of itself at any position;
+ * position in units of 2^-64, modulo one turn, rounded.  With it an angle is off by less than |position| 2^-64 + 2^-33 turns (frequencies of
+ * up to half a turn; 2^-32 at positions of up to 2^31), and by 2^-24 of itself, reduced to half a turn either way;
  * sarek_hip_rotary_turns brings radians (host memory) to that (host memory).                                                    */
 typedef struct {
   const uint64_t *turns;   /* device memory, `pairs` of them */

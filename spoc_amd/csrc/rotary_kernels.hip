@@ -1,9 +1,10 @@
 // Rotary positions, by themselves and on the way into a paged cache.
 //
 // Pair (a, b) of a head becomes amplitude (a cos t - b sin t, a sin t + b cos t), t = position * frequency.  The angle is formed in whole
-// numbers: position times the frequency in units of 2^-64 turns, modulo one turn by the overflow, of which the upper 32 bits are the
-// angle as a signed fraction of a turn.  That is right to 2^-33 turns at any position (a 32-bit product of both is 0.06 radians off at
-// position 10^6), and there is no reduction of the argument left for the sine.
+// numbers: position times the frequency in units of 2^-64 turns, modulo one turn by the overflow, of which the upper 32 bits, rounded, are the angle as a
+// signed fraction of a turn.  The table's entry is off by less than 2^-64 turns (frequencies of up to half a turn), so the angle is off by |position| 2^-64 + 2^-33 turns, up
+// to 2^-32 at positions of up to 2^31, and by 2^-24 of itself, float32's rounding (a 32-bit product of both is 0.06 radians off at position 10^6).  There is no reduction
+// of the argument left for the sine.
 //
 // Memory bounds both kernels (two products and a sum to a value); a thread takes 8 pairs of a head, two accesses of 16 bytes each way in
 // 16-bit types, and where there are many tokens 4 heads, for which it forms the sines once (8192 x 32 x 128 bf16: 22 us, 6.1 TB/s; a
@@ -52,7 +53,7 @@ __device__ __forceinline__ Turned angles(const RotaryArgs &r, int64_t position, 
   Turned t;
 #pragma unroll
   for (int j = 0; j < kPairs; ++j) {
-    const uint64_t turn = static_cast<uint64_t>(position) * r.turns[min(unit * kPairs + j, r.pairs - 1)];
+    const uint64_t turn = static_cast<uint64_t>(position) * r.turns[min(unit * kPairs + j, r.pairs - 1)] + 0x80000000u;
     sincospif(static_cast<float>(static_cast<int32_t>(turn >> 32)) * 0x1p-31f, &t.sin[j], &t.cos[j]);
     t.sin[j] *= r.inverse ? -r.amplitude : r.amplitude;
     t.cos[j] *= r.amplitude;
@@ -268,7 +269,8 @@ int sarek_hip_rotary_turns(const double *radians, uint64_t *turns, int pairs) {
   for (int i = 0; i < pairs; ++i) {
     if (!std::isfinite(radians[i])) return fail(SAREK_HIP_E_INVALID_ARG, "rotary_turns: frequency %d is not finite", i);
     const long double turn = radians[i] / 6.283185307179586476925286766559005768L, part = turn - std::floor(turn);
-    turns[i] = part * 0x1p64L < 0x1p64L ? static_cast<uint64_t>(part * 0x1p64L) : 0;
+    const long double rounded = std::nearbyint(part * 0x1p64L);
+    turns[i] = rounded < 0x1p64L ? static_cast<uint64_t>(rounded) : 0;
   }
   return SAREK_HIP_OK;
 }
