@@ -771,8 +771,16 @@ int sarek_hip_kv_append(const sarek_hip_kv_cache *cache, const void *k, int64_t 
 /* out = softmax(scale q . keys) . values, head h of q with head h / (q_heads / cache->heads) of the cache; causal not 0: a token sees its
  * sequence's keys up to its own.  A token that sees no key gets zeros.  lse (or NULL) [tokens, q_heads]: the natural logarithm of
  * the sum of the exponents, minus infinity for no key; one whose scores are all minus infinity counts as that.  out may be q itself, with
- * its strides, and must not overlap it otherwise.  Scores, their exponents' sums and the weighted values are held in float32.  A
- * key that a token does not see takes no part in its sums, whatever the cache holds there.  scale is positive and finite.
+ * its strides, and must not overlap it otherwise.  scale is positive and finite.
+ * A key that a token does not see takes no part in its sums, whatever the cache holds there.  An infinite value that it sees makes its sum
+ * infinite (NaN where the weight is 0 in the type).
+ * Scores, their exponents' sums and the sums of weighted values are held in float32.  The weights go into the product with the values in
+ * the cache's type.  Rows being tokens times the heads of q that share one of the cache, calls of up to 16 rows to a sequence on average
+ * take a weight in two parts, off by 2^-15 of itself in bf16 and 2^-21 in fp16, which the rounding of out hides.  Other calls, and the
+ * prefix of attention_shared where the rows of all tokens are more than 16, round it once, by up to 2^-8 and 2^-11: out is then off by
+ * 0.0022 of its norm in bf16, where its own rounding alone is 0.0016, and by 0.00028 for 0.0002 in fp16.  So the last bits of a token's
+ * row depend on what else is in its call.  fp16 besides drops up to 2^-32 of a row's largest weight from each.  lse has the weights as
+ * they are in float32.
  * workspace: sarek_hip_attention_workspace_bytes, for the same arguments, of device memory (16 bytes aligned), SAREK_HIP_E_WORKSPACE else;
  * one call at a time may use it.
  * attention_shared: every sequence begins with the prefix_length keys of prefix_pages (device memory, at least prefix_length / page_size

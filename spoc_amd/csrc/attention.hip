@@ -19,21 +19,24 @@ int64_t plane_bytes(const sarek_hip_kv_cache *cache, const Launch &r, int64_t to
 }
 // What is launched, by what the host knows: how many tokens, sequences and keys there are at most.
 //
-// Kernel.  Up to 16 rows to a sequence on average: the kernel of few rows; more: tiles of 128.  (us, 32 heads on 8 of 128, few rows / tiles: one
-// sequence of 4095 keys, 4 rows 16.3 / 19.0; 131071 keys 117 / 128; 64 of 2000, 20 rows 135 / 106, 16 rows 112 / 105.  Tiles are as fast from 8 rows on where
-// there are many sequences, but round the weights to 16 bits, which the kernel of few rows does not.)
-// Tiles of 256: heads of 65 to 128 values, long sequences that fill the card twice.  (One prompt, tiles of 256 / 128: 8192 tokens 526 / 537, 16384 2000 /
-// 2044; but 5000 231 / 219, and 16 prompts of 1000 242 / 222, for the rows past the ends and what the mask hides in a larger tile.)
+// Kernel.  Up to 16 rows to a sequence on average: the kernel of few rows; more: tiles of 128.  (us, calls without pauses, 32 heads on 8 of 128, few rows / tiles: one
+// sequence of 4095 keys, 4 rows 16.6 / 19.5; 131071 keys of 16 heads of 64, 113 / 121; 64 of 2000, 20 rows 135 / 105, 16 rows 107 / 104, 8 rows 104 / 103.  Tiles are as fast from 8 rows on
+// where there are many sequences, but round the weights to 16 bits, which the kernel of few rows does not.)  One kernel for the call: a chunk among single tokens, or one in a batch of
+// empty places, is not served by its own (127 tokens and a chunk of 380 265, each alone 246 and 42; a prompt of 1000 39, in a batch of 256 places 85).
+// Tiles of 256: heads of 65 to 128 values, long sequences that fill the card twice.  (One prompt, tiles of 256 / 128: 8192 tokens 516 / 522, 16384 1943 /
+// 1971; but 5000 229 / 217, and 16 prompts of 1000 242 / 217, for the rows past the ends and what the mask hides in a larger tile.)
 //
 // Stretches.  Where tiles are few for the card, the keys are cut: for as many workgroups as it takes at once if that comes out (find_item).  That is two to
 // a compute unit for tiles of 128 and few rows of more than 64 values, whose transfers it takes to keep the memory busy (one token each: 8 sequences of 4000 512
-// workgroups 33.4, 256 36.9, 768 40.4; 131071 keys of 16 heads 194, 211, 218), one otherwise, or where there is no room for two (the same of 64 values 120, 113, 118;
-// 12 of 4000, which do not fill 512: 480 42.6, 576 55.8).  Few rows that do not come out get half as many again (61 sequences of 100 to 11007: 768 207, 512
-// 225).  Tiles are cut below one to a compute unit: planes of 128 rows cost as much as 6 units of keys (2000 tokens behind 6000: uncut 249, cut 284); and for half as many
-// workgroups where a stretch would have less than 12 units (64 behind 8128: 4 units 36.3, 8 units 32.3; 500 behind 7692: 32 units 90, 64 units 99).
-// No more than 256 stretches: 30000 keys of one head, 235 of them 21.1, 469 25.3 (131071: 256 31.6, 512 35.7, 128 37.9).
+// workgroups 34.6, 256 37.1, 768 41.1; 131071 keys of 16 heads 195, 210, 218), one otherwise, or where there is no room for two (the same of 64 values 118, 113, 117;
+// 12 of 4000, which do not fill 512: 480 42.7, 576 56.3).  Few rows that do not come out get half as many again (61 sequences of 100 to 11007: 768 276, 512
+// 293).  Tiles are cut below one to a compute unit: planes of 128 rows cost as much as 6 units of keys (2000 tokens behind 6000: uncut 238, cut 248); and for half as many
+// workgroups where a stretch would have less than 12 units (64 behind 8128: 31.4, 34.9 without that; 500 behind 7692, which has more: 88.8, 95.1 with it).
+// No more than 256 stretches: 30000 keys of one head, 235 of them 20.1, 469 23.0 (131071: 256 30.0, 512 33.5, 128 36.6).
 // Own keys behind a prefix, few rows: a workgroup to each tile where these fill the card, which then finishes with the prefix's planes; no launch for
-// the join (61 sequences of up to 500 behind 8191: 57 with the join, 46).
+// the join (61 sequences of up to 500 behind 8191: 56 with the join, 47).
+// Whether keys are cut goes by how many tiles there are, not by how unlike the lengths are, which the host does not know: one sequence of 131071 keys among others of 500 takes 177 in a batch
+// of 90 single tokens, 2813 in one of 100, which is not cut any more.
 enum { kAlone, kBehindPrefix, kPrefix };
 Launch plan(const sarek_hip_kv_cache *cache, int q_heads, int64_t sequences, int64_t tokens, int64_t keys, int what) {
   const int d = cache->head_dim;

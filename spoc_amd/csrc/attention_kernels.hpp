@@ -337,8 +337,8 @@ template <int D, int kAtOnce> __device__ __forceinline__ void add_planes(const P
 
 // A wave takes every kWaves-th tile of 32 keys of the stretch by itself: its transfers go into its own part of LDS, one tile ahead, and there
 // is no barrier until the waves' sums are joined at the end.  The bytes of the cache bound it: 46 sequences of 100 to 11007 keys, 8 heads of
-// 128, 1.02 GB in 192 us, 5.3 TB/s (a large copy on this card: 5.1); 131071 keys of 16 heads of 64 in 98 us, 5.5.  The matrix unit is busy for 7 % of the time.  One
-// token of 4095 keys: 7.4 us for 17 MB, of which about 3 are a launch's start and the way to the first transfer (lengths, page, keys).
+// 128, 1.02 GB in 190 to 194 us, 5.3 TB/s (a large copy on this card: 5.1); 131071 keys of 16 heads of 64 in 99 us, 5.4.  The matrix unit is busy for 7 % of the time.  One
+// token of 4095 keys: 8.0 us for 17 MB, of which about 3 are a launch's start and the way to the first transfer (lengths, page, keys).
 template <class T, int D, int Used, bool Far>
 __global__ __launch_bounds__(64 * stream_waves(D)) void attention_stream_kernel(AttentionArgs s, Pass p, Pass before) {
   constexpr int kWaves = stream_waves(D), kRowBytes = 2 * D, kPieces = D / 8, kKeysMoved = 64 / kPieces, kMoves = kStreamKeys / kKeysMoved;
@@ -530,13 +530,15 @@ __global__ __launch_bounds__(64 * stream_waves(D)) void attention_stream_kernel(
 // unit, the matrix unit forms the scores of tile j + 1; then come the weighted values of tile j.  Used: the values of a head, rounded up to 32 (D, the
 // length of a row in LDS, is a power of two).
 //
-// A prompt of 8192 tokens, 32 heads on 8 of 128 (Waves 8): 526 us, 1045 TFLOP/s of what the mask leaves; a matrix product reaches 1410 here.  The matrix unit is
-// busy for 47 % of the time, at 2.1 to 2.2 GHz, the power's bound.  Without the exponentials it took 535 of then 567 us, without the scores' product 412, without the
+// A prompt of 8192 tokens, 32 heads on 8 of 128 (Waves 8): 514 us, 1070 TFLOP/s of what the mask leaves, right behind one another for 50 calls and more; the first ones, and
+// single calls, take 540 to 640, as the clock starts low.  A matrix product reaches 1410 here.  The matrix unit is busy for 48 % of the time, at 2.1 to 2.2 GHz, the power's bound.  (In its earlier
+// form:) without the exponentials it took 535 of then 567 us, without the scores' product 412, without the
 // values' 460, without transfers 462: what is left is the softmax's vector instructions (4.3 to a matrix instruction) beside the matrix unit.  First without the
 // scores ahead 641, with 32 x 32 matrix instructions 552 for 547; 64 rows to a wave, one wave to a SIMD, 855.
 //
-// The weights are rounded to 16 bits for the second product (in two parts, as in the other kernel, it would be twice the work): off by up to half a step
-// each, 2^-9 of a sum's size in bf16 where they add up at random, the size of out's own rounding.  l is the sum of the weights before that rounding, so lse is not touched.
+// The weights are rounded to 16 bits for the second product: off by up to half a step each, 2^-9 of a sum's size in bf16 where they add up at random, the size of out's own rounding (0.0022 of
+// out's norm for 0.0016, in fp16 0.00028 for 0.0002).  In two parts, as in the other kernel, a prompt of 8192 takes 707 us for 514, 5 chunks of 500 73 for 64, 61 tokens behind a prefix 50 for
+// 45.  l is the sum of the weights before that rounding, so lse is not touched.
 constexpr int kTileRing = 4;
 
 template <class T, int D, int Used, int Waves, bool Far>

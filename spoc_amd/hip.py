@@ -1346,7 +1346,10 @@ def attention_paged(q, cache, pages, lengths, starts=None, causal=True, scale=No
     scale None: head dim ^ -1/2.  The sequences' tokens, lengths and pages: as for kv_append, the tokens' own keys are in the cache
     already.  causal: a token sees its sequence's keys up to its own, otherwise all of them; a token that sees none gets zeros.
     out: where the result goes, which may be q itself (not q's memory in another order); lse (float32 [tokens, heads]): gets the logarithm of the sum of the exponents, -inf where there is none.
-    Rows of tokens before the first and behind the last sequence are left as they are."""
+    Rows of tokens before the first and behind the last sequence are left as they are.
+
+    All sums are float32.  Weights are multiplied with the values in the cache's type: in two parts (off by 2^-15 of themselves in bfloat16, 2^-21 in float16)
+    where the sequences have up to 16 rows each on average, tokens times the heads of q to one of the cache; rounded once (2^-8, 2^-11) otherwise."""
     if isinstance(cache, KvCache):
         got = _host.attention_tensors(q, cache._call, None, 0, pages, lengths, starts, causal, scale, out, lse)
         if got is not None:
@@ -1357,7 +1360,7 @@ def attention_paged(q, cache, pages, lengths, starts=None, causal=True, scale=No
 def attention_shared(q, cache, prefix_pages, prefix_length, pages, lengths, starts=None, causal=True, scale=None, out=None, lse=None):
     """attention_paged for sequences that all begin with the prefix_length keys of prefix_pages (int32, one page after the other), which
     are read once for all of them; pages and lengths are of what each sequence has behind the prefix (kv_append puts it there with
-    first=prefix_length)."""
+    first=prefix_length).  Before the prefix the rows of all tokens count together: where they are more than 16 its weights are rounded once."""
     if not isinstance(cache, KvCache):
         raise TypeError("cache: expected a KvCache")
     # (None would be a call without a prefix there)
