@@ -215,8 +215,8 @@ template <> struct Products<_Float16> {
   static constexpr float kRaised = 7.f;
 };
 // What is taken from a row's scores (log2) before the exponential: its maximum, less kRaised, so that weights, their sum and the weighted values are all held
-// 2^kRaised times as large.  fp16 has steps of 2^-24 below 2^-14 and nothing below 2^-25: of weights up to 1 thousands that are small would be lost to the product,
-// though not to their sum (131071 keys 18 natural units below another one, whose value is 0: 1e-4 for 2e-3).  With kLag they stay
+// 2^kRaised times as large.  fp16 has steps of 2^-24 below 2^-14 and nothing below 2^-25: with weights of up to 1, thousands of small ones would be lost to the
+// product, though not to their sum (131071 keys 18 natural units below another one, whose value is 0: 1e-4 for 2e-3).  With kLag they stay
 // below 2^15 and are off by 2^-32 of the largest at most.  bf16's exponents are float32's.
 template <class T> __device__ __forceinline__ float offset_of(float m, float scale) { return __builtin_fmaf(m, scale, -Products<T>::kRaised); }
 
